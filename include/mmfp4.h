@@ -189,6 +189,72 @@ int mm_fp4_gemm_multi(const uint16_t* A, int nmat, const uint32_t* const* B,
                       const uint16_t* const* S, uint16_t* const* C, const int* N, int M, int K,
                       int group_size, void* ws, size_t ws_bytes, void* stream);
 
+/* ------------------------------------------------- training on 4-bit weights */
+
+/* mm_fp4_gate_up (layout 0, Marlin words) / mm_fp4_gate_up_rowpacked (layout 1) with act = 1
+ * that keeps the two products for the backward pass:
+ *   C[M, N]        = silu(A . Wg) * (A . Wu)
+ *   gate_up[M, 2N] = [A . Wg | A . Wu]
+ * both rounded from the same fp32 sums, in one launch.  Requirements and workspace of the
+ * entry point that it extends; gate_up 8-byte aligned. */
+int mm_fp4_gate_up_keep(const uint16_t* A, const uint32_t* Bg, const uint16_t* Sg,
+                        const uint32_t* Bu, const uint16_t* Su, uint16_t* C, uint16_t* gate_up,
+                        int layout, int M, int N, int K, int group_size, void* ws,
+                        size_t ws_bytes, void* stream);
+
+/* Bytes of workspace mm_gemm_backward needs: arrival counters (zero before the first use,
+ * left at zero by every call), then partial sums. */
+size_t mm_gemm_backward_workspace_bytes(int nmat, const int* N, int M, int K);
+
+/* Input gradient of nmat <= 3 quantized products that share their input:
+ *   dA[M, K] = sum_p (dC[p] [M, N[p]] * row_mul[m]) . W_p[K, N[p]]^T
+ * dC[p] fp16 with row stride ldc[p]; row_mul fp32 [M] or NULL (ones).  W_p = dequant(B[p],
+ * S[p][, Z[p]]); Z NULL: FP4, else INT4 (layout 0 only).  layout 0: B[p] [K/8, N[p]] words;
+ * 1: row-packed [N[p], K/8] words.  Scales and zero points [K/g, N[p]].  out_type 0 fp32,
+ * 1 fp16, 2 bf16.  The tables are host arrays of device pointers.  N[p] % 8 == 0,
+ * ldc[p] % 8 == 0, K % 8 == 0 (layout 1: K % 32 == 0), group_size % 8 == 0 dividing K;
+ * every operand 16-byte aligned. */
+int mm_gemm_backward(const uint16_t* const* dC, const int* ldc, const float* row_mul, int nmat,
+                     const uint32_t* const* B, const uint16_t* const* S,
+                     const uint16_t* const* Z, const int* N, int layout, void* dA, int out_type,
+                     int M, int K, int group_size, void* ws, size_t ws_bytes, void* stream);
+
+/* Gradients carried in fp16 under one power of two per row: Y = X * 2^e with the row's
+ * largest magnitude in [2^14, 2^15), row_mul = 2^-e (a zero or non-finite row: e = 0).
+ * type 0 fp32, 1 fp16, 2 bf16; N % 8 == 0. */
+int mm_grad_rows(const void* X, int type, uint16_t* Y, float* row_mul, int M, int N,
+                 void* stream);
+
+/* Gradient of silu(g) * u, g and u the halves of gate_up [M, 2N] (mm_fp4_gate_up_keep):
+ * Y[M, 2N] = [dg | du] as mm_grad_rows carries it, one power of two per row. */
+int mm_swiglu_grad(const void* dH, int type, const uint16_t* gate_up, uint16_t* Y,
+                   float* row_mul, int M, int N, void* stream);
+
+/* Bytes of workspace of the adapter entry points below (arrival counters first, as above). */
+size_t mm_lora_workspace_bytes(int T, int K, int N, int rank, int adapters, int backward);
+
+/* Low-rank adapters of many requests added to a projection's output:
+ *   out[t] = base[t] + s_a * (x[t] . A_a^T) . B_a^T,   a = ids[t],  s_a = scale * scaling[a]
+ * x [T, K], out [T, N], A [adapters, rank, K] and B [adapters, N, rank] of one type (1 fp16,
+ * 2 bf16); base [T, N] fp16 or of that type (base_type); out may be base if the types agree.
+ * ids int32 (ids64 0) or int64 (1) [T]: an id outside [0, adapters) means no adapter; NULL:
+ * one adapter for all tokens.  scaling fp32 [adapters] or NULL (ones).  Any T, K, N and rank; at most 1024
+ * adapters. */
+int mm_lora_add(const uint16_t* x, int type, const uint16_t* base, int base_type, uint16_t* out,
+                const uint16_t* A, const uint16_t* B, const void* ids, int ids64,
+                const float* scaling, float scale, int T, int K, int N, int rank, int adapters,
+                void* ws, size_t ws_bytes, void* stream);
+
+/* Its gradients.  With h = s * x . A^T and dh = s * dy . B of each token:
+ *   dx[t] = dx_base[t] + dh[t] . A_a      (dx_base NULL: zeros; may be dx)
+ *   dA[a] = sum_t dh[t]^T x[t],  dB[a] = sum_t dy[t]^T h[t]   over the tokens of adapter a
+ * every tensor of the type of x; adapters without tokens get zeros. */
+int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type, const uint16_t* A,
+                     const uint16_t* B, const void* ids, int ids64, const float* scaling,
+                     float scale, const uint16_t* dx_base, uint16_t* dx, uint16_t* dA,
+                     uint16_t* dB, int T, int K, int N, int rank, int adapters, void* ws,
+                     size_t ws_bytes, void* stream);
+
 /* -------------------------------------------------------------------- MoE */
 
 /* Stable counting sort of the T*k (token, slot) assignments by expert.

@@ -48,11 +48,17 @@ MM_DEV float swiglu(float gate, float up) { return gate / (1.0f + __expf(-gate))
 //   SK_PAIR  : C[:, n] = A . Wg[:, n], C[:, N + n] = A . Wu[:, n]   (C is [M, 2N])
 //   SK_MULTI : up to three independent products sharing A and K (Q, K, V):
 //              the grid's column tiles are the three matrices' tiles in turn.
-enum { SK_PLAIN = 0, SK_SWIGLU = 1, SK_PAIR = 2, SK_MULTI = 3 };
+//   SK_KEEP  : SK_SWIGLU's C, and SK_PAIR's [M, 2N] products as well (`keep`), which the
+//              backward pass of the block starts from: the sums are in registers here, and
+//              a separate launch over the kept pair would read and write 6 M N bytes more.
+enum { SK_PLAIN = 0, SK_SWIGLU = 1, SK_PAIR = 2, SK_MULTI = 3, SK_KEEP = 4 };
+constexpr bool act_pair(int act) { return act == SK_SWIGLU || act == SK_PAIR || act == SK_KEEP; }
+constexpr bool act_glu(int act) { return act == SK_SWIGLU || act == SK_KEEP; }
+MM_DEV f16x4 to_f16x4(f32x4 v) { return f16x4{(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]}; }
 
 // SK_MULTI problem table: matrix p owns column tiles [tile0[p], tile0[p+1])
 // and partial-sum columns [cbase[p], cbase[p] + N[p]) of a [ksplit][M][ntot]
-// buffer; C[p] is [M, N[p]].
+// buffer; C[p] is [M, N[p]].  SK_KEEP: C[0] is the kept pair.
 struct SkMulti {
   const uint32_t* B[3];
   const f16* S[3];
@@ -181,8 +187,13 @@ k_skinny(const f16* __restrict__ A, int lda, const uint32_t* __restrict__ B,
     for (int k = 0; k < IPW; ++k) {
       const int row = item_row(k);
       if (row >= M) continue;
-      if constexpr (ACT == SK_SWIGLU) {
+      if constexpr (act_glu(ACT)) {
         const int col = n0 + 4 * c;
+        if (ACT == SK_KEEP && col < N) {
+          f16* kept = mp.C[0] + (size_t)row * (2 * N) + col;
+          *(f16x4*)kept = to_f16x4(rv[k][0]);
+          *(f16x4*)(kept + N) = to_f16x4(rv[k][1]);
+        }
         if (col < N)
           *(f16x4*)(C + (size_t)row * ldc + col) =
               f16x4{(f16)swiglu(rv[k][0][0], rv[k][1][0]), (f16)swiglu(rv[k][0][1], rv[k][1][1]),
@@ -236,7 +247,7 @@ k_skinny(const f16* __restrict__ A, int lda, const uint32_t* __restrict__ B,
   if (!s_last) return;
   // One thread per (row, 4-column) item sums the splits in order; the loads of
   // SK_RED_BATCH splits are issued together so the chain is ksplit/8 trips.
-  // SK_SWIGLU items carry the gate and the up columns of one 4-column group.
+  // SK_SWIGLU / SK_KEEP items carry the gate and the up columns of one 4-column group.
   auto sum_splits = [&](int row, int pc) {
     f32x4 v = {0, 0, 0, 0};
     for (int y0 = 0; y0 < ksplit; y0 += SK_RED_BATCH) {
@@ -252,14 +263,19 @@ k_skinny(const f16* __restrict__ A, int lda, const uint32_t* __restrict__ B,
     }
     return v;
   };
-  constexpr int GROUPS = (ACT == SK_SWIGLU ? 1 : NT) * SK_COLS / 4;   // 4-column items per row
+  constexpr int GROUPS = (act_glu(ACT) ? 1 : NT) * SK_COLS / 4;   // 4-column items per row
   const int nitems = min(M, MT * 16) * GROUPS;
   for (int e = threadIdx.x; e < nitems; e += NW * 64) {
     const int row = e / GROUPS, gi = e % GROUPS;
-    if constexpr (ACT == SK_SWIGLU) {
+    if constexpr (act_glu(ACT)) {
       const int col = n0 + 4 * gi;
       if (col >= N) continue;
       const f32x4 gt = sum_splits(row, col), up = sum_splits(row, N + col);
+      if constexpr (ACT == SK_KEEP) {
+        f16* kept = mp.C[0] + (size_t)row * (2 * N) + col;
+        *(f16x4*)kept = to_f16x4(gt);
+        *(f16x4*)(kept + N) = to_f16x4(up);
+      }
       *(f16x4*)(C + (size_t)row * ldc + col) =
           f16x4{(f16)swiglu(gt[0], up[0]), (f16)swiglu(gt[1], up[1]),
                 (f16)swiglu(gt[2], up[2]), (f16)swiglu(gt[3], up[3])};
@@ -581,7 +597,8 @@ __global__ void __launch_bounds__(WM * WN * 64)
 k_prefill2(const f16* __restrict__ A, int lda, const uint32_t* __restrict__ B,
            const f16* __restrict__ S, const f16* __restrict__ Z, const uint32_t* __restrict__ B2,
            const f16* __restrict__ S2, const f16* __restrict__ Z2, f16* __restrict__ C, int ldc,
-           int M, int N, int K, int g, float* __restrict__ part, int grp) {
+           int M, int N, int K, int g, float* __restrict__ part, int grp,
+           f16* __restrict__ keep) {
   // Wave tile: (32*RB) rows x (32*CW) LDS columns.  SK_PLAIN: lane l32 owns
   // CW adjacent columns (CW packed words of one word row feed CW column
   // tiles).  Pair modes (CW = 2, tile-major): column tile 0 is 32 gate
@@ -664,8 +681,12 @@ k_prefill2(const f16* __restrict__ A, int lda, const uint32_t* __restrict__ B,
         float* prow = part + ((size_t)bz * M + row) * PW;
         prow[ncol] = acc[rb][0][v];
         prow[N + ncol] = acc[rb][1][v];
-      } else if constexpr (ACT == SK_SWIGLU) {
+      } else if constexpr (act_glu(ACT)) {
         C[(size_t)row * ldc + ncol] = (f16)swiglu(acc[rb][0][v], acc[rb][1][v]);
+        if constexpr (ACT == SK_KEEP) {
+          keep[(size_t)row * (2 * N) + ncol] = (f16)acc[rb][0][v];
+          keep[(size_t)row * (2 * N) + N + ncol] = (f16)acc[rb][1][v];
+        }
       } else {
         C[(size_t)row * ldc + ncol] = (f16)acc[rb][0][v];
         C[(size_t)row * ldc + N + ncol] = (f16)acc[rb][1][v];
@@ -690,7 +711,7 @@ k_mid(const f16* __restrict__ A, int lda, const uint32_t* __restrict__ B,
       int N, int K, int g, int cps, float* __restrict__ part, uint32_t* __restrict__ counters,
       SkMulti mp) {
   using Sh = mmmid::MidShape<INT4, RB, WN>;
-  constexpr bool PAIR = ACT == SK_SWIGLU || ACT == SK_PAIR;
+  constexpr bool PAIR = act_pair(ACT);
   __shared__ __attribute__((aligned(16))) char smem[Sh::LDS_BYTES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wn = wave % WN, wk = wave / WN;
@@ -780,8 +801,12 @@ k_mid(const f16* __restrict__ A, int lda, const uint32_t* __restrict__ B,
       const float x = own[rb][0][i], y = own[rb][1][i];
       if constexpr (!PAIR) {
         *(f16x2*)(C + (size_t)row * ldc + ncol) = f16x2{(f16)x, (f16)y};
-      } else if constexpr (ACT == SK_SWIGLU) {
+      } else if constexpr (act_glu(ACT)) {
         C[(size_t)row * ldc + ncol] = (f16)swiglu(x, y);
+        if constexpr (ACT == SK_KEEP) {
+          mp.C[0][(size_t)row * (2 * N) + ncol] = (f16)x;
+          mp.C[0][(size_t)row * (2 * N) + N + ncol] = (f16)y;
+        }
       } else {
         C[(size_t)row * ldc + ncol] = (f16)x;
         C[(size_t)row * ldc + N + ncol] = (f16)y;
@@ -791,14 +816,14 @@ k_mid(const f16* __restrict__ A, int lda, const uint32_t* __restrict__ B,
 
 // Sum the K-split partials of the prefill kernel in split order -> fp16 C.
 // Partials are [ks][M][PW]; PW = N, or 2N for the pair modes (gate at n, up
-// at N + n).  SK_SWIGLU writes silu(gate) * up to C [M, N]; the others copy
-// the PW sums to C.
+// at N + n).  SK_SWIGLU writes silu(gate) * up to C [M, N], SK_KEEP that and the
+// sums to keep [M, 2N]; the others copy the PW sums to C.
 template <int ACT>
 __global__ void __launch_bounds__(256)
 k_splitk_reduce(const float* __restrict__ part, int ks, int M, int N, f16* __restrict__ C,
-                int ldc) {
+                int ldc, f16* __restrict__ keep) {
   const int PW = ACT == SK_PLAIN ? N : 2 * N;
-  const int OW = ACT == SK_SWIGLU ? N : PW;                       // output columns
+  const int OW = act_glu(ACT) ? N : PW;                       // output columns
   const size_t i4 = (size_t)blockIdx.x * 256 + threadIdx.x;     // 4-column item
   const size_t items = (size_t)M * (OW / 4);
   if (i4 >= items) return;
@@ -807,9 +832,13 @@ k_splitk_reduce(const float* __restrict__ part, int ks, int M, int N, f16* __res
   for (int z = 0; z < ks; ++z) {
     const float* prow = part + ((size_t)z * M + row) * PW;
     v += *(const f32x4*)(prow + col);
-    if constexpr (ACT == SK_SWIGLU) u += *(const f32x4*)(prow + N + col);
+    if constexpr (act_glu(ACT)) u += *(const f32x4*)(prow + N + col);
   }
-  if constexpr (ACT == SK_SWIGLU)
+  if constexpr (ACT == SK_KEEP) {
+    *(f16x4*)(keep + (size_t)row * PW + col) = to_f16x4(v);
+    *(f16x4*)(keep + (size_t)row * PW + N + col) = to_f16x4(u);
+  }
+  if constexpr (act_glu(ACT))
     v = f32x4{swiglu(v[0], u[0]), swiglu(v[1], u[1]), swiglu(v[2], u[2]), swiglu(v[3], u[3])};
   *(f16x4*)(C + (size_t)row * ldc + col) = f16x4{(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
 }
@@ -855,7 +884,7 @@ template <int MT> constexpr int sk_spw() { return MT == 1 ? MM_SK_SPW1 : MM_SK_S
 #define MM_SK_PAIR_SPW1 4
 #endif
 template <int MT, int ACT, int ROWP> constexpr int sk_spw_act() {
-  return (ACT == SK_SWIGLU || ACT == SK_PAIR) && MT == 1 && ROWP == 0 ? MM_SK_PAIR_SPW1
+  return act_pair(ACT) && MT == 1 && ROWP == 0 ? MM_SK_PAIR_SPW1
                                                                       : sk_spw<MT>();
 }
 // One 64-column virtual-tile quad per block: more column tiles means fewer
@@ -970,7 +999,7 @@ int launch_skinny(const f16* A, int lda, const uint32_t* B, const f16* S, const 
     case 8: MM_LAUNCH_SK(8 <= SPW ? 8 : 0, RP); break;                                      \
     default: MM_LAUNCH_SK(0, RP); break;                                                    \
   }
-  if constexpr ((ACT == SK_SWIGLU || ACT == SK_PAIR) && MT == 1 && ROWP == 2) {
+  if constexpr (act_pair(ACT) && MT == 1 && ROWP == 2) {
     static_assert(SPW == 8, "a round is 8 pieces of a column");
     if ((fl == 4 || fl == 8) && pair_rows_form(M, K, p, sk_nw<MT>() * SPW)) {
       if (fl == 4) MM_LAUNCH_SK(4, 4);
@@ -1197,7 +1226,7 @@ template <bool INT4, int ACT, bool ROWS = false>
 int launch_mid(const MidPlan& p, const f16* A, const uint32_t* B, const f16* S, const f16* Z,
                const uint32_t* B2, const f16* S2, const f16* Z2, f16* C, int ldc, int M, int N,
                int K, int g, void* ws, size_t ws_bytes, hipStream_t st, SkMulti* mp = nullptr) {
-  const int bn = 64 * p.wn / (ACT == SK_SWIGLU || ACT == SK_PAIR ? 2 : 1);
+  const int bn = 64 * p.wn / (act_pair(ACT) ? 2 : 1);
   int gx = mm_cdiv(N, bn);
   if (ACT == SK_MULTI) {
     gx = 0;
@@ -1238,23 +1267,24 @@ int prefill_row_group(int nx, int ny, int nz, int BM, int BN, bool int4) {
 template <bool INT4, int ACT, int WM, int WN, int RB, int CW, bool ROWS = false>
 int launch_prefill2(const f16* A, int lda, const uint32_t* B, const f16* S, const f16* Z,
                     const uint32_t* B2, const f16* S2, const f16* Z2, f16* C, int ldc, int M,
-                    int N, int K, int g, int ks, float* part, hipStream_t st) {
+                    int N, int K, int g, int ks, float* part, hipStream_t st,
+                    f16* keep = nullptr) {
   constexpr int BM = WM * 32 * RB, BN = WN * 32 * CW;
   dim3 grid(mm_cdiv(N, ACT == SK_PLAIN ? BN : BN / 2), mm_cdiv(M, BM), ks);
   const int grp = prefill_row_group((int)grid.x, (int)grid.y, (int)grid.z, BM, BN, INT4);
   if (g % PF2_BK == 0)
     hipLaunchKernelGGL((k_prefill2<INT4, WM, WN, RB, CW, true, ACT, ROWS>), grid,
                        dim3(WM * WN * 64), 0, st, A, lda, B, S, Z, B2, S2, Z2, C, ldc, M, N, K, g,
-                       part, grp);
+                       part, grp, keep);
   else if constexpr (!ROWS)
     hipLaunchKernelGGL((k_prefill2<INT4, WM, WN, RB, CW, false, ACT>), grid, dim3(WM * WN * 64),
-                       0, st, A, lda, B, S, Z, B2, S2, Z2, C, ldc, M, N, K, g, part, grp);
+                       0, st, A, lda, B, S, Z, B2, S2, Z2, C, ldc, M, N, K, g, part, grp, keep);
   MM_CHECK_LAUNCH("gemm(prefill2)");
   if (ks > 1) {
-    const int OW = ACT == SK_PLAIN ? N : (ACT == SK_SWIGLU ? N : 2 * N);
+    const int OW = ACT == SK_PAIR ? 2 * N : N;
     const size_t items = (size_t)M * (OW / 4);
     hipLaunchKernelGGL(k_splitk_reduce<ACT>, dim3((unsigned)((items + 255) / 256)), dim3(256), 0,
-                       st, part, ks, M, N, C, ldc);
+                       st, part, ks, M, N, C, ldc, keep);
     MM_CHECK_LAUNCH("gemm(prefill split-K reduce)");
   }
   return 0;
@@ -1350,7 +1380,8 @@ int gemm_dispatch(const char* who, const f16* A, const uint32_t* B, const f16* S
 template <bool INT4, int ACT>
 int pair_dispatch(const char* who, const f16* A, const uint32_t* Bg, const f16* Sg,
                   const f16* Zg, const uint32_t* Bu, const f16* Su, const f16* Zu, f16* C, int M,
-                  int N, int K, int g, void* ws, size_t ws_bytes, hipStream_t st) {
+                  int N, int K, int g, void* ws, size_t ws_bytes, hipStream_t st,
+                  f16* keep = nullptr) {
   MM_CHECK_ARG(M >= 0 && N > 0 && K > 0, "%s: bad shape M=%d N=%d K=%d", who, M, N, K);
   MM_CHECK_ARG(K % 8 == 0, "%s: K=%d must be divisible by 8", who, K);
   MM_CHECK_ARG(N % 8 == 0, "%s: N=%d must be divisible by 8", who, N);
@@ -1360,23 +1391,25 @@ int pair_dispatch(const char* who, const f16* A, const uint32_t* Bg, const f16* 
                PF2_BK);
   const uintptr_t a16 = (uintptr_t)A | (uintptr_t)Bg | (uintptr_t)Bu | (uintptr_t)Sg |
                         (uintptr_t)Su | (INT4 ? ((uintptr_t)Zg | (uintptr_t)Zu) : 0);
-  MM_CHECK_ARG((a16 & 15) == 0 && ((uintptr_t)C & 7) == 0,
+  MM_CHECK_ARG((a16 & 15) == 0 && (((uintptr_t)C | (uintptr_t)keep) & 7) == 0,
                "%s: A, packed weights, scales and zeros must be 16-byte aligned, C 8-byte", who);
   if (M == 0) return 0;
-  const int ldc = ACT == SK_SWIGLU ? N : 2 * N;
+  const int ldc = act_glu(ACT) ? N : 2 * N;
+  SkMulti mp{};
+  mp.C[0] = keep;
   const bool off32 = (size_t)(K / 8) * (size_t)N * 4 < ((size_t)1 << 32);
   MM_CHECK_ARG(off32 || K % PF2_BK == 0, "%s: weights over 4 GiB need K %% %d == 0", who,
                PF2_BK);
   if (off32 && M <= 16)
     return launch_skinny<INT4, 1, ACT>(A, K, Bg, Sg, Zg, Bu, Su, Zu, C, ldc, M, N, K, g, ws,
-                                       ws_bytes, st);
+                                       ws_bytes, st, &mp);
   if (off32 && M <= 32)
     return launch_skinny<INT4, 2, ACT>(A, K, Bg, Sg, Zg, Bu, Su, Zu, C, ldc, M, N, K, g, ws,
-                                       ws_bytes, st);
+                                       ws_bytes, st, &mp);
   if (const MidPlan mid = plan_mid(M, 2 * N, K, g, INT4);
       mid.wn != 0 && mid_ok<INT4>(Sg, Zg, N, g) && mid_ok<INT4>(Su, Zu, N, g))
     return launch_mid<INT4, ACT>(mid, A, Bg, Sg, Zg, Bu, Su, Zu, C, ldc, M, N, K, g, ws, ws_bytes,
-                                 st);
+                                 st, &mp);
   const PrefillPlan p = plan_prefill(M, 2 * N, K, g, INT4);
   float* part = nullptr;
   if (p.ksplit > 1) {
@@ -1389,13 +1422,13 @@ int pair_dispatch(const char* who, const f16* A, const uint32_t* Bg, const f16* 
   switch (p.cfg) {
     case 0:
       return launch_prefill2<INT4, ACT, PF2_BIG>(A, K, Bg, Sg, Zg, Bu, Su, Zu, C, ldc, M, N, K, g,
-                                                 p.ksplit, part, st);
+                                                 p.ksplit, part, st, keep);
     case 1:
       return launch_prefill2<INT4, ACT, PF2_MID>(A, K, Bg, Sg, Zg, Bu, Su, Zu, C, ldc, M, N, K, g,
-                                                 p.ksplit, part, st);
+                                                 p.ksplit, part, st, keep);
     default:
       return launch_prefill2<INT4, ACT, PF2_SMALL>(A, K, Bg, Sg, Zg, Bu, Su, Zu, C, ldc, M, N, K,
-                                                   g, p.ksplit, part, st);
+                                                   g, p.ksplit, part, st, keep);
   }
 }
 
@@ -1637,12 +1670,12 @@ extern "C" int mm_fp4_gemm_mmfp4(const uint16_t* A, const uint32_t* B, const uin
                                               ws, ws_bytes, (hipStream_t)stream);
 }
 
-extern "C" int mm_fp4_gate_up_rowpacked(const uint16_t* A, const uint32_t* Bg, const uint16_t* Sg,
-                                        const uint32_t* Bu, const uint16_t* Su, uint16_t* C,
-                                        int M, int N, int K, int g, int act, void* ws,
-                                        size_t ws_bytes, void* stream) {
-  const char* who = "mm_fp4_gate_up_rowpacked";
-  MM_CHECK_ARG(act == 0 || act == 1, "%s: act=%d must be 0 or 1", who, act);
+// The gate/up pair over row-packed words: act 0 both products, 1 SiLU and product, 2 (SK_KEEP)
+// all of them.
+static int pair_rows_dispatch(const char* who, const uint16_t* A, const uint32_t* Bg,
+                              const uint16_t* Sg, const uint32_t* Bu, const uint16_t* Su,
+                              uint16_t* C, int M, int N, int K, int g, int act, void* ws,
+                              size_t ws_bytes, void* stream, f16* keep) {
   MM_CHECK_ARG(M >= 0 && N > 0 && K > 0, "%s: bad shape M=%d N=%d K=%d", who, M, N, K);
   // The decode kernels take any multiple of 32 (one scale group per 32-k step
   // or more); the pipelined prefill kernel stages 64-k chunks of one group.
@@ -1654,13 +1687,19 @@ extern "C" int mm_fp4_gate_up_rowpacked(const uint16_t* A, const uint32_t* Bg, c
                "%s: each packed matrix must be under 4 GiB at M <= 32", who);
   const uintptr_t a16 = (uintptr_t)A | (uintptr_t)Bg | (uintptr_t)Bu;
   MM_CHECK_ARG((a16 & 15) == 0 && (((uintptr_t)Sg | (uintptr_t)Su) & 7) == 0 &&
-                   ((uintptr_t)C & 7) == 0,
+                   (((uintptr_t)C | (uintptr_t)keep) & 7) == 0,
                "%s: A and the packed weights must be 16-byte aligned, scales and C 8-byte", who);
   if (M == 0) return 0;
   const int ldc = act ? N : 2 * N;
+  SkMulti mp{};
+  mp.C[0] = keep;
   if (M > 16 && M <= 32) {
     // Two-row-block decode kernel over both matrices, as the Marlin-layout
     // pair at these sizes.
+    if (act == 2)
+      return launch_skinny<false, 2, SK_KEEP, 2>((const f16*)A, K, Bg, (const f16*)Sg, nullptr,
+                                                 Bu, (const f16*)Su, nullptr, (f16*)C, ldc, M, N,
+                                                 K, g, ws, ws_bytes, (hipStream_t)stream, &mp);
     if (act)
       return launch_skinny<false, 2, SK_SWIGLU, 2>((const f16*)A, K, Bg, (const f16*)Sg, nullptr,
                                                    Bu, (const f16*)Su, nullptr, (f16*)C, ldc, M,
@@ -1676,6 +1715,9 @@ extern "C" int mm_fp4_gate_up_rowpacked(const uint16_t* A, const uint32_t* Bg, c
     hipStream_t st = (hipStream_t)stream;
     if (const MidPlan mid = plan_mid(M, 2 * N, K, g, false);
         mid.wn != 0 && mid_ok<false>(sg, nullptr, N, g) && mid_ok<false>(su, nullptr, N, g)) {
+      if (act == 2)
+        return launch_mid<false, SK_KEEP, true>(mid, a, Bg, sg, nullptr, Bu, su, nullptr, (f16*)C,
+                                                ldc, M, N, K, g, ws, ws_bytes, st, &mp);
       if (act)
         return launch_mid<false, SK_SWIGLU, true>(mid, a, Bg, sg, nullptr, Bu, su, nullptr,
                                                   (f16*)C, ldc, M, N, K, g, ws, ws_bytes, st);
@@ -1693,18 +1735,24 @@ extern "C" int mm_fp4_gate_up_rowpacked(const uint16_t* A, const uint32_t* Bg, c
     }
 #define MM_LAUNCH_ROWS_PAIR(ACTV, CFG)                                                       \
   return launch_prefill2<false, ACTV, CFG, true>(a, K, Bg, sg, nullptr, Bu, su, nullptr,       \
-                                                 (f16*)C, ldc, M, N, K, g, p.ksplit, part, st)
+                                                 (f16*)C, ldc, M, N, K, g, p.ksplit, part, st, \
+                                                 keep)
 #define MM_LAUNCH_ROWS_PAIR_CFG(ACTV)                                                        \
   switch (p.cfg) {                                                                           \
     case 0: MM_LAUNCH_ROWS_PAIR(ACTV, PF2_BIG);                                              \
     case 1: MM_LAUNCH_ROWS_PAIR(ACTV, PF2_MID);                                              \
     default: MM_LAUNCH_ROWS_PAIR(ACTV, PF2_SMALL);                                           \
   }
+    if (act == 2) MM_LAUNCH_ROWS_PAIR_CFG(SK_KEEP)
     if (act) MM_LAUNCH_ROWS_PAIR_CFG(SK_SWIGLU)
     MM_LAUNCH_ROWS_PAIR_CFG(SK_PAIR)
 #undef MM_LAUNCH_ROWS_PAIR_CFG
 #undef MM_LAUNCH_ROWS_PAIR
   }
+  if (act == 2)
+    return launch_skinny<false, 1, SK_KEEP, 2>((const f16*)A, K, Bg, (const f16*)Sg, nullptr, Bu,
+                                               (const f16*)Su, nullptr, (f16*)C, ldc, M, N, K, g,
+                                               ws, ws_bytes, (hipStream_t)stream, &mp);
   if (act)
     return launch_skinny<false, 1, SK_SWIGLU, 2>((const f16*)A, K, Bg, (const f16*)Sg, nullptr,
                                                  Bu, (const f16*)Su, nullptr, (f16*)C, ldc, M,
@@ -1712,6 +1760,31 @@ extern "C" int mm_fp4_gate_up_rowpacked(const uint16_t* A, const uint32_t* Bg, c
   return launch_skinny<false, 1, SK_PAIR, 2>((const f16*)A, K, Bg, (const f16*)Sg, nullptr, Bu,
                                              (const f16*)Su, nullptr, (f16*)C, ldc, M, N, K, g, ws,
                                              ws_bytes, (hipStream_t)stream);
+}
+
+extern "C" int mm_fp4_gate_up_rowpacked(const uint16_t* A, const uint32_t* Bg, const uint16_t* Sg,
+                                        const uint32_t* Bu, const uint16_t* Su, uint16_t* C,
+                                        int M, int N, int K, int g, int act, void* ws,
+                                        size_t ws_bytes, void* stream) {
+  const char* who = "mm_fp4_gate_up_rowpacked";
+  MM_CHECK_ARG(act == 0 || act == 1, "%s: act=%d must be 0 or 1", who, act);
+  return pair_rows_dispatch(who, A, Bg, Sg, Bu, Su, C, M, N, K, g, act, ws, ws_bytes, stream,
+                            nullptr);
+}
+
+extern "C" int mm_fp4_gate_up_keep(const uint16_t* A, const uint32_t* Bg, const uint16_t* Sg,
+                                   const uint32_t* Bu, const uint16_t* Su, uint16_t* C,
+                                   uint16_t* gate_up, int layout, int M, int N, int K, int g,
+                                   void* ws, size_t ws_bytes, void* stream) {
+  const char* who = "mm_fp4_gate_up_keep";
+  MM_CHECK_ARG(layout == 0 || layout == 1, "%s: layout=%d must be 0 ([K/8, N] words) or 1 "
+               "([N, K/8])", who, layout);
+  if (layout == 1)
+    return pair_rows_dispatch(who, A, Bg, Sg, Bu, Su, C, M, N, K, g, 2, ws, ws_bytes, stream,
+                              (f16*)gate_up);
+  return pair_dispatch<false, SK_KEEP>(who, (const f16*)A, Bg, (const f16*)Sg, nullptr, Bu,
+                                       (const f16*)Su, nullptr, (f16*)C, M, N, K, g, ws, ws_bytes,
+                                       (hipStream_t)stream, (f16*)gate_up);
 }
 
 extern "C" int mm_u4_gemm(const uint16_t* A, const uint32_t* B, const uint16_t* S,

@@ -12,6 +12,10 @@ from .kernels import (FP4_PER_UINT, decode_gemv_fp4, dequant_fp4, dequant_fp4_de
 from .gpu_grouping import (GPUExpertGrouping, GPUGroupingResult, group_tokens_by_expert_auto,
                            group_tokens_by_expert_fast, group_tokens_by_expert_gpu_optimized)
 from .fp4_metal import FP4Metal, dequantize_fp4_metal, quantize_fp4_metal
+from .backward import (fused_gate_up_swiglu, fused_gate_up_swiglu_backward,
+                       marlin_gemm_fp4_backward, marlin_gemm_int4_backward,
+                       mmfp4_fused_qkv_backward, mmfp4_gemm_rowpacked_backward)
+from .adapters import lora_add, lora_backward
 from .layers import MMFP4Linear
 from .ops import GemmFp4, dispatch_gemm_fp4
 from .loader import QuantizedModel, convert_safetensors_to_fp4, load_and_quantize_safetensors

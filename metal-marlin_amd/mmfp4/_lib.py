@@ -46,6 +46,17 @@ SIGNATURES: dict[str, tuple] = {
                                 _c_int, _vp, _c_size, _vp]),
     "mm_fp4_gemm_multi": (_c_int, [_vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp,
                                    _c_size, _vp]),
+    "mm_fp4_gate_up_keep": (_c_int, [_vp] * 7 + [_c_int] * 5 + [_vp, _c_size, _vp]),
+    "mm_gemm_backward_workspace_bytes": (_c_size, [_c_int, _vp, _c_int, _c_int]),
+    "mm_gemm_backward": (_c_int, [_vp, _vp, _vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _vp, _c_int,
+                                  _c_int, _c_int, _c_int, _vp, _c_size, _vp]),
+    "mm_grad_rows": (_c_int, [_vp, _c_int, _vp, _vp, _c_int, _c_int, _vp]),
+    "mm_swiglu_grad": (_c_int, [_vp, _c_int, _vp, _vp, _vp, _c_int, _c_int, _vp]),
+    "mm_lora_workspace_bytes": (_c_size, [_c_int] * 6),
+    "mm_lora_add": (_c_int, [_vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _vp,
+                             ctypes.c_float] + [_c_int] * 5 + [_vp, _c_size, _vp]),
+    "mm_lora_backward": (_c_int, [_vp, _vp, _c_int, _vp, _vp, _vp, _c_int, _vp,
+                                  ctypes.c_float, _vp, _vp, _vp, _vp] + [_c_int] * 5 + [_vp, _c_size, _vp]),
     "mm_moe_sort": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp]),
     "mm_moe_sort_i64": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp]),
     "mm_moe_router_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
@@ -260,6 +271,14 @@ def release_workspaces() -> None:
     if b:
         b.release_workspaces()
     _ws.clear()
+
+
+def call_workspace(index: int, stream: int, nbytes: int) -> torch.Tensor:
+    """workspace_on, or under graph capture a zeroed buffer of the call's own (from the
+    graph's memory pool): two captured graphs never share it, so they may replay at once."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+    return workspace_on(index, stream, nbytes)
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
