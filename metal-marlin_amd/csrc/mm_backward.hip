@@ -21,7 +21,6 @@
 namespace {
 using namespace mmpf;
 
-constexpr int GR_BN = 64;                 // n per LDS chunk
 constexpr int GR_KP = 32;                 // word rows (8 k each) per tile
 constexpr int GR_COLS = 8 * GR_KP;        // output columns (k) per tile
 constexpr int GR_MAX_TILES = 16384;       // arrival counters at the head of the workspace
@@ -52,12 +51,15 @@ MM_DEV uint32_t sgpr_const(uint32_t v) {
 }
 
 // Non-finite scales count as zero (sanitize_scale), two at a time: x + 0x0400 carries the
-// all-ones exponent into the sign bit.
+// all-ones exponent into the sign bit, which the shift spreads.  (Written in C, the shift
+// becomes compares and selects, three times the instructions.)
 MM_DEV f16x2 sanitize2(f16x2 s) {
   typedef short s16x2 __attribute__((ext_vector_type(2)));
-  const s16x2 u = __builtin_bit_cast(s16x2, s);
-  const s16x2 e = (u & (short)0x7c00) + (short)0x0400;
-  return __builtin_bit_cast(f16x2, (s16x2)(u & ~(e >> 15)));
+  const uint32_t u = __builtin_bit_cast(uint32_t, s);
+  const s16x2 e = __builtin_bit_cast(s16x2, u & 0x7c007c00u) + s16x2{0x0400, 0x0400};
+  uint32_t m;
+  asm("v_pk_ashrrev_i16 %0, 15, %1 op_sel_hi:[0,1]" : "=v"(m) : "v"(__builtin_bit_cast(uint32_t, e)));
+  return __builtin_bit_cast(f16x2, u & ~m);
 }
 
 template <bool INT4>
@@ -123,23 +125,26 @@ struct PairWords<true> {
 };
 
 // ---------------------------------------------------------------------------
-// The product.  Tiles of BM = 32 * RB * WM rows x 256 columns (k); waves (wm, wn): rows of
-// wm, and of every word row's 8 columns the four 4 wn + j, so a wave's tile is 32 * RB rows
-// x 128 columns: lane l32 holds columns 8 (kp0 + l32) + 4 wn + j.  Operands go
-// global -> LDS directly, STAGES - 1 chunks of 64 n ahead:
-//   A  piece (r, c8), 8 halves, at r*8 + (c8 ^ ((r >> 1) & 7))   (as mm_prefill.h)
-//   B  Marlin: 32 word rows x 64 words, piece (row, p), 4 words, at row*16 + (p ^ (row & 15)):
-//      the 16 lanes of a read pass hit all banks; ROWS: 64 n x 32 words as they lie
-//   S, Z  SR group rows x 64 halves: the groups that the tile's 256 k touch
+// The product, more than 32 rows.  Tiles of BM = 32 * RB * WM rows x 256 columns (k); waves
+// (wk, wm, wn): wn takes of every word row's 8 columns the four 4 wn + j, so a wave's tile is
+// 32 * RB rows x 128 columns: lane l32 holds columns 8 (kp0 + l32) + 4 wn + j.  WK = 4 waves
+// share out the 16-n steps of every chunk and add up in LDS at the end: four times the waves
+// for a tile of 64 rows, with no weight converted more often.  Operands go global -> LDS
+// directly, STAGES - 1 chunks of BN n ahead:
+//   A  piece (r, c), 8 halves, at r * BN/8 + (c ^ sw(r)), sw = (r >> 1) & 7 (BN = 64) or
+//      r & 15: the 16 lanes of a read pass hit all banks
+//   B  Marlin: 32 word rows x BN words, piece (row, p), 4 words, at row * BN/4 +
+//      (p ^ (row & 15)); ROWS: BN n x 32 words as they lie
+//   S, Z  SR group rows x BN halves: the groups that the tile's 256 k touch
 // ks > 1: the chunks are split over gridDim.z and the last block of a tile adds the splits
 // in order (k_mid's hand-off: sc1 partials, an arrival counter per tile left at zero).
 // ot: the output's type, 0 fp32, 1 fp16, 2 bf16.
 // ---------------------------------------------------------------------------
-template <bool INT4, int WM, int RB, int SR>
+template <bool INT4, int WM, int WK, int RB, int SR, int BN, int STG>
 struct GradShape {
-  static constexpr int STAGES = 3;
-  static constexpr int NWAVE = 2 * WM, NTHR = 64 * NWAVE, BM = 32 * RB * WM;
-  static constexpr int A_PIECES = BM * 8, B_PIECES = GR_KP * GR_BN / 4, S_PIECES = SR * 8;
+  static constexpr int STAGES = STG;
+  static constexpr int NWAVE = 2 * WM * WK, NTHR = 64 * NWAVE, BM = 32 * RB * WM;
+  static constexpr int A_PIECES = BM * BN / 8, B_PIECES = GR_KP * BN / 4, S_PIECES = SR * BN / 8;
   static constexpr int A_IT = A_PIECES / NTHR, B_IT = B_PIECES / NTHR;
   static constexpr int S_IT = (S_PIECES + NTHR - 1) / NTHR;
   static_assert(A_PIECES % NTHR == 0 && B_PIECES % NTHR == 0 && S_PIECES % 64 == 0, "split");
@@ -148,25 +153,67 @@ struct GradShape {
   static constexpr int B_OFF = STAGES * A_BYTES, S_OFF = B_OFF + STAGES * B_BYTES;
   static constexpr int Z_OFF = S_OFF + STAGES * S_BYTES;
   static constexpr int D_OFF = Z_OFF + (INT4 ? STAGES * S_BYTES : 0);   // dump of idle waves
-  static constexpr int LDS_BYTES = D_OFF + 1024;
+  static constexpr int RED_BYTES = WK > 1 ? NWAVE * 4096 : 0;           // one (rb, j) of the sum
+  static constexpr int LDS_BYTES = D_OFF + 1024 > RED_BYTES ? D_OFF + 1024 : RED_BYTES;
 };
 
-MM_DEV uint16_t bf16_bits(float v) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, v);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40);   // NaN
-  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1)) >> 16);
+MM_DEV uint32_t bf16_bits(float v) {
+  return __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+// Four adjacent columns of a row.
+MM_DEV void store_grad4(void* out, int ot, size_t at, f32x4 v) {
+  if (ot == 1) {
+    *(f16x4*)((f16*)out + at) = f16x4{(f16)v[0], (f16)v[1], (f16)v[2], (f16)v[3]};
+  } else if (ot == 2) {
+    *(u32x2*)((uint16_t*)out + at) =
+        u32x2{bf16_bits(v[0]) | bf16_bits(v[1]) << 16, bf16_bits(v[2]) | bf16_bits(v[3]) << 16};
+  } else {
+    *(f32x4*)((float*)out + at) = v;
+  }
 }
 
-template <bool INT4, bool ROWS, int WM, int RB, int SR>
-__global__ void __launch_bounds__(WM * 128)
+// The hand-off's second half: true in the block that arrives last at the tile's counter.
+MM_DEV bool grad_last(uint32_t* counter, int ks, uint32_t* s_last) {
+  __builtin_amdgcn_s_waitcnt(0);   // this wave's partials have reached the coherence point
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t prev =
+        __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *s_last = prev == (uint32_t)ks - 1u;
+    if (*s_last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return *s_last != 0;
+}
+
+// Gradient values as the operands hold them: sanitised scales, negated clamped zero points.
+template <bool INT4>
+MM_DEV void grad_scales(f16x8 s, f16x8 z, f16x2 (&s2)[4], f16x2 (&nz2)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s2[i] = sanitize2(f16x2{s[2 * i], s[2 * i + 1]});
+    nz2[i] = f16x2{0, 0};
+    if constexpr (INT4) {
+      const f16x2 lim = {(f16)127.0f, (f16)127.0f};
+      nz2[i] = -__builtin_elementwise_min(
+          __builtin_elementwise_max(f16x2{z[2 * i], z[2 * i + 1]}, -lim), lim);
+    }
+  }
+}
+
+template <bool INT4, bool ROWS, int WM, int WK, int RB, int SR, int BN, int STG>
+__global__ void __launch_bounds__(WM * WK * 128)
 k_grad(GradSegs segs, void* __restrict__ out, int ot, const float* __restrict__ rowmul, int M,
        int K, int g, int cps, int grp, float* __restrict__ part, uint32_t* __restrict__ counters) {
-  using Sh = GradShape<INT4, WM, RB, SR>;
+  using Sh = GradShape<INT4, WM, WK, RB, SR, BN, STG>;
+  static_assert(WK == 1 || WK == 4, "a wave owns all or one of the four row quads");
   constexpr int NWAVE = Sh::NWAVE, STAGES = Sh::STAGES;
+  constexpr int PA = BN / 8, PB = BN / 4;      // pieces per row of A, of B
+  constexpr int STEPS = BN / 16 / WK;          // steps per wave and chunk
   __shared__ __attribute__((aligned(16))) char smem[Sh::LDS_BYTES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wn = wave & 1, wm = (wave >> 1) % WM, wk = (wave >> 1) / WM;
   const int l32 = lane & 31, h = lane >> 5;
   const int KP = K >> 3, ngroups = K / g;
   // Tile walk of k_prefill2: an XCD takes a run of tiles, groups of grp row tiles
@@ -183,48 +230,95 @@ k_grad(GradSegs segs, void* __restrict__ out, int ot, const float* __restrict__ 
   const int c_beg = bz * cps, c_end = min(segs.nch, c_beg + cps);
   const int g0 = 8 * kp0 / g;              // first group of the tile
 
-  // Source offsets within a segment that do not change from chunk to chunk.
-  int a_row[Sh::A_IT], a_c8[Sh::A_IT];
-#pragma unroll
-  for (int i = 0; i < Sh::A_IT; ++i) {
-    const int p = (i * NWAVE + wave) * 64 + lane, r = p >> 3;
-    a_row[i] = min(m0 + r, M - 1);
-    a_c8[i] = 8 * ((p & 7) ^ ((r >> 1) & 7));
-  }
-  auto issue = [&](int ch, int st) {
+  auto aswz = [](int r) { return BN == 64 ? (r >> 1) & 7 : r & 15; };
+  // Byte offsets of a lane's pieces from bases that are uniform: within a segment only the
+  // bases move from chunk to chunk, in scalar registers.
+  uint32_t a_off[Sh::A_IT], b_off[Sh::B_IT], s_src[Sh::S_IT];
+  const f16* a_base;
+  const uint32_t* b_base;
+  const f16 *s_base, *z_base;
+  int seg_n = 0, seg_n0 = 0, seg_next = 0;   // columns of the segment, the chunk's first, its last chunk
+  auto enter = [&](int ch) {                 // chunk ch opens a segment, or the block's range
     const int sg = ch >= segs.s[2].ch0 ? 2 : (ch >= segs.s[1].ch0 ? 1 : 0);
     const GradSeg& s = segs.s[sg];
-    const int N = s.N, n0 = (ch - s.ch0) * GR_BN;
+    const int N = s.N, n0 = (ch - s.ch0) * BN;
+    seg_n = N;
+    seg_n0 = n0;
+    seg_next = sg < 2 ? segs.s[sg + 1].ch0 : 0x7fffffff;
+    a_base = s.A + (size_t)m0 * s.lda + n0;
+    b_base = ROWS ? s.B + (size_t)n0 * KP + kp0 : s.B + (size_t)kp0 * N + n0;
+    s_base = s.S + (size_t)g0 * N + n0;
+    if constexpr (INT4) z_base = s.Z + (size_t)g0 * N + n0;
 #pragma unroll
     for (int i = 0; i < Sh::A_IT; ++i) {
-      const f16* src = s.A + (size_t)a_row[i] * s.lda + n0 + a_c8[i];
-      if (n0 + GR_BN > N) src = n0 + a_c8[i] < N ? src : (const f16*)gr_zeros;
-      gl2lds16(src, smem + st * Sh::A_BYTES + (i * NWAVE + wave) * 1024);
+      const int p = (i * NWAVE + wave) * 64 + lane, r = p / PA;
+      a_off[i] = (uint32_t)(min(r, M - 1 - m0) * s.lda + 8 * ((p % PA) ^ aswz(r))) * 2u;
     }
 #pragma unroll
     for (int i = 0; i < Sh::B_IT; ++i) {
       const int p = (i * NWAVE + wave) * 64 + lane;
-      const uint32_t* src;
-      if constexpr (ROWS) {
-        const int n = min(n0 + (p >> 3), N - 1), kp = min(kp0 + 4 * (p & 7), KP - 4);
-        src = s.B + (size_t)n * KP + kp;
-      } else {
-        const int row = p >> 4;
-        const int n = min(n0 + 4 * ((p & 15) ^ (row & 15)), N - 4);
-        src = s.B + (size_t)min(kp0 + row, KP - 1) * N + n;
+      if constexpr (ROWS)
+        b_off[i] = ((uint32_t)(p >> 3) * KP + min(4 * (p & 7), KP - 4 - kp0)) * 4u;
+      else
+        b_off[i] = ((uint32_t)min(p / PB, KP - 1 - kp0) * N + 4 * ((p % PB) ^ (p / PB & 15))) * 4u;
+    }
+#pragma unroll
+    for (int i = 0; i < Sh::S_IT; ++i) {
+      const int p = min((i * NWAVE + wave) * 64 + lane, Sh::S_PIECES - 1);
+      s_src[i] = ((uint32_t)min(p / PA, ngroups - 1 - g0) * N + 8 * (p % PA)) * 2u;
+    }
+  };
+  auto issue = [&](int st) {
+    // A segment's last chunk may reach past its columns: zeros for the gradient, any of the
+    // matrix's own words and scales.
+    const bool tail = seg_n0 + BN > seg_n;
+#pragma unroll
+    for (int i = 0; i < Sh::A_IT; ++i) {
+      const char* src = (const char*)a_base + a_off[i];
+      if (tail) {
+        const int p = (i * NWAVE + wave) * 64 + lane;
+        if (seg_n0 + 8 * ((p % PA) ^ aswz(p / PA)) >= seg_n) src = (const char*)gr_zeros;
+      }
+      gl2lds16(src, smem + st * Sh::A_BYTES + (i * NWAVE + wave) * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < Sh::B_IT; ++i) {
+      const char* src = (const char*)b_base + b_off[i];
+      if (tail) {
+        const int p = (i * NWAVE + wave) * 64 + lane;
+        const int over = ROWS ? seg_n0 + (p >> 3) - (seg_n - 1)
+                              : seg_n0 + 4 * ((p % PB) ^ (p / PB & 15)) - (seg_n - 4);
+        if (over > 0) src -= (size_t)over * (ROWS ? KP : 1) * 4;
       }
       gl2lds16(src, smem + Sh::B_OFF + st * Sh::B_BYTES + (i * NWAVE + wave) * 1024);
     }
 #pragma unroll
     for (int i = 0; i < Sh::S_IT; ++i) {
       const int wp = i * NWAVE + wave;
-      const int p = min(wp * 64 + lane, Sh::S_PIECES - 1);
-      const size_t off = (size_t)min(g0 + (p >> 3), ngroups - 1) * N + min(n0 + 8 * (p & 7), N - 8);
+      uint32_t off = s_src[i];
+      size_t back = 0;
+      if (tail) {
+        const int p = min(wp * 64 + lane, Sh::S_PIECES - 1);
+        back = (size_t)max(0, seg_n0 + 8 * (p % PA) - (seg_n - 8)) * 2;
+      }
       const bool live = wp * 64 < Sh::S_PIECES;
-      gl2lds16(s.S + off, smem + (live ? Sh::S_OFF + st * Sh::S_BYTES + wp * 1024 : Sh::D_OFF));
+      gl2lds16((const char*)s_base + off - back,
+               smem + (live ? Sh::S_OFF + st * Sh::S_BYTES + wp * 1024 : Sh::D_OFF));
       if constexpr (INT4)
-        gl2lds16(s.Z + off, smem + (live ? Sh::Z_OFF + st * Sh::S_BYTES + wp * 1024 : Sh::D_OFF));
+        gl2lds16((const char*)z_base + off - back,
+                 smem + (live ? Sh::Z_OFF + st * Sh::S_BYTES + wp * 1024 : Sh::D_OFF));
     }
+  };
+  auto advance = [&](int ch) {               // to chunk ch, the next one
+    if (ch >= seg_next) {
+      enter(ch);
+      return;
+    }
+    seg_n0 += BN;
+    a_base += BN;
+    b_base += ROWS ? (size_t)BN * KP : BN;
+    s_base += BN;
+    if constexpr (INT4) z_base += BN;
   };
 
   f32x16 acc[RB][4];
@@ -235,72 +329,76 @@ k_grad(GradSegs segs, void* __restrict__ out, int ot, const float* __restrict__ 
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[rb][j][v] = 0.0f;
 
+  enter(c_beg);
+  issue(0);
 #pragma unroll
-  for (int c = 0; c < STAGES - 1; ++c) issue(min(c_beg + c, c_end - 1), c);
+  for (int c = 1; c < STAGES; ++c) {
+    if (c_beg + c < c_end) advance(c_beg + c);
+    issue(c);
+  }
 
-  const int arow = wm * 32 * RB + l32, ax = (arow >> 1) & 7;   // rows of all row blocks share ax
+  const int arow = wm * 32 * RB + l32, ax = aswz(arow);   // rows of all row blocks share ax
   const int srow = 8 * min(kp0 + l32, KP - 1) / g - g0;
   const uint32_t half = wn ? 0x07060302u : 0x05040100u;
-  const uint32_t s_off = srow * 128 + h * 16;
-  const uint32_t b_row = ROWS ? (h * 8 * 32 + l32) * 4 : l32 * 256, bx15 = l32 & 15;
+  const uint32_t s_off = srow * (BN * 2) + h * 16;
+  const uint32_t b_row = ROWS ? (h * 8 * 32 + l32) * 4 : l32 * (BN * 4), bx15 = l32 & 15;
 
+  f16x8 af[2][RB], bq[2][4];
+  u32x4 w[2];
+  f16x8 sv, zv;
+  // Step t0 of this wave in the chunk at stage st: operands of the gradient, words and scales.
+  auto frag = [&](auto stc, int t0, int slot) {
+    constexpr int st = decltype(stc)::value;
+    const int t = wk * STEPS + t0;
+    if constexpr (ROWS) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        w[i >> 2][i & 3] = *(const uint32_t*)(smem + Sh::B_OFF + st * Sh::B_BYTES + b_row +
+                                              (16 * t + i) * 128);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        w[i] = *(const u32x4*)(smem + Sh::B_OFF + st * Sh::B_BYTES + b_row +
+                               ((4 * t + 2 * h + i) ^ bx15) * 16);
+    }
+    sv = *(const f16x8*)(smem + Sh::S_OFF + st * Sh::S_BYTES + s_off + t * 32);
+    if constexpr (INT4) zv = *(const f16x8*)(smem + Sh::Z_OFF + st * Sh::S_BYTES + s_off + t * 32);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+      af[slot][rb] = *(const f16x8*)(smem + st * Sh::A_BYTES + (arow + 32 * rb) * (BN * 2) +
+                                     ((2 * t + h) ^ ax) * 16);
+  };
+  auto decode = [&](int slot) {
+    f16x2 s2[4], nz2[4];
+    grad_scales<INT4>(sv, zv, s2, nz2);
+    PairWords<INT4>::run(w, s2, nz2, half, bq[slot]);
+  };
+  // A step is read and converted while the one before it occupies the matrix cores, across
+  // chunks too: before a chunk's last step every wave has read that chunk, so its stage is
+  // refilled there and the next one, which has landed once at most STAGES - 2 later ones are
+  // outstanding, is published by the same barrier.
   auto chunk = [&](int ch, auto stc) {
     constexpr int st = decltype(stc)::value;
-    // Chunk ch has landed once at most STAGES - 2 later chunks' loads are outstanding; the
-    // barrier publishes it and frees the stage that is refilled next.
-    wait_vmcnt<(STAGES - 2) * Sh::LOADS>();
-    __builtin_amdgcn_s_barrier();
-    issue(min(ch + STAGES - 1, c_end - 1), (st + STAGES - 1) % STAGES);
-    f16x8 af[2][RB], bq[2][4];
-    u32x4 w[2][2];
-    f16x8 sv[2], zv[2];
-    auto frag = [&](int t, int slot) {
-      if constexpr (ROWS) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          w[slot][i >> 2][i & 3] = *(const uint32_t*)(smem + Sh::B_OFF + st * Sh::B_BYTES + b_row +
-                                                      (16 * t + i) * 128);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          w[slot][i] = *(const u32x4*)(smem + Sh::B_OFF + st * Sh::B_BYTES + b_row +
-                                       ((4 * t + 2 * h + i) ^ bx15) * 16);
-      }
-      sv[slot] = *(const f16x8*)(smem + Sh::S_OFF + st * Sh::S_BYTES + s_off + t * 32);
-      if constexpr (INT4)
-        zv[slot] = *(const f16x8*)(smem + Sh::Z_OFF + st * Sh::S_BYTES + s_off + t * 32);
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-        af[slot][rb] = *(const f16x8*)(smem + st * Sh::A_BYTES + (arow + 32 * rb) * 128 +
-                                       ((2 * t + h) ^ ax) * 16);
-    };
-    auto decode = [&](int slot) {
-      f16x2 s2[4], nz2[4] = {};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s2[i] = sanitize2(f16x2{sv[slot][2 * i], sv[slot][2 * i + 1]});
-        if constexpr (INT4) {
-          const f16x2 lim = {(f16)127.0f, (f16)127.0f};
-          nz2[i] = -__builtin_elementwise_min(
-              __builtin_elementwise_max(f16x2{zv[slot][2 * i], zv[slot][2 * i + 1]}, -lim), lim);
-        }
-      }
-      PairWords<INT4>::run(w[slot], s2, nz2, half, bq[slot]);
-    };
-    // Step t + 1 is read and decoded while step t's products occupy the matrix cores.
-    frag(0, 0);
-    decode(0);
-#pragma unroll
-    for (int t = 0; t < GR_BN / 16; ++t) {
+    for (int t = 0; t < STEPS; ++t) {
       const int cur = t & 1;
-      if (t + 1 < GR_BN / 16) frag(t + 1, cur ^ 1);
+      if (t + 1 < STEPS) {
+        frag(stc, t + 1, cur ^ 1);
+      } else {
+        __builtin_amdgcn_s_waitcnt(0xc07f);            // lgkmcnt(0): this wave's reads are done
+        wait_vmcnt<(STAGES - 2) * Sh::LOADS>();
+        __builtin_amdgcn_s_barrier();
+        if (ch + STAGES < c_end) advance(ch + STAGES);
+        issue(st);                                     // behind the last chunk: again, never read
+        frag(std::integral_constant<int, (st + 1) % STAGES>{}, 0, cur ^ 1);
+      }
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           acc[rb][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[cur][rb], bq[cur][j], acc[rb][j],
                                                               0, 0, 0);
-      if (t + 1 < GR_BN / 16) decode(cur ^ 1);
+      decode(cur ^ 1);
 #pragma unroll
       for (int i = 0; i < RB * 4; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                    // MFMA
@@ -309,6 +407,11 @@ k_grad(GradSegs segs, void* __restrict__ out, int ot, const float* __restrict__ 
       }
     }
   };
+  static_assert(STEPS % 2 == 0, "the operand slots alternate within a chunk");
+  wait_vmcnt<(STAGES - 1) * Sh::LOADS>();
+  __builtin_amdgcn_s_barrier();
+  frag(std::integral_constant<int, 0>{}, 0, 0);
+  decode(0);
   for (int ch = c_beg; ch < c_end; ch += STAGES) {
     static_for(
         [&](auto stc) {
@@ -319,75 +422,212 @@ k_grad(GradSegs segs, void* __restrict__ out, int ot, const float* __restrict__ 
   }
   wait_vmcnt<0>();
 
-  const int ks = gridDim.z;
-  if (ks > 1) {
-    const int tile = by * nx + bx;
-    const __amdgpu_buffer_rsrc_t prs = mm_rsrc(part + (size_t)tile * ks * (Sh::BM * GR_COLS));
-    auto at = [&](int z, int rb, int j, int q) {
-      return 16u * (uint32_t)((((z * RB + rb) * 16 + j * 4 + q) * NWAVE + wave) * 64 + lane);
-    };
+  // own[rb][j][q]: rows 8 (q0 + q) + 4 h + i of row block rb.  WK = 4: wave wk sums quad wk
+  // of the four waves that share its tile, in their order.
+  constexpr int NQ = 4 / WK;
+  const int q0 = WK == 1 ? 0 : wk;
+  f32x4 own[RB][4][NQ];
+  if constexpr (WK == 1) {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          store_agent_x4(prs, at(bz, rb, j, q),
-                         f32x4{acc[rb][j][4 * q], acc[rb][j][4 * q + 1], acc[rb][j][4 * q + 2],
-                               acc[rb][j][4 * q + 3]});
-    __builtin_amdgcn_s_waitcnt(0);   // this wave's partials have reached the coherence point
-    __syncthreads();
-    uint32_t* const s_last = (uint32_t*)smem;
-    if (tid == 0) {
-      const uint32_t prev = __hip_atomic_fetch_add(&counters[tile], 1u, __ATOMIC_RELAXED,
-                                                   __HIP_MEMORY_SCOPE_AGENT);
-      *s_last = prev == (uint32_t)ks - 1u;
-    }
-    __syncthreads();
-    if (!*s_last) return;
+          own[rb][j][q] = f32x4{acc[rb][j][4 * q], acc[rb][j][4 * q + 1], acc[rb][j][4 * q + 2],
+                                acc[rb][j][4 * q + 3]};
+  } else {
+    f32x4* red = (f32x4*)smem;   // [wk][wm, wn][quad][lane]
+    const int wt = wave % (2 * WM);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          red[(wave * 4 + q) * 64 + lane] = f32x4{acc[rb][j][4 * q], acc[rb][j][4 * q + 1],
+                                                  acc[rb][j][4 * q + 2], acc[rb][j][4 * q + 3]};
+        __syncthreads();
+        own[rb][j][0] = red[(wt * 4 + wk) * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < WK; ++w) own[rb][j][0] += red[((w * 2 * WM + wt) * 4 + wk) * 64 + lane];
+      }
+  }
+  const int ks = gridDim.z;
+  if (ks > 1) {
+    const int tile = by * nx + bx;
+    const __amdgpu_buffer_rsrc_t prs = mm_rsrc(part + (size_t)tile * ks * (Sh::BM * GR_COLS));
+    auto at = [&](int z, int rb, int j, int q) {
+      return 16u * (uint32_t)((((z * RB + rb) * 4 + j) * NQ + q) * Sh::NTHR + tid);
+    };
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) store_agent_x4(prs, at(bz, rb, j, q), own[rb][j][q]);
+    // The flag lies in smem: a second LDS variable would have the compiler wait for every
+    // load to LDS before the reads of the main loop (M = 512, 4096 -> 4096 40 us so, 22 now).
+    if (!grad_last(counters + tile, ks, (uint32_t*)smem)) return;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
 #pragma unroll
-        for (int v = 0; v < 16; ++v) acc[rb][j][v] = 0.0f;
-        for (int z = 0; z < ks; z += 2) {
-          f32x4 ld[2][4];
+        for (int q = 0; q < NQ; ++q) own[rb][j][q] = f32x4{0, 0, 0, 0};
+        for (int z = 0; z < ks; z += 4) {
+          f32x4 ld[4][NQ];
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) ld[i][q] = load_agent_x4(prs, at(min(z + i, ks - 1), rb, j, q));
+            for (int q = 0; q < NQ; ++q) ld[i][q] = load_agent_x4(prs, at(min(z + i, ks - 1), rb, j, q));
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 4; ++i)
             if (z + i < ks)
 #pragma unroll
-              for (int v = 0; v < 16; ++v) acc[rb][j][v] += ld[i][v >> 2][v & 3];
+              for (int q = 0; q < NQ; ++q) own[rb][j][q] += ld[i][q];
         }
       }
-    if (tid == 0)
-      __hip_atomic_store(&counters[tile], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   const int kp = kp0 + l32;
   if (kp >= KP) return;
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-    for (int v = 0; v < 16; ++v) {
-      const int row = m0 + wm * 32 * RB + rb * 32 + 8 * (v >> 2) + 4 * h + (v & 3);
-      if (row >= M) continue;
-      const float f = rowmul != nullptr ? rowmul[row] : 1.0f;
-      const float x0 = acc[rb][0][v] * f, x1 = acc[rb][1][v] * f;
-      const float x2 = acc[rb][2][v] * f, x3 = acc[rb][3][v] * f;
-      const size_t at = (size_t)row * K + 8 * kp + 4 * wn;
-      if (ot == 1) {
-        *(f16x4*)((f16*)out + at) = f16x4{(f16)x0, (f16)x1, (f16)x2, (f16)x3};
-      } else if (ot == 2) {
-        *(u32x2*)((uint16_t*)out + at) = u32x2{bf16_bits(x0) | (uint32_t)bf16_bits(x1) << 16,
-                                               bf16_bits(x2) | (uint32_t)bf16_bits(x3) << 16};
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = m0 + wm * 32 * RB + rb * 32 + 8 * (q0 + q) + 4 * h + i;
+        if (row >= M) continue;
+        const float f = rowmul != nullptr ? rowmul[row] : 1.0f;
+        store_grad4(out, ot, (size_t)row * K + 8 * kp + 4 * wn,
+                    f * f32x4{own[rb][0][q][i], own[rb][1][q][i], own[rb][2][q][i],
+                              own[rb][3][q][i]});
+      }
+}
+
+// ---------------------------------------------------------------------------
+// Up to 32 rows: the weights stream HBM -> registers -> 16x16x32 MFMA, as in mm_skinny.h.
+// Tiles of 128 columns (16 word rows).  Lane (c, q) of a wave, at a step of 32 n: the words
+// of n0 + 8 q .. + 7 of word row kp0 + c (two 16-byte loads: 16 rows x 128 bytes a wave), and
+// the gradient's rows 16 mt + c at the same n; words give 8 operands, columns 8 (kp0 + c) + j.
+// Converting the words costs 96 VALU operations per 2 KiB of them, a third of what the
+// memory rate allows.  The NW waves of a block share out its steps, SPW at a time with all
+// loads in flight, and add up in LDS; blocks that split the steps hand over as in k_grad, M
+// rows each.
+// ---------------------------------------------------------------------------
+constexpr int GS_KP = 16, GS_COLS = 128, GS_NW = 8, GS_NTHR = 64 * GS_NW;
+
+template <bool INT4, bool ROWS, int MT, int SPW>
+__global__ void __launch_bounds__(GS_NTHR, MT == 1 ? 4 : 2)
+k_grad_skinny(GradSegs segs, void* __restrict__ out, int ot, const float* __restrict__ rowmul,
+              int M, int K, int g, int rounds, float* __restrict__ part,
+              uint32_t* __restrict__ counters) {
+  __shared__ __attribute__((aligned(16))) float red[GS_NW][16][GS_COLS];   // one row block
+  __shared__ uint32_t s_last;
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int KP = K >> 3, kp0 = blockIdx.x * GS_KP, kp = min(kp0 + c, KP - 1);
+  const int grow = 8 * kp / g;
+  f32x4 acc[MT][8];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[mt][j] = f32x4{0, 0, 0, 0};
+  for (int r = 0; r < rounds; ++r) {
+    const int st0 = ((blockIdx.y * rounds + r) * GS_NW + wave) * SPW;
+    if (st0 >= segs.nch) break;
+    u32x4 w[SPW][2];
+    f16x8 sv[SPW], zv[SPW], a[SPW][MT];
+#pragma unroll
+    for (int i = 0; i < SPW; ++i) {
+      const int st = min(st0 + i, segs.nch - 1);
+      const int sg = st >= segs.s[2].ch0 ? 2 : (st >= segs.s[1].ch0 ? 1 : 0);
+      const GradSeg& s = segs.s[sg];
+      const int N = s.N, n = (st - s.ch0) * 32 + 8 * q, nc = min(n, N - 8);
+      const size_t off = (size_t)grow * N + nc;
+      sv[i] = *(const f16x8*)(s.S + off);
+      if constexpr (INT4) zv[i] = *(const f16x8*)(s.Z + off);
+      if constexpr (ROWS) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          w[i][k >> 2][k & 3] = __builtin_nontemporal_load(s.B + (size_t)(nc + k) * KP + kp);
       } else {
-        *(f32x4*)((float*)out + at) = f32x4{x0, x1, x2, x3};
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          w[i][k] = __builtin_nontemporal_load((const u32x4*)(s.B + (size_t)kp * N + nc + 4 * k));
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        // rows past M, columns past N and steps past the last: zeros
+        const bool live = 16 * mt + c < M && n < N && st0 + i < segs.nch;
+        a[i][mt] = live ? *(const f16x8*)(s.A + (size_t)(16 * mt + c) * s.lda + n)
+                        : f16x8{0, 0, 0, 0, 0, 0, 0, 0};
       }
     }
+#pragma unroll
+    for (int i = 0; i < SPW; ++i) {
+      f16x2 s2[4], nz2[4];
+      grad_scales<INT4>(sv[i], zv[i], s2, nz2);
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        f16x8 b[4];
+        PairWords<INT4>::run(w[i], s2, nz2, hf ? 0x07060302u : 0x05040100u, b);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[mt][4 * hf + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                a[i][mt], b[j], acc[mt][4 * hf + j], 0, 0, 0);
+      }
+    }
+  }
+  const int ks = gridDim.y, tile = blockIdx.x;
+  const __amdgpu_buffer_rsrc_t prs = mm_rsrc(part + (size_t)tile * ks * M * GS_COLS);
+  // Item (row, 4 columns) of the tile.
+  auto finish = [&](int row, int c4, f32x4 v) {
+    if (8 * kp0 + 4 * c4 < K)
+      store_grad4(out, ot, (size_t)row * K + 8 * kp0 + 4 * c4,
+                  (rowmul != nullptr ? rowmul[row] : 1.0f) * v);
+  };
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    if (mt > 0) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (16 * mt + 4 * q + i < M)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+          *(f32x4*)&red[wave][4 * q + i][8 * c + 4 * hf] =
+              f32x4{acc[mt][4 * hf][i], acc[mt][4 * hf + 1][i], acc[mt][4 * hf + 2][i],
+                    acc[mt][4 * hf + 3][i]};
+    __syncthreads();
+    const int items = min(16, M - 16 * mt) * (GS_COLS / 4);
+    for (int e = tid; e < items; e += GS_NTHR) {
+      const int row = e / (GS_COLS / 4), c4 = e % (GS_COLS / 4);
+      f32x4 v = *(const f32x4*)&red[0][row][4 * c4];
+#pragma unroll
+      for (int k = 1; k < GS_NW; ++k) v += *(const f32x4*)&red[k][row][4 * c4];
+      if (ks == 1) finish(16 * mt + row, c4, v);
+      else store_agent_x4(prs, 4u * (uint32_t)((blockIdx.y * M + 16 * mt + row) * GS_COLS + 4 * c4), v);
+    }
+  }
+  if (ks == 1 || !grad_last(counters + tile, ks, &s_last)) return;
+  for (int e = tid; e < M * (GS_COLS / 4); e += GS_NTHR) {
+    const int row = e / (GS_COLS / 4), c4 = e % (GS_COLS / 4);
+    f32x4 v = {0, 0, 0, 0};
+    for (int z0 = 0; z0 < ks; z0 += 8) {
+      f32x4 ld[8];
+#pragma unroll
+      for (int z = 0; z < 8; ++z)
+        ld[z] = load_agent_x4(prs, 4u * (uint32_t)((min(z0 + z, ks - 1) * M + row) * GS_COLS + 4 * c4));
+#pragma unroll
+      for (int z = 0; z < 8; ++z)
+        if (z0 + z < ks) v += ld[z];
+    }
+    finish(row, c4, v);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -550,69 +790,118 @@ k_swiglu_grad(const void* __restrict__ dH, const f16* __restrict__ GU, f16* __re
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
+enum { G_SKINNY, G_64, G_256 };
 struct GradPlan {
-  int wm, rb;   // waves along the rows, 32-row blocks per wave
-  int ks, cps;
+  int kind;
+  int bn;       // n per chunk (step of the skinny kernel)
+  int bm, ks;   // rows per tile, splits
+  int per;      // chunks per split, or rounds per block
+  int spw;
+  size_t part;  // partial sums, bytes
 };
 
-GradPlan plan_grad(int M, long ntot_chunks, int K) {
-  GradPlan p{1, 1, 1, 0};
-  if (M > 128) p = {2, 4, 1, 0};
-  else if (M > 64) p = {1, 4, 1, 0};
-  else if (M > 32) p = {1, 2, 1, 0};
-  const int bm = 32 * p.rb * p.wm;
-  const long tiles = (long)mm_cdiv(K, GR_COLS) * mm_cdiv(M, bm);
-  const int want = p.rb == 4 && p.wm == 2 ? 200 : 512;
-  const int nch = (int)ntot_chunks;
-  while (tiles * p.ks < want && p.ks < 64 && nch / (p.ks + 1) >= 4) ++p.ks;
-  if (tiles > GR_MAX_TILES) p.ks = 1;
-  p.cps = mm_cdiv(nch, p.ks);
-  p.ks = mm_cdiv(nch, p.cps);
-  return p;
-}
-
-size_t grad_ws_bytes(const GradPlan& p, int M, int K) {
-  if (p.ks == 1) return GR_COUNTER_BYTES;
-  const int bm = 32 * p.rb * p.wm;
-  return GR_COUNTER_BYTES +
-         (size_t)mm_cdiv(K, GR_COLS) * mm_cdiv(M, bm) * p.ks * bm * GR_COLS * sizeof(float);
-}
-
-int grad_chunks(int nmat, const int* N) {
+int grad_chunks(int nmat, const int* N, int bn) {
   int c = 0;
-  for (int i = 0; i < nmat; ++i) c += mm_cdiv(N[i], GR_BN);
+  for (int i = 0; i < nmat; ++i) c += mm_cdiv(N[i], bn);
   return c;
 }
 
-template <bool INT4, bool ROWS, int WM, int RB, int SR>
+GradPlan plan_grad(int nmat, const int* N, int M, int K) {
+  GradPlan p{};
+  if (M <= 32) {
+    p = GradPlan{G_SKINNY, 32, M, 1, 1, 4, 0};
+    const int steps = grad_chunks(nmat, N, p.bn), tiles = mm_cdiv(K, GS_COLS);
+    if ((long)tiles * mm_cdiv(steps, GS_NW * 4) < 256) p.spw = 2;
+    const int blocks_n = mm_cdiv(steps, GS_NW * p.spw);
+    p.ks = blocks_n;
+    while (p.ks > 1 && ((long)tiles * p.ks > 1024 || p.ks > 32)) p.ks = mm_cdiv(p.ks, 2);
+    if (tiles > GR_MAX_TILES) p.ks = 1;
+    p.per = mm_cdiv(blocks_n, p.ks);
+    p.ks = mm_cdiv(blocks_n, p.per);
+    if (p.ks > 1) p.part = (size_t)tiles * p.ks * M * GS_COLS * sizeof(float);
+    return p;
+  }
+  // Tiles of 64 rows or of 256, and the split, by a time model (us; MI355X, FP4, K = 4096):
+  // rounds of 256 blocks, a time per chunk, and the hand-off of a split.  Measured, 64-row
+  // tiles split / 256-row ones: M = 64, N = 4096 4 ways 24 / 57; M = 512, N = 4096 2 ways 34 /
+  // 60; M = 1024 48 / 80; M = 2048, N = 4096 92 / 106 (2 ways), N = 14336 292 / 266; M = 4096
+  // 183 / 147.
+  double best = 0;
+  for (int kind = G_64; kind <= G_256; ++kind) {
+    const int bm = kind == G_64 ? 64 : 256, bn = kind == G_64 ? 128 : 64;
+    const long tiles = (long)mm_cdiv(K, GR_COLS) * mm_cdiv(M, bm);
+    const int nch = grad_chunks(nmat, N, bn);
+    for (int ks = 1; ks <= 16 && (ks == 1 || (nch / ks >= 2 && tiles <= GR_MAX_TILES)); ++ks) {
+      const int per = mm_cdiv(nch, ks);
+      if (mm_cdiv(nch, per) != ks) continue;
+      const double rounds = (double)((tiles * ks + 255) / 256);
+      const double us = kind == G_64
+                            ? rounds * per * (tiles * ks < 256 ? 1.06 : 1.25) + (ks > 1 ? 3 + 1.5 * ks : 0)
+                            : rounds * per * 2.2 + (ks > 1 ? 6 + 4 * ks : 0);
+      if (best == 0 || us < best) {
+        best = us;
+        p = GradPlan{kind, bn, bm, ks, per, 0,
+                     ks > 1 ? (size_t)tiles * ks * bm * GR_COLS * sizeof(float) : 0};
+      }
+    }
+  }
+  return p;
+}
+
+template <bool INT4, bool ROWS, int WM, int WK, int RB, int SR, int BN, int STG>
 int launch_grad(const GradSegs& s, void* out, int ot, const float* rowmul, int M, int K, int g,
                 const GradPlan& p, void* ws, hipStream_t st) {
-  using Sh = GradShape<INT4, WM, RB, SR>;
+  using Sh = GradShape<INT4, WM, WK, RB, SR, BN, STG>;
   const dim3 grid(mm_cdiv(K, GR_COLS), mm_cdiv(M, Sh::BM), p.ks);
-  // Row tiles walked together: the walk's A rows (128 B per n) against B words (4 B x 32).
   int grp = 1;
   while (grp * 2 <= (int)grid.y && grp < 4) grp *= 2;
-  hipLaunchKernelGGL((k_grad<INT4, ROWS, WM, RB, SR>), grid, dim3(Sh::NTHR), 0, st, s, out, ot,
-                     rowmul, M, K, g, p.cps, grp, (float*)((char*)ws + GR_COUNTER_BYTES),
+  hipLaunchKernelGGL((k_grad<INT4, ROWS, WM, WK, RB, SR, BN, STG>), grid, dim3(Sh::NTHR), 0, st, s,
+                     out, ot, rowmul, M, K, g, p.per, grp, (float*)((char*)ws + GR_COUNTER_BYTES),
                      (uint32_t*)ws);
   MM_CHECK_LAUNCH("gemm backward");
   return 0;
 }
 
-template <bool INT4, bool ROWS, int SR>
-int launch_grad_tile(const GradSegs& s, void* out, int ot, const float* rowmul, int M, int K,
-                     int g, const GradPlan& p, void* ws, hipStream_t st) {
-  if (p.wm == 2) return launch_grad<INT4, ROWS, 2, 4, SR>(s, out, ot, rowmul, M, K, g, p, ws, st);
-  if (p.rb == 4) return launch_grad<INT4, ROWS, 1, 4, SR>(s, out, ot, rowmul, M, K, g, p, ws, st);
-  if (p.rb == 2) return launch_grad<INT4, ROWS, 1, 2, SR>(s, out, ot, rowmul, M, K, g, p, ws, st);
-  return launch_grad<INT4, ROWS, 1, 1, SR>(s, out, ot, rowmul, M, K, g, p, ws, st);
+template <bool INT4, bool ROWS, int MT, int SPW>
+int launch_grad_skinny(const GradSegs& s, void* out, int ot, const float* rowmul, int M, int K,
+                       int g, const GradPlan& p, void* ws, hipStream_t st) {
+  hipLaunchKernelGGL((k_grad_skinny<INT4, ROWS, MT, SPW>), dim3(mm_cdiv(K, GS_COLS), p.ks),
+                     dim3(GS_NTHR), 0, st, s, out, ot, rowmul, M, K, g, p.per,
+                     (float*)((char*)ws + GR_COUNTER_BYTES), (uint32_t*)ws);
+  MM_CHECK_LAUNCH("gemm backward (few rows)");
+  return 0;
+}
+
+// A tile's 256 k touch at most 8 groups from g = 32 up, 32 below.
+template <bool INT4, bool ROWS>
+int dispatch_grad(const GradSegs& s, void* out, int ot, const float* rowmul, int M, int K, int g,
+                  const GradPlan& p, void* ws, hipStream_t st) {
+#define MM_GRAD(...) return launch_grad<INT4, ROWS, __VA_ARGS__>(s, out, ot, rowmul, M, K, g, p, ws, st)
+#define MM_GRAD_S(...) \
+  return launch_grad_skinny<INT4, ROWS, __VA_ARGS__>(s, out, ot, rowmul, M, K, g, p, ws, st)
+  if (p.kind == G_SKINNY) {
+    if (M <= 16 && p.spw == 2) MM_GRAD_S(1, 2);
+    if (M <= 16) MM_GRAD_S(1, 4);
+    if (p.spw == 2) MM_GRAD_S(2, 2);
+    MM_GRAD_S(2, 4);
+  }
+  if (g >= 32) {
+    if (p.kind == G_256) MM_GRAD(2, 1, 4, 8, 64, 3);
+    MM_GRAD(1, 4, 2, 8, 128, 3);
+  }
+  if (p.kind == G_256) MM_GRAD(2, 1, 4, 32, 64, 3);
+  MM_GRAD(1, 4, 2, 32, 128, 3);
+#undef MM_GRAD_S
+#undef MM_GRAD
 }
 
 }  // namespace
 
 extern "C" size_t mm_gemm_backward_workspace_bytes(int nmat, const int* N, int M, int K) {
   if (nmat < 1 || nmat > 3 || N == nullptr || M <= 0 || K <= 0) return GR_COUNTER_BYTES;
-  return grad_ws_bytes(plan_grad(M, grad_chunks(nmat, N), K), M, K);
+  for (int i = 0; i < nmat; ++i)
+    if (N[i] <= 0) return GR_COUNTER_BYTES;
+  return GR_COUNTER_BYTES + plan_grad(nmat, N, M, K).part;
 }
 
 extern "C" int mm_gemm_backward(const uint16_t* const* dC, const int* ldc,
@@ -636,7 +925,6 @@ extern "C" int mm_gemm_backward(const uint16_t* const* dC, const int* ldc,
                "%s: group_size=%d must be a multiple of 8 dividing K=%d", who, g, K);
   GradSegs s{};
   uintptr_t al = (uintptr_t)dA;
-  int ch = 0;
   for (int i = 0; i < 3; ++i) {
     s.s[i].ch0 = 0x7fffffff;
     if (i >= nmat) continue;
@@ -645,27 +933,30 @@ extern "C" int mm_gemm_backward(const uint16_t* const* dC, const int* ldc,
     MM_CHECK_ARG(ldc[i] >= N[i] && ldc[i] % 8 == 0,
                  "%s: ldc[%d]=%d must be a multiple of 8, at least N=%d", who, i, ldc[i], N[i]);
     s.s[i] = GradSeg{(const f16*)dC[i], B[i], (const f16*)S[i],
-                     Z != nullptr ? (const f16*)Z[i] : nullptr, ldc[i], N[i], ch};
-    ch += mm_cdiv(N[i], GR_BN);
+                     Z != nullptr ? (const f16*)Z[i] : nullptr, ldc[i], N[i], 0};
     al |= (uintptr_t)dC[i] | (uintptr_t)B[i] | (uintptr_t)S[i] |
           (Z != nullptr ? (uintptr_t)Z[i] : 0);
   }
-  s.nch = ch;
   MM_CHECK_ARG((al & 15) == 0, "%s: every operand must be 16-byte aligned", who);
+  // the kernels address a tile (256 gradient rows, 32 word rows or 128 columns) with 32 bits
+  for (int i = 0; i < nmat; ++i)
+    MM_CHECK_ARG(ldc[i] < (1 << 22) && N[i] < (1 << 24) && (layout == 0 || K < (1 << 24)),
+                 "%s: N[%d]=%d, ldc=%d, K=%d: rows are too long", who, i, N[i], ldc[i], K);
   if (M == 0) return 0;
-  const GradPlan p = plan_grad(M, ch, K);
-  const size_t need = grad_ws_bytes(p, M, K);
+  const GradPlan p = plan_grad(nmat, N, M, K);
+  for (int i = 0; i < nmat; ++i) {
+    s.s[i].ch0 = s.nch;
+    s.nch += mm_cdiv(N[i], p.bn);
+  }
+  const size_t need = GR_COUNTER_BYTES + p.part;
   MM_CHECK_ARG(p.ks == 1 || (ws != nullptr && ws_bytes >= need),
                "%s: workspace of %zu bytes is smaller than the %zu required", who, ws_bytes, need);
   hipStream_t st = (hipStream_t)stream;
-  // A tile's 256 k touch at most 8 groups from g = 32 up, 32 below.
-#define MM_GRAD(I4, RW)                                                                       \
-  return g >= 32 ? launch_grad_tile<I4, RW, 8>(s, dA, out_type, row_mul, M, K, g, p, ws, st)   \
-                 : launch_grad_tile<I4, RW, 32>(s, dA, out_type, row_mul, M, K, g, p, ws, st)
-  if (layout == 1) MM_GRAD(false, true);
-  if (Z != nullptr) MM_GRAD(true, false);
-  MM_GRAD(false, false);
-#undef MM_GRAD
+  if (layout == 1)
+    return dispatch_grad<false, true>(s, dA, out_type, row_mul, M, K, g, p, ws, st);
+  if (Z != nullptr)
+    return dispatch_grad<true, false>(s, dA, out_type, row_mul, M, K, g, p, ws, st);
+  return dispatch_grad<false, false>(s, dA, out_type, row_mul, M, K, g, p, ws, st);
 }
 
 extern "C" int mm_grad_rows(const void* X, int type, uint16_t* Y, float* row_mul, int M, int N,

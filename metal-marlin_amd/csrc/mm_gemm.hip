@@ -51,6 +51,10 @@ MM_DEV float swiglu(float gate, float up) { return gate / (1.0f + __expf(-gate))
 //   SK_KEEP  : SK_SWIGLU's C, and SK_PAIR's [M, 2N] products as well (`keep`), which the
 //              backward pass of the block starts from: the sums are in registers here, and
 //              a separate launch over the kept pair would read and write 6 M N bytes more.
+//              Up to 32 rows its weights are the exact fp16 ones, scaled before the products
+//              as above 32 rows: the backward pass starts from what is kept, and group sums
+//              scaled afterwards (2^-12 off the rounded weights) would move a quarter of the
+//              kept values by a step.
 enum { SK_PLAIN = 0, SK_SWIGLU = 1, SK_PAIR = 2, SK_MULTI = 3, SK_KEEP = 4 };
 constexpr bool act_pair(int act) { return act == SK_SWIGLU || act == SK_PAIR || act == SK_KEEP; }
 constexpr bool act_glu(int act) { return act == SK_SWIGLU || act == SK_KEEP; }
@@ -992,14 +996,16 @@ int launch_skinny(const f16* A, int lda, const uint32_t* B, const f16* S, const 
                      dim3(sk_nw<MT>() * 64), 0, st, A, lda, B, S, Z, B2, S2, Z2, C, ldc, M, N, \
                      K, g, p.nrounds, part, counters, mp ? *mp : none)
 #define MM_LAUNCH_SK_FL(RP)                                                                 \
-  switch (fl) {                                                                             \
+  if constexpr (ACT == SK_KEEP) {                                                           \
+    MM_LAUNCH_SK(0, RP);                                                                    \
+  } else switch (fl) {                                                                      \
     case 1: MM_LAUNCH_SK(1, RP); break;                                                     \
     case 2: MM_LAUNCH_SK(2, RP); break;                                                     \
     case 4: MM_LAUNCH_SK(4 <= SPW ? 4 : 0, RP); break;                                      \
     case 8: MM_LAUNCH_SK(8 <= SPW ? 8 : 0, RP); break;                                      \
     default: MM_LAUNCH_SK(0, RP); break;                                                    \
   }
-  if constexpr (act_pair(ACT) && MT == 1 && ROWP == 2) {
+  if constexpr (act_pair(ACT) && ACT != SK_KEEP && MT == 1 && ROWP == 2) {
     static_assert(SPW == 8, "a round is 8 pieces of a column");
     if ((fl == 4 || fl == 8) && pair_rows_form(M, K, p, sk_nw<MT>() * SPW)) {
       if (fl == 4) MM_LAUNCH_SK(4, 4);

@@ -47,6 +47,8 @@ def plain(t: torch.Tensor) -> torch.Tensor:
 
 
 def _pad_to(t: torch.Tensor, n: int, dim: int = 1, value: float = 0) -> torch.Tensor:
+    if t.shape[dim] == n:
+        return t
     pad = [0, 0] * (t.dim() - 1 - dim) + [0, n - t.shape[dim]]
     return torch.nn.functional.pad(t.view(torch.int32) if t.dtype == torch.uint32 else t, pad,
                                    value=value)

@@ -199,7 +199,8 @@ def test_block(M, N, K, g, dtype, rows):
     uw, us, Wu = make_fp4(gen, K, N, g, rows)
     x = torch.randn((M, K), generator=gen).to(DEV, dtype)
     h, gu = mmfp4.fused_gate_up_swiglu(x, gw, gs, uw, us, g, row_packed=rows)
-    # weights are not rounded to fp16 by the kernels that apply the scale to the sums: 2^-11
+    # the mid-sized kernel may apply a group's scale to its sum, where the weights have not been
+    # rounded to fp16: 2^-11
     xd = x.half().double()
     W = torch.cat([Wg, Wu], 1)
     terms = xd.abs() @ W.abs()
@@ -210,7 +211,7 @@ def test_block(M, N, K, g, dtype, rows):
     href = gr * sr * ur
     check(h, href, href.abs(), 16, F16,
           1.1 * eg * ur.abs() + (gr * sr).abs() * eu + 1.1 * eg * eu, "h")
-    if not rows and N % 8 == 0 and (M <= 32 or K % 64 == 0):
+    if not rows and M > 32 and N % 8 == 0 and K % 64 == 0:
         assert torch.equal(gu, mmfp4.fused_gate_up_gemm(x, gw, gs, uw, us, g))
         assert torch.equal(h, mmfp4.mmfp4_fused_gate_up_marlin(x, gw, gs, uw, us, g))
     dh = torch.randn((M, N), generator=gen).to(DEV, dtype) * 1e-3
