@@ -1,10 +1,12 @@
 // Python binding of the per-call hot path (marlin_gemm_fp4 / marlin_gemm_int4,
-// the fused QKV and gate/up projections and the row-packed product) for callers
+// the fused QKV and gate/up projections, the row-packed product, their input
+// gradients and the low-rank adapters) for callers
 // that issue one projection per Python call.  It does in C++ what the
 // ctypes path does in Python -- shape checks, the output allocation, the
 // per-(device, stream) workspace -- and calls the same C ABI entry points of
 // libmmfp4.so (mm_fp4_gemm / mm_u4_gemm).  torch is used only for tensor
 // arguments and the output allocation; the stream comes from the caller.
+#include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -232,6 +234,257 @@ pybind11::object rowpacked(const at::Tensor& A, const at::Tensor& W, const at::T
   return pybind11::cast(out);
 }
 
+// ---------------------------------------------------------------------------
+// Training and adapters.  As above: plain operands on the current device (contiguous,
+// 16-byte aligned, N % 8 == 0), or None.
+// ---------------------------------------------------------------------------
+int type_code(at::ScalarType t) {
+  return t == at::kFloat ? 0 : (t == at::kHalf ? 1 : (t == at::kBFloat16 ? 2 : -1));
+}
+bool on_current_device(int dev) {
+  return dev >= 0 &&
+         c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getDevice().index() == dev;
+}
+bool aligned(const at::Tensor& t) { return ((uintptr_t)t.data_ptr() & 15) == 0; }
+// [*, n] rows in plain form: their number, or -1.
+int64_t plain_rows(const at::Tensor& t, int dev, int64_t n) {
+  if (t.dim() < 1 || t.size(-1) != n || t.get_device() != dev || !t.is_contiguous() ||
+      !aligned(t) || type_code(t.scalar_type()) < 0)
+    return -1;
+  return t.numel() / n;
+}
+at::Tensor rows_like(const at::Tensor& t, int64_t n, at::ScalarType type) {
+  std::vector<int64_t> shape(t.sizes().begin(), t.sizes().end());
+  shape.back() = n;
+  return at::empty(shape, t.options().dtype(type));
+}
+struct Matrix {
+  const uint32_t* w;
+  const uint16_t *s, *z;
+  int64_t N, K;
+};
+// A quantized matrix in plain form; N = 0 if it is none.
+Matrix plain_matrix(const at::Tensor& W, const at::Tensor& S, const c10::optional<at::Tensor>& Z,
+                    bool rows, int64_t g, int dev) {
+  Matrix m{nullptr, nullptr, nullptr, 0, 0};
+  if (W.dim() != 2 || g <= 0) return m;
+  const int64_t N = W.size(rows ? 0 : 1), K = 8 * W.size(rows ? 1 : 0);
+  if (N <= 0 || N % 8 != 0 || K <= 0 || K % g != 0 || (rows && K % 32 != 0) ||
+      !plain_words(W, dev, W.size(0), W.size(1)) || !plain(S, at::kHalf, dev, K / g, N) ||
+      !aligned(W) || !aligned(S))
+    return m;
+  if (Z && (!plain(*Z, at::kHalf, dev, K / g, N) || !aligned(*Z))) return m;
+  m.w = (const uint32_t*)W.data_ptr();
+  m.s = (const uint16_t*)S.data_ptr();
+  m.z = Z ? (const uint16_t*)Z->data_ptr() : nullptr;
+  m.N = N;
+  m.K = K;
+  return m;
+}
+// dA of up to three matrices from fp16 gradients.
+at::Tensor backward(const at::Tensor& like, int nmat, const uint16_t* const* dC, const int* ldc,
+                    const float* mul, const Matrix* mats, bool rows, int64_t M, int64_t g,
+                    at::ScalarType out_type, int64_t stream) {
+  const int64_t K = mats[0].K;
+  at::Tensor out = rows_like(like, K, out_type);
+  if (M == 0) return out;
+  const uint32_t* w[3];
+  const uint16_t *s[3], *z[3];
+  int n[3];
+  for (int i = 0; i < nmat; ++i) {
+    w[i] = mats[i].w;
+    s[i] = mats[i].s;
+    z[i] = mats[i].z;
+    n[i] = (int)mats[i].N;
+  }
+  at::Tensor ws = workspace(like, stream, mm_gemm_backward_workspace_bytes(nmat, n, (int)M, (int)K));
+  const int rc = mm_gemm_backward(dC, ldc, mul, nmat, w, s, z[0] ? z : nullptr, n, rows,
+                                  out.data_ptr(), type_code(out_type), (int)M, (int)K, (int)g,
+                                  ws.data_ptr(), (size_t)ws.numel(), (void*)stream);
+  if (rc) fail(rc);
+  return out;
+}
+// fp16 values of M x N gradients and their rows' factors (undefined: ones).
+std::pair<at::Tensor, at::Tensor> carried(const at::Tensor& d, int64_t M, int64_t N,
+                                          int64_t stream) {
+  if (d.scalar_type() == at::kHalf) return {d, at::Tensor()};
+  at::Tensor y = at::empty({M, N}, d.options().dtype(at::kHalf));
+  at::Tensor mul = at::empty({M}, d.options().dtype(at::kFloat));
+  const int rc = mm_grad_rows(d.data_ptr(), type_code(d.scalar_type()), (uint16_t*)y.data_ptr(),
+                              (float*)mul.data_ptr(), (int)M, (int)N, (void*)stream);
+  if (rc) fail(rc);
+  return {y, mul};
+}
+
+pybind11::object linear_backward(const at::Tensor& dC, const at::Tensor& W, const at::Tensor& S,
+                                 const c10::optional<at::Tensor>& Z, bool rows, int64_t g,
+                                 int64_t stream) {
+  const int dev = (int)dC.get_device();
+  if (!on_current_device(dev)) return pybind11::none();
+  const Matrix m = plain_matrix(W, S, Z, rows, g, dev);
+  const int64_t M = m.N ? plain_rows(dC, dev, m.N) : -1;
+  if (M < 0) return pybind11::none();
+  const auto [d, mul] = carried(dC, M, m.N, stream);
+  const uint16_t* p[1] = {(const uint16_t*)d.data_ptr()};
+  const int ld[1] = {(int)m.N};
+  return pybind11::cast(backward(dC, 1, p, ld, mul.defined() ? (const float*)mul.data_ptr() : nullptr,
+                                 &m, rows, M, g, dC.scalar_type(), stream));
+}
+
+pybind11::object qkv_backward(const std::array<at::Tensor, 3>& dC,
+                              const std::array<at::Tensor, 3>& W,
+                              const std::array<at::Tensor, 3>& S, int64_t g, int64_t stream) {
+  const int dev = (int)dC[0].get_device();
+  if (!on_current_device(dev) || dC[0].scalar_type() != at::kHalf) return pybind11::none();
+  Matrix m[3];
+  const uint16_t* p[3];
+  int ld[3];
+  int64_t M = 0;
+  for (int i = 0; i < 3; ++i) {
+    m[i] = plain_matrix(W[i], S[i], c10::nullopt, false, g, dev);
+    const int64_t rows = m[i].N ? plain_rows(dC[i], dev, m[i].N) : -1;
+    if (rows < 0 || dC[i].scalar_type() != at::kHalf || m[i].K != m[0].K ||
+        dC[i].sizes().slice(0, dC[i].dim() - 1) != dC[0].sizes().slice(0, dC[0].dim() - 1))
+      return pybind11::none();
+    M = rows;
+    p[i] = (const uint16_t*)dC[i].data_ptr();
+    ld[i] = (int)m[i].N;
+  }
+  return pybind11::cast(backward(dC[0], 3, p, ld, nullptr, m, false, M, g, at::kHalf, stream));
+}
+
+pybind11::object gate_up_keep(const at::Tensor& A, const at::Tensor& Wg, const at::Tensor& Sg,
+                              const at::Tensor& Wu, const at::Tensor& Su, int64_t g, bool rows,
+                              int64_t stream) {
+  const int dev = (int)A.get_device();
+  if (!on_current_device(dev) || A.scalar_type() != at::kHalf) return pybind11::none();
+  const Matrix mg = plain_matrix(Wg, Sg, c10::nullopt, rows, g, dev);
+  const Matrix mu = plain_matrix(Wu, Su, c10::nullopt, rows, g, dev);
+  const int64_t N = mg.N, K = mg.K, M = N ? plain_rows(A, dev, K) : -1;
+  if (M <= 0 || mu.N != N || mu.K != K || (M > 32 && K % 64 != 0) ||
+      (rows && g % (M <= 32 ? 32 : 64) != 0))
+    return pybind11::none();
+  at::Tensor h = rows_like(A, N, at::kHalf), keep = rows_like(A, 2 * N, at::kHalf);
+  at::Tensor ws = workspace(A, stream, mm_gemm_workspace_bytes((int)M, (int)(2 * N), (int)K));
+  const int rc = mm_fp4_gate_up_keep((const uint16_t*)A.data_ptr(), mg.w, mg.s, mu.w, mu.s,
+                                     (uint16_t*)h.data_ptr(), (uint16_t*)keep.data_ptr(), rows,
+                                     (int)M, (int)N, (int)K, (int)g, ws.data_ptr(),
+                                     (size_t)ws.numel(), (void*)stream);
+  if (rc) fail(rc);
+  return pybind11::make_tuple(h, keep);
+}
+
+pybind11::object gate_up_backward(const at::Tensor& dH, const at::Tensor& keep,
+                                  const at::Tensor& Wg, const at::Tensor& Sg,
+                                  const at::Tensor& Wu, const at::Tensor& Su, int64_t g, bool rows,
+                                  int64_t stream) {
+  const int dev = (int)dH.get_device();
+  if (!on_current_device(dev)) return pybind11::none();
+  const Matrix m[2] = {plain_matrix(Wg, Sg, c10::nullopt, rows, g, dev),
+                       plain_matrix(Wu, Su, c10::nullopt, rows, g, dev)};
+  const int64_t N = m[0].N, M = N ? plain_rows(dH, dev, N) : -1;
+  if (M <= 0 || m[1].N != N || m[1].K != m[0].K || keep.scalar_type() != at::kHalf ||
+      keep.dim() != dH.dim() || plain_rows(keep, dev, 2 * N) != M)
+    return pybind11::none();
+  at::Tensor d = at::empty({M, 2 * N}, keep.options());
+  at::Tensor mul = at::empty({M}, keep.options().dtype(at::kFloat));
+  const int rc = mm_swiglu_grad(dH.data_ptr(), type_code(dH.scalar_type()),
+                                (const uint16_t*)keep.data_ptr(), (uint16_t*)d.data_ptr(),
+                                (float*)mul.data_ptr(), (int)M, (int)N, (void*)stream);
+  if (rc) fail(rc);
+  const uint16_t* p[2] = {(const uint16_t*)d.data_ptr(), (const uint16_t*)d.data_ptr() + N};
+  const int ld[2] = {(int)(2 * N), (int)(2 * N)};
+  return pybind11::cast(backward(dH, 2, p, ld, (const float*)mul.data_ptr(), m, rows, M, g,
+                                 dH.scalar_type(), stream));
+}
+
+// The adapters' operands in plain form.
+struct Lora {
+  int64_t T, K, N, r, L;
+  int type, ids64;
+  const void* ids;
+  const float* scaling;
+};
+bool plain_lora(const at::Tensor& x, const at::Tensor& a, const at::Tensor& b,
+                const c10::optional<at::Tensor>& ids, const c10::optional<at::Tensor>& scaling,
+                Lora* l) {
+  const int dev = (int)x.get_device();
+  const auto t = x.scalar_type();
+  if (!on_current_device(dev) || (t != at::kHalf && t != at::kBFloat16) || a.dim() != 3 ||
+      b.dim() != 3)
+    return false;
+  *l = Lora{0, a.size(2), b.size(1), a.size(1), a.size(0), type_code(t), 0, nullptr, nullptr};
+  if (l->K <= 0 || l->N <= 0 || l->r <= 0 || l->L <= 0 || x.dim() < 1 || x.size(-1) != l->K ||
+      !x.is_contiguous() || b.size(0) != l->L || b.size(2) != l->r)
+    return false;
+  l->T = x.numel() / l->K;
+  for (const at::Tensor* w : {&a, &b})
+    if (w->get_device() != dev || w->scalar_type() != t || !w->is_contiguous()) return false;
+  if (ids) {
+    l->ids64 = ids->scalar_type() == at::kLong;
+    if (ids->get_device() != dev || (!l->ids64 && ids->scalar_type() != at::kInt) ||
+        !ids->is_contiguous() || ids->dim() != 1 || ids->numel() != l->T)
+      return false;
+    l->ids = ids->data_ptr();
+  } else if (l->L != 1) {
+    return false;
+  }
+  if (scaling) {
+    if (scaling->get_device() != dev || scaling->scalar_type() != at::kFloat ||
+        !scaling->is_contiguous() || scaling->dim() != 1 || scaling->numel() != l->L)
+      return false;
+    l->scaling = (const float*)scaling->data_ptr();
+  }
+  return l->T > 0;
+}
+bool same_rows(const at::Tensor& t, const at::Tensor& x, int64_t n) {
+  return t.dim() == x.dim() && t.get_device() == x.get_device() && t.is_contiguous() &&
+         t.size(-1) == n && t.sizes().slice(0, t.dim() - 1) == x.sizes().slice(0, x.dim() - 1);
+}
+
+pybind11::object lora_add(const at::Tensor& base, const at::Tensor& x, const at::Tensor& a,
+                          const at::Tensor& b, const c10::optional<at::Tensor>& ids,
+                          const c10::optional<at::Tensor>& scaling, double factor,
+                          int64_t stream) {
+  Lora l;
+  if (!plain_lora(x, a, b, ids, scaling, &l) || !same_rows(base, x, l.N) ||
+      (base.scalar_type() != at::kHalf && base.scalar_type() != x.scalar_type()))
+    return pybind11::none();
+  at::Tensor out = rows_like(x, l.N, x.scalar_type());
+  at::Tensor ws = workspace(x, stream, mm_lora_workspace_bytes((int)l.T, (int)l.K, (int)l.N,
+                                                               (int)l.r, (int)l.L, 0));
+  const int rc = mm_lora_add((const uint16_t*)x.data_ptr(), l.type,
+                             (const uint16_t*)base.data_ptr(), type_code(base.scalar_type()),
+                             (uint16_t*)out.data_ptr(), (const uint16_t*)a.data_ptr(),
+                             (const uint16_t*)b.data_ptr(), l.ids, l.ids64, l.scaling,
+                             (float)factor, (int)l.T, (int)l.K, (int)l.N, (int)l.r, (int)l.L,
+                             ws.data_ptr(), (size_t)ws.numel(), (void*)stream);
+  if (rc) fail(rc);
+  return pybind11::cast(out);
+}
+
+pybind11::object lora_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& a,
+                               const at::Tensor& b, const c10::optional<at::Tensor>& ids,
+                               const c10::optional<at::Tensor>& scaling, double factor,
+                               const c10::optional<at::Tensor>& dx_base, int64_t stream) {
+  Lora l;
+  if (!plain_lora(x, a, b, ids, scaling, &l) || !same_rows(dy, x, l.N) ||
+      dy.scalar_type() != x.scalar_type() ||
+      (dx_base && (!same_rows(*dx_base, x, l.K) || dx_base->scalar_type() != x.scalar_type())))
+    return pybind11::none();
+  at::Tensor dx = at::empty_like(x), da = at::empty_like(a), db = at::empty_like(b);
+  at::Tensor ws = workspace(x, stream, mm_lora_workspace_bytes((int)l.T, (int)l.K, (int)l.N,
+                                                               (int)l.r, (int)l.L, 1));
+  const int rc = mm_lora_backward(
+      (const uint16_t*)dy.data_ptr(), (const uint16_t*)x.data_ptr(), l.type,
+      (const uint16_t*)a.data_ptr(), (const uint16_t*)b.data_ptr(), l.ids, l.ids64, l.scaling,
+      (float)factor, dx_base ? (const uint16_t*)dx_base->data_ptr() : nullptr,
+      (uint16_t*)dx.data_ptr(), (uint16_t*)da.data_ptr(), (uint16_t*)db.data_ptr(), (int)l.T,
+      (int)l.K, (int)l.N, (int)l.r, (int)l.L, ws.data_ptr(), (size_t)ws.numel(), (void*)stream);
+  if (rc) fail(rc);
+  return pybind11::make_tuple(dx, da, db);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -242,6 +495,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qkv", &qkv, "mm_fp4_gemm_multi on plain operands, else None");
   m.def("gate_up", &gate_up, "mm_fp4_gate_up[_rowpacked] on plain operands, else None");
   m.def("rowpacked", &rowpacked, "mm_fp4_gemm_rowpacked on plain operands, else None");
+  m.def("linear_backward", &linear_backward, "mm_gemm_backward on plain operands, else None");
+  m.def("qkv_backward", &qkv_backward, "mm_gemm_backward over three matrices, else None");
+  m.def("gate_up_keep", &gate_up_keep, "mm_fp4_gate_up_keep on plain operands, else None");
+  m.def("gate_up_backward", &gate_up_backward,
+        "mm_swiglu_grad and mm_gemm_backward on plain operands, else None");
+  m.def("lora_add", &lora_add, "mm_lora_add on plain operands, else None");
+  m.def("lora_backward", &lora_backward, "mm_lora_backward on plain operands, else None");
   m.def("workspace", &workspace_for,
         "the zero-initialised workspace of (device index, raw stream), at least nbytes",
         pybind11::arg("device"), pybind11::arg("stream"), pybind11::arg("nbytes"));

@@ -273,6 +273,21 @@ def release_workspaces() -> None:
     _ws.clear()
 
 
+def fast(name: str, tensor: torch.Tensor, *args):
+    """The per-call binding's entry `name` on the current stream of the tensor's device: its
+    result, or None when the binding is absent, the stream is being captured (call_workspace)
+    or the operands are not in the plain form it takes."""
+    b = binding()
+    if b is None or tensor.get_device() < 0 or torch.cuda.is_current_stream_capturing():
+        return None
+    try:
+        return getattr(b, name)(*args, _raw_stream(tensor.get_device()))
+    except RuntimeError as e:
+        if type(e) is RuntimeError:
+            raise MMError(str(e)) from None
+        raise
+
+
 def call_workspace(index: int, stream: int, nbytes: int) -> torch.Tensor:
     """workspace_on, or under graph capture a zeroed buffer of the call's own (from the
     graph's memory pool): two captured graphs never share it, so they may replay at once."""

@@ -63,7 +63,16 @@ def _scaling(scaling, adapters: int, dev: torch.device):
     return scaling.to(torch.float32).contiguous(), 1.0
 
 
+def _plain_scaling(scaling):
+    return (scaling, 1.0) if isinstance(scaling, torch.Tensor) else (None, float(scaling))
+
+
 def _add(base, x, lora_a, lora_b, adapter_ids, scaling, out=None):
+    if out is None and isinstance(x, torch.Tensor):
+        got = _lib.fast("lora_add", x, base, x, lora_a, lora_b, adapter_ids,
+                        *_plain_scaling(scaling))
+        if got is not None:
+            return got
     dev = _lib.require_device(base, x, lora_a, lora_b, adapter_ids, out)
     a, b = _factors(lora_a, lora_b)
     L, r, K = a.shape
@@ -133,6 +142,11 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_
     as lora_a and lora_b (zeros for adapters without tokens), dx of x's type.  dx_base, the
     gradient that reached x through the projection itself (marlin_gemm_fp4_backward), is
     added to dx before it is rounded."""
+    if isinstance(x, torch.Tensor):
+        got = _lib.fast("lora_backward", x, dy, x, lora_a, lora_b, adapter_ids,
+                        *_plain_scaling(scaling), dx_base)
+        if got is not None:
+            return got
     dev = _lib.require_device(dy, x, lora_a, lora_b, adapter_ids, dx_base)
     a, b = _factors(lora_a, lora_b)
     L, r, K = a.shape

@@ -119,6 +119,10 @@ def _linear(dC: torch.Tensor, words: torch.Tensor, scales: torch.Tensor,
     dev = _lib.require_device(dC, words, scales, zeros)
     N = scales.shape[1]
     dtype = out_dtype or dC.dtype
+    if dtype == dC.dtype:
+        out = _lib.fast("linear_backward", dC, dC, words, scales, zeros, bool(layout), group_size)
+        if out is not None:
+            return out
     _type("out_dtype", dtype)
     with on_device(dev):
         g, mul = _carried(_flat(dC, N, "dC"))
@@ -189,6 +193,11 @@ def mmfp4_fused_qkv_backward(dQ: torch.Tensor, dK: torch.Tensor, dV: torch.Tenso
     the sum rounded once."""
     dev = _lib.require_device(dQ, dK, dV, Q_packed, Q_scales, K_packed, K_scales, V_packed,
                               V_scales)
+    if out_dtype in (None, dQ.dtype):
+        out = _lib.fast("qkv_backward", dQ, (dQ, dK, dV), (Q_packed, K_packed, V_packed),
+                        (Q_scales, K_scales, V_scales), group_size)
+        if out is not None:
+            return out
     grads, mats, widths = [], [], []
     Kdim = Q_packed.shape[0] * kernels.FP4_PER_UINT
     dtype = out_dtype or dQ.dtype
@@ -242,6 +251,10 @@ def fused_gate_up_swiglu(x: torch.Tensor, gate_packed: torch.Tensor, gate_scales
     dev = _lib.require_device(x, gate_packed, gate_scales, up_packed, up_scales)
     if x.dim() == 0 or not x.is_floating_point():
         raise ValueError(f"x must be a floating tensor [*, K], got {x.dtype} {tuple(x.shape)}")
+    out = _lib.fast("gate_up_keep", x, x, gate_packed, gate_scales, up_packed, up_scales,
+                    group_size, row_packed)
+    if out is not None:
+        return out
     N, K = _check_pair(x.shape[-1], gate_packed, gate_scales, up_packed, up_scales, group_size,
                        row_packed)
     lead = x.shape[:-1]
@@ -282,6 +295,11 @@ def fused_gate_up_swiglu_backward(dh: torch.Tensor, gate_up: torch.Tensor,
     dev = _lib.require_device(dh, gate_up, gate_packed, gate_scales, up_packed, up_scales)
     N, K = _check_pair(None, gate_packed, gate_scales, up_packed, up_scales, group_size,
                        row_packed)
+    if out_dtype in (None, dh.dtype):
+        out = _lib.fast("gate_up_backward", dh, dh, gate_up, gate_packed, gate_scales, up_packed,
+                        up_scales, group_size, row_packed)
+        if out is not None:
+            return out
     if tuple(gate_up.shape) != (*dh.shape[:-1], 2 * N):
         raise ValueError(f"gate_up shape {tuple(gate_up.shape)} != "
                          f"{(*dh.shape[:-1], 2 * N)}")
