@@ -5,19 +5,20 @@
 // with A [L, r, K], B [L, N, r], s = scale * scaling[a] (scaling fp32 [L], or none).
 //
 // Few tokens: every token on its own, two launches of fp32 dot products (k_vec_down,
-// k_vec_up).  Otherwise the tokens are sorted by adapter (mm_moe_sort) and cut into tiles
-// of 32 of one adapter:
+// k_vec_up).  Otherwise the tokens are sorted by adapter and cut into tiles of 64 of one
+// adapter (k_plan), and
 //   k_down   H of a tile, over the whole width: 16x16x32 MFMAs, the width split over the
 //            waves and over blocks.  The block that finishes a tile leaves a record of it:
 //            H as hi + lo in the operands' type, under one power of two per tile that puts
 //            the tile's largest value in [2^14, 2^15): 16 (bf16) or 22 (fp16) bits of H
 //            reach the second product, whatever its size.  The record has H by token and
 //            by rank, the operand orders of the two kernels that follow.
-//   k_up     out of a tile: MFMAs over [hi | lo] of 16 ranks at a time.
-//   k_wgrad  dA_a or dB_a: MFMAs over the 32 tokens of a tile, tile after tile.
-// All sums are fp32 and in a fixed order.  All three kernels stream activations that are
-// read once (x, dy) or read and written once (out): HBM bounds them, the factors stay in L2.
+//   up       out of a tile: MFMAs over [hi | lo] of 16 ranks at a time.
+//   wgrad    dA_a or dB_a: MFMAs over 32 tokens at a time, tile after tile.
+// All sums are fp32 and in a fixed order.  All of them stream activations that are read
+// once (x, dy) or read and written once (out): HBM bounds them, the factors stay in L2.
 #include <algorithm>
+#include <type_traits>
 
 #include "mm_common.h"
 #include "mmfp4.h"
@@ -28,14 +29,16 @@ typedef __bf16 bf16;
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
-typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 // Rows of any width start at any even address.
 typedef u16x4 u16x4_any __attribute__((aligned(2)));
 typedef u16x8 u16x8_any __attribute__((aligned(2)));
 
-constexpr int LO_TM = 32;               // tokens per tile
-constexpr int LO_NT = 256;              // threads per block
-constexpr int LO_COLS = 256;            // columns per block of k_up and k_wgrad: 64 a wave
+constexpr int LO_TM = 64;               // tokens per tile
+constexpr int LO_NT = 256;              // threads per block of the dot products, up and wgrad
+constexpr int LO_DW = 8;                // waves of a k_down block
+constexpr int LO_UP_COLS = 256;         // columns per block of up: 64 a wave
+constexpr int LO_WG_COLS = 64;          // columns per block of wgrad
+constexpr int LO_MAX_ADAPTERS = 1024;
 // Arrival counters at the head of the workspace, where every entry point has them.
 constexpr size_t LO_COUNTER_BYTES = (size_t)16384 * sizeof(uint32_t);
 
@@ -86,6 +89,19 @@ MM_DEV void store4(uint16_t* p, u16x4 v, int n) {
   for (int i = 0; i < 3; ++i)
     if (i < n) p[i] = v[i];
 }
+// The same where the caller knows that all are there: a guard costs a branch and a wait for
+// every load before it, so the kernels have a form of each for whole pieces.
+template <bool WHOLE>
+MM_DEV u16x4 ld4(const uint16_t* p, int n) {
+  if constexpr (WHOLE) return *(const u16x4_any*)p;
+  else return load4(p, n);
+}
+template <bool WHOLE>
+MM_DEV void st4(uint16_t* p, u16x4 v, int n) {
+  if constexpr (WHOLE) *(u16x4_any*)p = v;
+  else store4(p, v, n);
+}
+
 // Eight rows of four values -> four columns of eight (the MFMA operand of each column).
 MM_DEV void transpose84(const u16x4 (&v)[8], u16x8 (&o)[4]) {
 #pragma unroll
@@ -102,18 +118,37 @@ MM_DEV void transpose84(const u16x4 (&v)[8], u16x8 (&o)[4]) {
 }
 
 // ---------------------------------------------------------------------------
-// Tokens sorted by adapter: group e (e < L: adapter e; e == L: none) holds sorted rows
-// [first(e), first(e + 1)); order maps them to tokens.  offsets == nullptr: one adapter
-// for all tokens, in their own order.
+// Tokens sorted by adapter, and the tiles: tile b has `rows` tokens of group e (e < L:
+// adapter e; e == L: no adapter; e < 0: no such tile), listed in tokens[64 b ..], the last one
+// repeated behind them.  tiles == nullptr: one adapter for all tokens, as they come.
 // ---------------------------------------------------------------------------
-struct Groups {
-  const int *offsets, *order;
+struct TileInfo {
+  int e, rows;
+};
+struct Plan {
+  const TileInfo* tiles;
+  const int *tokens, *first;   // first[e]: first tile of group e
   int T, L;
-  MM_DEV int first(int e) const {
-    if (offsets == nullptr) return e == 0 ? 0 : T;
-    return e <= L ? offsets[e] : T;
+  MM_DEV TileInfo tile(int b) const {
+    if (tiles == nullptr)
+      return LO_TM * b < T ? TileInfo{0, min(LO_TM, T - LO_TM * b)} : TileInfo{-1, 0};
+    return tiles[b];
   }
-  MM_DEV int token(int row) const { return order != nullptr ? order[row] : row; }
+  MM_DEV int first_tile(int e) const {
+    if (tiles == nullptr) return e == 0 ? 0 : mm_cdiv(T, LO_TM);
+    return first[e];
+  }
+  // Tokens at[k] of tile b (the list does not wait for the tile's entry).
+  template <int N>
+  MM_DEV void get(int b, const int (&at)[N], int (&tok)[N]) const {
+    if (tiles != nullptr) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) tok[k] = tokens[LO_TM * b + at[k]];
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) tok[k] = min(LO_TM * b + at[k], T - 1);
+    }
+  }
 };
 
 struct Scaling {
@@ -122,51 +157,147 @@ struct Scaling {
   MM_DEV float at(int e) const { return p != nullptr ? scale * p[e] : scale; }
 };
 
-struct Tile {
-  int e, row0, rows;   // group, first sorted row, rows; e < 0: no such tile
-};
-// Tile b of the groups' tiles, counted group by group over `ngroups` groups.  Every lane
-// of the wave takes part.
-MM_DEV Tile find_tile(const Groups& gs, int ngroups, int b) {
-  const int lane = threadIdx.x & 63;
-  int base = 0;
-  for (int e0 = 0; e0 < ngroups; e0 += 64) {
-    const int e = e0 + lane;
-    const int f = e < ngroups ? gs.first(e) : 0, l = e < ngroups ? gs.first(e + 1) : 0;
-    const int n = mm_cdiv(l - f, LO_TM);
-    int inc = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int v = __shfl_up(inc, d);
-      if (lane >= d) inc += v;
-    }
-    const uint64_t hit = __ballot(base + inc > b);
-    if (hit != 0) {
-      const int src = __builtin_ctzll(hit);
-      const int k = b - base - __shfl(inc - n, src);
-      const int row0 = __shfl(f, src) + k * LO_TM;
-      return Tile{e0 + src, row0, min(LO_TM, __shfl(l, src) - row0)};
-    }
-    base += __shfl(inc, 63);
+struct Ids {
+  const void* p;   // nullptr: adapter 0
+  int wide, L;     // int64 ids
+  MM_DEV int64_t raw(int t) const { return wide ? ((const int64_t*)p)[t] : ((const int32_t*)p)[t]; }
+  MM_DEV int at(int t) const {   // the token's adapter, or -1
+    if (p == nullptr) return 0;
+    const int64_t a = raw(t);
+    return a >= 0 && a < L ? (int)a : -1;
   }
-  return Tile{-1, 0, 0};
-}
-// Number of tiles of the groups before e.
-MM_DEV int tiles_before(const Groups& gs, int e) {
-  const int lane = threadIdx.x & 63;
-  int n = 0;
-  for (int i = lane; i < e; i += 64) n += mm_cdiv(gs.first(i + 1) - gs.first(i), LO_TM);
+};
+
+// Stable counting sort of the tokens by group in one block, and the tile table.  Each wave
+// counts and places its own stretch of the tokens, 64 at a time; requests lie one after
+// another, so that a step mostly has one or two groups.  Latency bounds it: the ids of eight
+// steps are loaded together and kept for the second pass (up to 8192 tokens).
+constexpr int PL_NT = 1024, PL_NW = PL_NT / 64, PL_HOLD = 8;
+__global__ void __launch_bounds__(PL_NT)
+k_plan(Ids ids, int T, int max_tiles, TileInfo* __restrict__ tiles, int* __restrict__ tokens,
+       int* __restrict__ first) {
+  __shared__ int cnt[PL_NW][LO_MAX_ADAPTERS + 1];
+  __shared__ int rows_of[LO_MAX_ADAPTERS + 2], tile0[LO_MAX_ADAPTERS + 2];   // rows, first tile
+  __shared__ int last[LO_MAX_ADAPTERS + 1];                               // last token
+  __shared__ int wsum[PL_NW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int G = ids.L + 1;
+  const int steps = mm_cdiv(T, 64 * PL_NW), t0 = wave * steps * 64 + lane;   // per wave
+  int hold[PL_HOLD];
+  auto load = [&](int s0) {
+    int64_t raw[PL_HOLD];
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d);
-  return n;
+    for (int i = 0; i < PL_HOLD; ++i) raw[i] = ids.raw(min(t0 + 64 * (s0 + i), T - 1));
+#pragma unroll
+    for (int i = 0; i < PL_HOLD; ++i)
+      hold[i] = s0 + i < steps && t0 + 64 * (s0 + i) < T
+                    ? (raw[i] >= 0 && raw[i] < ids.L ? (int)raw[i] : ids.L)
+                    : -1;                     // no token
+  };
+  load(0);
+  for (int i = tid; i < PL_NW * G; i += PL_NT) cnt[i / G][i % G] = 0;
+  __syncthreads();
+  for (int s0 = 0; s0 < steps; s0 += PL_HOLD) {
+    if (s0 > 0) load(s0);
+#pragma unroll
+    for (int i = 0; i < PL_HOLD; ++i) {
+      const int g = hold[i], g0 = __builtin_amdgcn_readfirstlane(g);
+      const uint64_t live = __ballot(g >= 0);
+      if (live == 0) continue;
+      if (__ballot(g == g0) == live) {
+        if (lane == 0) cnt[wave][g0] += __popcll(live);
+      } else if (g >= 0) {
+        atomicAdd(&cnt[wave][g], 1);
+      }
+    }
+  }
+  __syncthreads();
+  // Groups 2 tid and 2 tid + 1: rows of each wave in front of one another, then both scans.
+  int n[2] = {0, 0};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int g = 2 * tid + k;
+    if (g >= G) continue;
+#pragma unroll
+    for (int w = 0; w < PL_NW; ++w) {
+      const int c = cnt[w][g];
+      cnt[w][g] = n[k];
+      n[k] += c;
+    }
+    rows_of[g] = n[k];                           // the group's rows
+  }
+  const int nt = mm_cdiv(n[0], LO_TM) + mm_cdiv(n[1], LO_TM);
+  int it = nt;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int b = __shfl_up(it, d);
+    if (lane >= d) it += b;
+  }
+  if (lane == 63) wsum[wave] = it;
+  __syncthreads();
+  int b = it - nt;
+  for (int w = 0; w < wave; ++w) b += wsum[w];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int g = 2 * tid + k;
+    if (g > G) continue;                      // entry G: the end
+    tile0[g] = b;
+    first[g] = b;
+    b += mm_cdiv(n[k], LO_TM);
+  }
+  __syncthreads();
+  const int total = tile0[G];
+  for (int i = tid; i < max_tiles; i += PL_NT) {
+    TileInfo t = {-1, 0};
+    if (i < total) {
+      int lo = 0, hi = G;                     // tile0[lo] <= i < tile0[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tile0[mid] <= i) lo = mid;
+        else hi = mid;
+      }
+      t = TileInfo{lo, min(LO_TM, rows_of[lo] - (i - tile0[lo]) * LO_TM)};
+    }
+    tiles[i] = t;
+  }
+  const uint64_t below = ((uint64_t)1 << lane) - 1;
+  for (int s0 = 0; s0 < steps; s0 += PL_HOLD) {
+    if (steps > PL_HOLD) load(s0);
+#pragma unroll
+    for (int i = 0; i < PL_HOLD; ++i) {
+      const int g = hold[i], t = t0 + 64 * (s0 + i);
+      uint64_t left = __ballot(g >= 0);
+      while (left != 0) {
+        const int src = __builtin_ctzll(left);
+        const int g0 = __builtin_amdgcn_readlane(g, src);
+        const uint64_t m = __ballot(g == g0);
+        volatile int* next = &cnt[wave][g0];  // read by all lanes, moved on by one
+        const int at = *next;
+        if (lane == src) *next = at + __popcll(m);
+        if ((m >> lane) & 1) {
+          const int row = at + __popcll(m & below);   // of the group
+          tokens[LO_TM * tile0[g0] + row] = t;
+          if (row == rows_of[g0] - 1) last[g0] = t;
+        }
+        left &= ~m;
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int g = 2 * tid + k;
+    if (g >= G) continue;
+    int* list = tokens + LO_TM * tile0[g];
+    for (int i = n[k]; i < LO_TM * mm_cdiv(n[k], LO_TM); ++i) list[i] = last[g];
+  }
 }
 
 // The records of a launch's tiles; rp ranks (of a chunk) each, nrc chunks.
 struct Records {
-  uint16_t* by_token;   // [tile][chunk][hi, lo][32][rp]
-  uint16_t* by_rank;    // [tile][chunk][hi, lo][rp][32]
+  uint16_t* by_token;   // [tile][chunk][hi, lo][64][rp]
+  uint16_t* by_rank;    // [tile][chunk][hi, lo][rp][64]
   float* scale;         // [tile][chunk]: H = scale * (hi + lo)
-  int* tokens;          // [tile][32], the last one repeated behind the tile's rows
   int rp, nrc;
 };
 
@@ -189,78 +320,156 @@ MM_DEV bool last_of(uint32_t* counter, int n, uint32_t* s_last) {
 // ---------------------------------------------------------------------------
 // k_down.  One launch does up to two problems (H from x and A, dH from dy and B); block
 // (tile, split, problem x rank chunk).  CR: the factor is [C, r] (B), else [r, C] (A).
-// Wave w of a block takes every fourth pair of 32-wide steps of the block's range.
+// Wave w of a block takes every eighth pair of 32-wide steps of the block's range.  Rows of
+// 16 that hold no token are skipped.
 // ---------------------------------------------------------------------------
 struct DownProblem {
   const uint16_t *V, *W;   // activations [T, C], factors
   int C, ks, per;          // width, splits, 64-wide step pairs per split
   Records rec;
-  float* part;             // [tile][chunk][ks][32 * rp]
+  float* part;             // [tile][chunk][ks][64 * rp]
   uint32_t* counters;      // [tile][chunk]
   int by_token, by_rank;   // which records are wanted
 };
 
-template <int T, bool CR, int RT>
-MM_DEV void down_tile(const DownProblem& p, const Groups& gs, const Scaling& scaling, int r,
-                      int chunk, float* lds) {
-  constexpr int RP = 16 * RT;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, q = lane >> 4;
-  const int b = blockIdx.x;
-  const Tile t = find_tile(gs, gs.L, b);
-  if (t.e < 0) return;
-  const int r0 = chunk * RP;
-  const uint16_t* W = p.W + (size_t)t.e * r * p.C;
-  const uint16_t* v[2];
+template <int T, bool CR, int RT, int NR>
+MM_DEV void down_sum(const DownProblem& p, const Plan& plan, int b, int e, int r, int r0,
+                     f32x4 (&acc)[4][RT]) {
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint16_t* W = p.W + (size_t)e * r * p.C;
+  const uint16_t* v[NR];
+  int at[NR], tok[NR];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    v[i] = p.V + (size_t)gs.token(t.row0 + min(16 * i + c, t.rows - 1)) * p.C;
-  f32x4 acc[2][RT];
+  for (int i = 0; i < NR; ++i) at[i] = 16 * i + c;
+  plan.get(b, at, tok);
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < NR; ++i) v[i] = p.V + (size_t)tok[i] * p.C;
+  // A stage: SS steps of 32 (a pair, or with 64 ranks half of one): its operands, and its
+  // products.  D rows: ranks 4q + i, columns: tokens c.  CR's factors stay as they are loaded
+  // until they are used: packing them waits for them.
+  constexpr int SS = RT == 4 ? 1 : 2, STAGES = 2 / SS;   // steps a stage, stages a pair
+  struct Stage {
+    u16x8 x[SS][NR];
+    std::conditional_t<CR, uint32_t[8], u16x8> w[SS][RT];
+  };
+  auto load = [&](Stage& o, int u) {
 #pragma unroll
-    for (int k = 0; k < RT; ++k) acc[i][k] = f32x4{0, 0, 0, 0};
-  const int pairs = mm_cdiv(p.C, 64);
-  const int p_end = min(pairs, ((int)blockIdx.y + 1) * p.per);
-  for (int pr = blockIdx.y * p.per + wave; pr < p_end; pr += 4) {
+    for (int s = 0; s < SS; ++s) {
+      const int k0 = 32 * (SS * u + s) + 8 * q;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int k0 = 64 * pr + 32 * s + 8 * q, left = p.C - k0;
-      u16x8 x[2], w[RT];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) x[i] = load8(v[i] + k0, left);
+      for (int i = 0; i < NR; ++i) o.x[s][i] = *(const u16x8_any*)(v[i] + k0);
 #pragma unroll
       for (int k = 0; k < RT; ++k) {
         const int rank = min(r0 + 16 * k + c, r - 1);
         if constexpr (!CR) {
-          w[k] = load8(W + (size_t)rank * p.C + k0, left);
+          o.w[s][k] = *(const u16x8_any*)(W + (size_t)rank * p.C + k0);
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            w[k][i] = i < left ? W[(size_t)(k0 + i) * r + rank] : (uint16_t)0;
+          for (int i = 0; i < 8; ++i) o.w[s][k][i] = W[(size_t)(k0 + i) * r + rank];
         }
       }
-      // D rows: ranks 4q + i, columns: tokens c
+    }
+  };
+  auto multiply = [&](const Stage& o) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+    for (int s = 0; s < SS; ++s)
 #pragma unroll
-        for (int k = 0; k < RT; ++k) acc[i][k] = mfma<T>(w[k], x[i], acc[i][k]);
+      for (int k = 0; k < RT; ++k) {
+        u16x8 w;
+        if constexpr (CR) {
+          u32x4 pk;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) pk[i] = o.w[s][k][2 * i] | o.w[s][k][2 * i + 1] << 16;
+          w = __builtin_bit_cast(u16x8, pk);
+        } else {
+          w = o.w[s][k];
+        }
+#pragma unroll
+        for (int i = 0; i < NR; ++i) acc[i][k] = mfma<T>(w, o.x[s][i], acc[i][k]);
+      }
+  };
+  const int beg = blockIdx.y * p.per, end = min(p.C / 64, beg + p.per);   // whole pairs
+  // The next stage is on its way while one is multiplied (the last again at the end).
+  // Stage n of a wave: stage n % STAGES of pair beg + wave + LO_DW * (n / STAGES).
+  const int np = beg + wave < end ? (end - beg - wave + LO_DW - 1) / LO_DW : 0;
+  const int ns = np * STAGES;
+  auto at_stage = [&](int n) {
+    n = min(n, ns - 1);
+    return (beg + wave + LO_DW * (n / STAGES)) * STAGES + n % STAGES;
+  };
+  if (ns > 0) {
+    Stage even, odd;
+    load(even, at_stage(0));
+    for (int n = 0; n < ns; n += 2) {
+      load(odd, at_stage(n + 1));
+      __builtin_amdgcn_sched_barrier(0);   // or the loads sink to where they are used
+      multiply(even);
+      if (n + 1 >= ns) break;
+      load(even, at_stage(n + 2));
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(odd);
     }
   }
-  // Sum over the waves: lds[wave][token][rank].
+  // What is left of a width that is no multiple of 64.
+  const int rest = p.C / 64;
+  if (64 * rest < p.C && rest >= beg && rest < beg + p.per && wave == (rest - beg) % LO_DW) {
+    for (int s = 0; s < 2; ++s) {
+      const int k0 = 64 * rest + 32 * s + 8 * q, left = p.C - k0;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+      for (int k = 0; k < RT; ++k) {
+        const int rank = min(r0 + 16 * k + c, r - 1);
+        u16x8 w;
+        if constexpr (!CR) {
+          w = load8(W + (size_t)rank * p.C + k0, left);
+        } else {
 #pragma unroll
-    for (int k = 0; k < RT; ++k)
-      *(f32x4*)(lds + (wave * LO_TM + 16 * i + c) * RP + 16 * k + 4 * q) = acc[i][k];
-  __syncthreads();
-  constexpr int PER = LO_TM * RP / 4 / LO_NT > 0 ? LO_TM * RP / 4 / LO_NT : 1;   // f32x4 a thread
-  constexpr int ITEMS = LO_TM * RP / 4;
-  __shared__ uint32_t s_last;
-  __shared__ float s_max[4];
+          for (int i = 0; i < 8; ++i) w[i] = i < left ? W[(size_t)(k0 + i) * r + rank] : (uint16_t)0;
+        }
+#pragma unroll
+        for (int i = 0; i < NR; ++i) acc[i][k] = mfma<T>(w, load8(v[i] + k0, left), acc[i][k]);
+      }
+    }
+  }
+}
+
+template <int T, bool CR, int RT>
+MM_DEV void down_tile(const DownProblem& p, const Plan& plan, const Scaling& scaling, int r,
+                      int chunk, float* lds) {
+  constexpr int RP = 16 * RT, NT = 64 * LO_DW, ITEMS = LO_TM * RP / 4;   // f32x4 items
+  constexpr int PER = ITEMS / NT > 0 ? ITEMS / NT : 1;                   // per thread
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, q = lane >> 4;
+  const int b = blockIdx.x;
+  const TileInfo t = plan.tile(b);
+  if (t.e < 0 || t.e >= plan.L) return;
+  const int r0 = chunk * RP;
+  f32x4 acc[4][RT];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int k = 0; k < RT; ++k) acc[i][k] = f32x4{0, 0, 0, 0};
+  if (t.rows > 32) down_sum<T, CR, RT, 4>(p, plan, b, t.e, r, r0, acc);
+  else if (t.rows > 16) down_sum<T, CR, RT, 2>(p, plan, b, t.e, r, r0, acc);
+  else down_sum<T, CR, RT, 1>(p, plan, b, t.e, r, r0, acc);
+  // Sum over the waves, half of them at a time: lds[wave % 4][token][rank].
+  uint32_t* s_last = (uint32_t*)(lds + 4 * LO_TM * RP);
+  float* s_max = lds + 4 * LO_TM * RP + 4;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    if (wave / 4 == half)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < RT; ++k) {
+          f32x4* at = (f32x4*)(lds + ((wave & 3) * LO_TM + 16 * i + c) * RP + 16 * k + 4 * q);
+          *at = half == 0 ? acc[i][k] : *at + acc[i][k];
+        }
+    __syncthreads();
+  }
   f32x4 h[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int it = threadIdx.x + k * LO_NT;
+    const int it = threadIdx.x + k * NT;
     h[k] = f32x4{0, 0, 0, 0};
     if (it < ITEMS)
 #pragma unroll
@@ -271,23 +480,25 @@ MM_DEV void down_tile(const DownProblem& p, const Groups& gs, const Scaling& sca
     const __amdgpu_buffer_rsrc_t prs = mm_rsrc(p.part + (size_t)slot * p.ks * (LO_TM * RP));
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int it = threadIdx.x + k * LO_NT;
+      const int it = threadIdx.x + k * NT;
       if (it < ITEMS) store_agent_x4(prs, 16u * (uint32_t)(blockIdx.y * ITEMS + it), h[k]);
     }
-    if (!last_of(p.counters + slot, p.ks, &s_last)) return;
+    if (!last_of(p.counters + slot, p.ks, s_last)) return;
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const int it = min((int)threadIdx.x + k * LO_NT, ITEMS - 1);
-      h[k] = f32x4{0, 0, 0, 0};
-      for (int z0 = 0; z0 < p.ks; z0 += 4) {
-        f32x4 ld[4];
+    for (int k = 0; k < PER; ++k) h[k] = f32x4{0, 0, 0, 0};
+    for (int z0 = 0; z0 < p.ks; z0 += 8) {
+      f32x4 ld[8][PER];
 #pragma unroll
-        for (int z = 0; z < 4; ++z)
-          ld[z] = load_agent_x4(prs, 16u * (uint32_t)(min(z0 + z, p.ks - 1) * ITEMS + it));
+      for (int z = 0; z < 8; ++z)
 #pragma unroll
-        for (int z = 0; z < 4; ++z)
-          if (z0 + z < p.ks) h[k] += ld[z];
-      }
+        for (int k = 0; k < PER; ++k)
+          ld[z][k] = load_agent_x4(prs, 16u * (uint32_t)(min(z0 + z, p.ks - 1) * ITEMS +
+                                                        min((int)threadIdx.x + k * NT, ITEMS - 1)));
+#pragma unroll
+      for (int z = 0; z < 8; ++z)
+        if (z0 + z < p.ks)
+#pragma unroll
+          for (int k = 0; k < PER; ++k) h[k] += ld[z][k];
     }
   }
   // The record.  Ranks and rows past the last are zero.
@@ -295,7 +506,7 @@ MM_DEV void down_tile(const DownProblem& p, const Groups& gs, const Scaling& sca
   float m = 0.0f;
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int it = threadIdx.x + k * LO_NT, row = 4 * it / RP, rank = 4 * it % RP;
+    const int it = threadIdx.x + k * NT, row = 4 * it / RP, rank = 4 * it % RP;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       h[k][i] = row < t.rows && r0 + rank + i < r ? h[k][i] * s : 0.0f;
@@ -306,7 +517,8 @@ MM_DEV void down_tile(const DownProblem& p, const Groups& gs, const Scaling& sca
   for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
   if (lane == 0) s_max[wave] = m;
   __syncthreads();
-  m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+#pragma unroll
+  for (int w = 0; w < LO_DW; ++w) m = fmaxf(m, s_max[w]);
   int ex = 0;
   if (m > 0.0f && m < __builtin_inff()) {
     (void)frexpf(m, &ex);                      // m = f * 2^ex, f in [0.5, 1)
@@ -317,7 +529,7 @@ MM_DEV void down_tile(const DownProblem& p, const Groups& gs, const Scaling& sca
   uint16_t* br = p.rec.by_rank + (size_t)slot * 2 * LO_TM * RP;
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int it = threadIdx.x + k * LO_NT, row = 4 * it / RP, rank = 4 * it % RP;
+    const int it = threadIdx.x + k * NT, row = 4 * it / RP, rank = 4 * it % RP;
     if (it >= ITEMS) continue;
     u16x4 hi, lo;
 #pragma unroll
@@ -339,226 +551,319 @@ MM_DEV void down_tile(const DownProblem& p, const Groups& gs, const Scaling& sca
       }
   }
   if (threadIdx.x == 0) p.rec.scale[slot] = ldexpf(1.0f, -ex);
-  if (chunk == 0 && threadIdx.x < LO_TM)
-    p.rec.tokens[b * LO_TM + threadIdx.x] = gs.token(t.row0 + min((int)threadIdx.x, t.rows - 1));
 }
 
 template <int T, int RT>
-__global__ void __launch_bounds__(LO_NT)
-k_down(DownProblem p0, DownProblem p1, Groups gs, Scaling scaling, int r) {
-  __shared__ __attribute__((aligned(16))) float lds[4 * LO_TM * 16 * RT];
+__global__ void __launch_bounds__(64 * LO_DW)
+k_down(DownProblem p0, DownProblem p1, Plan plan, Scaling scaling, int r) {
+  __shared__ __attribute__((aligned(16))) float lds[4 * LO_TM * 16 * RT + 4 + LO_DW];
   const int nrc = p0.rec.nrc;
   const bool second = (int)blockIdx.z >= nrc;
   if ((int)blockIdx.y >= (second ? p1.ks : p0.ks)) return;
-  if (!second) down_tile<T, false, RT>(p0, gs, scaling, r, blockIdx.z, lds);
-  else down_tile<T, true, RT>(p1, gs, scaling, r, blockIdx.z - nrc, lds);
+  if (!second) down_tile<T, false, RT>(p0, plan, scaling, r, blockIdx.z, lds);
+  else down_tile<T, true, RT>(p1, plan, scaling, r, blockIdx.z - nrc, lds);
 }
 
 // ---------------------------------------------------------------------------
-// k_up.  Block (tile, 256 columns): wave: 64 columns, lane (c, q): columns 4c .. 4c + 3 of
-// tokens 4q + i of both halves of the tile.  CR: the factor is [C, r] (B), else [r, C] (A).
-// BT: the base's type (0: no base, zeros).  Group L (no adapter) copies the base.
+// up.  Block (tile, 256 columns): wave: 64 columns, lane (c, q): columns 4c .. 4c + 3 of
+// tokens 16 i + 4 q + k.  CR: the factor is [C, r] (B), else [r, C] (A).  BT: the base's
+// type (0: no base, zeros).  Group L (no adapter) copies the base.
 // ---------------------------------------------------------------------------
-template <int T, bool CR, int RT, int BT>
-__global__ void __launch_bounds__(LO_NT)
-k_up(const uint16_t* __restrict__ W, const uint16_t* base, uint16_t* out, int C, int r,
-     Groups gs, Records rec) {
+struct UpProblem {
+  const uint16_t *W, *base;
+  uint16_t* out;
+  int C;
+  Records rec;
+};
+
+template <int T, bool CR, int RT, int BT, bool WHOLE>
+MM_DEV void up_rows(const UpProblem& p, const Plan& plan, TileInfo t, int r, int b, int col0) {
   constexpr int RP = 16 * RT;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, q = lane >> 4;
-  const int b = blockIdx.x, n0 = blockIdx.y * LO_COLS + wave * 64 + 4 * c;
-  const Tile t = find_tile(gs, gs.L + 1, b);
-  if (t.e < 0) return;
-  const bool none = t.e >= gs.L;
-  if (none && base == out) return;
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  const int C = p.C, n0 = col0 + 4 * c;
+  const bool none = t.e >= plan.L;
   const int left = C - n0;
-  u16x4 bv[2][4];
-  size_t at[2][4];
+  const Records& rec = p.rec;
+  const uint16_t* W = p.W + (none ? 0 : (size_t)t.e * r * C);
+  // Factors of the first rank chunk: they serve all rows.
+  u16x8 w[RT][4];
+  auto load_w = [&](int ch) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int k = 0; k < RT; ++k) {
+      const int rank = ch * RP + 16 * k + 8 * (q & 1);   // the first of this lane's eight
+      if constexpr (CR) {
+        // ranks past the last: any, the record has zeros there
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      at[i][k] = (size_t)gs.token(t.row0 + min(16 * i + 4 * q + k, t.rows - 1)) * C + n0;
-      if constexpr (BT != 0) bv[i][k] = load4(base + at[i][k], left);
-      else bv[i][k] = u16x4{0, 0, 0, 0};
-    }
-  f32x4 sum[2][4];   // [half][column j]: tokens 4q + i
+        for (int j = 0; j < 4; ++j)
+          w[k][j] = WHOLE ? *(const u16x8_any*)(W + (size_t)(n0 + j) * r + min(rank, r - 8))
+                          : load8(W + (size_t)min(n0 + j, C - 1) * r + rank, r - rank);
+      } else {
+        u16x4 rows[8];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum[i][j] = f32x4{0, 0, 0, 0};
-  if (!none) {
-    W += (size_t)t.e * r * C;
-    for (int ch = 0; ch < rec.nrc; ++ch) {
-      const size_t slot = (size_t)b * rec.nrc + ch;
-      const uint16_t* H = rec.by_token + slot * 2 * LO_TM * RP + (q >> 1) * LO_TM * RP + 8 * (q & 1);
-      f32x4 acc[2][4];
-#pragma unroll
-      for (int k = 0; k < RT; ++k) {
-        const int rank = ch * RP + 16 * k + 8 * (q & 1);   // the first of this lane's eight
-        u16x8 w[4], hv[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) hv[i] = *(const u16x8*)(H + (16 * i + c) * RP + 16 * k);
-        if constexpr (CR) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            w[j] = load8(W + (size_t)min(n0 + j, C - 1) * r + rank, r - rank);
-        } else {
-          u16x4 rows[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            rows[i] = load4(W + (size_t)min(rank + i, r - 1) * C + n0, left);
-          transpose84(rows, w);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            acc[i][j] = mfma<T>(hv[i], w[j], k == 0 ? f32x4{0, 0, 0, 0} : acc[i][j]);
+        for (int i = 0; i < 8; ++i)
+          rows[i] = ld4<WHOLE>(W + (size_t)min(rank + i, r - 1) * C + n0, left);
+        transpose84(rows, w[k]);
       }
-      const float f = rec.scale[slot];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum[i][j] += f * acc[i][j];
     }
-  }
+  };
+  // The bases of all rows are on their way before anything else.
+  constexpr int NR = LO_TM / 16;
+  u16x4 bv[NR * 4];
+  int at[NR * 4], token[NR * 4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < NR * 4; ++i) at[i] = 16 * (i / 4) + 4 * q + i % 4;
+  plan.get(b, at, token);
+#pragma unroll
+  for (int i = 0; i < NR * 4; ++i)
+    if constexpr (BT != 0) bv[i] = ld4<WHOLE>(p.base + (size_t)token[i] * C + n0, left);
+    else bv[i] = u16x4{0, 0, 0, 0};
+  if (!none) load_w(0);
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {   // 16 rows at a time
+    if (16 * i >= t.rows) break;
+    f32x4 sum[4];   // [column j]: tokens 4q + k
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] = f32x4{0, 0, 0, 0};
+    if (!none) {
+      for (int ch = 0; ch < rec.nrc; ++ch) {
+        if (rec.nrc > 1) load_w(ch);
+        const size_t slot = (size_t)b * rec.nrc + ch;
+        const uint16_t* H = rec.by_token + slot * 2 * LO_TM * RP + (q >> 1) * LO_TM * RP +
+                            (16 * i + c) * RP + 8 * (q & 1);
+        f32x4 acc[4];
+#pragma unroll
+        for (int k = 0; k < RT; ++k) {
+          const u16x8 hv = *(const u16x8*)(H + 16 * k);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[j] = mfma<T>(hv, w[k][j], k == 0 ? f32x4{0, 0, 0, 0} : acc[j]);
+        }
+        const float f = rec.scale[slot];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] += f * acc[j];
+      }
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (16 * i + 4 * q + k >= t.rows) continue;
       u16x4 o;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        o[j] = from_f32<T>(BT != 0 ? to_f32<BT != 0 ? BT : T>(bv[i][k][j]) + sum[i][j][k]
-                                   : sum[i][j][k]);
-      store4(out + at[i][k], o, left);
+        o[j] = from_f32<T>(BT != 0 ? to_f32<BT != 0 ? BT : T>(bv[4 * i + k][j]) + sum[j][k]
+                                   : sum[j][k]);
+      st4<WHOLE>(p.out + (size_t)token[4 * i + k] * C + n0, o, left);
     }
+  }
+}
+
+template <int T, bool CR, int RT, int BT>
+MM_DEV void up_tile(const UpProblem& p, const Plan& plan, int r, int b, int colblock) {
+  const TileInfo t = plan.tile(b);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col0 = colblock * LO_UP_COLS + wave * 64;
+  if (t.e < 0 || (t.e >= plan.L && p.base == p.out) || col0 >= p.C) return;
+  if (col0 + 64 <= p.C && (!CR || r % 8 == 0))
+    up_rows<T, CR, RT, BT, true>(p, plan, t, r, b, col0);
+  else
+    up_rows<T, CR, RT, BT, false>(p, plan, t, r, b, col0);
+}
+
+template <int T, int RT, int BT>
+__global__ void __launch_bounds__(LO_NT)
+k_up(UpProblem p, Plan plan, int r) {
+  up_tile<T, true, RT, BT>(p, plan, r, blockIdx.x, blockIdx.y);
 }
 
 // ---------------------------------------------------------------------------
-// k_wgrad.  Up to two problems: dA_a [r, K] from dH and x, dB_a [N, r] from H and dy.
-// Block (256 columns, adapter, problem x chunk x split): wave: 64 columns, all tiles of its
-// share of the adapter's.  D rows: ranks 4q + i, columns 4c + j.
+// wgrad.  Up to two problems: dA_a [r, K] from dH and x, dB_a [N, r] from H and dy.  Block
+// (64 columns, adapter, problem x chunk x split): its waves take every fourth 32 tokens of
+// the adapter's tiles in its share and add up in LDS.  D rows: ranks 4q + i, columns 4c + j.
 // ---------------------------------------------------------------------------
 struct GradProblem {
   const uint16_t* V;    // [T, C]
   uint16_t* G;          // [L, r, C] or, CR, [L, C, r]
   int C, ks;
   Records rec;
-  float* part;          // [adapter][chunk][column block][ks][LO_COLS * rp]
+  float* part;          // [adapter][chunk][column block][ks][64 * rp]
   uint32_t* counters;   // [adapter][chunk][column block]
 };
 
-template <int T, bool CR, int RT>
-MM_DEV void wgrad_tile(const GradProblem& p, const Groups& gs, int r, int chunk, int split) {
+template <int T, bool CR, int RT, bool WHOLE>
+MM_DEV void wgrad_tile(const GradProblem& p, const Plan& plan, int r, int colblock, int e,
+                       int chunk, int split, f32x4* lds) {
   constexpr int RP = 16 * RT;
-  __shared__ uint32_t s_last;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, q = lane >> 4;
-  const int e = blockIdx.y, n0 = blockIdx.x * LO_COLS + wave * 64 + 4 * c, left = p.C - n0;
-  if ((int)blockIdx.x * LO_COLS >= p.C) return;
-  const int nt = mm_cdiv(gs.first(e + 1) - gs.first(e), LO_TM);
-  const int per = mm_cdiv(nt, p.ks), tb = tiles_before(gs, e);
-  const int t_beg = tb + split * per, t_end = tb + min(nt, (split + 1) * per);
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = colblock * LO_WG_COLS + 4 * c, left = p.C - n0;
+  const int tb = plan.first_tile(e), nt = plan.first_tile(e + 1) - tb;
+  const int steps = 2 * nt, per = mm_cdiv(steps, p.ks);
+  const int s_end = min(steps, (split + 1) * per);
   f32x4 sum[RT][4];
 #pragma unroll
   for (int k = 0; k < RT; ++k)
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[k][j] = f32x4{0, 0, 0, 0};
-  for (int b = t_beg; b < t_end; ++b) {
-    const i32x4 t0 = *(const i32x4*)(p.rec.tokens + b * LO_TM + 8 * q);
-    const i32x4 t1 = *(const i32x4*)(p.rec.tokens + b * LO_TM + 8 * q + 4);
+  // Tokens two steps ahead, their rows and the records one step ahead (the last again).
+  struct Step {
     u16x4 rows[8];
-    u16x8 w[4];
+    u16x8 hi[RT], lo[RT];
+    float f;
+  };
+  int token[8];
+  auto find = [&](int st) {
+    int at[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      rows[i] = load4(p.V + (size_t)(i < 4 ? t0[i & 3] : t1[i & 3]) * p.C + n0, left);
-    transpose84(rows, w);
-    const size_t slot = (size_t)b * p.rec.nrc + chunk;
-    const uint16_t* H = p.rec.by_rank + slot * 2 * LO_TM * RP + c * LO_TM + 8 * q;
-    const float f = p.rec.scale[slot];
+    for (int i = 0; i < 8; ++i) at[i] = 32 * (st & 1) + 8 * q + i;
+    plan.get(tb + (st >> 1), at, token);
+  };
+  auto load = [&](Step& o, int st) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o.rows[i] = ld4<WHOLE>(p.V + (size_t)token[i] * p.C + n0, left);
+    const size_t slot = (size_t)(tb + (st >> 1)) * p.rec.nrc + chunk;
+    const uint16_t* H =
+        p.rec.by_rank + slot * 2 * LO_TM * RP + c * LO_TM + 32 * (st & 1) + 8 * q;
 #pragma unroll
     for (int k = 0; k < RT; ++k) {
-      const u16x8 hi = *(const u16x8*)(H + 16 * k * LO_TM);
-      const u16x8 lo = *(const u16x8*)(H + LO_TM * RP + 16 * k * LO_TM);
+      o.hi[k] = *(const u16x8*)(H + 16 * k * LO_TM);
+      o.lo[k] = *(const u16x8*)(H + LO_TM * RP + 16 * k * LO_TM);
+    }
+    o.f = p.rec.scale[slot];
+  };
+  auto multiply = [&](const Step& o) {
+    u16x8 w[4];
+    transpose84(o.rows, w);
+#pragma unroll
+    for (int k = 0; k < RT; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        sum[k][j] += f * mfma<T>(hi, w[j], mfma<T>(lo, w[j], f32x4{0, 0, 0, 0}));
+        sum[k][j] += o.f * mfma<T>(o.hi[k], w[j], mfma<T>(o.lo[k], w[j], f32x4{0, 0, 0, 0}));
+  };
+  Step even, odd;
+  int st = split * per + wave;
+  if (st < s_end) {
+    const int last = s_end - 1;
+    find(st);
+    load(even, st);
+    find(min(st + 4, last));
+    while (true) {
+      load(odd, min(st + 4, last));
+      find(min(st + 8, last));
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(even);
+      if ((st += 4) >= s_end) break;
+      load(even, min(st + 4, last));
+      find(min(st + 8, last));
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(odd);
+      if ((st += 4) >= s_end) break;
     }
   }
-  if (p.ks > 1) {
-    const int slot = (e * p.rec.nrc + chunk) * mm_cdiv(p.C, LO_COLS) + blockIdx.x;
-    const __amdgpu_buffer_rsrc_t prs = mm_rsrc(p.part + (size_t)slot * p.ks * (LO_COLS * RP));
-    auto at = [&](int z, int k, int j) {
-      return 16u * (uint32_t)(((z * RT + k) * 4 + j) * LO_NT + threadIdx.x);
-    };
+  // lds[wave][k, j][lane]; wave w then owns columns j = w of every rank tile.
+  uint32_t* s_last = (uint32_t*)(lds + 4 * RT * 4 * 64);
 #pragma unroll
-    for (int k = 0; k < RT; ++k)
+  for (int k = 0; k < RT; ++k)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) store_agent_x4(prs, at(split, k, j), sum[k][j]);
-    if (!last_of(p.counters + slot, p.ks, &s_last)) return;
-#pragma unroll
-    for (int k = 0; k < RT; ++k)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        sum[k][j] = f32x4{0, 0, 0, 0};
-        for (int z0 = 0; z0 < p.ks; z0 += 4) {
-          f32x4 ld[4];
-#pragma unroll
-          for (int z = 0; z < 4; ++z) ld[z] = load_agent_x4(prs, at(min(z0 + z, p.ks - 1), k, j));
-#pragma unroll
-          for (int z = 0; z < 4; ++z)
-            if (z0 + z < p.ks) sum[k][j] += ld[z];
-        }
-      }
-  }
-  uint16_t* G = p.G + (size_t)e * r * p.C;
+    for (int j = 0; j < 4; ++j) lds[((wave * RT + k) * 4 + j) * 64 + lane] = sum[k][j];
+  __syncthreads();
+  f32x4 own[RT];
 #pragma unroll
   for (int k = 0; k < RT; ++k) {
-    const int rank = chunk * RP + 16 * k + 4 * q;
-    if constexpr (CR) {
+    own[k] = lds[(k * 4 + wave) * 64 + lane];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        u16x4 o;
+    for (int w = 1; w < 4; ++w) own[k] += lds[((w * RT + k) * 4 + wave) * 64 + lane];
+  }
+  if (p.ks > 1) {
+    const int slot = (e * p.rec.nrc + chunk) * mm_cdiv(p.C, LO_WG_COLS) + colblock;
+    const __amdgpu_buffer_rsrc_t prs = mm_rsrc(p.part + (size_t)slot * p.ks * (LO_WG_COLS * RP));
+    auto at = [&](int z, int k) { return 16u * (uint32_t)((z * RT + k) * LO_NT + threadIdx.x); };
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = from_f32<T>(sum[k][j][i]);
-        if (j < left) store4(G + (size_t)(n0 + j) * r + rank, o, r - rank);
-      }
-    } else {
+    for (int k = 0; k < RT; ++k) store_agent_x4(prs, at(split, k), own[k]);
+    if (!last_of(p.counters + slot, p.ks, s_last)) return;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        u16x4 o;
+    for (int k = 0; k < RT; ++k) own[k] = f32x4{0, 0, 0, 0};
+    for (int z0 = 0; z0 < p.ks; z0 += 8) {
+      f32x4 ld[8][RT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = from_f32<T>(sum[k][j][i]);
-        if (rank + i < r) store4(G + (size_t)(rank + i) * p.C + n0, o, left);
-      }
+      for (int z = 0; z < 8; ++z)
+#pragma unroll
+        for (int k = 0; k < RT; ++k) ld[z][k] = load_agent_x4(prs, at(min(z0 + z, p.ks - 1), k));
+#pragma unroll
+      for (int z = 0; z < 8; ++z)
+        if (z0 + z < p.ks)
+#pragma unroll
+          for (int k = 0; k < RT; ++k) own[k] += ld[z][k];
+    }
+  } else {
+    __syncthreads();
+  }
+  // Wave w holds column 4c + w, ranks 4q + i.  dB has the ranks of a column side by side;
+  // dA, columns side by side, goes through LDS once more.
+  uint16_t* G = p.G + (size_t)e * r * p.C;
+  if constexpr (CR) {
+#pragma unroll
+    for (int k = 0; k < RT; ++k) {
+      const int rank = chunk * RP + 16 * k + 4 * q;
+      u16x4 o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = from_f32<T>(own[k][i]);
+      if (wave < left)
+        store4(G + (size_t)(n0 + wave) * r + rank, o, r - rank);
+    }
+  } else {
+    float* tr = (float*)lds;   // [rank][64 columns]
+#pragma unroll
+    for (int k = 0; k < RT; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        tr[(16 * k + 4 * q + i) * LO_WG_COLS + 4 * c + wave] = own[k][i];
+    __syncthreads();
+    for (int it = threadIdx.x; it < RP * LO_WG_COLS / 4; it += LO_NT) {
+      const int rank = it / (LO_WG_COLS / 4), col = 4 * (it % (LO_WG_COLS / 4));
+      const f32x4 v = *(const f32x4*)(tr + rank * LO_WG_COLS + col);
+      const int n = colblock * LO_WG_COLS + col;
+      u16x4 o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = from_f32<T>(v[j]);
+      if (chunk * RP + rank < r)
+        st4<WHOLE>(G + (size_t)(chunk * RP + rank) * p.C + n, o, p.C - n);
     }
   }
 }
 
-template <int T, int RT>
+// The backward pass behind k_down: dA's blocks, dB's, then dx's.  They do not depend on one
+// another, and one launch lets them fill one another's gaps.
+template <int T, int RT, int BT>
 __global__ void __launch_bounds__(LO_NT)
-k_wgrad(GradProblem pa, GradProblem pb, Groups gs, int r) {
-  const int nrc = pa.rec.nrc, za = nrc * pa.ks;
-  const int z = blockIdx.z;
-  if (z < za) wgrad_tile<T, false, RT>(pa, gs, r, z / pa.ks, z % pa.ks);
-  else wgrad_tile<T, true, RT>(pb, gs, r, (z - za) / pb.ks, (z - za) % pb.ks);
+k_back(GradProblem pa, GradProblem pb, UpProblem pu, Plan plan, int r, int na, int nb) {
+  __shared__ __attribute__((aligned(16))) f32x4 lds[4 * RT * 4 * 64 + 1];
+  const int nrc = pa.rec.nrc;
+  int b = blockIdx.x;
+  if (b < na + nb) {
+    const GradProblem& p = b < na ? pa : pb;
+    const int cols = mm_cdiv(p.C, LO_WG_COLS), first = b < na ? 0 : na;
+    b -= first;
+    const int cb = b % cols, e = b / cols % plan.L, z = b / cols / plan.L;
+    const bool whole = (cb + 1) * LO_WG_COLS <= p.C;
+#define MM_WGRAD(CR, P)                                                                     \
+  if (whole) wgrad_tile<T, CR, RT, true>(P, plan, r, cb, e, z / P.ks, z % P.ks, lds);        \
+  else wgrad_tile<T, CR, RT, false>(P, plan, r, cb, e, z / P.ks, z % P.ks, lds)
+    if (first == 0 && (int)blockIdx.x < na) {
+      MM_WGRAD(false, pa);
+    } else {
+      MM_WGRAD(true, pb);
+    }
+#undef MM_WGRAD
+    return;
+  }
+  b -= na + nb;
+  const int cols = mm_cdiv(pu.C, LO_UP_COLS);
+  up_tile<T, false, RT, BT>(pu, plan, r, b / cols, b % cols);
 }
 
 // ---------------------------------------------------------------------------
 // Few tokens.  k_vec_down: block (token, RG ranks), the width over 256 threads; H fp32
 // [T, r].  k_vec_up: block (256 columns, token), a column per thread.
 // ---------------------------------------------------------------------------
-struct Ids {
-  const void* p;   // nullptr: adapter 0
-  int wide, L;     // int64 ids
-  MM_DEV int at(int t) const {   // the token's adapter, or -1
-    if (p == nullptr) return 0;
-    const int64_t a = wide ? ((const int64_t*)p)[t] : ((const int32_t*)p)[t];
-    return a >= 0 && a < L ? (int)a : -1;
-  }
-};
-
 template <int T, int RG>
 __global__ void __launch_bounds__(LO_NT)
 k_vec_down(const uint16_t* __restrict__ X, const uint16_t* __restrict__ A, Ids ids,
@@ -621,69 +926,74 @@ k_vec_up(const float* __restrict__ H, const uint16_t* __restrict__ B, Ids ids,
 // Host side
 // ---------------------------------------------------------------------------
 constexpr int LO_VEC_TOKENS = 64;   // up to here k_vec_*
-// Sums are split over blocks while a launch has fewer than these: two a CU.  A split
-// launch therefore has fewer arrival counters than this in use per problem.
+// No sum of a launch with this many blocks per problem is split: a split launch therefore has
+// fewer arrival counters than this in use per problem.
 constexpr int LO_SPLIT_BELOW = 512;
 
 int rank_tiles(int r) { return r <= 16 ? 1 : (r <= 32 ? 2 : 4); }
 
 struct LoraPlan {
-  int rt, rp, nrc, tiles;          // tiles: upper bound of the adapters' tiles
-  size_t sort, rec[2], part, total;
+  int rt, rp, nrc;
+  int tiles;                       // upper bound of the adapters' tiles
+  int all;                         // with those of the tokens without one
+  int kx, ky;                      // splits of k_down over K and (backward) N
+  size_t tokens, first, rec[2], part, total;   // byte offsets; the tile table comes first
 };
 
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-int down_split(int tiles, int nrc, int C) {
+// A k_down block costs about 8 us besides its sums (launch, lists, the hand-off), so the width
+// is split only until all `blocks` of the launch fill the CUs once.  us, splits 1 / 2 / 4 / 8 /
+// 16: forward of 1111 tokens, K = 14336, rank 64 123 / 78 / 54 / 44 / 52; 4096, 14336, 16 85 /
+// 58 / 45 / 50 / 59; backward of 4096, K = 4096, N = 14336 126 / 104 / 101 / 107 / 119; 8192
+// tokens, 4096, 4096 101 / 106 / 110 / 127 / 147.
+int down_split(int blocks, int C) {
   const int pairs = mm_cdiv(C, 64);
   int ks = 1;
-  while (tiles * nrc * ks < LO_SPLIT_BELOW && pairs / (2 * ks) >= 8) ks *= 2;
+  while (blocks * ks * 2 <= 288 && pairs / (2 * ks) >= LO_DW) ks *= 2;
   return ks;
 }
+// Splits of an adapter's tokens: while a wave has more than 16 steps of 32 on average.  us,
+// splits 1 / 2 / 4: backward of 4096 tokens 113 / 104 / 107, 2048 of 2 adapters 81 / 90 / 100.
 int wgrad_split(int T, int L, int nrc, int C) {
-  const long blocks = (long)mm_cdiv(C, LO_COLS) * L * nrc;
-  const int most = std::max(1, mm_cdiv(T, LO_TM) / 4);
+  const long blocks = (long)mm_cdiv(C, LO_WG_COLS) * L * nrc;
   int ks = 1;
-  while (blocks * ks < LO_SPLIT_BELOW && ks * 2 <= most && ks < 32) ks *= 2;
+  while (blocks * ks < LO_SPLIT_BELOW && T / 32 / L / (4 * ks) > 16) ks *= 2;
   return ks;
 }
 
 size_t record_bytes(const LoraPlan& p) {
   const size_t h = (size_t)p.tiles * p.nrc * 2 * LO_TM * p.rp * 2;
-  return 2 * align256(h) + align256((size_t)p.tiles * p.nrc * 4) +
-         align256((size_t)p.tiles * LO_TM * 4);
+  return 2 * align256(h) + align256((size_t)p.tiles * p.nrc * 4);
 }
 Records record_at(const LoraPlan& p, char* at) {
   const size_t h = align256((size_t)p.tiles * p.nrc * 2 * LO_TM * p.rp * 2);
-  Records r{};
-  r.by_token = (uint16_t*)at;
-  r.by_rank = (uint16_t*)(at + h);
-  r.scale = (float*)(at + 2 * h);
-  r.tokens = (int*)(at + 2 * h + align256((size_t)p.tiles * p.nrc * 4));
-  r.rp = p.rp;
-  r.nrc = p.nrc;
-  return r;
+  return Records{(uint16_t*)at, (uint16_t*)(at + h), (float*)(at + 2 * h), p.rp, p.nrc};
 }
 
-// Workspace: counters, the sort's arrays, the records of both problems, partial sums (of
-// k_down and then of k_wgrad, one after the other in the same memory).
+// Workspace: counters, the plan, the records of both problems, partial sums (of k_down and
+// then of wgrad, one after the other in the same memory).
 LoraPlan plan_lora(int T, int K, int N, int r, int L, bool backward) {
   LoraPlan p{};
   p.rt = rank_tiles(r);
   p.rp = 16 * p.rt;
   p.nrc = mm_cdiv(r, p.rp);
   p.tiles = T / LO_TM + std::min(L, T);
-  p.sort = LO_COUNTER_BYTES;
-  p.rec[0] = p.sort + align256(((size_t)L + 1 + 2 * (size_t)T) * 4);
+  p.all = T / LO_TM + std::min(L + 1, T);
+  p.tokens = LO_COUNTER_BYTES + align256((size_t)p.all * sizeof(TileInfo));
+  p.first = p.tokens + align256((size_t)p.all * LO_TM * 4);
+  p.rec[0] = p.first + align256(((size_t)L + 2) * 4);
   p.rec[1] = p.rec[0] + record_bytes(p);
   p.part = p.rec[1] + (backward ? record_bytes(p) : 0);
   const size_t tile = (size_t)p.tiles * p.nrc * LO_TM * p.rp * 4;
-  size_t part = tile * down_split(p.tiles, p.nrc, K);
+  p.kx = down_split(p.tiles * p.nrc * (backward ? 2 : 1), K);
+  p.ky = down_split(p.tiles * p.nrc * 2, N);
+  size_t part = tile * p.kx;
   if (backward) {
-    part += tile * down_split(p.tiles, p.nrc, N);
-    const size_t col = (size_t)L * p.nrc * LO_COLS * p.rp * 4;
-    part = std::max(part, col * (mm_cdiv(K, LO_COLS) * (size_t)wgrad_split(T, L, p.nrc, K) +
-                                 mm_cdiv(N, LO_COLS) * (size_t)wgrad_split(T, L, p.nrc, N)));
+    part += tile * p.ky;
+    const size_t col = (size_t)L * p.nrc * LO_WG_COLS * p.rp * 4;
+    part = std::max(part, col * (mm_cdiv(K, LO_WG_COLS) * (size_t)wgrad_split(T, L, p.nrc, K) +
+                                 mm_cdiv(N, LO_WG_COLS) * (size_t)wgrad_split(T, L, p.nrc, N)));
   }
   p.total = p.part + align256(part);
   return p;
@@ -697,25 +1007,25 @@ int check_common(const char* who, int type, int T, int K, int N, int r, int L, c
   MM_CHECK_ARG(ids == nullptr || ids64 == 0 || ids64 == 1, "%s: ids64=%d must be 0 or 1", who,
                ids64);
   MM_CHECK_ARG(ids != nullptr || L == 1, "%s: %d adapters need ids", who, L);
-  MM_CHECK_ARG(L <= 1024, "%s: at most 1024 adapters, got %d", who, L);
-  MM_CHECK_ARG((long)mm_cdiv(N, LO_COLS) <= 65535 && (long)mm_cdiv(K, LO_COLS) <= 65535,
-               "%s: K=%d, N=%d exceed %ld columns", who, K, N, 65535L * LO_COLS);
+  MM_CHECK_ARG(L <= LO_MAX_ADAPTERS, "%s: at most %d adapters, got %d", who, LO_MAX_ADAPTERS, L);
+  MM_CHECK_ARG(T <= (1 << 24) && K <= (1 << 24) && N <= (1 << 24) && r <= (1 << 12),
+               "%s: T=%d, K=%d, N=%d or rank=%d is too large", who, T, K, N, r);
   return 0;
 }
 
 // Sorts the tokens by adapter (none needed for a single adapter without ids).
-int make_groups(const char* who, const LoraPlan& p, const void* ids, int ids64, int T, int L,
-                void* ws, void* stream, Groups* gs) {
-  *gs = Groups{nullptr, nullptr, T, L};
+int make_plan(const char* who, const LoraPlan& p, const void* ids, int ids64, int T, int L,
+              void* ws, hipStream_t st, Plan* plan) {
+  *plan = Plan{nullptr, nullptr, nullptr, T, L};
   if (ids == nullptr) return 0;
-  int32_t* off = (int32_t*)((char*)ws + p.sort);
-  int32_t* order = off + L + 1;
-  int32_t* inverse = order + T;
-  const int rc = ids64 ? mm_moe_sort_i64((const int64_t*)ids, T, 1, L, off, order, inverse, stream)
-                       : mm_moe_sort((const int32_t*)ids, T, 1, L, off, order, inverse, stream);
-  gs->offsets = off;
-  gs->order = order;
-  return rc;
+  TileInfo* tiles = (TileInfo*)((char*)ws + LO_COUNTER_BYTES);
+  int* tokens = (int*)((char*)ws + p.tokens);
+  int* first = (int*)((char*)ws + p.first);
+  hipLaunchKernelGGL(k_plan, dim3(1), dim3(PL_NT), 0, st, Ids{ids, ids64, L}, T, p.all, tiles,
+                     tokens, first);
+  MM_CHECK_LAUNCH(who);
+  *plan = Plan{tiles, tokens, first, T, L};
+  return 0;
 }
 
 #define MM_LORA_RT(F, ...)                    \
@@ -771,21 +1081,21 @@ extern "C" int mm_lora_add(const uint16_t* x, int type, const uint16_t* base, in
     return 0;
   }
   const LoraPlan p = plan_lora(T, K, N, r, L, false);
-  Groups gs;
-  if (const int rc = make_groups(who, p, ids, ids64, T, L, ws, stream, &gs)) return rc;
+  Plan plan;
+  if (const int rc = make_plan(who, p, ids, ids64, T, L, ws, st, &plan)) return rc;
   const Records rec = record_at(p, (char*)ws + p.rec[0]);
-  const int ks = down_split(p.tiles, p.nrc, K);
+  const int ks = p.kx;
   const DownProblem d{x, A, K, ks, mm_cdiv(mm_cdiv(K, 64), ks), rec, (float*)((char*)ws + p.part),
                       (uint32_t*)ws, 1, 0};
 #define MM_DOWN(RTV, TV)                                                                       \
-  hipLaunchKernelGGL((k_down<TV, RTV>), dim3(p.tiles, ks, p.nrc), dim3(LO_NT), 0, st, d, d, gs, \
-                     sc, r)
+  hipLaunchKernelGGL((k_down<TV, RTV>), dim3(p.tiles, ks, p.nrc), dim3(64 * LO_DW), 0, st, d, d, \
+                     plan, sc, r)
   if (type == 1) { MM_LORA_RT(MM_DOWN, 1) } else { MM_LORA_RT(MM_DOWN, 2) }
   MM_CHECK_LAUNCH(who);
-  // group L (tokens without an adapter) has tiles of its own
-  const dim3 grid(p.tiles + (ids != nullptr ? mm_cdiv(T, LO_TM) : 0), mm_cdiv(N, LO_COLS));
-#define MM_UP(RTV, TV, BV)                                                                     \
-  hipLaunchKernelGGL((k_up<TV, true, RTV, BV>), grid, dim3(LO_NT), 0, st, B, base, out, N, r, gs, rec)
+  const UpProblem u{B, base, out, N, rec};
+  const dim3 grid(p.all, mm_cdiv(N, LO_UP_COLS));
+#define MM_UP(RTV, TV, BV) \
+  hipLaunchKernelGGL((k_up<TV, RTV, BV>), grid, dim3(LO_NT), 0, st, u, plan, r)
   if (type == 1) { MM_LORA_RT(MM_UP, 1, 1) }
   else if (base_type == 1) { MM_LORA_RT(MM_UP, 2, 1) }
   else { MM_LORA_RT(MM_UP, 2, 2) }
@@ -809,43 +1119,41 @@ extern "C" int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type,
   hipStream_t st = (hipStream_t)stream;
   const Scaling sc{scaling, scale};
   const LoraPlan p = plan_lora(T, K, N, r, L, true);
-  Groups gs;
-  if (const int rc = make_groups(who, p, ids, ids64, T, L, ws, stream, &gs)) return rc;
+  Plan plan;
+  if (const int rc = make_plan(who, p, ids, ids64, T, L, ws, st, &plan)) return rc;
   const Records rx = record_at(p, (char*)ws + p.rec[0]), ry = record_at(p, (char*)ws + p.rec[1]);
   float* part = (float*)((char*)ws + p.part);
   uint32_t* counters = (uint32_t*)ws;
-  const int kx = down_split(p.tiles, p.nrc, K), ky = down_split(p.tiles, p.nrc, N);
+  const int kx = p.kx, ky = p.ky;
   const size_t tile = (size_t)p.tiles * p.nrc * LO_TM * p.rp;
   const DownProblem px{x, A, K, kx, mm_cdiv(mm_cdiv(K, 64), kx), rx, part, counters, 0, 1};
   const DownProblem py{dy, B, N, ky, mm_cdiv(mm_cdiv(N, 64), ky), ry, part + tile * kx,
                        counters + LO_SPLIT_BELOW, 1, 1};
 #define MM_DOWN(RTV, TV)                                                                       \
-  hipLaunchKernelGGL((k_down<TV, RTV>), dim3(p.tiles, std::max(kx, ky), 2 * p.nrc), dim3(LO_NT), \
-                     0, st, px, py, gs, sc, r)
+  hipLaunchKernelGGL((k_down<TV, RTV>), dim3(p.tiles, std::max(kx, ky), 2 * p.nrc),              \
+                     dim3(64 * LO_DW), 0, st, px, py, plan, sc, r)
   if (type == 1) { MM_LORA_RT(MM_DOWN, 1) } else { MM_LORA_RT(MM_DOWN, 2) }
 #undef MM_DOWN
   MM_CHECK_LAUNCH(who);
-  const int ca = mm_cdiv(K, LO_COLS), cb = mm_cdiv(N, LO_COLS);
+  const int ca = mm_cdiv(K, LO_WG_COLS), cb = mm_cdiv(N, LO_WG_COLS);
   const int ga = wgrad_split(T, L, p.nrc, K), gb = wgrad_split(T, L, p.nrc, N);
   const GradProblem pa{x, dA, K, ga, ry, part, counters};
-  const GradProblem pb{dy, dB, N, gb, rx, part + (size_t)L * p.nrc * ca * ga * LO_COLS * p.rp,
+  const GradProblem pb{dy, dB, N, gb, rx, part + (size_t)L * p.nrc * ca * ga * LO_WG_COLS * p.rp,
                        counters + LO_SPLIT_BELOW};
-#define MM_WGRAD(RTV, TV)                                                                      \
-  hipLaunchKernelGGL((k_wgrad<TV, RTV>), dim3(std::max(ca, cb), L, p.nrc * (ga + gb)),           \
-                     dim3(LO_NT), 0, st, pa, pb, gs, r)
-  if (type == 1) { MM_LORA_RT(MM_WGRAD, 1) } else { MM_LORA_RT(MM_WGRAD, 2) }
-#undef MM_WGRAD
-  MM_CHECK_LAUNCH(who);
-  const dim3 grid(p.tiles + (ids != nullptr ? mm_cdiv(T, LO_TM) : 0), ca);
-#define MM_UP(RTV, TV, BV)                                                                     \
-  hipLaunchKernelGGL((k_up<TV, false, RTV, BV>), grid, dim3(LO_NT), 0, st, A, dx_base, dx, K, r, \
-                     gs, ry)
+  const UpProblem pu{A, dx_base, dx, K, ry};
+  const long na = (long)ca * L * p.nrc * ga, nb = (long)cb * L * p.nrc * gb;
+  const long nu = (long)p.all * mm_cdiv(K, LO_UP_COLS);
+  MM_CHECK_ARG(na + nb + nu < 0x7fffffffL, "%s: K=%d, N=%d with %d adapters is too large", who, K,
+               N, L);
+#define MM_BACK(RTV, TV, BV)                                                                   \
+  hipLaunchKernelGGL((k_back<TV, RTV, BV>), dim3((unsigned)(na + nb + nu)), dim3(LO_NT), 0, st, pa, \
+                     pb, pu, plan, r, (int)na, (int)nb)
   if (dx_base != nullptr) {
-    if (type == 1) { MM_LORA_RT(MM_UP, 1, 1) } else { MM_LORA_RT(MM_UP, 2, 2) }
+    if (type == 1) { MM_LORA_RT(MM_BACK, 1, 1) } else { MM_LORA_RT(MM_BACK, 2, 2) }
   } else {
-    if (type == 1) { MM_LORA_RT(MM_UP, 1, 0) } else { MM_LORA_RT(MM_UP, 2, 0) }
+    if (type == 1) { MM_LORA_RT(MM_BACK, 1, 0) } else { MM_LORA_RT(MM_BACK, 2, 0) }
   }
-#undef MM_UP
+#undef MM_BACK
   MM_CHECK_LAUNCH(who);
   return 0;
 }
