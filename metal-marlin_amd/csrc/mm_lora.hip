@@ -18,7 +18,6 @@
 // All sums are fp32 and in a fixed order.  All of them stream activations that are read
 // once (x, dy) or read and written once (out): HBM bounds them, the factors stay in L2.
 #include <algorithm>
-#include <type_traits>
 
 #include "mm_common.h"
 #include "mmfp4.h"
@@ -284,12 +283,9 @@ k_plan(Ids ids, int T, int max_tiles, TileInfo* __restrict__ tiles, int* __restr
     }
   }
   __syncthreads();
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int g = 2 * tid + k;
-    if (g >= G) continue;
-    int* list = tokens + LO_TM * tile0[g];
-    for (int i = n[k]; i < LO_TM * mm_cdiv(n[k], LO_TM); ++i) list[i] = last[g];
+  for (int g = wave; g < G; g += PL_NW) {
+    const int i = rows_of[g] + lane;
+    if (i < LO_TM * mm_cdiv(rows_of[g], LO_TM)) tokens[LO_TM * tile0[g] + i] = last[g];
   }
 }
 
@@ -332,12 +328,114 @@ struct DownProblem {
   int by_token, by_rank;   // which records are wanted
 };
 
+// LDS of a wave: its pair's activations, 64 rows of 128 bytes, 16-byte piece (row, p) at
+// row * 8 + (p ^ ((row >> 1) & 7)); then the factors, 16 * RT rows laid out the same, or (CR) 64
+// rows of 16 * RT ranks and 16 bytes.  A load of a whole row's 128 bytes by 8 lanes is one
+// request; straight into the operands' layout, 64 bytes a row, it is two, and those are what a
+// CU has a limited number of in flight (117 MB of dy 33 us so, 3.5 TB/s).
+template <int RT>
+constexpr int down_lds_wave() { return LO_TM * 128 + 64 * (32 * RT + 16); }
+
 template <int T, bool CR, int RT, int NR>
 MM_DEV void down_sum(const DownProblem& p, const Plan& plan, int b, int e, int r, int r0,
-                     f32x4 (&acc)[4][RT]) {
+                     char* lds, f32x4 (&acc)[4][RT]) {
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint16_t* W = p.W + (size_t)e * r * p.C;
+  const int beg = blockIdx.y * p.per, end = min(p.C / 64, beg + p.per);   // whole pairs
+  constexpr int WROW = 32 * RT + 16;   // CR: bytes of a factor row in LDS
+  char* xs = lds + wave * down_lds_wave<RT>();
+  char* ws = xs + LO_TM * 128;
+  if (!CR || r % 8 == 0) {
+    constexpr int NX = 2 * NR, NW = 2 * RT;   // load instructions of a pair
+    const uint16_t* v[NX];
+    int at[NX], tok[NX];
+#pragma unroll
+    for (int i = 0; i < NX; ++i) at[i] = 8 * i + (lane >> 3);
+    plan.get(b, at, tok);
+#pragma unroll
+    for (int i = 0; i < NX; ++i) v[i] = p.V + (size_t)tok[i] * p.C + 8 * (lane & 7);
+    uint32_t woff[NW], wlds[NW];   // element offset of the lane's pieces at k = 0, place in LDS
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      if constexpr (!CR) {
+        const int row = 8 * i + (lane >> 3);
+        woff[i] = (uint32_t)min(r0 + row, r - 1) * p.C + 8 * (lane & 7);
+        wlds[i] = row * 128 + ((lane & 7) ^ ((row >> 1) & 7)) * 16;
+      } else {
+        const int n = (64 * i + lane) / (2 * RT), piece = (64 * i + lane) % (2 * RT);
+        woff[i] = (uint32_t)n * r + min(r0 + 8 * piece, r - 8);
+        wlds[i] = n * WROW + piece * 16;
+      }
+    }
+    struct Stage {
+      u16x8 x[NX], w[NW];
+    };
+    auto load = [&](Stage& o, int pr) {
+#pragma unroll
+      for (int i = 0; i < NX; ++i) o.x[i] = *(const u16x8_any*)(v[i] + 64 * pr);
+      const uint16_t* w = W + (size_t)64 * pr * (CR ? r : 1);
+#pragma unroll
+      for (int i = 0; i < NW; ++i) o.w[i] = *(const u16x8_any*)(w + woff[i]);
+    };
+    // Through the wave's own LDS (no barrier) into the operands' order.  D rows: ranks
+    // 4q + i, columns: tokens c.
+    auto park = [&](const Stage& o) {
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const int row = 8 * i + (lane >> 3);
+        *(u16x8*)(xs + row * 128 + ((lane & 7) ^ ((row >> 1) & 7)) * 16) = o.x[i];
+      }
+#pragma unroll
+      for (int i = 0; i < NW; ++i) *(u16x8*)(ws + wlds[i]) = o.w[i];
+    };
+    auto multiply = [&]() {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        u16x8 x[NR], w[RT];
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+          x[i] = *(const u16x8*)(xs + (16 * i + c) * 128 + ((4 * s + q) ^ ((c >> 1) & 7)) * 16);
+#pragma unroll
+        for (int k = 0; k < RT; ++k) {
+          if constexpr (!CR) {
+            w[k] = *(const u16x8*)(ws + (16 * k + c) * 128 + ((4 * s + q) ^ ((c >> 1) & 7)) * 16);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              w[k][i] = *(const uint16_t*)(ws + (32 * s + 8 * q + i) * WROW + (16 * k + c) * 2);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+          for (int k = 0; k < RT; ++k) acc[i][k] = mfma<T>(w[k], x[i], acc[i][k]);
+      }
+    };
+    // A pair (with up to 32 ranks two) is on its way while one is multiplied; behind the last
+    // it is the last again.
+    constexpr int SETS = RT == 4 ? 1 : 2;
+    const int np = beg + wave < end ? (end - beg - wave + LO_DW - 1) / LO_DW : 0;
+    auto pair = [&](int n) { return beg + wave + LO_DW * min(n, np - 1); };
+    if (np > 0) {
+      Stage set[SETS];
+#pragma unroll
+      for (int d = 0; d < SETS; ++d) load(set[d], pair(d));
+      for (int n = 0; n < np; n += SETS) {
+#pragma unroll
+        for (int d = 0; d < SETS; ++d) {
+          if (n + d >= np) break;
+          park(set[d]);
+          __builtin_amdgcn_sched_barrier(0);   // or the loads sink to where they are used
+          load(set[d], pair(n + d + SETS));
+          __builtin_amdgcn_sched_barrier(0);
+          multiply();
+        }
+      }
+    }
+  }
+  // What is left of a width that is no multiple of 64; all of it where the rows of B are not
+  // made of 16-byte pieces: straight into the operands.
   const uint16_t* v[NR];
   int at[NR], tok[NR];
 #pragma unroll
@@ -345,77 +443,11 @@ MM_DEV void down_sum(const DownProblem& p, const Plan& plan, int b, int e, int r
   plan.get(b, at, tok);
 #pragma unroll
   for (int i = 0; i < NR; ++i) v[i] = p.V + (size_t)tok[i] * p.C;
-  // A stage: SS steps of 32 (a pair, or with 64 ranks half of one): its operands, and its
-  // products.  D rows: ranks 4q + i, columns: tokens c.  CR's factors stay as they are loaded
-  // until they are used: packing them waits for them.
-  constexpr int SS = RT == 4 ? 1 : 2, STAGES = 2 / SS;   // steps a stage, stages a pair
-  struct Stage {
-    u16x8 x[SS][NR];
-    std::conditional_t<CR, uint32_t[8], u16x8> w[SS][RT];
-  };
-  auto load = [&](Stage& o, int u) {
-#pragma unroll
-    for (int s = 0; s < SS; ++s) {
-      const int k0 = 32 * (SS * u + s) + 8 * q;
-#pragma unroll
-      for (int i = 0; i < NR; ++i) o.x[s][i] = *(const u16x8_any*)(v[i] + k0);
-#pragma unroll
-      for (int k = 0; k < RT; ++k) {
-        const int rank = min(r0 + 16 * k + c, r - 1);
-        if constexpr (!CR) {
-          o.w[s][k] = *(const u16x8_any*)(W + (size_t)rank * p.C + k0);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o.w[s][k][i] = W[(size_t)(k0 + i) * r + rank];
-        }
-      }
-    }
-  };
-  auto multiply = [&](const Stage& o) {
-#pragma unroll
-    for (int s = 0; s < SS; ++s)
-#pragma unroll
-      for (int k = 0; k < RT; ++k) {
-        u16x8 w;
-        if constexpr (CR) {
-          u32x4 pk;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) pk[i] = o.w[s][k][2 * i] | o.w[s][k][2 * i + 1] << 16;
-          w = __builtin_bit_cast(u16x8, pk);
-        } else {
-          w = o.w[s][k];
-        }
-#pragma unroll
-        for (int i = 0; i < NR; ++i) acc[i][k] = mfma<T>(w, o.x[s][i], acc[i][k]);
-      }
-  };
-  const int beg = blockIdx.y * p.per, end = min(p.C / 64, beg + p.per);   // whole pairs
-  // The next stage is on its way while one is multiplied (the last again at the end).
-  // Stage n of a wave: stage n % STAGES of pair beg + wave + LO_DW * (n / STAGES).
-  const int np = beg + wave < end ? (end - beg - wave + LO_DW - 1) / LO_DW : 0;
-  const int ns = np * STAGES;
-  auto at_stage = [&](int n) {
-    n = min(n, ns - 1);
-    return (beg + wave + LO_DW * (n / STAGES)) * STAGES + n % STAGES;
-  };
-  if (ns > 0) {
-    Stage even, odd;
-    load(even, at_stage(0));
-    for (int n = 0; n < ns; n += 2) {
-      load(odd, at_stage(n + 1));
-      __builtin_amdgcn_sched_barrier(0);   // or the loads sink to where they are used
-      multiply(even);
-      if (n + 1 >= ns) break;
-      load(even, at_stage(n + 2));
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(odd);
-    }
-  }
-  // What is left of a width that is no multiple of 64.
-  const int rest = p.C / 64;
-  if (64 * rest < p.C && rest >= beg && rest < beg + p.per && wave == (rest - beg) % LO_DW) {
+  const int direct_end = min(mm_cdiv(p.C, 64), beg + p.per);
+  for (int pr = beg + wave; pr < direct_end; pr += LO_DW) {
+    if (pr < p.C / 64 && (!CR || r % 8 == 0)) continue;
     for (int s = 0; s < 2; ++s) {
-      const int k0 = 64 * rest + 32 * s + 8 * q, left = p.C - k0;
+      const int k0 = 64 * pr + 32 * s + 8 * q, left = p.C - k0;
 #pragma unroll
       for (int k = 0; k < RT; ++k) {
         const int rank = min(r0 + 16 * k + c, r - 1);
@@ -448,9 +480,10 @@ MM_DEV void down_tile(const DownProblem& p, const Plan& plan, const Scaling& sca
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int k = 0; k < RT; ++k) acc[i][k] = f32x4{0, 0, 0, 0};
-  if (t.rows > 32) down_sum<T, CR, RT, 4>(p, plan, b, t.e, r, r0, acc);
-  else if (t.rows > 16) down_sum<T, CR, RT, 2>(p, plan, b, t.e, r, r0, acc);
-  else down_sum<T, CR, RT, 1>(p, plan, b, t.e, r, r0, acc);
+  if (t.rows > 32) down_sum<T, CR, RT, 4>(p, plan, b, t.e, r, r0, (char*)lds, acc);
+  else if (t.rows > 16) down_sum<T, CR, RT, 2>(p, plan, b, t.e, r, r0, (char*)lds, acc);
+  else down_sum<T, CR, RT, 1>(p, plan, b, t.e, r, r0, (char*)lds, acc);
+  __syncthreads();   // every wave is done with its staging area
   // Sum over the waves, half of them at a time: lds[wave % 4][token][rank].
   uint32_t* s_last = (uint32_t*)(lds + 4 * LO_TM * RP);
   float* s_max = lds + 4 * LO_TM * RP + 4;
@@ -556,7 +589,8 @@ MM_DEV void down_tile(const DownProblem& p, const Plan& plan, const Scaling& sca
 template <int T, int RT>
 __global__ void __launch_bounds__(64 * LO_DW)
 k_down(DownProblem p0, DownProblem p1, Plan plan, Scaling scaling, int r) {
-  __shared__ __attribute__((aligned(16))) float lds[4 * LO_TM * 16 * RT + 4 + LO_DW];
+  constexpr int SUM = 4 * LO_TM * 16 * RT + 4 + LO_DW, STAGE = LO_DW * down_lds_wave<RT>() / 4;
+  __shared__ __attribute__((aligned(16))) float lds[SUM > STAGE ? SUM : STAGE];
   const int nrc = p0.rec.nrc;
   const bool second = (int)blockIdx.z >= nrc;
   if ((int)blockIdx.y >= (second ? p1.ks : p0.ks)) return;
@@ -585,27 +619,6 @@ MM_DEV void up_rows(const UpProblem& p, const Plan& plan, TileInfo t, int r, int
   const int left = C - n0;
   const Records& rec = p.rec;
   const uint16_t* W = p.W + (none ? 0 : (size_t)t.e * r * C);
-  // Factors of the first rank chunk: they serve all rows.
-  u16x8 w[RT][4];
-  auto load_w = [&](int ch) {
-#pragma unroll
-    for (int k = 0; k < RT; ++k) {
-      const int rank = ch * RP + 16 * k + 8 * (q & 1);   // the first of this lane's eight
-      if constexpr (CR) {
-        // ranks past the last: any, the record has zeros there
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w[k][j] = WHOLE ? *(const u16x8_any*)(W + (size_t)(n0 + j) * r + min(rank, r - 8))
-                          : load8(W + (size_t)min(n0 + j, C - 1) * r + rank, r - rank);
-      } else {
-        u16x4 rows[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          rows[i] = ld4<WHOLE>(W + (size_t)min(rank + i, r - 1) * C + n0, left);
-        transpose84(rows, w[k]);
-      }
-    }
-  };
   // The bases of all rows are on their way before anything else.
   constexpr int NR = LO_TM / 16;
   u16x4 bv[NR * 4];
@@ -617,42 +630,68 @@ MM_DEV void up_rows(const UpProblem& p, const Plan& plan, TileInfo t, int r, int
   for (int i = 0; i < NR * 4; ++i)
     if constexpr (BT != 0) bv[i] = ld4<WHOLE>(p.base + (size_t)token[i] * C + n0, left);
     else bv[i] = u16x4{0, 0, 0, 0};
-  if (!none) load_w(0);
+  constexpr int NI = 2;   // blocks of 16 rows at a time (all four take the registers of a wave)
+  u16x8 w[RT][4];
 #pragma unroll
-  for (int i = 0; i < NR; ++i) {   // 16 rows at a time
-    if (16 * i >= t.rows) break;
-    f32x4 sum[4];   // [column j]: tokens 4q + k
+  for (int i0 = 0; i0 < NR; i0 += NI) {
+    if (16 * i0 >= t.rows) break;
+    f32x4 sum[NI][4];     // [16 rows][column j]: tokens 4q + k
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j] = f32x4{0, 0, 0, 0};
-    if (!none) {
-      for (int ch = 0; ch < rec.nrc; ++ch) {
-        if (rec.nrc > 1) load_w(ch);
-        const size_t slot = (size_t)b * rec.nrc + ch;
-        const uint16_t* H = rec.by_token + slot * 2 * LO_TM * RP + (q >> 1) * LO_TM * RP +
-                            (16 * i + c) * RP + 8 * (q & 1);
-        f32x4 acc[4];
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[i][j] = f32x4{0, 0, 0, 0};
+    for (int ch = 0; ch < (none ? 0 : rec.nrc); ++ch) {
+      const size_t slot = (size_t)b * rec.nrc + ch;
+      const uint16_t* H = rec.by_token + slot * 2 * LO_TM * RP + (q >> 1) * LO_TM * RP +
+                          (16 * i0 + c) * RP + 8 * (q & 1);
+      const float f = rec.scale[slot];
+      u16x8 hv[NI][RT];
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int k = 0; k < RT; ++k) hv[i][k] = *(const u16x8*)(H + 16 * i * RP + 16 * k);
+      if (i0 == 0 || rec.nrc > 1) {
 #pragma unroll
         for (int k = 0; k < RT; ++k) {
-          const u16x8 hv = *(const u16x8*)(H + 16 * k);
+          const int rank = ch * RP + 16 * k + 8 * (q & 1);   // the first of this lane's eight
+          if constexpr (CR) {
+            // ranks past the last: any, the record has zeros there
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            acc[j] = mfma<T>(hv, w[k][j], k == 0 ? f32x4{0, 0, 0, 0} : acc[j]);
+            for (int j = 0; j < 4; ++j)
+              w[k][j] = WHOLE ? *(const u16x8_any*)(W + (size_t)(n0 + j) * r + min(rank, r - 8))
+                              : load8(W + (size_t)min(n0 + j, C - 1) * r + rank, r - rank);
+          } else {
+            u16x4 rows[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              rows[i] = ld4<WHOLE>(W + (size_t)min(rank + i, r - 1) * C + n0, left);
+            transpose84(rows, w[k]);
+          }
         }
-        const float f = rec.scale[slot];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum[j] += f * acc[j];
       }
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+          for (int k = 0; k < RT; ++k) acc = mfma<T>(hv[i][k], w[k][j], acc);
+          sum[i][j] += f * acc;
+        }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (16 * i + 4 * q + k >= t.rows) continue;
-      u16x4 o;
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        o[j] = from_f32<T>(BT != 0 ? to_f32<BT != 0 ? BT : T>(bv[4 * i + k][j]) + sum[j][k]
-                                   : sum[j][k]);
-      st4<WHOLE>(p.out + (size_t)token[4 * i + k] * C + n0, o, left);
-    }
+      for (int k = 0; k < 4; ++k) {
+        const int row = 4 * (i0 + i) + k;
+        if (16 * (i0 + i) + 4 * q + k >= t.rows) continue;
+        u16x4 o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          o[j] = from_f32<T>(BT != 0 ? to_f32<BT != 0 ? BT : T>(bv[row][j]) + sum[i][j][k]
+                                     : sum[i][j][k]);
+        st4<WHOLE>(p.out + (size_t)token[row] * C + n0, o, left);
+      }
   }
 }
 
@@ -936,22 +975,19 @@ struct LoraPlan {
   int rt, rp, nrc;
   int tiles;                       // upper bound of the adapters' tiles
   int all;                         // with those of the tokens without one
-  int kx, ky;                      // splits of k_down over K and (backward) N
+  int kx, ky, per;                 // splits of k_down over K and (backward) N, pairs of each
   size_t tokens, first, rec[2], part, total;   // byte offsets; the tile table comes first
 };
 
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-// A k_down block costs about 8 us besides its sums (launch, lists, the hand-off), so the width
-// is split only until all `blocks` of the launch fill the CUs once.  us, splits 1 / 2 / 4 / 8 /
-// 16: forward of 1111 tokens, K = 14336, rank 64 123 / 78 / 54 / 44 / 52; 4096, 14336, 16 85 /
-// 58 / 45 / 50 / 59; backward of 4096, K = 4096, N = 14336 126 / 104 / 101 / 107 / 119; 8192
-// tokens, 4096, 4096 101 / 106 / 110 / 127 / 147.
-int down_split(int blocks, int C) {
-  const int pairs = mm_cdiv(C, 64);
-  int ks = 1;
-  while (blocks * ks * 2 <= 288 && pairs / (2 * ks) >= LO_DW) ks *= 2;
-  return ks;
+// A k_down block costs about 8 us besides its sums (launch, lists, the hand-off) and one fits
+// a CU, so the widths of the launch are cut into equal ranges, as many as fill the CUs once,
+// of at least a pair per wave.  us, splits 1 / 2 / 4 / 8 / 16: forward of 1111 tokens, K =
+// 14336, rank 64 71 / 55 / 45 / 43 / 52; 4096, 14336, 16 68 / 52 / 43 / 48 / 57; backward of
+// 8192 tokens, 4096, 4096 96 / 101 / 108 / 122 / 142.
+int down_range(long tiles, int pairs) {
+  return std::max(LO_DW, (int)((tiles * pairs + 223) / 224));
 }
 // Splits of an adapter's tokens: while a wave has more than 16 steps of 32 on average.  us,
 // splits 1 / 2 / 4: backward of 4096 tokens 113 / 104 / 107, 2048 of 2 adapters 81 / 90 / 100.
@@ -986,8 +1022,10 @@ LoraPlan plan_lora(int T, int K, int N, int r, int L, bool backward) {
   p.rec[1] = p.rec[0] + record_bytes(p);
   p.part = p.rec[1] + (backward ? record_bytes(p) : 0);
   const size_t tile = (size_t)p.tiles * p.nrc * LO_TM * p.rp * 4;
-  p.kx = down_split(p.tiles * p.nrc * (backward ? 2 : 1), K);
-  p.ky = down_split(p.tiles * p.nrc * 2, N);
+  const int px = mm_cdiv(K, 64), py = backward ? mm_cdiv(N, 64) : 0;
+  p.per = down_range((long)p.tiles * p.nrc, px + py);
+  p.kx = mm_cdiv(px, p.per);
+  p.ky = mm_cdiv(py, p.per);
   size_t part = tile * p.kx;
   if (backward) {
     part += tile * p.ky;
@@ -1085,7 +1123,7 @@ extern "C" int mm_lora_add(const uint16_t* x, int type, const uint16_t* base, in
   if (const int rc = make_plan(who, p, ids, ids64, T, L, ws, st, &plan)) return rc;
   const Records rec = record_at(p, (char*)ws + p.rec[0]);
   const int ks = p.kx;
-  const DownProblem d{x, A, K, ks, mm_cdiv(mm_cdiv(K, 64), ks), rec, (float*)((char*)ws + p.part),
+  const DownProblem d{x, A, K, ks, p.per, rec, (float*)((char*)ws + p.part),
                       (uint32_t*)ws, 1, 0};
 #define MM_DOWN(RTV, TV)                                                                       \
   hipLaunchKernelGGL((k_down<TV, RTV>), dim3(p.tiles, ks, p.nrc), dim3(64 * LO_DW), 0, st, d, d, \
@@ -1126,8 +1164,8 @@ extern "C" int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type,
   uint32_t* counters = (uint32_t*)ws;
   const int kx = p.kx, ky = p.ky;
   const size_t tile = (size_t)p.tiles * p.nrc * LO_TM * p.rp;
-  const DownProblem px{x, A, K, kx, mm_cdiv(mm_cdiv(K, 64), kx), rx, part, counters, 0, 1};
-  const DownProblem py{dy, B, N, ky, mm_cdiv(mm_cdiv(N, 64), ky), ry, part + tile * kx,
+  const DownProblem px{x, A, K, kx, p.per, rx, part, counters, 0, 1};
+  const DownProblem py{dy, B, N, ky, p.per, ry, part + tile * kx,
                        counters + LO_SPLIT_BELOW, 1, 1};
 #define MM_DOWN(RTV, TV)                                                                       \
   hipLaunchKernelGGL((k_down<TV, RTV>), dim3(p.tiles, std::max(kx, ky), 2 * p.nrc),              \
