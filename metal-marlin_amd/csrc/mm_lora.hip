@@ -4,8 +4,8 @@
 //   dB_a = sum dy[t]^T H[t]     over the tokens t of adapter a
 // with A [L, r, K], B [L, N, r], s = scale * scaling[a] (scaling fp32 [L], or none).
 //
-// Few tokens: every token on its own, two launches of fp32 dot products (k_vec_down,
-// k_vec_up).  Otherwise the tokens are sorted by adapter and cut into tiles of 64 of one
+// Few tokens: every token on its own, one launch of fp32 dot products (k_vec) or two
+// (k_vec_down, k_vec_up).  Otherwise the tokens are sorted by adapter and cut into tiles of 64 of one
 // adapter (k_plan), and
 //   k_down   H of a tile, over the whole width: 16x16x32 MFMAs, the width split over the
 //            waves and over blocks.  The block that finishes a tile leaves a record of it:
@@ -900,7 +900,80 @@ k_back(GradProblem pa, GradProblem pb, UpProblem pu, Plan plan, int r, int na, i
 }
 
 // ---------------------------------------------------------------------------
-// Few tokens.  k_vec_down: block (token, RG ranks), the width over 256 threads; H fp32
+// Few tokens, and so few factors that every block may read its adapter's A itself: one
+// launch.  Block (512 columns, token): its waves take the ranks in pairs and leave H in LDS,
+// then a thread has a column, whose factors were on their way meanwhile.
+// ---------------------------------------------------------------------------
+constexpr int VE_NT = 512, VE_RANKS = 128;
+template <int T, int BT>
+__global__ void __launch_bounds__(VE_NT)
+k_vec(const uint16_t* __restrict__ X, const uint16_t* __restrict__ A,
+      const uint16_t* __restrict__ B, Ids ids, Scaling scaling, const uint16_t* base,
+      uint16_t* out, int K, int N, int r) {
+  __shared__ float h[VE_RANKS];
+  const int t = blockIdx.y, n = blockIdx.x * VE_NT + threadIdx.x, a = ids.at(t);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const size_t at = (size_t)t * N + min(n, N - 1);
+  float v = to_f32<BT>(base[at]);
+  if (a >= 0) {
+    const uint16_t* w = B + ((size_t)a * N + min(n, N - 1)) * r;
+    const u16x8 w0 = load8(w, r), w1 = load8(w + 8, r - 8);
+    const uint16_t* x = X + (size_t)t * K;
+    for (int r0 = 2 * wave; r0 < r; r0 += 2 * (VE_NT / 64)) {
+      const uint16_t* a0 = A + ((size_t)a * r + r0) * K;
+      const uint16_t* a1 = A + ((size_t)a * r + min(r0 + 1, r - 1)) * K;
+      float s0 = 0.0f, s1 = 0.0f;
+      auto add = [&](u16x8 xv, u16x8 p, u16x8 q) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float f = to_f32<T>(xv[j]);
+          s0 += f * to_f32<T>(p[j]);
+          s1 += f * to_f32<T>(q[j]);
+        }
+      };
+      int k = 8 * lane;
+      for (; k + 3 * 512 + 8 <= K; k += 4 * 512) {
+        u16x8 xv[4], p[4], q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          xv[i] = *(const u16x8_any*)(x + k + 512 * i);
+          p[i] = *(const u16x8_any*)(a0 + k + 512 * i);
+          q[i] = *(const u16x8_any*)(a1 + k + 512 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) add(xv[i], p[i], q[i]);
+      }
+      for (; k < K; k += 512) add(load8(x + k, K - k), load8(a0 + k, K - k), load8(a1 + k, K - k));
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) {
+        s0 += __shfl_xor(s0, d);
+        s1 += __shfl_xor(s1, d);
+      }
+      if (lane == 0) {
+        h[r0] = s0 * scaling.at(a);
+        if (r0 + 1 < r) h[r0 + 1] = s1 * scaling.at(a);
+      }
+    }
+    __syncthreads();
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j < r) s += h[j] * to_f32<T>(w0[j]);
+      if (j + 8 < r) s += h[j + 8] * to_f32<T>(w1[j]);
+    }
+    for (int k = 16; k < r; k += 8) {
+      const u16x8 wv = load8(w + k, r - k);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (k + j < r) s += h[k + j] * to_f32<T>(wv[j]);
+    }
+    v += s;
+  }
+  if (n < N) out[at] = from_f32<T>(v);
+}
+
+// ---------------------------------------------------------------------------
+// Few tokens, two launches.  k_vec_down: block (token, RG ranks), the width over 256 threads; H fp32
 // [T, r].  k_vec_up: block (256 columns, token), a column per thread.
 // ---------------------------------------------------------------------------
 template <int T, int RG>
@@ -964,7 +1037,20 @@ k_vec_up(const float* __restrict__ H, const uint16_t* __restrict__ B, Ids ids,
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-constexpr int LO_VEC_TOKENS = 64;   // up to here k_vec_*
+// Whether every token goes on its own (k_vec*) rather than in tiles of its adapter: two time
+// models, us.  On its own a token reads its factors itself, at about 5 TB/s whether from L2 or
+// HBM; by tiles there are three launches and a tile per adapter in use, at most L.  Measured,
+// on their own / by tiles: 64 tokens of 64 adapters, 4096 -> 4096, rank 16 8.7 / 35; 64 of 8,
+// 4096 -> 14336, rank 64 37 / 29; 32 of 32, 14336 -> 4096, rank 64 19 / 42; 128 of 8, 4096 ->
+// 4096, rank 16 12 / 16.
+bool tokens_alone(int T, int K, int N, int r, int L) {
+  if (T > 4096) return false;
+  const double factors = 2e-6 * r * ((double)K + N), used = std::min(L, T);
+  const double alone = 6 + T * factors / 5;
+  const double tiles = 16 + 0.3 * used * mm_cdiv(r, 64) + used * factors / 3.5 +
+                       2e-6 * T * (K + 2.0 * N) / 4;
+  return alone < tiles;
+}
 // No sum of a launch with this many blocks per problem is split: a split launch therefore has
 // fewer arrival counters than this in use per problem.
 constexpr int LO_SPLIT_BELOW = 512;
@@ -987,7 +1073,7 @@ size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 // 14336, rank 64 71 / 55 / 45 / 43 / 52; 4096, 14336, 16 68 / 52 / 43 / 48 / 57; backward of
 // 8192 tokens, 4096, 4096 96 / 101 / 108 / 122 / 142.
 int down_range(long tiles, int pairs) {
-  return std::max(LO_DW, (int)((tiles * pairs + 223) / 224));
+  return std::max(LO_DW, (int)((tiles * pairs + 255) / 256));
 }
 // Splits of an adapter's tokens: while a wave has more than 16 steps of 32 on average.  us,
 // splits 1 / 2 / 4: backward of 4096 tokens 113 / 104 / 107, 2048 of 2 adapters 81 / 90 / 100.
@@ -1077,7 +1163,7 @@ int make_plan(const char* who, const LoraPlan& p, const void* ids, int ids64, in
 
 extern "C" size_t mm_lora_workspace_bytes(int T, int K, int N, int r, int L, int backward) {
   if (T <= 0 || K <= 0 || N <= 0 || r <= 0 || L <= 0) return LO_COUNTER_BYTES;
-  if (!backward && T <= LO_VEC_TOKENS) return LO_COUNTER_BYTES + (size_t)T * r * 4;
+  if (!backward && tokens_alone(T, K, N, r, L)) return LO_COUNTER_BYTES + (size_t)T * r * 4;
   return plan_lora(T, K, N, r, L, backward != 0).total;
 }
 
@@ -1097,9 +1183,24 @@ extern "C" int mm_lora_add(const uint16_t* x, int type, const uint16_t* base, in
                "%s: workspace of %zu bytes is smaller than the %zu required", who, ws_bytes, need);
   hipStream_t st = (hipStream_t)stream;
   const Scaling sc{scaling, scale};
-  if (T <= LO_VEC_TOKENS) {
+  if (tokens_alone(T, K, N, r, L)) {
     float* H = (float*)((char*)ws + LO_COUNTER_BYTES);
     const Ids id{ids, ids64, L};
+    // One launch while a block's read of A (at 50 GB/s and CU) costs less than a launch.  us,
+    // one / two launches: 1 token, 4096 -> 4096, rank 16 4.8 / 7.2; 8 tokens 5.1 / 8.0; 32
+    // tokens, 4096 -> 6144 9.5 / 8.0; 1 token, 14336 -> 4096, rank 64 29 / 9.4.
+    const long a_bytes = 2L * r * K;
+    if (r <= VE_RANKS && a_bytes <= 256 << 10 && mm_cdiv(N, VE_NT) * T * a_bytes <= 24L << 20) {
+#define MM_VEC(TV, BV)                                                                         \
+  hipLaunchKernelGGL((k_vec<TV, BV>), dim3(mm_cdiv(N, VE_NT), T), dim3(VE_NT), 0, st, x, A, B, id, \
+                     sc, base, out, K, N, r)
+      if (type == 1) MM_VEC(1, 1);
+      else if (base_type == 1) MM_VEC(2, 1);
+      else MM_VEC(2, 2);
+#undef MM_VEC
+      MM_CHECK_LAUNCH(who);
+      return 0;
+    }
     // Fewer ranks a block while that leaves CUs idle.
 #define MM_VEC_DOWN(TV, RG)                                                                    \
   hipLaunchKernelGGL((k_vec_down<TV, RG>), dim3(mm_cdiv(r, RG), T), dim3(LO_NT), 0, st, x, A, id, \
