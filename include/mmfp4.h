@@ -248,11 +248,12 @@ int mm_lora_add(const uint16_t* x, int type, const uint16_t* base, int base_type
 /* Its gradients.  With h = s * x . A^T and dh = s * dy . B of each token:
  *   dx[t] = dx_base[t] + dh[t] . A_a      (dx_base NULL: zeros; may be dx)
  *   dA[a] = sum_t dh[t]^T x[t],  dB[a] = sum_t dy[t]^T h[t]   over the tokens of adapter a
- * every tensor of the type of x; adapters without tokens get zeros. */
+ * every tensor of the type of x, but dA and dB fp32 with grad_type 0 (else grad_type is that
+ * type); adapters without tokens get zeros. */
 int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type, const uint16_t* A,
                      const uint16_t* B, const void* ids, int ids64, const float* scaling,
-                     float scale, const uint16_t* dx_base, uint16_t* dx, uint16_t* dA,
-                     uint16_t* dB, int T, int K, int N, int rank, int adapters, void* ws,
+                     float scale, const uint16_t* dx_base, uint16_t* dx, void* dA, void* dB,
+                     int grad_type, int T, int K, int N, int rank, int adapters, void* ws,
                      size_t ws_bytes, void* stream);
 
 /* -------------------------------------------------------------------- MoE */

@@ -720,8 +720,8 @@ k_up(UpProblem p, Plan plan, int r) {
 // ---------------------------------------------------------------------------
 struct GradProblem {
   const uint16_t* V;    // [T, C]
-  uint16_t* G;          // [L, r, C] or, CR, [L, C, r]
-  int C, ks;
+  void* G;              // [L, r, C] or, CR, [L, C, r]; fp32 or the operands' type
+  int C, ks, f32;
   Records rec;
   float* part;          // [adapter][chunk][column block][ks][64 * rp]
   uint32_t* counters;   // [adapter][chunk][column block]
@@ -837,16 +837,26 @@ MM_DEV void wgrad_tile(const GradProblem& p, const Plan& plan, int r, int colblo
   }
   // Wave w holds column 4c + w, ranks 4q + i.  dB has the ranks of a column side by side;
   // dA, columns side by side, goes through LDS once more.
-  uint16_t* G = p.G + (size_t)e * r * p.C;
+  const size_t G = (size_t)e * r * p.C;
+  auto store = [&](size_t at, f32x4 v, bool whole, int n) {
+    if (p.f32) {
+      float* o = (float*)p.G + at;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < n) o[i] = v[i];
+      return;
+    }
+    u16x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = from_f32<T>(v[i]);
+    if (whole) *(u16x4_any*)((uint16_t*)p.G + at) = o;
+    else store4((uint16_t*)p.G + at, o, n);
+  };
   if constexpr (CR) {
 #pragma unroll
     for (int k = 0; k < RT; ++k) {
       const int rank = chunk * RP + 16 * k + 4 * q;
-      u16x4 o;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = from_f32<T>(own[k][i]);
-      if (wave < left)
-        store4(G + (size_t)(n0 + wave) * r + rank, o, r - rank);
+      if (wave < left) store(G + (size_t)(n0 + wave) * r + rank, own[k], false, r - rank);
     }
   } else {
     float* tr = (float*)lds;   // [rank][64 columns]
@@ -860,11 +870,8 @@ MM_DEV void wgrad_tile(const GradProblem& p, const Plan& plan, int r, int colblo
       const int rank = it / (LO_WG_COLS / 4), col = 4 * (it % (LO_WG_COLS / 4));
       const f32x4 v = *(const f32x4*)(tr + rank * LO_WG_COLS + col);
       const int n = colblock * LO_WG_COLS + col;
-      u16x4 o;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = from_f32<T>(v[j]);
       if (chunk * RP + rank < r)
-        st4<WHOLE>(G + (size_t)(chunk * RP + rank) * p.C + n, o, p.C - n);
+        store(G + (size_t)(chunk * RP + rank) * p.C + n, v, WHOLE, p.C - n);
     }
   }
 }
@@ -1247,10 +1254,12 @@ extern "C" int mm_lora_add(const uint16_t* x, int type, const uint16_t* base, in
 extern "C" int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type,
                                 const uint16_t* A, const uint16_t* B, const void* ids, int ids64,
                                 const float* scaling, float scale, const uint16_t* dx_base,
-                                uint16_t* dx, uint16_t* dA, uint16_t* dB, int T, int K, int N,
-                                int r, int L, void* ws, size_t ws_bytes, void* stream) {
+                                uint16_t* dx, void* dA, void* dB, int grad_type, int T, int K,
+                                int N, int r, int L, void* ws, size_t ws_bytes, void* stream) {
   const char* who = "mm_lora_backward";
   if (const int rc = check_common(who, type, T, K, N, r, L, ids, ids64)) return rc;
+  MM_CHECK_ARG(grad_type == 0 || grad_type == type,
+               "%s: grad_type=%d must be 0 (fp32) or the type of x", who, grad_type);
   MM_CHECK_ARG(T > 0, "%s: no tokens (the gradients are zeros)", who);
   const size_t need = mm_lora_workspace_bytes(T, K, N, r, L, 1);
   MM_CHECK_ARG(ws != nullptr && ws_bytes >= need,
@@ -1276,8 +1285,8 @@ extern "C" int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type,
   MM_CHECK_LAUNCH(who);
   const int ca = mm_cdiv(K, LO_WG_COLS), cb = mm_cdiv(N, LO_WG_COLS);
   const int ga = wgrad_split(T, L, p.nrc, K), gb = wgrad_split(T, L, p.nrc, N);
-  const GradProblem pa{x, dA, K, ga, ry, part, counters};
-  const GradProblem pb{dy, dB, N, gb, rx, part + (size_t)L * p.nrc * ca * ga * LO_WG_COLS * p.rp,
+  const GradProblem pa{x, dA, K, ga, grad_type == 0, ry, part, counters};
+  const GradProblem pb{dy, dB, N, gb, grad_type == 0, rx, part + (size_t)L * p.nrc * ca * ga * LO_WG_COLS * p.rp,
                        counters + LO_SPLIT_BELOW};
   const UpProblem pu{A, dx_base, dx, K, ry};
   const long na = (long)ca * L * p.nrc * ga, nb = (long)cb * L * p.nrc * gb;

@@ -7,6 +7,8 @@
 // libmmfp4.so (mm_fp4_gemm / mm_u4_gemm).  torch is used only for tensor
 // arguments and the output allocation; the stream comes from the caller.
 #include <c10/core/impl/DeviceGuardImplInterface.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -479,10 +481,18 @@ pybind11::object lora_backward(const at::Tensor& dy, const at::Tensor& x, const 
       (const uint16_t*)dy.data_ptr(), (const uint16_t*)x.data_ptr(), l.type,
       (const uint16_t*)a.data_ptr(), (const uint16_t*)b.data_ptr(), l.ids, l.ids64, l.scaling,
       (float)factor, dx_base ? (const uint16_t*)dx_base->data_ptr() : nullptr,
-      (uint16_t*)dx.data_ptr(), (uint16_t*)da.data_ptr(), (uint16_t*)db.data_ptr(), (int)l.T,
-      (int)l.K, (int)l.N, (int)l.r, (int)l.L, ws.data_ptr(), (size_t)ws.numel(), (void*)stream);
+      (uint16_t*)dx.data_ptr(), da.data_ptr(), db.data_ptr(), l.type, (int)l.T, (int)l.K, (int)l.N,
+      (int)l.r, (int)l.L, ws.data_ptr(), (size_t)ws.numel(), (void*)stream);
   if (rc) fail(rc);
   return pybind11::make_tuple(dx, da, db);
+}
+
+// Stream id of a leaf's gradient accumulator, or -1 where it has none (yet).
+int64_t accumulator_stream(const at::Tensor& leaf) {
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  if (!node) return -1;
+  const auto stream = node->stream();
+  return stream ? (int64_t)stream->id() : -1;
 }
 
 }  // namespace
@@ -502,6 +512,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "mm_swiglu_grad and mm_gemm_backward on plain operands, else None");
   m.def("lora_add", &lora_add, "mm_lora_add on plain operands, else None");
   m.def("lora_backward", &lora_backward, "mm_lora_backward on plain operands, else None");
+  m.def("accumulator_stream", &accumulator_stream,
+        "stream id of a leaf's gradient accumulator, -1 without one");
   m.def("workspace", &workspace_for,
         "the zero-initialised workspace of (device index, raw stream), at least nbytes",
         pybind11::arg("device"), pybind11::arg("stream"), pybind11::arg("nbytes"));

@@ -16,6 +16,7 @@ from .backward import (fused_gate_up_swiglu, fused_gate_up_swiglu_backward,
                        marlin_gemm_fp4_backward, marlin_gemm_int4_backward,
                        mmfp4_fused_qkv_backward, mmfp4_gemm_rowpacked_backward)
 from .adapters import lora_add, lora_backward
+from .autograd import gate_up_swiglu
 from .layers import MMFP4Linear
 from .ops import GemmFp4, dispatch_gemm_fp4
 from .loader import QuantizedModel, convert_safetensors_to_fp4, load_and_quantize_safetensors
@@ -31,7 +32,7 @@ from .moe_dispatch import (FusedMoEDispatcher, MoEDispatcher, _fused_expert_mlp,
                            scatter_expert_outputs)
 from .quantize_fp4 import (E2M1_VALUES, compute_quantization_error, pack_u4_weights,
                            quantize_fp4, unpack_fp4, unpack_u4_weights)
-from .quantized_linear import (KernelLibrary, MarlinLinear, QuantizedLinear, QuantizedTensor,
+from .quantized_linear import (KernelLibrary, LoRALinear, MarlinLinear, QuantizedLinear, QuantizedTensor,
                                dequant_fp4_bulk, dequant_int4_bulk, get_default_library,
                                quantized_linear)
 

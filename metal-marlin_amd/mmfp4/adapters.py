@@ -63,6 +63,19 @@ def _scaling(scaling, adapters: int, dev: torch.device):
     return scaling.to(torch.float32).contiguous(), 1.0
 
 
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses of t's first element and of the byte behind its last."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
 def _plain_scaling(scaling):
     return (scaling, 1.0) if isinstance(scaling, torch.Tensor) else (None, float(scaling))
 
@@ -87,6 +100,12 @@ def _add(base, x, lora_a, lora_b, adapter_ids, scaling, out=None):
                             not out.is_contiguous()):
         raise ValueError(f"out must be contiguous {dt} {tuple(base.shape)}, got {out.dtype} "
                          f"{tuple(out.shape)}")
+    if out is not None:
+        for name, t in (("base", base), ("x", x), ("lora_a", lora_a), ("lora_b", lora_b)):
+            itself = t is base and t.dtype == dt and t.is_contiguous() and \
+                t.data_ptr() == out.data_ptr()
+            if not itself and _overlap(out, t):
+                raise ValueError(f"out shares memory with {name}")
     with on_device(dev):
         st, factor = _scaling(scaling, L, dev)
         xf = x.reshape(-1, K).to(dt).contiguous()
@@ -129,6 +148,8 @@ def lora_add(base: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     if torch.is_grad_enabled() and any(t.requires_grad for t in (base, x, lora_a, lora_b)
                                        if isinstance(t, torch.Tensor)):
         from .autograd import LoraAdd
+        if isinstance(scaling, torch.Tensor) and scaling.requires_grad:
+            raise ValueError("scaling gets no gradient: pass scaling.detach()")
         if out is not None:
             raise ValueError("out= takes no part in autograd: use torch.no_grad()")
         return LoraAdd.apply(base, x, lora_a, lora_b, adapter_ids, scaling)
@@ -141,7 +162,9 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_
     """The gradients of lora_add for dy [*, N]: (dx [*, K], da, db), da and db shaped and typed
     as lora_a and lora_b (zeros for adapters without tokens), dx of x's type.  dx_base, the
     gradient that reached x through the projection itself (marlin_gemm_fp4_backward), is
-    added to dx before it is rounded."""
+    added to dx before it is rounded.  dy is rounded to the type that x is computed in: fp32
+    gradients are computed as fp16 and want a loss scale, fp32 factors beside fp16 or bf16
+    tokens get fp32 gradients."""
     if isinstance(x, torch.Tensor):
         got = _lib.fast("lora_backward", x, dy, x, lora_a, lora_b, adapter_ids,
                         *_plain_scaling(scaling), dx_base)
@@ -168,13 +191,16 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_
         if T == 0:
             return x.new_empty(x.shape), torch.zeros_like(lora_a), torch.zeros_like(lora_b)
         dx = torch.empty((T, K), dtype=dt, device=dev)
-        da, db = torch.empty_like(ac), torch.empty_like(bc)
+        # factors that are not of the type they are computed in (fp32 masters) get their
+        # gradients from the fp32 sums
+        gt = dt if lora_a.dtype == lora_b.dtype == dt else torch.float32
+        da, db = torch.empty_like(ac, dtype=gt), torch.empty_like(bc, dtype=gt)
         stream = _lib.raw_stream(dev.index)
         ws = _lib.call_workspace(dev.index, stream,
                                  _lib.load().mm_lora_workspace_bytes(T, K, N, r, L, 1))
         _lib.call("mm_lora_backward", _lib.ptr(dyf), _lib.ptr(xf), _TYPES[dt], _lib.ptr(ac),
                   _lib.ptr(bc), _lib.ptr(ids), int(ids is not None and ids.dtype == torch.int64),
                   _lib.ptr(st), factor, _lib.ptr(dxb), _lib.ptr(dx), _lib.ptr(da), _lib.ptr(db),
-                  T, K, N, r, L, _lib.ptr(ws), ws.numel(), stream)
+                  _TYPES[gt], T, K, N, r, L, _lib.ptr(ws), ws.numel(), stream)
     return (dx.view(x.shape).to(x.dtype), da.view(lora_a.shape).to(lora_a.dtype),
             db.view(lora_b.shape).to(lora_b.dtype))

@@ -1,0 +1,139 @@
+"""Autograd over the quantized products: gradients of the input through frozen 4-bit weights,
+and of low-rank adapters.  The layers (QuantizedLinear, MarlinLinear, MMFP4Linear, LoRALinear)
+and lora_add use these by themselves where an operand requires a gradient; calls that need
+none take the same path as ever.  They are differentiable once: a gradient of a gradient is
+an error, not a silent zero.
+
+A backward pass may be captured into a graph.  torch then refuses, by ending the process, one
+thing that a caller cannot see: a leaf whose gradient accumulator belongs to another stream
+because an eager graph of that leaf is still alive.  refuse_foreign_leaf raises before that.
+"""
+
+from __future__ import annotations
+
+from collections.abc import Callable
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib, adapters, backward
+
+__all__ = ["linear", "gate_up_swiglu", "LoraAdd", "LoraLinear"]
+
+
+def refuse_foreign_leaf(*tensors: torch.Tensor | None) -> None:
+    """Under graph capture, raises for a leaf whose gradient accumulator lives on another
+    stream than the captured one."""
+    if not torch.cuda.is_current_stream_capturing():
+        return
+    b = _lib.binding()
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.is_leaf and t.requires_grad and b is not None:
+            stream = b.accumulator_stream(t)
+            if stream >= 0 and stream != torch.cuda.current_stream(t.device).stream_id:
+                raise RuntimeError(
+                    "backward under graph capture: a leaf's gradient accumulator belongs to "
+                    "another stream, because a graph built there is still alive. Drop it (del "
+                    "its outputs) before capturing, or build it on the capture stream too")
+
+
+def wants_grad(*tensors: torch.Tensor | None) -> bool:
+    return torch.is_grad_enabled() and any(
+        isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+
+
+class _Linear(torch.autograd.Function):
+    """y = forward(x) in x's type, dx = input_grad(dy); neither depends on anything trained."""
+
+    @staticmethod
+    def forward(ctx, x, product, input_grad):
+        refuse_foreign_leaf(x)
+        ctx.input_grad, ctx.dtype, ctx.shape = input_grad, x.dtype, x.shape
+        return product(x).to(x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return ctx.input_grad(dy, ctx.dtype).view(ctx.shape), None, None
+
+
+def linear(x: torch.Tensor, product: Callable, input_grad: Callable) -> torch.Tensor:
+    """product(x) in x's type, differentiable in x: input_grad(dy, dtype) is its gradient."""
+    if wants_grad(x):
+        return _Linear.apply(x, product, input_grad)
+    return product(x).to(x.dtype)
+
+
+class _GateUp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate_packed, gate_scales, up_packed, up_scales, group_size, row_packed):
+        refuse_foreign_leaf(x)
+        h, gate_up = backward.fused_gate_up_swiglu(x, gate_packed, gate_scales, up_packed,
+                                                   up_scales, group_size, row_packed)
+        ctx.save_for_backward(gate_up, gate_packed, gate_scales, up_packed, up_scales)
+        ctx.group_size, ctx.row_packed, ctx.dtype = group_size, row_packed, x.dtype
+        return h.to(x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        gate_up, *weights = ctx.saved_tensors
+        dx = backward.fused_gate_up_swiglu_backward(dh, gate_up, *weights, ctx.group_size,
+                                                    ctx.row_packed, out_dtype=ctx.dtype)
+        return dx, None, None, None, None, None, None
+
+
+def gate_up_swiglu(x: torch.Tensor, gate_packed: torch.Tensor, gate_scales: torch.Tensor,
+                   up_packed: torch.Tensor, up_scales: torch.Tensor, group_size: int = 128,
+                   row_packed: bool = False) -> torch.Tensor:
+    """silu(x @ Wg) * (x @ Wu) in x's type, differentiable in x: fused_gate_up_swiglu and its
+    backward pass as one differentiable call."""
+    return _GateUp.apply(x, gate_packed, gate_scales, up_packed, up_scales, group_size,
+                         row_packed)
+
+
+class LoraAdd(torch.autograd.Function):
+    """lora_add, differentiable in base, x, lora_a and lora_b."""
+
+    @staticmethod
+    def forward(ctx, base, x, lora_a, lora_b, adapter_ids, scaling):
+        refuse_foreign_leaf(base, x, lora_a, lora_b)
+        ctx.save_for_backward(x, lora_a, lora_b, adapter_ids,
+                              scaling if isinstance(scaling, torch.Tensor) else None)
+        ctx.scaling = scaling
+        ctx.base_dtype = base.dtype
+        return adapters._add(base, x, lora_a, lora_b, adapter_ids, scaling)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, a, b, ids, scaling = ctx.saved_tensors
+        dx = da = db = None
+        if any(ctx.needs_input_grad[1:4]):
+            dx, da, db = adapters.lora_backward(dy.contiguous(), x, a, b, ids,
+                                                ctx.scaling if scaling is None else scaling)
+        return dy.to(ctx.base_dtype), dx, da, db, None, None
+
+
+class LoraLinear(torch.autograd.Function):
+    """A layer and its adapters in one node, so that the two gradients of x are added before
+    they are rounded."""
+
+    @staticmethod
+    def forward(ctx, x, lora_a, lora_b, adapter_ids, scaling, layer):
+        refuse_foreign_leaf(x, lora_a, lora_b)
+        ctx.save_for_backward(x, lora_a, lora_b, adapter_ids,
+                              scaling if isinstance(scaling, torch.Tensor) else None)
+        ctx.scaling, ctx.layer = scaling, layer
+        return adapters._add(layer(x), x, lora_a, lora_b, adapter_ids, scaling).to(x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, a, b, ids, scaling = ctx.saved_tensors
+        dy = dy.contiguous()
+        base = ctx.layer.input_grad(dy, x.dtype) if ctx.needs_input_grad[0] else None
+        dx, da, db = adapters.lora_backward(dy, x, a, b, ids,
+                                            ctx.scaling if scaling is None else scaling,
+                                            dx_base=base)
+        return (dx if ctx.needs_input_grad[0] else None), da, db, None, None, None

@@ -21,7 +21,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
-from .. import kernels
+from .. import autograd, backward, kernels
 
 __all__ = ["MMFP4Linear", "mmfp4_gemm", "rowpacked_to_marlin"]
 
@@ -81,7 +81,7 @@ class MMFP4Linear(nn.Module):
     """y = x @ W^T (+ bias) with row-packed FP4 weights
     (mmfp4_linear.py:600-960).  Same constructor arguments, validation and
     errors as the reference.  `activation` is stored and, as in the
-    reference's forward, not applied."""
+    reference's forward, not applied.  Differentiable in x; the weights are frozen."""
 
     def __init__(self, packed_weights: torch.Tensor, scales: torch.Tensor,
                  bias: torch.Tensor | None = None, group_size: int = 128,
@@ -140,19 +140,28 @@ class MMFP4Linear(nn.Module):
             raise ValueError(f"Expected input last dim={self.in_features}, got {x.shape[-1]}")
         if not x.is_floating_point():
             raise ValueError(f"x must be a floating tensor, got dtype={x.dtype}")
-        x2 = x.reshape(-1, self.in_features)
+        out = autograd.linear(x.reshape(-1, self.in_features), self._product, self.input_grad)
+        return out.reshape(*x.shape[:-1], self.out_features)
+
+    def input_grad(self, dy: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """The gradient of the input for dy [*, out] -> [*, in], in dy's type or `dtype`."""
+        return backward.mmfp4_gemm_rowpacked_backward(
+            dy, self.packed_weights.to(dy.device), self.scales.to(dy.device), self.group_size,
+            out_dtype=dtype)
+
+    def _product(self, x2: torch.Tensor) -> torch.Tensor:
+        """x2 [M, in] -> [M, out] fp16, with the bias."""
         if kernels.rowpacked_gemm_supported(x2.shape[0], self.out_features, self.in_features,
                                             self.group_size):
             # row-packed words and [n_groups, out] scales in place
-            out = kernels.mmfp4_gemm_rowpacked(x2, self.packed_weights.to(x.device),
-                                               self.scales.to(x.device), self.group_size)
+            out = kernels.mmfp4_gemm_rowpacked(x2, self.packed_weights.to(x2.device),
+                                               self.scales.to(x2.device), self.group_size)
         else:
-            kp, ks = self._kernel_weights(x.device)
+            kp, ks = self._kernel_weights(x2.device)
             if ks is None:
-                out = kernels.marlin_gemm_fp4(x2, kp, self.scales.to(x.device), self.group_size)
+                out = kernels.marlin_gemm_fp4(x2, kp, self.scales.to(x2.device), self.group_size)
             else:
                 out = kernels.marlin_gemm_fp4(x2, kp, ks, self.group_size)[:, :self.out_features]
         if self.bias is not None:
             out = out + self.bias.to(device=out.device, dtype=out.dtype)
-        out = out.reshape(*x.shape[:-1], self.out_features)
-        return out.to(x.dtype) if out.dtype != x.dtype else out
+        return out

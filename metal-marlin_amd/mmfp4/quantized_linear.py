@@ -9,7 +9,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 
-from . import kernels
+from . import adapters, autograd, backward, kernels
 from .quantize_fp4 import quantize_fp4
 
 
@@ -27,6 +27,15 @@ class QuantizedTensor:
     zeros: torch.Tensor | None = None
 
 
+def _fp4(x: torch.Tensor, weight: torch.Tensor, scales: torch.Tensor,
+         group_size: int) -> torch.Tensor:
+    """marlin_gemm_fp4 in x's type, differentiable in x."""
+    return autograd.linear(
+        x, lambda v: kernels.marlin_gemm_fp4(v, weight, scales, group_size),
+        lambda dy, dt: backward.marlin_gemm_fp4_backward(dy, weight, scales, group_size,
+                                                         out_dtype=dt))
+
+
 class KernelLibrary:
     """The GEMM methods QuantizedLinear dispatches to
     (metal_dispatch.py:1791-1937, MetalKernelLibrary.fp4_gemm / int4_gemm)."""
@@ -35,7 +44,7 @@ class KernelLibrary:
                  K: int, group_size: int = 128) -> torch.Tensor:
         if weight.shape[1] != N or weight.shape[0] * 8 != K:
             raise ValueError(f"weight shape {tuple(weight.shape)} != ({K // 8}, {N})")
-        return kernels.marlin_gemm_fp4(input, weight, scales, group_size).to(input.dtype)
+        return _fp4(input, weight, scales, group_size)
 
     def int4_gemm(self, input: torch.Tensor, weight: torch.Tensor, scales: torch.Tensor, N: int,
                   K: int, group_size: int = 128, zeros: torch.Tensor | None = None) -> torch.Tensor:
@@ -46,7 +55,10 @@ class KernelLibrary:
             raise ValueError(f"weight shape {tuple(weight.shape)} != ({K // 8}, {N})")
         if zeros is None:
             zeros = torch.full(scales.shape, 8.0, dtype=torch.float16, device=scales.device)
-        return kernels.marlin_gemm_int4(input, weight, scales, zeros, group_size).to(input.dtype)
+        return autograd.linear(
+            input, lambda x: kernels.marlin_gemm_int4(x, weight, scales, zeros, group_size),
+            lambda dy, dt: backward.marlin_gemm_int4_backward(dy, weight, scales, zeros,
+                                                              group_size, out_dtype=dt))
 
 
 _LIB: KernelLibrary | None = None
@@ -62,7 +74,8 @@ def get_default_library() -> KernelLibrary:
 
 class QuantizedLinear(nn.Module):
     """Linear layer over FP4/INT4 weights (quantized_linear.py:12-78): flatten,
-    optional Hadamard rotation, fused dequant-GEMM, in-place bias add."""
+    optional Hadamard rotation, fused dequant-GEMM, in-place bias add.  Differentiable in x;
+    the weights are frozen."""
 
     def __init__(self, quantized_weight: QuantizedTensor, bias: torch.Tensor | None = None):
         super().__init__()
@@ -87,6 +100,24 @@ class QuantizedLinear(nn.Module):
             out.add_(self.bias)
         return out.view(*batch_shape, self.out_features)
 
+    def input_grad(self, dy: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """The gradient of the input for dy [*, out] -> [*, in], in dy's type or `dtype`."""
+        w, s, g = self.weight_data, self.weight_scales, self.group_size
+        rotate = self.needs_hadamard and self.hadamard is not None
+        dt = torch.float32 if rotate else dtype
+        if self.format == "fp4":
+            dx = backward.marlin_gemm_fp4_backward(dy, w, s, g, out_dtype=dt)
+        elif self.format == "int4":
+            z = self.weight_zeros
+            if z is None:
+                z = torch.full(s.shape, 8.0, dtype=torch.float16, device=s.device)
+            dx = backward.marlin_gemm_int4_backward(dy, w, s, z, g, out_dtype=dt)
+        else:
+            raise ValueError(f"Unsupported quantized format: {self.format}")
+        if rotate:
+            dx = (dx @ self.hadamard.to(dx.device, dx.dtype).t()).to(dtype or dy.dtype)
+        return dx
+
     def _dispatch_quantized_gemm(self, x: torch.Tensor) -> torch.Tensor:
         if self.format == "fp4":
             return self._lib.fp4_gemm(x, self.weight_data, self.weight_scales, self.out_features,
@@ -102,8 +133,9 @@ def quantized_linear(x: torch.Tensor, weight_packed: torch.Tensor, scales: torch
     """x @ dequant(weight_packed, scales) with weight_packed in the Marlin
     layout [K/8, N] (metal_marlin.py:389-438).  The reference's docstring
     mentions an N-packed [K, N/8] layout but its body calls marlin_gemm_fp4,
-    which takes [K/8, N]; this follows the body.  Output dtype = x.dtype."""
-    return kernels.marlin_gemm_fp4(x, weight_packed, scales, group_size).to(x.dtype)
+    which takes [K/8, N]; this follows the body.  Output dtype = x.dtype.
+    Differentiable in x."""
+    return _fp4(x, weight_packed, scales, group_size)
 
 
 class MarlinLinear:
@@ -123,6 +155,11 @@ class MarlinLinear:
             out.add_(self.bias)
         return out
 
+    def input_grad(self, dy: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """The gradient of the input for dy [*, out] -> [*, in], in dy's type or `dtype`."""
+        return backward.marlin_gemm_fp4_backward(dy, self.weight_packed, self.scales,
+                                                 self.group_size, out_dtype=dtype)
+
     @staticmethod
     def from_linear(linear: nn.Linear, quant_type: str = "fp4", group_size: int = 32,
                     device: torch.device | str | None = None) -> "MarlinLinear":
@@ -136,6 +173,53 @@ class MarlinLinear:
         packed, scales = quantize_fp4(linear.weight.data.to(dev), group_size=group_size)
         bias = linear.bias.data.to(dev, torch.float16) if linear.bias is not None else None
         return MarlinLinear(packed, scales, bias, group_size=group_size)
+
+
+class LoRALinear(nn.Module):
+    """A quantized layer (QuantizedLinear, MarlinLinear, MMFP4Linear) with low-rank adapters of
+    several requests or users beside it: y = layer(x) + scaling[a] * (x @ lora_a[a]^T) @
+    lora_b[a]^T with a = adapter_ids[t], one id per token; ids outside [0, num_adapters) mean
+    no adapter.  The layer is frozen, lora_a [num_adapters, rank, in] (normal) and lora_b
+    [num_adapters, out, rank] (zeros) are the parameters.  `scaling`: a number, or one per
+    adapter.  fp16 or bf16 inputs; fp32 ones are computed as fp16, as the layer does."""
+
+    def __init__(self, layer, rank: int, num_adapters: int = 1,
+                 scaling: float | torch.Tensor = 1.0, dtype: torch.dtype = torch.float16,
+                 device: torch.device | str | None = None) -> None:
+        super().__init__()
+        if rank < 1 or num_adapters < 1:
+            raise ValueError(f"rank={rank} and num_adapters={num_adapters} must be positive")
+        self.layer = layer
+        n_in, n_out, dev = _features(layer)
+        dev = torch.device(device) if device is not None else dev
+        self.in_features, self.out_features = n_in, n_out
+        self.rank, self.num_adapters = rank, num_adapters
+        a = torch.randn(num_adapters, rank, n_in, device=dev) * n_in ** -0.5
+        self.lora_a = nn.Parameter(a.to(dtype))
+        self.lora_b = nn.Parameter(torch.zeros(num_adapters, n_out, rank, device=dev,
+                                               dtype=dtype))
+        if isinstance(scaling, torch.Tensor):
+            self.register_buffer("scaling", scaling.detach().to(dev, torch.float32))
+        else:
+            self.scaling = float(scaling)
+
+    def forward(self, x: torch.Tensor, adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
+        if autograd.wants_grad(x, self.lora_a, self.lora_b):
+            return autograd.LoraLinear.apply(x, self.lora_a, self.lora_b, adapter_ids,
+                                             self.scaling, self.layer)
+        return adapters.lora_add(self.layer(x), x, self.lora_a, self.lora_b, adapter_ids,
+                                 self.scaling).to(x.dtype)
+
+
+def _features(layer) -> tuple[int, int, torch.device]:
+    """(in, out, device) of a quantized layer."""
+    if isinstance(layer, MarlinLinear):
+        return 8 * layer.weight_packed.shape[0], layer.weight_packed.shape[1], \
+            layer.weight_packed.device
+    if not hasattr(layer, "input_grad"):
+        raise TypeError(f"LoRALinear needs a quantized layer, got {type(layer).__name__}")
+    words = layer.weight_data if isinstance(layer, QuantizedLinear) else layer.packed_weights
+    return layer.in_features, layer.out_features, words.device
 
 
 def dequant_fp4_bulk(packed: torch.Tensor, scales: torch.Tensor, K: int,

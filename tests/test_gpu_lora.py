@@ -109,6 +109,10 @@ SIZES = [  # T, K, N, r, L
     (65, 64, 64, 16, 1), (65, 520, 100, 8, 4), (100, 33, 1, 3, 5), (130, 1, 65, 17, 2),
     (257, 2048, 264, 33, 3), (300, 200, 515, 64, 9), (500, 776, 320, 100, 2),
     (1111, 328, 136, 16, 100), (900, 64, 72, 200, 1), (2100, 512, 256, 16, 1),
+    # forward by tiles (many tokens per adapter, wide factors)
+    (300, 4096, 515, 40, 2), (1111, 2048, 264, 64, 3), (700, 1000, 1030, 130, 2),
+    (400, 2056, 1001, 33, 4), (1500, 4000, 96, 16, 1), (260, 64, 8200, 24, 1),
+    (9000, 256, 200, 64, 3),
 ]
 
 
@@ -222,10 +226,30 @@ def test_forms_of_the_operands():
     assert f32.dtype == F16 and torch.equal(f32, ref)
     g = mmfp4.lora_backward(c.dy, c.x, c.a.float(), c.b.float(), c.ids, c.s)
     assert g[0].dtype == F16 and g[1].dtype == F32 and g[2].dtype == F32
+    half = mmfp4.lora_backward(c.dy, c.x, c.a, c.b, c.ids, c.s)
+    assert torch.equal(g[1].half(), half[1]) and torch.equal(g[2].half(), half[2])
     empty = mmfp4.lora_add(c.base[:0], c.x[:0], c.a, c.b, c.ids[:0], c.s)
     assert empty.shape == (0, 72)
     g = mmfp4.lora_backward(c.dy[:0], c.x[:0], c.a, c.b, c.ids[:0], c.s)
     assert g[0].shape == (0, 64) and not g[1].any() and not g[2].any()
+
+
+def test_out_beside_the_operands():
+    """out may be base itself; anything else that shares its memory is refused."""
+    gen = torch.Generator().manual_seed(31)
+    T, K = 6, 64
+    a, b = (torch.randn((1, *s), generator=gen).to(DEV, F16) for s in ((4, K), (K, 4)))
+    both = torch.randn((T + 1, K), generator=gen).to(DEV, F16)
+    x, base = both[:T], torch.randn((T, K), generator=gen).to(DEV, F16)
+    for name, out, bs in (("x", x, base), ("x", both[1:], base), ("base", both[1:], both[:T])):
+        with pytest.raises(ValueError, match=f"memory with {name}"):
+            mmfp4.lora_add(bs, x if name == "x" else base, a, b, out=out)
+    want = mmfp4.lora_add(base, x, a, b)
+    assert torch.equal(mmfp4.lora_add(base, x, a, b, out=base), want)
+    # columns of one tensor are not contiguous as `out`, but may be base and x
+    wide = torch.randn((T, 2 * K), generator=gen).to(DEV, F16)
+    want = mmfp4.lora_add(wide[:, :K].contiguous(), wide[:, K:].contiguous(), a, b)
+    assert torch.equal(mmfp4.lora_add(wide[:, :K], wide[:, K:], a, b, out=base), want)
 
 
 def test_gradients_by_differences():
@@ -247,11 +271,11 @@ def test_gradients_by_differences():
         assert abs(float((got.double() * d).sum()) - num) <= 2.0 ** -10 * terms
 
 
-@pytest.mark.parametrize("T", [4, 150])
-def test_capture(T):
+@pytest.mark.parametrize("T,K", [(4, 256), (150, 256), (500, 4096)])
+def test_capture(T, K):
     """Captured once, replayed on new tokens, ids and factors with eager work between; two
     graphs in turn."""
-    c = Case(T, 256, 200, 16, 4, BF16)
+    c = Case(T, K, 200, 16, 4, BF16)
 
     def step():
         out = mmfp4.lora_add(c.base, c.x, c.a, c.b, c.ids, c.s)
