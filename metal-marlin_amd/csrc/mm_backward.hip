@@ -125,7 +125,7 @@ struct PairWords<true> {
 };
 
 // ---------------------------------------------------------------------------
-// The product, more than 32 rows.  Tiles of BM = 32 * RB * WM rows x 256 columns (k); waves
+// The product, many rows.  Tiles of BM = 32 * RB * WM rows x 256 columns (k); waves
 // (wk, wm, wn): wn takes of every word row's 8 columns the four 4 wn + j, so a wave's tile is
 // 32 * RB rows x 128 columns: lane l32 holds columns 8 (kp0 + l32) + 4 wn + j.  WK = 4 waves
 // share out the 16-n steps of every chunk and add up in LDS at the end: four times the waves
@@ -140,11 +140,13 @@ struct PairWords<true> {
 // in order (k_mid's hand-off: sc1 partials, an arrival counter per tile left at zero).
 // ot: the output's type, 0 fp32, 1 fp16, 2 bf16.
 // ---------------------------------------------------------------------------
-template <bool INT4, int WM, int WK, int RB, int SR, int BN, int STG>
+// LDS of a block of NW waves that takes BM rows x KPT word rows (8 k each) in chunks of BN n,
+// and its loads.  RED: bytes of the sum over its waves at the end, in the same place.
+template <bool INT4, int NW, int BM_, int KPT, int SR, int BN, int STG, int RED>
 struct GradShape {
-  static constexpr int STAGES = STG;
-  static constexpr int NWAVE = 2 * WM * WK, NTHR = 64 * NWAVE, BM = 32 * RB * WM;
-  static constexpr int A_PIECES = BM * BN / 8, B_PIECES = GR_KP * BN / 4, S_PIECES = SR * BN / 8;
+  static constexpr int STAGES = STG, BM = BM_;
+  static constexpr int NWAVE = NW, NTHR = 64 * NWAVE;
+  static constexpr int A_PIECES = BM * BN / 8, B_PIECES = KPT * BN / 4, S_PIECES = SR * BN / 8;
   static constexpr int A_IT = A_PIECES / NTHR, B_IT = B_PIECES / NTHR;
   static constexpr int S_IT = (S_PIECES + NTHR - 1) / NTHR;
   static_assert(A_PIECES % NTHR == 0 && B_PIECES % NTHR == 0 && S_PIECES % 64 == 0, "split");
@@ -153,8 +155,147 @@ struct GradShape {
   static constexpr int B_OFF = STAGES * A_BYTES, S_OFF = B_OFF + STAGES * B_BYTES;
   static constexpr int Z_OFF = S_OFF + STAGES * S_BYTES;
   static constexpr int D_OFF = Z_OFF + (INT4 ? STAGES * S_BYTES : 0);   // dump of idle waves
-  static constexpr int RED_BYTES = WK > 1 ? NWAVE * 4096 : 0;           // one (rb, j) of the sum
-  static constexpr int LDS_BYTES = D_OFF + 1024 > RED_BYTES ? D_OFF + 1024 : RED_BYTES;
+  static constexpr int LDS_BYTES = D_OFF + 1024 > RED ? D_OFF + 1024 : RED;
+  static_assert(LDS_BYTES <= 160 * 1024, "LDS");
+};
+
+// The tile of a block, walked as in k_prefill2: an XCD takes a run of tiles, groups of grp row
+// tiles column by column.
+struct GradTile {
+  int bx, by, bz;
+};
+MM_DEV GradTile grad_tile(int grp) {
+  const int nx = gridDim.x, ny = gridDim.y, ntile = nx * ny * gridDim.z;
+  const int L = blockIdx.x + nx * (blockIdx.y + ny * blockIdx.z);
+  const int xq = ntile >> 3, xr = ntile & 7, xcd = L & 7;
+  const int lin = xcd * xq + min(xcd, xr) + (L >> 3);
+  const int bz = lin / (nx * ny), lt = lin - bz * (nx * ny);
+  const int gi = lt / (grp * nx), gw = lt - gi * (grp * nx);
+  const int gr = min(grp, ny - gi * grp);
+  return GradTile{gw / gr, gi * grp + gw % gr, bz};
+}
+
+// The chunks of a tile on their way to LDS.  Byte offsets of a lane's pieces from bases that
+// are uniform: within a segment only the bases move from chunk to chunk, in scalar registers.
+template <typename Sh, bool INT4, bool ROWS, int KPT, int BN>
+struct GradFeed {
+  static constexpr int PA = BN / 8, PB = BN / 4;   // pieces per row of A, of B
+  static constexpr int PR = KPT / 4;               // pieces per n of row-packed words
+  const GradSegs& segs;
+  char* smem;
+  int wave, lane, M, KP, ngroups, m0, kp0, g0;
+  uint32_t a_off[Sh::A_IT], b_off[Sh::B_IT], s_src[Sh::S_IT];
+  const f16* a_base;
+  const uint32_t* b_base;
+  const f16 *s_base, *z_base;
+  int seg_n, seg_n0, seg_next;   // columns of the segment, the chunk's first, its last chunk
+
+  MM_DEV static int aswz(int r) { return BN == 64 ? (r >> 1) & 7 : r & 15; }
+  MM_DEV int piece(int i) const { return (i * Sh::NWAVE + wave) * 64 + lane; }
+  // n of a row-packed piece.  Tiles of 16 word rows: the four n that the quarters of a wave
+  // read together (8 apart) lie side by side, 256 bytes.
+  MM_DEV static int rows_n(int p) {
+    const int n = p / PR;
+    return KPT == 16 ? (n & ~31) | (n & 3) << 3 | (n >> 2 & 7) : n;
+  }
+
+  MM_DEV void enter(int ch) {   // chunk ch opens a segment, or the block's range
+    const int sg = ch >= segs.s[2].ch0 ? 2 : (ch >= segs.s[1].ch0 ? 1 : 0);
+    const GradSeg& s = segs.s[sg];
+    const int N = s.N, n0 = (ch - s.ch0) * BN;
+    seg_n = N;
+    seg_n0 = n0;
+    seg_next = sg < 2 ? segs.s[sg + 1].ch0 : 0x7fffffff;
+    a_base = s.A + (size_t)m0 * s.lda + n0;
+    b_base = ROWS ? s.B + (size_t)n0 * KP + kp0 : s.B + (size_t)kp0 * N + n0;
+    s_base = s.S + (size_t)g0 * N + n0;
+    if constexpr (INT4) z_base = s.Z + (size_t)g0 * N + n0;
+#pragma unroll
+    for (int i = 0; i < Sh::A_IT; ++i) {
+      const int p = piece(i), r = p / PA;
+      a_off[i] = (uint32_t)(min(r, M - 1 - m0) * s.lda + 8 * ((p % PA) ^ aswz(r))) * 2u;
+    }
+#pragma unroll
+    for (int i = 0; i < Sh::B_IT; ++i) {
+      const int p = piece(i);
+      if constexpr (ROWS)
+        b_off[i] = ((uint32_t)rows_n(p) * KP + min(4 * (p % PR), KP - 4 - kp0)) * 4u;
+      else
+        b_off[i] = ((uint32_t)min(p / PB, KP - 1 - kp0) * N + 4 * ((p % PB) ^ (p / PB & 15))) * 4u;
+    }
+#pragma unroll
+    for (int i = 0; i < Sh::S_IT; ++i) {
+      const int p = min(piece(i), Sh::S_PIECES - 1);
+      s_src[i] = ((uint32_t)min(p / PA, ngroups - 1 - g0) * N + 8 * (p % PA)) * 2u;
+    }
+  }
+  // A segment's last chunk may reach past its columns: zeros for the gradient, any of the
+  // matrix's own words and scales.  (In two forms, so that the common one adds 32-bit offsets
+  // to scalar bases.)
+  MM_DEV void issue(int st) {
+    if (seg_n0 + BN > seg_n) load<true>(st);
+    else load<false>(st);
+  }
+  template <bool TAIL>
+  MM_DEV void load(int st) {
+#pragma unroll
+    for (int i = 0; i < Sh::A_IT; ++i) {
+      const char* src = (const char*)a_base + a_off[i];
+      if constexpr (TAIL) {
+        const int p = piece(i);
+        if (seg_n0 + 8 * ((p % PA) ^ aswz(p / PA)) >= seg_n) src = (const char*)gr_zeros;
+      }
+      gl2lds16(src, smem + st * Sh::A_BYTES + (i * Sh::NWAVE + wave) * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < Sh::B_IT; ++i) {
+      const char* src = (const char*)b_base + b_off[i];
+      if constexpr (TAIL) {
+        const int p = piece(i);
+        const int over = ROWS ? seg_n0 + rows_n(p) - (seg_n - 1)
+                              : seg_n0 + 4 * ((p % PB) ^ (p / PB & 15)) - (seg_n - 4);
+        if (over > 0) src -= (size_t)over * (ROWS ? KP : 1) * 4;
+      }
+      gl2lds16(src, smem + Sh::B_OFF + st * Sh::B_BYTES + (i * Sh::NWAVE + wave) * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < Sh::S_IT; ++i) {
+      const int wp = i * Sh::NWAVE + wave;
+      const uint32_t off = s_src[i];
+      size_t back = 0;
+      if constexpr (TAIL) {
+        const int p = min(wp * 64 + lane, Sh::S_PIECES - 1);
+        back = (size_t)max(0, seg_n0 + 8 * (p % PA) - (seg_n - 8)) * 2;
+      }
+      const bool live = wp * 64 < Sh::S_PIECES;
+      gl2lds16((const char*)s_base - back + off,
+               smem + (live ? Sh::S_OFF + st * Sh::S_BYTES + wp * 1024 : Sh::D_OFF));
+      if constexpr (INT4)
+        gl2lds16((const char*)z_base - back + off,
+                 smem + (live ? Sh::Z_OFF + st * Sh::S_BYTES + wp * 1024 : Sh::D_OFF));
+    }
+  }
+  MM_DEV void advance(int ch) {   // to chunk ch, the next one
+    if (ch >= seg_next) {
+      enter(ch);
+      return;
+    }
+    seg_n0 += BN;
+    a_base += BN;
+    b_base += ROWS ? (size_t)BN * KP : BN;
+    s_base += BN;
+    if constexpr (INT4) z_base += BN;
+  }
+  // The first STAGES chunks of [beg, end).
+  MM_DEV void start(int beg, int end) {
+    enter(beg);
+    issue(0);
+#pragma unroll
+    for (int c = 1; c < Sh::STAGES; ++c) {
+      if (beg + c < end) advance(beg + c);
+      issue(c);
+    }
+  }
 };
 
 MM_DEV uint32_t bf16_bits(float v) {
@@ -201,125 +342,29 @@ MM_DEV void grad_scales(f16x8 s, f16x8 z, f16x2 (&s2)[4], f16x2 (&nz2)[4]) {
   }
 }
 
+template <bool INT4, int WM, int WK, int RB, int SR, int BN, int STG>
+using GradTall = GradShape<INT4, 2 * WM * WK, 32 * RB * WM, GR_KP, SR, BN, STG,
+                           (WK > 1 ? 2 * WM * WK * 4096 : 0)>;   // one (rb, j) of the sum
+
 template <bool INT4, bool ROWS, int WM, int WK, int RB, int SR, int BN, int STG>
 __global__ void __launch_bounds__(WM * WK * 128)
 k_grad(GradSegs segs, void* __restrict__ out, int ot, const float* __restrict__ rowmul, int M,
        int K, int g, int cps, int grp, float* __restrict__ part, uint32_t* __restrict__ counters) {
-  using Sh = GradShape<INT4, WM, WK, RB, SR, BN, STG>;
+  using Sh = GradTall<INT4, WM, WK, RB, SR, BN, STG>;
   static_assert(WK == 1 || WK == 4, "a wave owns all or one of the four row quads");
-  constexpr int NWAVE = Sh::NWAVE, STAGES = Sh::STAGES;
-  constexpr int PA = BN / 8, PB = BN / 4;      // pieces per row of A, of B
+  constexpr int STAGES = Sh::STAGES;
   constexpr int STEPS = BN / 16 / WK;          // steps per wave and chunk
   __shared__ __attribute__((aligned(16))) char smem[Sh::LDS_BYTES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wave & 1, wm = (wave >> 1) % WM, wk = (wave >> 1) / WM;
   const int l32 = lane & 31, h = lane >> 5;
-  const int KP = K >> 3, ngroups = K / g;
-  // Tile walk of k_prefill2: an XCD takes a run of tiles, groups of grp row tiles
-  // column by column.
-  const int nx = gridDim.x, ny = gridDim.y, ntile = nx * ny * gridDim.z;
-  const int L = blockIdx.x + nx * (blockIdx.y + ny * blockIdx.z);
-  const int xq = ntile >> 3, xr = ntile & 7, xcd = L & 7;
-  const int lin = xcd * xq + min(xcd, xr) + (L >> 3);
-  const int bz = lin / (nx * ny), lt = lin - bz * (nx * ny);
-  const int gi = lt / (grp * nx), gw = lt - gi * (grp * nx);
-  const int gr = min(grp, ny - gi * grp);
-  const int by = gi * grp + gw % gr, bx = gw / gr;
+  const int KP = K >> 3;
+  const auto [bx, by, bz] = grad_tile(grp);
   const int m0 = by * Sh::BM, kp0 = bx * GR_KP;
   const int c_beg = bz * cps, c_end = min(segs.nch, c_beg + cps);
   const int g0 = 8 * kp0 / g;              // first group of the tile
-
-  auto aswz = [](int r) { return BN == 64 ? (r >> 1) & 7 : r & 15; };
-  // Byte offsets of a lane's pieces from bases that are uniform: within a segment only the
-  // bases move from chunk to chunk, in scalar registers.
-  uint32_t a_off[Sh::A_IT], b_off[Sh::B_IT], s_src[Sh::S_IT];
-  const f16* a_base;
-  const uint32_t* b_base;
-  const f16 *s_base, *z_base;
-  int seg_n = 0, seg_n0 = 0, seg_next = 0;   // columns of the segment, the chunk's first, its last chunk
-  auto enter = [&](int ch) {                 // chunk ch opens a segment, or the block's range
-    const int sg = ch >= segs.s[2].ch0 ? 2 : (ch >= segs.s[1].ch0 ? 1 : 0);
-    const GradSeg& s = segs.s[sg];
-    const int N = s.N, n0 = (ch - s.ch0) * BN;
-    seg_n = N;
-    seg_n0 = n0;
-    seg_next = sg < 2 ? segs.s[sg + 1].ch0 : 0x7fffffff;
-    a_base = s.A + (size_t)m0 * s.lda + n0;
-    b_base = ROWS ? s.B + (size_t)n0 * KP + kp0 : s.B + (size_t)kp0 * N + n0;
-    s_base = s.S + (size_t)g0 * N + n0;
-    if constexpr (INT4) z_base = s.Z + (size_t)g0 * N + n0;
-#pragma unroll
-    for (int i = 0; i < Sh::A_IT; ++i) {
-      const int p = (i * NWAVE + wave) * 64 + lane, r = p / PA;
-      a_off[i] = (uint32_t)(min(r, M - 1 - m0) * s.lda + 8 * ((p % PA) ^ aswz(r))) * 2u;
-    }
-#pragma unroll
-    for (int i = 0; i < Sh::B_IT; ++i) {
-      const int p = (i * NWAVE + wave) * 64 + lane;
-      if constexpr (ROWS)
-        b_off[i] = ((uint32_t)(p >> 3) * KP + min(4 * (p & 7), KP - 4 - kp0)) * 4u;
-      else
-        b_off[i] = ((uint32_t)min(p / PB, KP - 1 - kp0) * N + 4 * ((p % PB) ^ (p / PB & 15))) * 4u;
-    }
-#pragma unroll
-    for (int i = 0; i < Sh::S_IT; ++i) {
-      const int p = min((i * NWAVE + wave) * 64 + lane, Sh::S_PIECES - 1);
-      s_src[i] = ((uint32_t)min(p / PA, ngroups - 1 - g0) * N + 8 * (p % PA)) * 2u;
-    }
-  };
-  auto issue = [&](int st) {
-    // A segment's last chunk may reach past its columns: zeros for the gradient, any of the
-    // matrix's own words and scales.
-    const bool tail = seg_n0 + BN > seg_n;
-#pragma unroll
-    for (int i = 0; i < Sh::A_IT; ++i) {
-      const char* src = (const char*)a_base + a_off[i];
-      if (tail) {
-        const int p = (i * NWAVE + wave) * 64 + lane;
-        if (seg_n0 + 8 * ((p % PA) ^ aswz(p / PA)) >= seg_n) src = (const char*)gr_zeros;
-      }
-      gl2lds16(src, smem + st * Sh::A_BYTES + (i * NWAVE + wave) * 1024);
-    }
-#pragma unroll
-    for (int i = 0; i < Sh::B_IT; ++i) {
-      const char* src = (const char*)b_base + b_off[i];
-      if (tail) {
-        const int p = (i * NWAVE + wave) * 64 + lane;
-        const int over = ROWS ? seg_n0 + (p >> 3) - (seg_n - 1)
-                              : seg_n0 + 4 * ((p % PB) ^ (p / PB & 15)) - (seg_n - 4);
-        if (over > 0) src -= (size_t)over * (ROWS ? KP : 1) * 4;
-      }
-      gl2lds16(src, smem + Sh::B_OFF + st * Sh::B_BYTES + (i * NWAVE + wave) * 1024);
-    }
-#pragma unroll
-    for (int i = 0; i < Sh::S_IT; ++i) {
-      const int wp = i * NWAVE + wave;
-      uint32_t off = s_src[i];
-      size_t back = 0;
-      if (tail) {
-        const int p = min(wp * 64 + lane, Sh::S_PIECES - 1);
-        back = (size_t)max(0, seg_n0 + 8 * (p % PA) - (seg_n - 8)) * 2;
-      }
-      const bool live = wp * 64 < Sh::S_PIECES;
-      gl2lds16((const char*)s_base + off - back,
-               smem + (live ? Sh::S_OFF + st * Sh::S_BYTES + wp * 1024 : Sh::D_OFF));
-      if constexpr (INT4)
-        gl2lds16((const char*)z_base + off - back,
-                 smem + (live ? Sh::Z_OFF + st * Sh::S_BYTES + wp * 1024 : Sh::D_OFF));
-    }
-  };
-  auto advance = [&](int ch) {               // to chunk ch, the next one
-    if (ch >= seg_next) {
-      enter(ch);
-      return;
-    }
-    seg_n0 += BN;
-    a_base += BN;
-    b_base += ROWS ? (size_t)BN * KP : BN;
-    s_base += BN;
-    if constexpr (INT4) z_base += BN;
-  };
+  GradFeed<Sh, INT4, ROWS, GR_KP, BN> feed{segs, smem, wave, lane, M, KP, K / g, m0, kp0, g0};
 
   f32x16 acc[RB][4];
 #pragma unroll
@@ -329,15 +374,9 @@ k_grad(GradSegs segs, void* __restrict__ out, int ot, const float* __restrict__ 
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[rb][j][v] = 0.0f;
 
-  enter(c_beg);
-  issue(0);
-#pragma unroll
-  for (int c = 1; c < STAGES; ++c) {
-    if (c_beg + c < c_end) advance(c_beg + c);
-    issue(c);
-  }
+  feed.start(c_beg, c_end);
 
-  const int arow = wm * 32 * RB + l32, ax = aswz(arow);   // rows of all row blocks share ax
+  const int arow = wm * 32 * RB + l32, ax = feed.aswz(arow);   // rows of all row blocks share ax
   const int srow = 8 * min(kp0 + l32, KP - 1) / g - g0;
   const uint32_t half = wn ? 0x07060302u : 0x05040100u;
   const uint32_t s_off = srow * (BN * 2) + h * 16;
@@ -388,8 +427,8 @@ k_grad(GradSegs segs, void* __restrict__ out, int ot, const float* __restrict__ 
         __builtin_amdgcn_s_waitcnt(0xc07f);            // lgkmcnt(0): this wave's reads are done
         wait_vmcnt<(STAGES - 2) * Sh::LOADS>();
         __builtin_amdgcn_s_barrier();
-        if (ch + STAGES < c_end) advance(ch + STAGES);
-        issue(st);                                     // behind the last chunk: again, never read
+        if (ch + STAGES < c_end) feed.advance(ch + STAGES);
+        feed.issue(st);                                // behind the last chunk: again, never read
         frag(std::integral_constant<int, (st + 1) % STAGES>{}, 0, cur ^ 1);
       }
 #pragma unroll
@@ -456,7 +495,7 @@ k_grad(GradSegs segs, void* __restrict__ out, int ot, const float* __restrict__ 
   }
   const int ks = gridDim.z;
   if (ks > 1) {
-    const int tile = by * nx + bx;
+    const int tile = by * gridDim.x + bx;
     const __amdgpu_buffer_rsrc_t prs = mm_rsrc(part + (size_t)tile * ks * (Sh::BM * GR_COLS));
     auto at = [&](int z, int rb, int j, int q) {
       return 16u * (uint32_t)((((z * RB + rb) * 4 + j) * NQ + q) * Sh::NTHR + tid);
@@ -468,7 +507,7 @@ k_grad(GradSegs segs, void* __restrict__ out, int ot, const float* __restrict__ 
 #pragma unroll
         for (int q = 0; q < NQ; ++q) store_agent_x4(prs, at(bz, rb, j, q), own[rb][j][q]);
     // The flag lies in smem: a second LDS variable would have the compiler wait for every
-    // load to LDS before the reads of the main loop (M = 512, 4096 -> 4096 40 us so, 22 now).
+    // load to LDS before the reads of the main loop (M = 512, 4096 -> 4096 2 ways 40 us, 35 so).
     if (!grad_last(counters + tile, ks, (uint32_t*)smem)) return;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
@@ -505,6 +544,199 @@ k_grad(GradSegs segs, void* __restrict__ out, int ot, const float* __restrict__ 
                     f * f32x4{own[rb][0][q][i], own[rb][1][q][i], own[rb][2][q][i],
                               own[rb][3][q][i]});
       }
+}
+
+// ---------------------------------------------------------------------------
+// The product, 33 rows up: tiles of 64 rows x 128 columns (16 word rows), 16x16x32 MFMA.  Lane
+// (c, q): columns 8 (kp0 + c) + j of word row kp0 + c, gradient rows 16 rb + c, n 8 q .. + 7
+// of a step of 32.  A chunk has one step for each of the 8 waves, so every word and every
+// gradient value is read from LDS once, and the waves add up in LDS at the end.  While the
+// matrix cores take one half of a step's columns, the other half of the next operands is
+// converted.  ks > 1: as in k_grad.
+//
+// Against tiles of 64 x 256: half the columns leave no split to be joined up to 512 rows of K =
+// 4096, and every weight costs 1.7 VALU operations (2.3 there, where a wave converts half
+// words).  M = 512, 4096 -> 4096: 24.7 us, 700 TFLOP/s (34 there).  A chunk takes 1.3 us, of
+// which the matrix cores are busy 0.43: the two waves of a SIMD wait a third of the time for
+// each other, and what they issue does not overlap fully.  Reading the next operands before
+// the first half (double words) spills and gains nothing.
+// ---------------------------------------------------------------------------
+constexpr int GN_KP = 16, GN_COLS = 8 * GN_KP, GN_BM = 64, GN_NW = 8, GN_BN = 32 * GN_NW;
+constexpr int GN_NTHR = 64 * GN_NW, GN_RED = GN_NW * 2 * 16 * GN_COLS * 4;   // two row blocks
+
+template <bool INT4, int SR, int STG>
+using GradNarrow = GradShape<INT4, GN_NW, GN_BM, GN_KP, SR, GN_BN, STG, GN_RED>;
+
+template <bool INT4, bool ROWS, int SR, int STG>
+__global__ void __launch_bounds__(GN_NTHR)
+k_grad_narrow(GradSegs segs, void* __restrict__ out, int ot, const float* __restrict__ rowmul,
+              int M, int K, int g, int cps, int grp, float* __restrict__ part,
+              uint32_t* __restrict__ counters) {
+  using Sh = GradNarrow<INT4, SR, STG>;
+  __shared__ __attribute__((aligned(16))) char smem[Sh::LDS_BYTES];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int KP = K >> 3;
+  const auto [bx, by, bz] = grad_tile(grp);
+  const int m0 = by * GN_BM, kp0 = bx * GN_KP;
+  const int c_beg = bz * cps, c_end = min(segs.nch, c_beg + cps);
+  const int g0 = 8 * kp0 / g;
+  GradFeed<Sh, INT4, ROWS, GN_KP, GN_BN> feed{segs, smem, wave, lane, M, KP, K / g, m0, kp0, g0};
+  f32x4 acc[4][8];
+#pragma unroll
+  for (int rb = 0; rb < 4; ++rb)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[rb][j] = f32x4{0, 0, 0, 0};
+  feed.start(c_beg, c_end);
+
+  const int srow = 8 * min(kp0 + c, KP - 1) / g - g0;
+  const uint32_t s_off = srow * (GN_BN * 2) + (4 * wave + q) * 16;
+  const uint32_t a_off = c * (GN_BN * 2) + ((4 * wave + q) ^ c) * 16;
+  f16x8 af[2][4], bq[2][4];
+  u32x4 w[2];
+  f16x8 sv, zv;
+  f16x2 s2[4], nz2[4];
+  auto frag = [&](auto stc, int slot) __attribute__((always_inline)) {
+    constexpr int st = decltype(stc)::value;
+    if constexpr (ROWS) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        w[i >> 2][i & 3] = *(const uint32_t*)(smem + Sh::B_OFF + st * Sh::B_BYTES +
+                                              (32 * wave + 4 * i + q) * 64 + c * 4);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        w[i] = *(const u32x4*)(smem + Sh::B_OFF + st * Sh::B_BYTES + c * (GN_BN * 4) +
+                               ((8 * wave + 2 * q + i) ^ c) * 16);
+    }
+    sv = *(const f16x8*)(smem + Sh::S_OFF + st * Sh::S_BYTES + s_off);
+    if constexpr (INT4) zv = *(const f16x8*)(smem + Sh::Z_OFF + st * Sh::S_BYTES + s_off);
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb)
+      af[slot][rb] = *(const f16x8*)(smem + st * Sh::A_BYTES + a_off + rb * 16 * (GN_BN * 2));
+  };
+  auto decode = [&](int hf) __attribute__((always_inline)) {
+    if (hf == 0) grad_scales<INT4>(sv, zv, s2, nz2);
+    PairWords<INT4>::run(w, s2, nz2, hf ? 0x07060302u : 0x05040100u, bq[hf]);
+  };
+  auto half = [&](int slot, int hf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int rb = 0; rb < 4; ++rb)
+        acc[rb][4 * hf + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af[slot][rb], bq[hf][j],
+                                                                     acc[rb][4 * hf + j], 0, 0, 0);
+  };
+  auto order = [] {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // MFMA
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // DS read
+      __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);   // VALU
+    }
+  };
+  auto chunk = [&](int ch, auto stc, int cur) __attribute__((always_inline)) {
+    constexpr int st = decltype(stc)::value;
+    half(cur, 0);
+    decode(1);
+    order();
+    // Every wave has read this chunk: its stage is refilled, and the next one, which has
+    // landed once at most STAGES - 2 later ones are outstanding, is published.
+    __builtin_amdgcn_s_waitcnt(0xc07f);            // lgkmcnt(0)
+    wait_vmcnt<(STG - 2) * Sh::LOADS>();
+    __builtin_amdgcn_s_barrier();
+    if (ch + STG < c_end) feed.advance(ch + STG);
+    feed.issue(st);                                // behind the last chunk: again, never read
+    frag(std::integral_constant<int, (st + 1) % STG>{}, cur ^ 1);
+    half(cur, 1);
+    decode(0);
+    order();
+  };
+  wait_vmcnt<(STG - 1) * Sh::LOADS>();
+  __builtin_amdgcn_s_barrier();
+  frag(std::integral_constant<int, 0>{}, 0);
+  decode(0);
+  // an even number of stages in a round, so that the operand slots are constants
+  for (int ch = c_beg; ch < c_end; ch += 2 * STG) {
+    static_for(
+        [&](auto ic) __attribute__((always_inline)) {
+          constexpr int i = decltype(ic)::value;
+          if (i == 0 || ch + i < c_end)
+            chunk(ch + i, std::integral_constant<int, i % STG>{}, i & 1);
+        },
+        std::make_integer_sequence<int, 2 * STG>{});
+  }
+  wait_vmcnt<0>();
+
+  // The sum over the waves, two row blocks at a time: thread (wave, lane) owns row
+  // 16 (2 t + wave / 4) + 4 q + wave % 4 and its 8 columns.
+  f32x4 own[2][2];
+  f32x4* red = (f32x4*)smem;   // [wave][row block][row of a lane][column half][lane]
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    __syncthreads();
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const f32x4(&a)[8] = acc[2 * t + rb];
+          red[(((wave * 2 + rb) * 4 + v) * 2 + hf) * 64 + lane] =
+              f32x4{a[4 * hf][v], a[4 * hf + 1][v], a[4 * hf + 2][v], a[4 * hf + 3][v]};
+        }
+    __syncthreads();
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      own[t][hf] = red[(wave * 2 + hf) * 64 + lane];
+#pragma unroll
+      for (int k = 1; k < GN_NW; ++k) own[t][hf] += red[((k * 8 + wave) * 2 + hf) * 64 + lane];
+    }
+  }
+  const int ks = gridDim.z;
+  if (ks > 1) {
+    const int tile = by * gridDim.x + bx;
+    const __amdgpu_buffer_rsrc_t prs = mm_rsrc(part + (size_t)tile * ks * (GN_BM * GN_COLS));
+    auto at = [&](int z, int t, int hf) {
+      return 16u * (uint32_t)(((z * 2 + t) * 2 + hf) * GN_NTHR + tid);
+    };
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) store_agent_x4(prs, at(bz, t, hf), own[t][hf]);
+    // the flag lies in smem for k_grad's reason
+    if (!grad_last(counters + tile, ks, (uint32_t*)smem)) return;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) own[t][hf] = f32x4{0, 0, 0, 0};
+    for (int z = 0; z < ks; z += 4) {
+      f32x4 ld[4][2][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) ld[i][t][hf] = load_agent_x4(prs, at(min(z + i, ks - 1), t, hf));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (z + i < ks)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) own[t][hf] += ld[i][t][hf];
+    }
+  }
+  if (kp0 + c >= KP) return;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int row = m0 + 16 * (2 * t + (wave >> 2)) + 4 * q + (wave & 3);
+    if (row >= M) continue;
+    const float f = rowmul != nullptr ? rowmul[row] : 1.0f;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+      store_grad4(out, ot, (size_t)row * K + 8 * (kp0 + c) + 4 * hf, f * own[t][hf]);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -790,7 +1022,7 @@ k_swiglu_grad(const void* __restrict__ dH, const f16* __restrict__ GU, f16* __re
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-enum { G_SKINNY, G_64, G_256 };
+enum { G_SKINNY, G_NARROW, G_64, G_256 };
 struct GradPlan {
   int kind;
   int bn;       // n per chunk (step of the skinny kernel)
@@ -821,27 +1053,30 @@ GradPlan plan_grad(int nmat, const int* N, int M, int K) {
     if (p.ks > 1) p.part = (size_t)tiles * p.ks * M * GS_COLS * sizeof(float);
     return p;
   }
-  // Tiles of 64 rows or of 256, and the split, by a time model (us; MI355X, FP4, K = 4096):
-  // rounds of 256 blocks, a time per chunk, and the hand-off of a split.  Measured, 64-row
-  // tiles split / 256-row ones: M = 64, N = 4096 4 ways 24 / 57; M = 512, N = 4096 2 ways 34 /
-  // 60; M = 1024 48 / 80; M = 2048, N = 4096 92 / 106 (2 ways), N = 14336 292 / 266; M = 4096
-  // 183 / 147.
+  // The tile and the split by a time model (us; MI355X, FP4): rounds of 256 blocks, each its
+  // start, a time per chunk (more where all CUs share the memory) and its end, and the
+  // hand-off of a split.  Measured, K = 4096, 64 x 128 tiles / 64 x 256 / 256 x 256, each at its
+  // best split: M = 64, N = 4096 16.3 (4 ways) / 23 / 82; M = 300 24 / 28 / 89; M = 512 25 / 34 /
+  // 89, N = 14336 77 / 82 / 228; M = 1024, N = 4096 50 / 47 / 92; M = 2048 99 / 92 / 103, N =
+  // 14336 - / 292 / 266; M = 4096, N = 4096 - / 183 / 147.
+  struct { int kind, bm, cols, bn; double start, chunk, full, split, each; } const kinds[] = {
+      {G_NARROW, GN_BM, GN_COLS, GN_BN, 3.6, 1.32, 1.32, 2.2, 1.25},
+      {G_64, 64, GR_COLS, 128, 7.8, 1.05, 1.21, 7, 0},
+      {G_256, 256, GR_COLS, 64, 16, 1.75, 2.05, 20, 0}};
   double best = 0;
-  for (int kind = G_64; kind <= G_256; ++kind) {
-    const int bm = kind == G_64 ? 64 : 256, bn = kind == G_64 ? 128 : 64;
-    const long tiles = (long)mm_cdiv(K, GR_COLS) * mm_cdiv(M, bm);
-    const int nch = grad_chunks(nmat, N, bn);
-    for (int ks = 1; ks <= 16 && (ks == 1 || (nch / ks >= 2 && tiles <= GR_MAX_TILES)); ++ks) {
+  for (const auto& k : kinds) {
+    const long tiles = (long)mm_cdiv(K, k.cols) * mm_cdiv(M, k.bm);
+    const int nch = grad_chunks(nmat, N, k.bn);
+    for (int ks = 1; ks <= 16 && ks <= nch && (ks == 1 || tiles <= GR_MAX_TILES); ++ks) {
       const int per = mm_cdiv(nch, ks);
       if (mm_cdiv(nch, per) != ks) continue;
-      const double rounds = (double)((tiles * ks + 255) / 256);
-      const double us = kind == G_64
-                            ? rounds * per * (tiles * ks < 256 ? 1.06 : 1.25) + (ks > 1 ? 3 + 1.5 * ks : 0)
-                            : rounds * per * 2.2 + (ks > 1 ? 6 + 4 * ks : 0);
+      const long rounds = (tiles * ks + 255) / 256;
+      const double us = rounds * (k.start + per * (tiles * ks > 192 ? k.full : k.chunk) +
+                                  (ks > 1 ? k.split + ks * k.each : 0));
       if (best == 0 || us < best) {
         best = us;
-        p = GradPlan{kind, bn, bm, ks, per, 0,
-                     ks > 1 ? (size_t)tiles * ks * bm * GR_COLS * sizeof(float) : 0};
+        p = GradPlan{k.kind, k.bn, k.bm, ks, per, 0,
+                     ks > 1 ? (size_t)tiles * ks * k.bm * k.cols * sizeof(float) : 0};
       }
     }
   }
@@ -851,12 +1086,25 @@ GradPlan plan_grad(int nmat, const int* N, int M, int K) {
 template <bool INT4, bool ROWS, int WM, int WK, int RB, int SR, int BN, int STG>
 int launch_grad(const GradSegs& s, void* out, int ot, const float* rowmul, int M, int K, int g,
                 const GradPlan& p, void* ws, hipStream_t st) {
-  using Sh = GradShape<INT4, WM, WK, RB, SR, BN, STG>;
+  using Sh = GradTall<INT4, WM, WK, RB, SR, BN, STG>;
   const dim3 grid(mm_cdiv(K, GR_COLS), mm_cdiv(M, Sh::BM), p.ks);
   int grp = 1;
   while (grp * 2 <= (int)grid.y && grp < 4) grp *= 2;
   hipLaunchKernelGGL((k_grad<INT4, ROWS, WM, WK, RB, SR, BN, STG>), grid, dim3(Sh::NTHR), 0, st, s,
                      out, ot, rowmul, M, K, g, p.per, grp, (float*)((char*)ws + GR_COUNTER_BYTES),
+                     (uint32_t*)ws);
+  MM_CHECK_LAUNCH("gemm backward");
+  return 0;
+}
+
+template <bool INT4, bool ROWS, int SR, int STG>
+int launch_grad_narrow(const GradSegs& s, void* out, int ot, const float* rowmul, int M, int K,
+                       int g, const GradPlan& p, void* ws, hipStream_t st) {
+  const dim3 grid(mm_cdiv(K, GN_COLS), mm_cdiv(M, GN_BM), p.ks);
+  int grp = 1;
+  while (grp * 2 <= (int)grid.y && grp < 4) grp *= 2;
+  hipLaunchKernelGGL((k_grad_narrow<INT4, ROWS, SR, STG>), grid, dim3(GN_NTHR), 0, st, s, out, ot,
+                     rowmul, M, K, g, p.per, grp, (float*)((char*)ws + GR_COUNTER_BYTES),
                      (uint32_t*)ws);
   MM_CHECK_LAUNCH("gemm backward");
   return 0;
@@ -885,6 +1133,13 @@ int dispatch_grad(const GradSegs& s, void* out, int ot, const float* rowmul, int
     if (p.spw == 2) MM_GRAD_S(2, 2);
     MM_GRAD_S(2, 4);
   }
+#define MM_GRAD_N(...) \
+  return launch_grad_narrow<INT4, ROWS, __VA_ARGS__>(s, out, ot, rowmul, M, K, g, p, ws, st)
+  if (p.kind == G_NARROW) {
+    if (g >= 64) MM_GRAD_N(4, 3);
+    if (g >= 32) MM_GRAD_N(8, INT4 ? 2 : 3);
+    MM_GRAD_N(16, 2);
+  }
   if (g >= 32) {
     if (p.kind == G_256) MM_GRAD(2, 1, 4, 8, 64, 3);
     MM_GRAD(1, 4, 2, 8, 128, 3);
@@ -892,6 +1147,7 @@ int dispatch_grad(const GradSegs& s, void* out, int ot, const float* rowmul, int
   if (p.kind == G_256) MM_GRAD(2, 1, 4, 32, 64, 3);
   MM_GRAD(1, 4, 2, 32, 128, 3);
 #undef MM_GRAD_S
+#undef MM_GRAD_N
 #undef MM_GRAD
 }
 
