@@ -108,6 +108,30 @@ def test_rowpacked(M, N, K, g, dtype):
     assert torch.equal(out, marlin)
 
 
+# Sizes at which the time model takes each tile (64 x 128, 64 x 256, 256 x 256), whole and split,
+# with chunks that end inside a tile, small groups and large.
+TILES = [(64, 2056, 480, 8), (256, 2056, 480, 48), (70, 4104, 96, 96), (64, 8200, 480, 24),
+         (256, 8200, 480, 32), (1000, 264, 2080, 8), (1030, 520, 2080, 104), (2050, 200, 4096, 16),
+         (2050, 520, 4096, 64), (1000, 8200, 2080, 32)]
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "int4", "rows"])
+@pytest.mark.parametrize("M,N,K,g", TILES)
+def test_tiles(M, N, K, g, fmt):
+    announce(f"tiles {M} {N} {K} {g} {fmt}")
+    gen = torch.Generator().manual_seed(M + N + K)
+    dC = torch.randn((M, N), generator=gen).to(DEV, F16)
+    if fmt == "int4":
+        words, scales, zeros, W = make_int4(gen, K, N, g)
+        out = mmfp4.marlin_gemm_int4_backward(dC, words, scales, zeros, g)
+    else:
+        words, scales, W = make_fp4(gen, K, N, g, rows=fmt == "rows")
+        call = mmfp4.mmfp4_gemm_rowpacked_backward if fmt == "rows" else \
+            mmfp4.marlin_gemm_fp4_backward
+        out = call(dC, words, scales, g)
+    check_linear(out, dC, W, F16, fmt)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("M,Ns", [(1, (512, 128, 128)), (50, (72, 8, 40)), (260, (256, 65, 64))])
 def test_qkv(M, Ns, dtype):
