@@ -1194,6 +1194,7 @@ extern "C" int mm_gemm_backward(const uint16_t* const* dC, const int* ldc,
           (Z != nullptr ? (uintptr_t)Z[i] : 0);
   }
   MM_CHECK_ARG((al & 15) == 0, "%s: every operand must be 16-byte aligned", who);
+  MM_CHECK_ARG(M <= 64 * 65535, "%s: M=%d is too large", who, M);
   // the kernels address a tile (256 gradient rows, 32 word rows or 128 columns) with 32 bits
   for (int i = 0; i < nmat; ++i)
     MM_CHECK_ARG(ldc[i] < (1 << 22) && N[i] < (1 << 24) && (layout == 0 || K < (1 << 24)),

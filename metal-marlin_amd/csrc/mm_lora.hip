@@ -5,8 +5,8 @@
 // with A [L, r, K], B [L, N, r], s = scale * scaling[a] (scaling fp32 [L], or none).
 //
 // Few tokens: every token on its own, one launch of fp32 dot products (k_vec) or two
-// (k_vec_down, k_vec_up).  Otherwise the tokens are sorted by adapter and cut into tiles of 64 of one
-// adapter (k_plan), and
+// (k_vec_down, k_vec_up).  Otherwise the tokens are sorted by adapter and cut into tiles of 64
+// of one adapter (k_plan), and
 //   k_down   H of a tile, over the whole width: 16x16x32 MFMAs, the width split over the
 //            waves and over blocks.  The block that finishes a tile leaves a record of it:
 //            H as hi + lo in the operands' type, under one power of two per tile that puts
@@ -204,7 +204,7 @@ k_plan(Ids ids, int T, int max_tiles, TileInfo* __restrict__ tiles, int* __restr
       const uint64_t live = __ballot(g >= 0);
       if (live == 0) continue;
       if (__ballot(g == g0) == live) {
-        if (lane == 0) cnt[wave][g0] += __popcll(live);
+        if (lane == 0) atomicAdd(&cnt[wave][g0], __popcll(live));
       } else if (g >= 0) {
         atomicAdd(&cnt[wave][g], 1);
       }
@@ -543,7 +543,8 @@ MM_DEV void down_tile(const DownProblem& p, const Plan& plan, const Scaling& sca
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       h[k][i] = row < t.rows && r0 + rank + i < r ? h[k][i] * s : 0.0f;
-      m = fmaxf(m, fabsf(h[k][i]));
+      const float a = fabsf(h[k][i]);
+      m = a < __builtin_inff() ? fmaxf(m, a) : m;   // a non-finite token leaves the others their bits
     }
   }
 #pragma unroll
@@ -553,7 +554,7 @@ MM_DEV void down_tile(const DownProblem& p, const Plan& plan, const Scaling& sca
 #pragma unroll
   for (int w = 0; w < LO_DW; ++w) m = fmaxf(m, s_max[w]);
   int ex = 0;
-  if (m > 0.0f && m < __builtin_inff()) {
+  if (m > 0.0f) {
     (void)frexpf(m, &ex);                      // m = f * 2^ex, f in [0.5, 1)
     ex = max(-110, min(110, 15 - ex));
   }
@@ -980,8 +981,8 @@ k_vec(const uint16_t* __restrict__ X, const uint16_t* __restrict__ A,
 }
 
 // ---------------------------------------------------------------------------
-// Few tokens, two launches.  k_vec_down: block (token, RG ranks), the width over 256 threads; H fp32
-// [T, r].  k_vec_up: block (256 columns, token), a column per thread.
+// Few tokens, two launches.  k_vec_down: block (token, RG ranks), the width over 256 threads;
+// H fp32 [T, r].  k_vec_up: block (256 columns, token), a column per thread.
 // ---------------------------------------------------------------------------
 template <int T, int RG>
 __global__ void __launch_bounds__(LO_NT)
@@ -1141,6 +1142,9 @@ int check_common(const char* who, int type, int T, int K, int N, int r, int L, c
   MM_CHECK_ARG(L <= LO_MAX_ADAPTERS, "%s: at most %d adapters, got %d", who, LO_MAX_ADAPTERS, L);
   MM_CHECK_ARG(T <= (1 << 24) && K <= (1 << 24) && N <= (1 << 24) && r <= (1 << 12),
                "%s: T=%d, K=%d, N=%d or rank=%d is too large", who, T, K, N, r);
+  // an adapter's factors are addressed with 32 bits
+  MM_CHECK_ARG((long)r * K < (1L << 31) && (long)r * N < (1L << 31),
+               "%s: rank=%d times K=%d or N=%d is too large", who, r, K, N);
   return 0;
 }
 

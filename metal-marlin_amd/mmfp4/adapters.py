@@ -162,7 +162,7 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_
     """The gradients of lora_add for dy [*, N]: (dx [*, K], da, db), da and db shaped and typed
     as lora_a and lora_b (zeros for adapters without tokens), dx of x's type.  dx_base, the
     gradient that reached x through the projection itself (marlin_gemm_fp4_backward), is
-    added to dx before it is rounded.  dy is rounded to the type that x is computed in: fp32
+    added to dx before it is rounded (in fp32 for an fp32 x).  dy is rounded to the type that x is computed in: fp32
     gradients are computed as fp16 and want a loss scale, fp32 factors beside fp16 or bf16
     tokens get fp32 gradients."""
     if isinstance(x, torch.Tensor):
@@ -186,7 +186,10 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_
         st, factor = _scaling(scaling, L, dev)
         xf, dyf = (t.reshape(-1, t.shape[-1]).to(dt).contiguous() for t in (x, dy))
         T = xf.shape[0]
-        dxb = None if dx_base is None else dx_base.reshape(T, K).to(dt).contiguous()
+        # an fp32 x: its own gradient has come through fp16, what arrives beside it has not
+        late = dx_base if x.dtype == torch.float32 else None
+        dxb = None if dx_base is None or late is not None else \
+            dx_base.reshape(T, K).to(dt).contiguous()
         ac, bc = a.to(dt).contiguous(), b.to(dt).contiguous()
         if T == 0:
             return x.new_empty(x.shape), torch.zeros_like(lora_a), torch.zeros_like(lora_b)
@@ -202,5 +205,6 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_
                   _lib.ptr(bc), _lib.ptr(ids), int(ids is not None and ids.dtype == torch.int64),
                   _lib.ptr(st), factor, _lib.ptr(dxb), _lib.ptr(dx), _lib.ptr(da), _lib.ptr(db),
                   _TYPES[gt], T, K, N, r, L, _lib.ptr(ws), ws.numel(), stream)
-    return (dx.view(x.shape).to(x.dtype), da.view(lora_a.shape).to(lora_a.dtype),
+    dx = dx.view(x.shape).to(x.dtype)
+    return (dx if late is None else dx + late, da.view(lora_a.shape).to(lora_a.dtype),
             db.view(lora_b.shape).to(lora_b.dtype))

@@ -22,19 +22,38 @@ __all__ = ["linear", "gate_up_swiglu", "LoraAdd", "LoraLinear"]
 
 
 def refuse_foreign_leaf(*tensors: torch.Tensor | None) -> None:
-    """Under graph capture, raises for a leaf whose gradient accumulator lives on another
-    stream than the captured one."""
-    if not torch.cuda.is_current_stream_capturing():
-        return
+    """Under graph capture, raises for a leaf behind `tensors` whose gradient accumulator lives
+    on another stream than the captured one."""
     b = _lib.binding()
+    if b is None or not torch.cuda.is_current_stream_capturing():
+        return
+    for t in _leaves(tensors):
+        stream = b.accumulator_stream(t)
+        if stream >= 0 and stream != torch.cuda.current_stream(t.device).stream_id:
+            raise RuntimeError(
+                "backward under graph capture: a leaf's gradient accumulator belongs to "
+                "another stream, because a graph built there is still alive. Drop it (del "
+                "its outputs) before capturing, or build it on the capture stream too")
+
+
+def _leaves(tensors):
+    """The leaves on the device that gradients of `tensors` will reach."""
+    seen, nodes = set(), []
     for t in tensors:
-        if isinstance(t, torch.Tensor) and t.is_leaf and t.requires_grad and b is not None:
-            stream = b.accumulator_stream(t)
-            if stream >= 0 and stream != torch.cuda.current_stream(t.device).stream_id:
-                raise RuntimeError(
-                    "backward under graph capture: a leaf's gradient accumulator belongs to "
-                    "another stream, because a graph built there is still alive. Drop it (del "
-                    "its outputs) before capturing, or build it on the capture stream too")
+        if isinstance(t, torch.Tensor) and t.requires_grad:
+            if t.is_leaf:
+                yield t
+            else:
+                nodes.append(t.grad_fn)
+    while nodes:
+        node = nodes.pop()
+        if node is None or node in seen:
+            continue
+        seen.add(node)
+        leaf = getattr(node, "variable", None)
+        if isinstance(leaf, torch.Tensor) and leaf.is_cuda:
+            yield leaf
+        nodes += [n for n, _ in node.next_functions]
 
 
 def wants_grad(*tensors: torch.Tensor | None) -> bool:

@@ -226,3 +226,20 @@ def test_capture_beside_a_living_graph_is_refused():
                 m(x, ids)
     torch.cuda.synchronize()
     assert alive.isfinite().all()
+
+
+def test_capture_behind_other_operations_is_refused():
+    """The same where the leaf lies behind torch's own operations."""
+    gen = torch.Generator().manual_seed(8)
+    layer = next(iter(layers(gen, 64, 64, 64)))[1]
+    p = torch.randn((5, 64), generator=gen).to(DEV, F16).requires_grad_(True)
+    alive = p * 2
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with pytest.raises(RuntimeError, match="another stream"):
+            with torch.cuda.graph(graph, stream=side):
+                layer((p + 1).relu())
+    torch.cuda.synchronize()
+    assert alive.isfinite().all()

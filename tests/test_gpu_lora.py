@@ -210,6 +210,33 @@ def test_non_finite_tokens_stay_by_themselves(T):
     assert out.isfinite().all()
 
 
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_non_finite_tokens_leave_the_others_their_bits(bad):
+    """Small H beside an infinite one in the same tile: 1e-5 would be a subnormal of fp16."""
+    c = Case(4200, 64, 72, 8, 1, F16, x_scale=1e-5, ids=torch.zeros(4200, dtype=torch.int64))
+    c.b *= 100
+    c.base.zero_()
+    clean = mmfp4.lora_add(c.base, c.x, c.a, c.b, c.ids, c.s)
+    row = c.x[5].clone()
+    c.x[5, 3] = bad
+    out = mmfp4.lora_add(c.base, c.x, c.a, c.b, c.ids, c.s)
+    assert not out[5].isfinite().any()
+    c.x[5], out[5] = row, clean[5]
+    check_add(c, out)
+
+
+def test_fp32_base_of_dx_stays_fp32():
+    """What reaches an fp32 x through the projection does not pass through fp16."""
+    c = Case(70, 64, 48, 8, 2, F32)
+    dx, da, db = mmfp4.lora_backward(c.dy, c.x, c.a, c.b, c.ids, c.s)
+    small = c.dx_base * 1e-9
+    got = mmfp4.lora_backward(c.dy, c.x, c.a, c.b, c.ids, c.s, dx_base=small)
+    assert got[0].dtype == F32 and torch.equal(got[0], dx + small)
+    assert torch.equal(got[1], da) and torch.equal(got[2], db)
+    none = (c.ids < 0) | (c.ids >= 2)
+    assert none.any() and torch.equal(got[0][none], small[none])
+
+
 def test_forms_of_the_operands():
     """Leading axes, strides, odd offsets, factors of another type, fp32 tokens, no tokens."""
     c = Case(12, 64, 72, 8, 3, F16)

@@ -36,7 +36,7 @@ def backward(nmat=1, N=(64,), ldc=(64,), layout=0, out_type=1, M=4, K=64, g=32, 
     ({"K": 60}, "divisible by 8"), ({"K": 72, "layout": 1, "g": 8}, "divisible by 32"),
     ({"g": 12}, "group_size"), ({"g": 48}, "group_size"), ({"a": 8}, "aligned"),
     ({"layout": 1, "z": table(16)}, "zero points"), ({"M": -1}, "bad shape"),
-    ({"ldc": (1 << 23,)}, "too long"),
+    ({"ldc": (1 << 23,)}, "too long"), ({"M": 1 << 23}, "too large"),
     ({"M": 4, "K": 256, "N": (65536,), "ldc": (65536,)}, "workspace"),
 ])
 def test_backward_product(kw, msg):
@@ -69,7 +69,8 @@ def lora(T=4, K=64, N=64, r=8, L=2, type=1, base_type=1, ids=P16, ids64=0, out=P
     ({"type": 0}, "type"), ({"base_type": 2}, "base_type"), ({"K": 0}, "bad shape"),
     ({"r": 0}, "bad shape"), ({"L": 0}, "bad shape"), ({"T": -1}, "bad shape"),
     ({"ids": None}, "need ids"), ({"L": 1025}, "at most 1024"), ({"ids64": 2}, "ids64"),
-    ({"r": 5000}, "too large"), ({"type": 2, "base": P16}, "in place"), ({}, "workspace"),
+    ({"r": 5000}, "too large"), ({"r": 4096, "K": 1 << 20}, "too large"),
+    ({"r": 4096, "N": 1 << 20}, "too large"), ({"type": 2, "base": P16}, "in place"), ({}, "workspace"),
 ])
 def test_adapters(kw, msg):
     with pytest.raises(ValueError, match=msg):
