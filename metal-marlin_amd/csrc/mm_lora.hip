@@ -289,6 +289,102 @@ k_plan(Ids ids, int T, int max_tiles, TileInfo* __restrict__ tiles, int* __restr
   }
 }
 
+// The same for up to DP_TOKENS tokens, by each block of k_down for its own tile: a launch less,
+// and a pass over the ids costs a block less than the launch.  Block (b, 0, 0) also leaves tile
+// b's entry and list, and block 0 the first tiles, for the kernels that follow.
+// us, a launch of its own / this: forward of 256 tokens of 4 adapters, 4096 -> 4096, rank 16
+// 17.9 / 15.1; 2000 tokens 26.7 / 24.5; 1111 tokens, 14336 -> 4096, rank 64 41.9 / 39.0; backward
+// of 777 tokens, 2048 -> 5632, rank 8 23.9 / 20.8; with several blocks to a CU the other way, 128
+// tokens of 8 adapters, 4096 -> 14336, rank 64, 71.6 / 74.5; 4000 tokens no gain.
+constexpr int DP_NT = 64 * LO_DW, DP_HOLD = 4, DP_TOKENS = DP_NT * DP_HOLD;
+struct PlanOut {
+  Ids ids;             // ids.p == nullptr: the plan is there
+  TileInfo* tiles;
+  int *tokens, *first;
+};
+MM_DEV TileInfo own_tile(const PlanOut& o, int T, int b, bool write, int* cnt, int* list) {
+  __shared__ int wsum[LO_DW], found[3];        // group, first row, rows
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int L = o.ids.L, G = L + 1;
+  const int steps = mm_cdiv(T, DP_NT), t0 = wave * steps * 64 + lane;
+  int64_t raw[DP_HOLD];
+  int hold[DP_HOLD];
+#pragma unroll
+  for (int i = 0; i < DP_HOLD; ++i)
+    raw[i] = i < steps ? o.ids.raw(min(t0 + 64 * i, T - 1)) : -1;
+  for (int i = tid; i < LO_DW * G; i += DP_NT) cnt[i] = 0;
+  if (tid == 0) found[0] = -1;
+#pragma unroll
+  for (int i = 0; i < DP_HOLD; ++i)
+    hold[i] = i < steps && t0 + 64 * i < T ? (raw[i] >= 0 && raw[i] < L ? (int)raw[i] : L) : -1;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < DP_HOLD; ++i) {
+    const int g = hold[i], g0 = __builtin_amdgcn_readfirstlane(g);
+    const uint64_t live = __ballot(g >= 0);
+    if (live == 0) continue;
+    if (__ballot(g == g0) == live) {
+      if (lane == 0) atomicAdd(&cnt[wave * G + g0], __popcll(live));
+    } else if (g >= 0) {
+      atomicAdd(&cnt[wave * G + g], 1);
+    }
+  }
+  __syncthreads();
+  constexpr int PER = (LO_MAX_ADAPTERS + 2 + DP_NT - 1) / DP_NT;   // groups of a thread, entry G
+  int n[PER], nt = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    n[k] = 0;
+    if (PER * tid + k < G)
+#pragma unroll
+      for (int w = 0; w < LO_DW; ++w) n[k] += cnt[w * G + PER * tid + k];
+    nt += mm_cdiv(n[k], LO_TM);
+  }
+  int at = nt;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int v = __shfl_up(at, d);
+    if (lane >= d) at += v;
+  }
+  if (lane == 63) wsum[wave] = at;
+  __syncthreads();
+  at -= nt;
+  for (int w = 0; w < wave; ++w) at += wsum[w];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int g = PER * tid + k, tiles = mm_cdiv(n[k], LO_TM);
+    if (write && b == 0 && g <= G) o.first[g] = at;
+    if (b >= at && b < at + tiles) {
+      found[0] = g;
+      found[1] = (b - at) * LO_TM;
+      found[2] = min(LO_TM, n[k] - found[1]);
+    }
+    at += tiles;
+  }
+  __syncthreads();
+  const TileInfo t{found[0], found[0] < 0 ? 0 : found[2]};
+  if (write && tid == 0) o.tiles[b] = t;
+  if (t.e < 0) return t;
+  int row = -found[1];
+  for (int w = 0; w < wave; ++w) row += cnt[w * G + t.e];
+#pragma unroll
+  for (int i = 0; i < DP_HOLD; ++i) {
+    const uint64_t m = __ballot(hold[i] == t.e);
+    const int mine = row + __popcll(m & (((uint64_t)1 << lane) - 1));
+    if (hold[i] == t.e && mine >= 0 && mine < LO_TM) list[mine] = t0 + 64 * i;
+    row += __popcll(m);
+  }
+  __syncthreads();
+  if (tid < LO_TM) {
+    const int token = list[min(tid, t.rows - 1)];
+    if (write) o.tokens[LO_TM * b + tid] = token;
+    if (tid >= t.rows) list[tid] = token;
+  }
+  __syncthreads();
+  return t;
+}
+
 // The records of a launch's tiles; rp ranks (of a chunk) each, nrc chunks.
 struct Records {
   uint16_t* by_token;   // [tile][chunk][hi, lo][64][rp]
@@ -336,9 +432,21 @@ struct DownProblem {
 template <int RT>
 constexpr int down_lds_wave() { return LO_TM * 128 + 64 * (32 * RT + 16); }
 
+// Tokens at[k] of tile b: of own_tile's list in LDS, or of the plan.
+template <int N>
+MM_DEV void tokens_of(const Plan& plan, const int* list, int b, const int (&at)[N],
+                      int (&tok)[N]) {
+  if (list == nullptr) {
+    plan.get(b, at, tok);
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) tok[k] = list[at[k]];
+}
+
 template <int T, bool CR, int RT, int NR>
-MM_DEV void down_sum(const DownProblem& p, const Plan& plan, int b, int e, int r, int r0,
-                     char* lds, f32x4 (&acc)[4][RT]) {
+MM_DEV void down_sum(const DownProblem& p, const Plan& plan, const int* list, int b, int e,
+                     int r, int r0, char* lds, f32x4 (&acc)[4][RT]) {
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint16_t* W = p.W + (size_t)e * r * p.C;
@@ -352,7 +460,7 @@ MM_DEV void down_sum(const DownProblem& p, const Plan& plan, int b, int e, int r
     int at[NX], tok[NX];
 #pragma unroll
     for (int i = 0; i < NX; ++i) at[i] = 8 * i + (lane >> 3);
-    plan.get(b, at, tok);
+    tokens_of(plan, list, b, at, tok);
 #pragma unroll
     for (int i = 0; i < NX; ++i) v[i] = p.V + (size_t)tok[i] * p.C + 8 * (lane & 7);
     uint32_t woff[NW], wlds[NW];   // element offset of the lane's pieces at k = 0, place in LDS
@@ -440,7 +548,7 @@ MM_DEV void down_sum(const DownProblem& p, const Plan& plan, int b, int e, int r
   int at[NR], tok[NR];
 #pragma unroll
   for (int i = 0; i < NR; ++i) at[i] = 16 * i + c;
-  plan.get(b, at, tok);
+  tokens_of(plan, list, b, at, tok);
 #pragma unroll
   for (int i = 0; i < NR; ++i) v[i] = p.V + (size_t)tok[i] * p.C;
   const int direct_end = min(mm_cdiv(p.C, 64), beg + p.per);
@@ -466,23 +574,20 @@ MM_DEV void down_sum(const DownProblem& p, const Plan& plan, int b, int e, int r
 }
 
 template <int T, bool CR, int RT>
-MM_DEV void down_tile(const DownProblem& p, const Plan& plan, const Scaling& scaling, int r,
-                      int chunk, float* lds) {
+MM_DEV void down_tile(const DownProblem& p, const Plan& plan, const int* list, TileInfo t,
+                      const Scaling& scaling, int r, int chunk, float* lds) {
   constexpr int RP = 16 * RT, NT = 64 * LO_DW, ITEMS = LO_TM * RP / 4;   // f32x4 items
   constexpr int PER = ITEMS / NT > 0 ? ITEMS / NT : 1;                   // per thread
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, q = lane >> 4;
-  const int b = blockIdx.x;
-  const TileInfo t = plan.tile(b);
-  if (t.e < 0 || t.e >= plan.L) return;
-  const int r0 = chunk * RP;
+  const int b = blockIdx.x, r0 = chunk * RP;
   f32x4 acc[4][RT];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int k = 0; k < RT; ++k) acc[i][k] = f32x4{0, 0, 0, 0};
-  if (t.rows > 32) down_sum<T, CR, RT, 4>(p, plan, b, t.e, r, r0, (char*)lds, acc);
-  else if (t.rows > 16) down_sum<T, CR, RT, 2>(p, plan, b, t.e, r, r0, (char*)lds, acc);
-  else down_sum<T, CR, RT, 1>(p, plan, b, t.e, r, r0, (char*)lds, acc);
+  if (t.rows > 32) down_sum<T, CR, RT, 4>(p, plan, list, b, t.e, r, r0, (char*)lds, acc);
+  else if (t.rows > 16) down_sum<T, CR, RT, 2>(p, plan, list, b, t.e, r, r0, (char*)lds, acc);
+  else down_sum<T, CR, RT, 1>(p, plan, list, b, t.e, r, r0, (char*)lds, acc);
   __syncthreads();   // every wave is done with its staging area
   // Sum over the waves, half of them at a time: lds[wave % 4][token][rank].
   uint32_t* s_last = (uint32_t*)(lds + 4 * LO_TM * RP);
@@ -589,14 +694,25 @@ MM_DEV void down_tile(const DownProblem& p, const Plan& plan, const Scaling& sca
 
 template <int T, int RT>
 __global__ void __launch_bounds__(64 * LO_DW)
-k_down(DownProblem p0, DownProblem p1, Plan plan, Scaling scaling, int r) {
+k_down(DownProblem p0, DownProblem p1, Plan plan, PlanOut own, Scaling scaling, int r) {
   constexpr int SUM = 4 * LO_TM * 16 * RT + 4 + LO_DW, STAGE = LO_DW * down_lds_wave<RT>() / 4;
+  static_assert(LO_DW * (LO_MAX_ADAPTERS + 1) <= STAGE, "own_tile's counts");
   __shared__ __attribute__((aligned(16))) float lds[SUM > STAGE ? SUM : STAGE];
   const int nrc = p0.rec.nrc;
   const bool second = (int)blockIdx.z >= nrc;
   if ((int)blockIdx.y >= (second ? p1.ks : p0.ks)) return;
-  if (!second) down_tile<T, false, RT>(p0, plan, scaling, r, blockIdx.z, lds);
-  else down_tile<T, true, RT>(p1, plan, scaling, r, blockIdx.z - nrc, lds);
+  __shared__ int list[LO_TM];
+  const int* own_list = nullptr;
+  TileInfo t;
+  if (own.ids.p != nullptr) {
+    t = own_tile(own, plan.T, blockIdx.x, blockIdx.y == 0 && blockIdx.z == 0, (int*)lds, list);
+    own_list = list;
+  } else {
+    t = plan.tile(blockIdx.x);
+  }
+  if (t.e < 0 || t.e >= plan.L) return;
+  if (!second) down_tile<T, false, RT>(p0, plan, own_list, t, scaling, r, blockIdx.z, lds);
+  else down_tile<T, true, RT>(p1, plan, own_list, t, scaling, r, blockIdx.z - nrc, lds);
 }
 
 // ---------------------------------------------------------------------------
@@ -1148,18 +1264,23 @@ int check_common(const char* who, int type, int T, int K, int N, int r, int L, c
   return 0;
 }
 
-// Sorts the tokens by adapter (none needed for a single adapter without ids).
+// The tokens sorted by adapter: by a launch, by k_down's blocks (`own`), or as they come (a
+// single adapter without ids).
 int make_plan(const char* who, const LoraPlan& p, const void* ids, int ids64, int T, int L,
-              void* ws, hipStream_t st, Plan* plan) {
+              void* ws, hipStream_t st, Plan* plan, PlanOut* own) {
   *plan = Plan{nullptr, nullptr, nullptr, T, L};
+  *own = PlanOut{};
   if (ids == nullptr) return 0;
-  TileInfo* tiles = (TileInfo*)((char*)ws + LO_COUNTER_BYTES);
-  int* tokens = (int*)((char*)ws + p.tokens);
-  int* first = (int*)((char*)ws + p.first);
-  hipLaunchKernelGGL(k_plan, dim3(1), dim3(PL_NT), 0, st, Ids{ids, ids64, L}, T, p.all, tiles,
-                     tokens, first);
+  const PlanOut o{Ids{ids, ids64, L}, (TileInfo*)((char*)ws + LO_COUNTER_BYTES),
+                  (int*)((char*)ws + p.tokens), (int*)((char*)ws + p.first)};
+  *plan = Plan{o.tiles, o.tokens, o.first, T, L};
+  if (T <= DP_TOKENS) {
+    *own = o;
+    return 0;
+  }
+  hipLaunchKernelGGL(k_plan, dim3(1), dim3(PL_NT), 0, st, o.ids, T, p.all, o.tiles, o.tokens,
+                     o.first);
   MM_CHECK_LAUNCH(who);
-  *plan = Plan{tiles, tokens, first, T, L};
   return 0;
 }
 
@@ -1232,14 +1353,16 @@ extern "C" int mm_lora_add(const uint16_t* x, int type, const uint16_t* base, in
   }
   const LoraPlan p = plan_lora(T, K, N, r, L, false);
   Plan plan;
-  if (const int rc = make_plan(who, p, ids, ids64, T, L, ws, st, &plan)) return rc;
+  PlanOut own;
+  if (const int rc = make_plan(who, p, ids, ids64, T, L, ws, st, &plan, &own)) return rc;
+  const int down_tiles = own.ids.p != nullptr ? p.all : p.tiles;
   const Records rec = record_at(p, (char*)ws + p.rec[0]);
   const int ks = p.kx;
   const DownProblem d{x, A, K, ks, p.per, rec, (float*)((char*)ws + p.part),
                       (uint32_t*)ws, 1, 0};
 #define MM_DOWN(RTV, TV)                                                                       \
-  hipLaunchKernelGGL((k_down<TV, RTV>), dim3(p.tiles, ks, p.nrc), dim3(64 * LO_DW), 0, st, d, d, \
-                     plan, sc, r)
+  hipLaunchKernelGGL((k_down<TV, RTV>), dim3(down_tiles, ks, p.nrc), dim3(64 * LO_DW), 0, st, d,  \
+                     d, plan, own, sc, r)
   if (type == 1) { MM_LORA_RT(MM_DOWN, 1) } else { MM_LORA_RT(MM_DOWN, 2) }
   MM_CHECK_LAUNCH(who);
   const UpProblem u{B, base, out, N, rec};
@@ -1272,7 +1395,9 @@ extern "C" int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type,
   const Scaling sc{scaling, scale};
   const LoraPlan p = plan_lora(T, K, N, r, L, true);
   Plan plan;
-  if (const int rc = make_plan(who, p, ids, ids64, T, L, ws, st, &plan)) return rc;
+  PlanOut own;
+  if (const int rc = make_plan(who, p, ids, ids64, T, L, ws, st, &plan, &own)) return rc;
+  const int down_tiles = own.ids.p != nullptr ? p.all : p.tiles;
   const Records rx = record_at(p, (char*)ws + p.rec[0]), ry = record_at(p, (char*)ws + p.rec[1]);
   float* part = (float*)((char*)ws + p.part);
   uint32_t* counters = (uint32_t*)ws;
@@ -1282,8 +1407,8 @@ extern "C" int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type,
   const DownProblem py{dy, B, N, ky, p.per, ry, part + tile * kx,
                        counters + LO_SPLIT_BELOW, 1, 1};
 #define MM_DOWN(RTV, TV)                                                                       \
-  hipLaunchKernelGGL((k_down<TV, RTV>), dim3(p.tiles, std::max(kx, ky), 2 * p.nrc),              \
-                     dim3(64 * LO_DW), 0, st, px, py, plan, sc, r)
+  hipLaunchKernelGGL((k_down<TV, RTV>), dim3(down_tiles, std::max(kx, ky), 2 * p.nrc),             \
+                     dim3(64 * LO_DW), 0, st, px, py, plan, own, sc, r)
   if (type == 1) { MM_LORA_RT(MM_DOWN, 1) } else { MM_LORA_RT(MM_DOWN, 2) }
 #undef MM_DOWN
   MM_CHECK_LAUNCH(who);
