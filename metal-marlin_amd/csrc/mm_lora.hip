@@ -839,22 +839,37 @@ struct GradProblem {
   const uint16_t* V;    // [T, C]
   void* G;              // [L, r, C] or, CR, [L, C, r]; fp32 or the operands' type
   int C, ks, f32;
+  int wide;             // every wave has 64 columns of its own and all of the adapter's tokens
   Records rec;
   float* part;          // [adapter][chunk][column block][ks][64 * rp]
   uint32_t* counters;   // [adapter][chunk][column block]
+
+  MM_DEV int cols() const { return mm_cdiv(C, wide ? 4 * LO_WG_COLS : LO_WG_COLS); }
+  // n of four adjacent values of the gradient.
+  template <int T>
+  MM_DEV void store(size_t at, f32x4 v, bool whole, int n) const {
+    if (f32) {
+      float* o = (float*)G + at;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < n) o[i] = v[i];
+      return;
+    }
+    u16x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = from_f32<T>(v[i]);
+    if (whole) *(u16x4_any*)((uint16_t*)G + at) = o;
+    else store4((uint16_t*)G + at, o, n);
+  }
 };
 
-template <int T, bool CR, int RT, bool WHOLE>
-MM_DEV void wgrad_tile(const GradProblem& p, const Plan& plan, int r, int colblock, int e,
-                       int chunk, int split, f32x4* lds) {
+// sum[k][j]: ranks 16 k + 4 q + i of column n0 + j, over the steps st, st + stride, .. < s_end of
+// 32 tokens each, from the adapter's first tile tb on.
+template <int T, int RT, bool WHOLE>
+MM_DEV void wgrad_sum(const GradProblem& p, const Plan& plan, int n0, int tb, int chunk, int st,
+                      int stride, int s_end, f32x4 (&sum)[RT][4]) {
   constexpr int RP = 16 * RT;
-  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = colblock * LO_WG_COLS + 4 * c, left = p.C - n0;
-  const int tb = plan.first_tile(e), nt = plan.first_tile(e + 1) - tb;
-  const int steps = 2 * nt, per = mm_cdiv(steps, p.ks);
-  const int s_end = min(steps, (split + 1) * per);
-  f32x4 sum[RT][4];
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4, left = p.C - n0;
 #pragma unroll
   for (int k = 0; k < RT; ++k)
 #pragma unroll
@@ -895,25 +910,38 @@ MM_DEV void wgrad_tile(const GradProblem& p, const Plan& plan, int r, int colblo
         sum[k][j] += o.f * mfma<T>(o.hi[k], w[j], mfma<T>(o.lo[k], w[j], f32x4{0, 0, 0, 0}));
   };
   Step even, odd;
-  int st = split * per + wave;
   if (st < s_end) {
     const int last = s_end - 1;
     find(st);
     load(even, st);
-    find(min(st + 4, last));
+    find(min(st + stride, last));
     while (true) {
-      load(odd, min(st + 4, last));
-      find(min(st + 8, last));
+      load(odd, min(st + stride, last));
+      find(min(st + 2 * stride, last));
       __builtin_amdgcn_sched_barrier(0);
       multiply(even);
-      if ((st += 4) >= s_end) break;
-      load(even, min(st + 4, last));
-      find(min(st + 8, last));
+      if ((st += stride) >= s_end) break;
+      load(even, min(st + stride, last));
+      find(min(st + 2 * stride, last));
       __builtin_amdgcn_sched_barrier(0);
       multiply(odd);
-      if ((st += 4) >= s_end) break;
+      if ((st += stride) >= s_end) break;
     }
   }
+}
+
+template <int T, bool CR, int RT, bool WHOLE>
+MM_DEV void wgrad_tile(const GradProblem& p, const Plan& plan, int r, int colblock, int e,
+                       int chunk, int split, f32x4* lds) {
+  constexpr int RP = 16 * RT;
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = colblock * LO_WG_COLS + 4 * c, left = p.C - n0;
+  const int tb = plan.first_tile(e), nt = plan.first_tile(e + 1) - tb;
+  const int steps = 2 * nt, per = mm_cdiv(steps, p.ks);
+  f32x4 sum[RT][4];
+  wgrad_sum<T, RT, WHOLE>(p, plan, n0, tb, chunk, split * per + wave, 4,
+                          min(steps, (split + 1) * per), sum);
   // lds[wave][k, j][lane]; wave w then owns columns j = w of every rank tile.
   uint32_t* s_last = (uint32_t*)(lds + 4 * RT * 4 * 64);
 #pragma unroll
@@ -955,25 +983,11 @@ MM_DEV void wgrad_tile(const GradProblem& p, const Plan& plan, int r, int colblo
   // Wave w holds column 4c + w, ranks 4q + i.  dB has the ranks of a column side by side;
   // dA, columns side by side, goes through LDS once more.
   const size_t G = (size_t)e * r * p.C;
-  auto store = [&](size_t at, f32x4 v, bool whole, int n) {
-    if (p.f32) {
-      float* o = (float*)p.G + at;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < n) o[i] = v[i];
-      return;
-    }
-    u16x4 o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = from_f32<T>(v[i]);
-    if (whole) *(u16x4_any*)((uint16_t*)p.G + at) = o;
-    else store4((uint16_t*)p.G + at, o, n);
-  };
   if constexpr (CR) {
 #pragma unroll
     for (int k = 0; k < RT; ++k) {
       const int rank = chunk * RP + 16 * k + 4 * q;
-      if (wave < left) store(G + (size_t)(n0 + wave) * r + rank, own[k], false, r - rank);
+      if (wave < left) p.store<T>(G + (size_t)(n0 + wave) * r + rank, own[k], false, r - rank);
     }
   } else {
     float* tr = (float*)lds;   // [rank][64 columns]
@@ -988,8 +1002,32 @@ MM_DEV void wgrad_tile(const GradProblem& p, const Plan& plan, int r, int colblo
       const f32x4 v = *(const f32x4*)(tr + rank * LO_WG_COLS + col);
       const int n = colblock * LO_WG_COLS + col;
       if (chunk * RP + rank < r)
-        store(G + (size_t)(chunk * RP + rank) * p.C + n, v, WHOLE, p.C - n);
+        p.store<T>(G + (size_t)(chunk * RP + rank) * p.C + n, v, WHOLE, p.C - n);
     }
+  }
+}
+
+// The same where an adapter has few tokens: a wave takes all of them, for 64 columns of its own.
+template <int T, bool CR, int RT, bool WHOLE>
+MM_DEV void wgrad_wave(const GradProblem& p, const Plan& plan, int r, int col0, int e,
+                       int chunk) {
+  constexpr int RP = 16 * RT;
+  const int lane = threadIdx.x & 63, n0 = col0 + 4 * (lane & 15), q = lane >> 4;
+  const int tb = plan.first_tile(e), nt = plan.first_tile(e + 1) - tb;
+  f32x4 sum[RT][4];
+  wgrad_sum<T, RT, WHOLE>(p, plan, n0, tb, chunk, 0, 1, 2 * nt, sum);
+  const size_t G = (size_t)e * r * p.C;
+#pragma unroll
+  for (int k = 0; k < RT; ++k) {
+    const int rank = chunk * RP + 16 * k + 4 * q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if constexpr (CR) {
+        if (n0 + i < p.C) p.store<T>(G + (size_t)(n0 + i) * r + rank, sum[k][i], false, r - rank);
+      } else if (rank + i < r) {
+        p.store<T>(G + (size_t)(rank + i) * p.C + n0,
+                   f32x4{sum[k][0][i], sum[k][1][i], sum[k][2][i], sum[k][3][i]}, WHOLE, p.C - n0);
+      }
   }
 }
 
@@ -1003,9 +1041,25 @@ k_back(GradProblem pa, GradProblem pb, UpProblem pu, Plan plan, int r, int na, i
   int b = blockIdx.x;
   if (b < na + nb) {
     const GradProblem& p = b < na ? pa : pb;
-    const int cols = mm_cdiv(p.C, LO_WG_COLS), first = b < na ? 0 : na;
+    const int cols = p.cols(), first = b < na ? 0 : na;
     b -= first;
     const int cb = b % cols, e = b / cols % plan.L, z = b / cols / plan.L;
+    if (p.wide) {
+      const int col0 =
+          (4 * cb + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * LO_WG_COLS;
+      if (col0 >= p.C) return;
+      const bool whole = col0 + LO_WG_COLS <= p.C;
+#define MM_WGRAD(CR, P)                                                       \
+  if (whole) wgrad_wave<T, CR, RT, true>(P, plan, r, col0, e, z);              \
+  else wgrad_wave<T, CR, RT, false>(P, plan, r, col0, e, z)
+      if (first == 0 && (int)blockIdx.x < na) {
+        MM_WGRAD(false, pa);
+      } else {
+        MM_WGRAD(true, pb);
+      }
+#undef MM_WGRAD
+      return;
+    }
     const bool whole = (cb + 1) * LO_WG_COLS <= p.C;
 #define MM_WGRAD(CR, P)                                                                     \
   if (whole) wgrad_tile<T, CR, RT, true>(P, plan, r, cb, e, z / P.ks, z % P.ks, lds);        \
@@ -1199,9 +1253,18 @@ size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 int down_range(long tiles, int pairs) {
   return std::max(LO_DW, (int)((tiles * pairs + 255) / 256));
 }
+// Whether a wave of wgrad takes all of an adapter's tokens: where they are few, and the blocks
+// still a fair number.  us, backward, four waves an adapter and 64 columns / a wave: 1000 tokens of
+// 64 adapters, 4096 -> 4096, rank 16 54.9 / 38.2; 2000 of 16 37.9 / 32.8; 512 of 4, rank 64 40.7 /
+// 33.8; 4000 of 1000 771 / 452; the other way 2000 of 4, rank 16 33.0 / 35.0, 128 of 1 15.1 / 16.1.
+bool wgrad_wide(int T, int L, int nrc, int C) {
+  return T / 32 / L <= 4 && (long)mm_cdiv(C, 4 * LO_WG_COLS) * L * nrc >= 64;
+}
+
 // Splits of an adapter's tokens: while a wave has more than 16 steps of 32 on average.  us,
 // splits 1 / 2 / 4: backward of 4096 tokens 113 / 104 / 107, 2048 of 2 adapters 81 / 90 / 100.
 int wgrad_split(int T, int L, int nrc, int C) {
+  if (wgrad_wide(T, L, nrc, C)) return 1;
   const long blocks = (long)mm_cdiv(C, LO_WG_COLS) * L * nrc;
   int ks = 1;
   while (blocks * ks < LO_SPLIT_BELOW && T / 32 / L / (4 * ks) > 16) ks *= 2;
@@ -1412,10 +1475,12 @@ extern "C" int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type,
   if (type == 1) { MM_LORA_RT(MM_DOWN, 1) } else { MM_LORA_RT(MM_DOWN, 2) }
 #undef MM_DOWN
   MM_CHECK_LAUNCH(who);
-  const int ca = mm_cdiv(K, LO_WG_COLS), cb = mm_cdiv(N, LO_WG_COLS);
+  const bool wa = wgrad_wide(T, L, p.nrc, K), wb = wgrad_wide(T, L, p.nrc, N);
+  const int ca = mm_cdiv(K, wa ? 4 * LO_WG_COLS : LO_WG_COLS);
+  const int cb = mm_cdiv(N, wb ? 4 * LO_WG_COLS : LO_WG_COLS);
   const int ga = wgrad_split(T, L, p.nrc, K), gb = wgrad_split(T, L, p.nrc, N);
-  const GradProblem pa{x, dA, K, ga, grad_type == 0, ry, part, counters};
-  const GradProblem pb{dy, dB, N, gb, grad_type == 0, rx, part + (size_t)L * p.nrc * ca * ga * LO_WG_COLS * p.rp,
+  const GradProblem pa{x, dA, K, ga, grad_type == 0, wa, ry, part, counters};
+  const GradProblem pb{dy, dB, N, gb, grad_type == 0, wb, rx, part + (size_t)L * p.nrc * ca * ga * LO_WG_COLS * p.rp,
                        counters + LO_SPLIT_BELOW};
   const UpProblem pu{A, dx_base, dx, K, ry};
   const long na = (long)ca * L * p.nrc * ga, nb = (long)cb * L * p.nrc * gb;
