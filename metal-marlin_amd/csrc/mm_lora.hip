@@ -1033,8 +1033,10 @@ MM_DEV void wgrad_wave(const GradProblem& p, const Plan& plan, int r, int col0, 
 
 // The backward pass behind k_down: dA's blocks, dB's, then dx's.  They do not depend on one
 // another, and one launch lets them fill one another's gaps.
+// 256 registers, so that two waves share a SIMD: rank 64 by itself takes 309 (backward of 1111
+// tokens, 14336 -> 4096, rank 64 105 us; 85 so, with 10 of them spilled outside the loop).
 template <int T, int RT, int BT>
-__global__ void __launch_bounds__(LO_NT)
+__global__ void __launch_bounds__(LO_NT, 2)
 k_back(GradProblem pa, GradProblem pb, UpProblem pu, Plan plan, int r, int na, int nb) {
   __shared__ __attribute__((aligned(16))) f32x4 lds[4 * RT * 4 * 64 + 1];
   const int nrc = pa.rec.nrc;
