@@ -224,6 +224,10 @@ int mm_gemm_backward(const uint16_t* const* dC, const int* ldc, const float* row
  * type 0 fp32, 1 fp16, 2 bf16; N % 8 == 0. */
 int mm_grad_rows(const void* X, int type, uint16_t* Y, float* row_mul, int M, int N,
                  void* stream);
+/* The same for up to three matrices X[p] [M, N[p]] side by side: Y [M, sum N], one power of two
+ * for the whole row.  The tables are host arrays. */
+int mm_grad_rows_multi(const void* const* X, int type, int nmat, const int* N, uint16_t* Y,
+                       float* row_mul, int M, void* stream);
 
 /* Gradient of silu(g) * u, g and u the halves of gate_up [M, 2N] (mm_fp4_gate_up_keep):
  * Y[M, 2N] = [dg | du] as mm_grad_rows carries it, one power of two per row. */

@@ -920,26 +920,37 @@ MM_DEV void store8(f16* p, const float (&v)[8], float mul) {
   *(f16x8*)p = o;
 }
 
+// A row's parts, from up to three matrices: pieces of 8 up to the end of each.
+struct RowParts {
+  const void* x[3];
+  int end[3];
+  template <int T>
+  MM_DEV void load(int row, int p, float (&v)[8]) const {
+    const int i = p < end[0] ? 0 : (p < end[1] ? 1 : 2), first = i > 0 ? end[i - 1] : 0;
+    load8<T>(x[i], 8 * ((size_t)row * (end[i] - first) + (p - first)), v);
+  }
+};
+
 // One block per row; up to RW_NT * 8 * RW_HOLD columns are read once, wider rows twice.
 template <int T>
 __global__ void __launch_bounds__(RW_NT)
-k_grad_rows(const void* __restrict__ X, f16* __restrict__ Y, float* __restrict__ rowmul, int N) {
+k_grad_rows(RowParts parts, f16* __restrict__ Y, float* __restrict__ rowmul) {
   __shared__ float red[RW_NT / 64];
-  const size_t base = (size_t)blockIdx.x * N;
-  const int np = N / 8;
+  const int row = blockIdx.x, np = parts.end[2];
+  const size_t base = 8 * (size_t)row * np;
   float hold[RW_HOLD][8], m = 0.0f;
 #pragma unroll
   for (int i = 0; i < RW_HOLD; ++i) {
     const int p = threadIdx.x + i * RW_NT;
     if (p < np) {
-      load8<T>(X, base + 8 * (size_t)p, hold[i]);
+      parts.load<T>(row, p, hold[i]);
 #pragma unroll
       for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(hold[i][k]));
     }
   }
   for (int p = threadIdx.x + RW_HOLD * RW_NT; p < np; p += RW_NT) {
     float v[8];
-    load8<T>(X, base + 8 * (size_t)p, v);
+    parts.load<T>(row, p, v);
 #pragma unroll
     for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(v[k]));
   }
@@ -953,7 +964,7 @@ k_grad_rows(const void* __restrict__ X, f16* __restrict__ Y, float* __restrict__
   }
   for (int p = threadIdx.x + RW_HOLD * RW_NT; p < np; p += RW_NT) {
     float v[8];
-    load8<T>(X, base + 8 * (size_t)p, v);
+    parts.load<T>(row, p, v);
     store8(Y + base + 8 * (size_t)p, v, mul);
   }
 }
@@ -1216,23 +1227,44 @@ extern "C" int mm_gemm_backward(const uint16_t* const* dC, const int* ldc,
   return dispatch_grad<false, false>(s, dA, out_type, row_mul, M, K, g, p, ws, st);
 }
 
-extern "C" int mm_grad_rows(const void* X, int type, uint16_t* Y, float* row_mul, int M, int N,
-                            void* stream) {
+extern "C" int mm_grad_rows_multi(const void* const* X, int type, int nmat, const int* N,
+                                  uint16_t* Y, float* row_mul, int M, void* stream) {
   const char* who = "mm_grad_rows";
+  MM_CHECK_ARG(nmat >= 1 && nmat <= 3 && X != nullptr && N != nullptr,
+               "%s: nmat=%d must be 1..3", who, nmat);
   MM_CHECK_ARG(type >= 0 && type <= 2, "%s: type=%d must be 0 (fp32), 1 (fp16) or 2 (bf16)", who,
                type);
-  MM_CHECK_ARG(M >= 0 && N > 0 && N % 8 == 0, "%s: bad shape M=%d N=%d (N %% 8 == 0)", who, M, N);
-  MM_CHECK_ARG((((uintptr_t)X | (uintptr_t)Y) & 15) == 0 && ((uintptr_t)row_mul & 3) == 0,
+  RowParts parts{};
+  uintptr_t al = (uintptr_t)Y;
+  long pieces = 0;
+  for (int i = 0; i < 3; ++i) {
+    if (i < nmat) {
+      MM_CHECK_ARG(M >= 0 && N[i] > 0 && N[i] % 8 == 0,
+                   "%s: bad shape M=%d N=%d (N %% 8 == 0)", who, M, N[i]);
+      al |= (uintptr_t)X[i];
+      parts.x[i] = X[i];
+      pieces += N[i] / 8;
+    }
+    parts.end[i] = (int)pieces;
+  }
+  MM_CHECK_ARG(pieces < (1 << 28), "%s: rows are too long", who);
+  MM_CHECK_ARG((al & 15) == 0 && ((uintptr_t)row_mul & 3) == 0,
                "%s: X and Y must be 16-byte aligned", who);
   if (M == 0) return 0;
   hipStream_t st = (hipStream_t)stream;
-  switch (type) {
-    case 0: hipLaunchKernelGGL(k_grad_rows<0>, dim3(M), dim3(RW_NT), 0, st, X, (f16*)Y, row_mul, N); break;
-    case 1: hipLaunchKernelGGL(k_grad_rows<1>, dim3(M), dim3(RW_NT), 0, st, X, (f16*)Y, row_mul, N); break;
-    default: hipLaunchKernelGGL(k_grad_rows<2>, dim3(M), dim3(RW_NT), 0, st, X, (f16*)Y, row_mul, N);
-  }
+#define MM_GR(T) \
+  hipLaunchKernelGGL(k_grad_rows<T>, dim3(M), dim3(RW_NT), 0, st, parts, (f16*)Y, row_mul)
+  if (type == 0) MM_GR(0);
+  else if (type == 1) MM_GR(1);
+  else MM_GR(2);
+#undef MM_GR
   MM_CHECK_LAUNCH(who);
   return 0;
+}
+
+extern "C" int mm_grad_rows(const void* X, int type, uint16_t* Y, float* row_mul, int M, int N,
+                            void* stream) {
+  return mm_grad_rows_multi(&X, type, 1, &N, Y, row_mul, M, stream);
 }
 
 extern "C" int mm_swiglu_grad(const void* dH, int type, const uint16_t* gate_up, uint16_t* Y,

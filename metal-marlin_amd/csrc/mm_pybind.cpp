@@ -306,16 +306,42 @@ at::Tensor backward(const at::Tensor& like, int nmat, const uint16_t* const* dC,
   if (rc) fail(rc);
   return out;
 }
-// fp16 values of M x N gradients and their rows' factors (undefined: ones).
-std::pair<at::Tensor, at::Tensor> carried(const at::Tensor& d, int64_t M, int64_t N,
+// fp16 values [M, sum N] of gradients side by side, and their rows' factors.
+std::pair<at::Tensor, at::Tensor> carried(const at::Tensor* d, const int* N, int nmat, int64_t M,
                                           int64_t stream) {
-  if (d.scalar_type() == at::kHalf) return {d, at::Tensor()};
-  at::Tensor y = at::empty({M, N}, d.options().dtype(at::kHalf));
-  at::Tensor mul = at::empty({M}, d.options().dtype(at::kFloat));
-  const int rc = mm_grad_rows(d.data_ptr(), type_code(d.scalar_type()), (uint16_t*)y.data_ptr(),
-                              (float*)mul.data_ptr(), (int)M, (int)N, (void*)stream);
+  int64_t n = 0;
+  const void* x[3];
+  for (int i = 0; i < nmat; ++i) {
+    n += N[i];
+    x[i] = d[i].data_ptr();
+  }
+  at::Tensor y = at::empty({M, n}, d[0].options().dtype(at::kHalf));
+  at::Tensor mul = at::empty({M}, d[0].options().dtype(at::kFloat));
+  const int rc = mm_grad_rows_multi(x, type_code(d[0].scalar_type()), nmat, N,
+                                    (uint16_t*)y.data_ptr(), (float*)mul.data_ptr(), (int)M,
+                                    (void*)stream);
   if (rc) fail(rc);
   return {y, mul};
+}
+// dA of up to three matrices, all gradients of one type.
+at::Tensor backward_any(const at::Tensor* dC, int nmat, const Matrix* mats, bool rows, int64_t M,
+                        int64_t g, int64_t stream) {
+  const uint16_t* p[3];
+  int n[3], ld[3];
+  for (int i = 0; i < nmat; ++i) {
+    p[i] = (const uint16_t*)dC[i].data_ptr();
+    ld[i] = n[i] = (int)mats[i].N;
+  }
+  const auto type = dC[0].scalar_type();
+  if (type == at::kHalf) return backward(dC[0], nmat, p, ld, nullptr, mats, rows, M, g, type, stream);
+  const auto [y, mul] = carried(dC, n, nmat, M, stream);
+  const uint16_t* at = (const uint16_t*)y.data_ptr();
+  for (int i = 0; i < nmat; ++i) {
+    p[i] = at;
+    at += n[i];
+    ld[i] = (int)y.size(1);
+  }
+  return backward(dC[0], nmat, p, ld, (const float*)mul.data_ptr(), mats, rows, M, g, type, stream);
 }
 
 pybind11::object linear_backward(const at::Tensor& dC, const at::Tensor& W, const at::Tensor& S,
@@ -326,33 +352,25 @@ pybind11::object linear_backward(const at::Tensor& dC, const at::Tensor& W, cons
   const Matrix m = plain_matrix(W, S, Z, rows, g, dev);
   const int64_t M = m.N ? plain_rows(dC, dev, m.N) : -1;
   if (M < 0) return pybind11::none();
-  const auto [d, mul] = carried(dC, M, m.N, stream);
-  const uint16_t* p[1] = {(const uint16_t*)d.data_ptr()};
-  const int ld[1] = {(int)m.N};
-  return pybind11::cast(backward(dC, 1, p, ld, mul.defined() ? (const float*)mul.data_ptr() : nullptr,
-                                 &m, rows, M, g, dC.scalar_type(), stream));
+  return pybind11::cast(backward_any(&dC, 1, &m, rows, M, g, stream));
 }
 
 pybind11::object qkv_backward(const std::array<at::Tensor, 3>& dC,
                               const std::array<at::Tensor, 3>& W,
                               const std::array<at::Tensor, 3>& S, int64_t g, int64_t stream) {
   const int dev = (int)dC[0].get_device();
-  if (!on_current_device(dev) || dC[0].scalar_type() != at::kHalf) return pybind11::none();
+  if (!on_current_device(dev)) return pybind11::none();
   Matrix m[3];
-  const uint16_t* p[3];
-  int ld[3];
   int64_t M = 0;
   for (int i = 0; i < 3; ++i) {
     m[i] = plain_matrix(W[i], S[i], c10::nullopt, false, g, dev);
     const int64_t rows = m[i].N ? plain_rows(dC[i], dev, m[i].N) : -1;
-    if (rows < 0 || dC[i].scalar_type() != at::kHalf || m[i].K != m[0].K ||
+    if (rows < 0 || dC[i].scalar_type() != dC[0].scalar_type() || m[i].K != m[0].K ||
         dC[i].sizes().slice(0, dC[i].dim() - 1) != dC[0].sizes().slice(0, dC[0].dim() - 1))
       return pybind11::none();
     M = rows;
-    p[i] = (const uint16_t*)dC[i].data_ptr();
-    ld[i] = (int)m[i].N;
   }
-  return pybind11::cast(backward(dC[0], 3, p, ld, nullptr, m, false, M, g, at::kHalf, stream));
+  return pybind11::cast(backward_any(dC.data(), 3, m, false, M, g, stream));
 }
 
 pybind11::object gate_up_keep(const at::Tensor& A, const at::Tensor& Wg, const at::Tensor& Sg,

@@ -51,6 +51,7 @@ SIGNATURES: dict[str, tuple] = {
     "mm_gemm_backward": (_c_int, [_vp, _vp, _vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _vp, _c_int,
                                   _c_int, _c_int, _c_int, _vp, _c_size, _vp]),
     "mm_grad_rows": (_c_int, [_vp, _c_int, _vp, _vp, _c_int, _c_int, _vp]),
+    "mm_grad_rows_multi": (_c_int, [_vp, _c_int, _c_int, _vp, _vp, _vp, _c_int, _vp]),
     "mm_swiglu_grad": (_c_int, [_vp, _c_int, _vp, _vp, _vp, _c_int, _c_int, _vp]),
     "mm_lora_workspace_bytes": (_c_size, [_c_int] * 6),
     "mm_lora_add": (_c_int, [_vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _vp,

@@ -216,8 +216,13 @@ def mmfp4_fused_qkv_backward(dQ: torch.Tensor, dK: torch.Tensor, dV: torch.Tenso
         mul = None
         if dQ.dtype != torch.float16:
             # one power of two per row for all three
-            whole, mul = _carried(torch.cat(grads, 1))
-            n = whole.shape[1]
+            M, n = grads[0].shape[0], sum(widths)
+            whole = torch.empty((M, n), dtype=torch.float16, device=dev)
+            mul = torch.empty(M, dtype=torch.float32, device=dev)
+            _lib.call("mm_grad_rows_multi",
+                      (ctypes.c_void_p * 3)(*[g.data_ptr() for g in grads]), _TYPES[dQ.dtype], 3,
+                      (ctypes.c_int * 3)(*widths), _lib.ptr(whole), _lib.ptr(mul), M,
+                      _lib.stream_of(whole))
             grads = list(whole.split(widths, 1))
             widths = [n] * 3
         out = _launch(grads, widths, mul, mats, 0, Kdim, group_size, dtype)

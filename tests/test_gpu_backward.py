@@ -156,6 +156,24 @@ def test_range_of_bf16_gradients():
     assert not out[5].any()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_qkv_of_one_tensor(dtype):
+    """The three gradients as columns of one tensor (strided views), and no rows at all: the
+    per-call binding and the checked path give the same bits."""
+    K, g, Ns = 256, 64, (256, 72, 64)
+    gen = torch.Generator().manual_seed(9)
+    mats = [make_fp4(gen, K, n, g) for n in Ns]
+    args = [t for w, s, _ in mats for t in (w, s)]
+    whole = torch.randn((77, sum(Ns)), generator=gen).to(DEV, dtype) * 1e-3
+    views = whole.split(Ns, 1)
+    out = mmfp4.mmfp4_fused_qkv_backward(*[v.contiguous() for v in views], *args, g)
+    check_linear(out, whole, torch.cat([W for _, _, W in mats], 1), dtype, "qkv")
+    assert torch.equal(out, mmfp4.mmfp4_fused_qkv_backward(*views, *args, g))
+    none = mmfp4.mmfp4_fused_qkv_backward(*[v[:0] for v in views], *args, g)
+    assert none.shape == (0, K) and none.dtype == dtype
+    assert mmfp4.marlin_gemm_fp4_backward(views[0][:0], *args[:2], g).shape == (0, K)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_non_finite_rows_stay_by_themselves(dtype):
     gen = torch.Generator().manual_seed(6)
