@@ -1785,6 +1785,7 @@ extern "C" int mm_fp4_gate_up_keep(const uint16_t* A, const uint32_t* Bg, const 
   const char* who = "mm_fp4_gate_up_keep";
   MM_CHECK_ARG(layout == 0 || layout == 1, "%s: layout=%d must be 0 ([K/8, N] words) or 1 "
                "([N, K/8])", who, layout);
+  MM_CHECK_ARG(M <= 0 || gate_up != nullptr, "%s: null gate_up", who);
   if (layout == 1)
     return pair_rows_dispatch(who, A, Bg, Sg, Bu, Su, C, M, N, K, g, 2, ws, ws_bytes, stream,
                               (f16*)gate_up);
