@@ -6,7 +6,7 @@
 //
 // Few tokens: every token on its own, one launch of fp32 dot products (k_vec) or two
 // (k_vec_down, k_vec_up).  Otherwise the tokens are sorted by adapter and cut into tiles of 64
-// of one adapter (k_plan), and
+// of one adapter (k_plan, or up to 2048 tokens each block of k_down for its own tile), and
 //   k_down   H of a tile, over the whole width: 16x16x32 MFMAs, the width split over the
 //            waves and over blocks.  The block that finishes a tile leaves a record of it:
 //            H as hi + lo in the operands' type, under one power of two per tile that puts
@@ -14,7 +14,8 @@
 //            reach the second product, whatever its size.  The record has H by token and
 //            by rank, the operand orders of the two kernels that follow.
 //   up       out of a tile: MFMAs over [hi | lo] of 16 ranks at a time.
-//   wgrad    dA_a or dB_a: MFMAs over 32 tokens at a time, tile after tile.
+//   wgrad    dA_a or dB_a: MFMAs over 32 tokens at a time, tile after tile; the tiles are shared
+//            out over a block's waves, or a wave has them all where an adapter has few tokens.
 // All sums are fp32 and in a fixed order.  All of them stream activations that are read
 // once (x, dy) or read and written once (out): HBM bounds them, the factors stay in L2.
 #include <algorithm>
@@ -1034,7 +1035,7 @@ MM_DEV void wgrad_wave(const GradProblem& p, const Plan& plan, int r, int col0, 
 // The backward pass behind k_down: dA's blocks, dB's, then dx's.  They do not depend on one
 // another, and one launch lets them fill one another's gaps.
 // 256 registers, so that two waves share a SIMD: rank 64 by itself takes 309 (backward of 1111
-// tokens, 14336 -> 4096, rank 64 105 us; 85 so, with 10 of them spilled outside the loop).
+// tokens, 14336 -> 4096, rank 64 105 us; 85 so, with 10 of them spilled, nearly all outside the loops).
 template <int T, int RT, int BT>
 __global__ void __launch_bounds__(LO_NT, 2)
 k_back(GradProblem pa, GradProblem pb, UpProblem pu, Plan plan, int r, int na, int nb) {

@@ -68,7 +68,9 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, product, input_grad):
         refuse_foreign_leaf(x)
         ctx.input_grad, ctx.dtype, ctx.shape = input_grad, x.dtype, x.shape
-        return product(x).to(x.dtype)
+        y = product(x).to(x.dtype)
+        # a view (columns of a padded product) could not be changed in place, as a bias is added
+        return y.clone() if y._is_view() else y
 
     @staticmethod
     @once_differentiable

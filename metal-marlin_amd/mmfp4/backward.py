@@ -272,12 +272,12 @@ def fused_gate_up_swiglu(x: torch.Tensor, gate_packed: torch.Tensor, gate_scales
             if row_packed:
                 gate_packed, up_packed = (kernels._packed(w.t()) for w in
                                           (gate_packed, up_packed))
-            g = kernels.marlin_gemm_fp4(a, gate_packed, gate_scales, group_size)
-            u = kernels.marlin_gemm_fp4(a, up_packed, up_scales, group_size)
+            g, u = (kernels.marlin_gemm_fp4(a, w, s, group_size).reshape(*lead, N) for w, s in
+                    ((gate_packed, gate_scales), (up_packed, up_scales)))
             h = (torch.nn.functional.silu(g.float()) * u.float()).half()
-            return h.view(*lead, N), torch.cat([g, u], 1).view(*lead, 2 * N)
-        h = torch.empty((M, N), dtype=torch.float16, device=dev)
-        gate_up = torch.empty((M, 2 * N), dtype=torch.float16, device=dev)
+            return h, torch.cat([g, u], -1)
+        h = torch.empty((*lead, N), dtype=torch.float16, device=dev)
+        gate_up = torch.empty((*lead, 2 * N), dtype=torch.float16, device=dev)
         if M > 0:
             stream = _lib.raw_stream(dev.index)
             ws = _lib.call_workspace(dev.index, stream, kernels._ws_bytes(M, 2 * N, K))
@@ -286,7 +286,7 @@ def fused_gate_up_swiglu(x: torch.Tensor, gate_packed: torch.Tensor, gate_scales
             _lib.call("mm_fp4_gate_up_keep", _lib.ptr(a), *map(_lib.ptr, ops), _lib.ptr(h),
                       _lib.ptr(gate_up), int(row_packed), M, N, K, group_size, _lib.ptr(ws),
                       ws.numel(), stream)
-    return h.view(*lead, N), gate_up.view(*lead, 2 * N)
+    return h, gate_up
 
 
 def fused_gate_up_swiglu_backward(dh: torch.Tensor, gate_up: torch.Tensor,

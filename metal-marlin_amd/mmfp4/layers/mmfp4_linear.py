@@ -140,7 +140,12 @@ class MMFP4Linear(nn.Module):
             raise ValueError(f"Expected input last dim={self.in_features}, got {x.shape[-1]}")
         if not x.is_floating_point():
             raise ValueError(f"x must be a floating tensor, got dtype={x.dtype}")
-        out = autograd.linear(x.reshape(-1, self.in_features), self._product, self.input_grad)
+        x2 = x.reshape(-1, self.in_features)
+        if self.bias is not None and self.bias.requires_grad and autograd.wants_grad(x):
+            out = autograd.linear(x2, self._product, self.input_grad)
+            out = out + self.bias.to(device=out.device, dtype=out.dtype)
+        else:
+            out = autograd.linear(x2, self._biased_product, self.input_grad)
         return out.reshape(*x.shape[:-1], self.out_features)
 
     def input_grad(self, dy: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -150,7 +155,7 @@ class MMFP4Linear(nn.Module):
             out_dtype=dtype)
 
     def _product(self, x2: torch.Tensor) -> torch.Tensor:
-        """x2 [M, in] -> [M, out] fp16, with the bias."""
+        """x2 [M, in] -> [M, out] fp16, without the bias."""
         if kernels.rowpacked_gemm_supported(x2.shape[0], self.out_features, self.in_features,
                                             self.group_size):
             # row-packed words and [n_groups, out] scales in place
@@ -162,6 +167,10 @@ class MMFP4Linear(nn.Module):
                 out = kernels.marlin_gemm_fp4(x2, kp, self.scales.to(x2.device), self.group_size)
             else:
                 out = kernels.marlin_gemm_fp4(x2, kp, ks, self.group_size)[:, :self.out_features]
+        return out
+
+    def _biased_product(self, x2: torch.Tensor) -> torch.Tensor:
+        out = self._product(x2)
         if self.bias is not None:
             out = out + self.bias.to(device=out.device, dtype=out.dtype)
         return out

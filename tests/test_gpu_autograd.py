@@ -81,6 +81,27 @@ def test_gate_up(dtype, rows):
     assert torch.equal(dx, mmfp4.fused_gate_up_swiglu_backward(dh, gu, *mats, g, rows))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("N", [128, 36])
+def test_results_may_be_changed_in_place(N, dtype):
+    gen = torch.Generator().manual_seed(12)
+    K, g = 64, 64
+    w, s = mmfp4.quantize_fp4(weight(gen, N, K), group_size=g)
+    lib = mmfp4.get_default_library()
+    w4, s4, z4 = mmfp4.pack_u4_weights(weight(gen, N, K), group_size=g)
+    for shape in ((K,), (3, K), (2, 20, K)):
+        x = torch.randn(shape, generator=gen).to(DEV, dtype).requires_grad_(True)
+        calls = [lambda: mmfp4.quantized_linear(x, w, s, g),
+                 lambda: lib.fp4_gemm(x, w, s, N, K, g),
+                 lambda: lib.int4_gemm(x, w4, s4, N, K, g, z4),
+                 lambda: mmfp4.gate_up_swiglu(x, w, s, w, s, g)]
+        for f in calls if len(shape) > 1 else calls[-1:]:
+            y = f()
+            dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+            dx2, = torch.autograd.grad(f().mul_(2), x, torch.ones_like(y))
+            assert dx.shape == x.shape and torch.equal(dx2, 2 * dx)
+
+
 @pytest.mark.parametrize("T", [5, 300])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_adapters(dtype, T):
@@ -107,6 +128,43 @@ def test_adapters(dtype, T):
             assert a.dtype == b.dtype and torch.equal(a, b), name
         with torch.no_grad():
             assert torch.equal(m(x, ids), y)
+
+
+@pytest.mark.parametrize("K,N,g", [(72, 35, 24), (264, 100, 8), (64, 4, 64)])
+@pytest.mark.parametrize("M", [1, 50])
+def test_odd_layers(M, K, N, g):
+    """Widths that the kernels take on padded or transposed copies."""
+    gen = torch.Generator().manual_seed(10)
+    for name, layer, W in layers(gen, K, N, g):
+        x = torch.randn((M, K), generator=gen).to(DEV, F16).requires_grad_(True)
+        layer(x).mul_(2)                                       # results may be changed in place
+        m = mmfp4.LoRALinear(layer, rank=3)
+        dy = torch.randn((M, N), generator=gen).to(DEV, F16)
+        ref, terms = dy.double() @ W, dy.double().abs() @ W.abs()
+        tol = 2.0 ** -11 * ref.abs() + 2.0 ** -11 * terms      # as in test_layers
+        if name == "rotated":
+            tol = tol + 2.0 ** -10 * terms.max()
+        for f in (layer, m):                                   # lora_b is zeros
+            dx, = torch.autograd.grad(f(x), x, dy)
+            # LoRALinear rounds the sum of two gradients once more
+            assert ((dx.double() - ref).abs() <= 2 * tol).all(), (name, f)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_bias_gets_its_gradient(dtype):
+    gen = torch.Generator().manual_seed(9)
+    for name, layer, _ in layers(gen, 256, 96, 64):
+        if isinstance(layer, mmfp4.QuantizedLinear) or name == "marlin":
+            layer.bias = layer.bias.to(dtype)
+        layer.bias.requires_grad_(True)
+        x = torch.randn((5, 256), generator=gen).to(DEV, dtype)
+        dy = torch.randn((5, 96), generator=gen).to(DEV, dtype)
+        for wants in (False, True):
+            x.requires_grad_(wants)
+            db, = torch.autograd.grad(layer(x), layer.bias, dy)
+            # five terms, each sum rounded to the type
+            tol = 5 * torch.finfo(dtype).eps * dy.double().abs().sum(0) + 1e-6
+            assert ((db.double() - dy.double().sum(0)).abs() <= tol).all(), (name, wants)
 
 
 def test_twice_is_refused():
