@@ -555,8 +555,8 @@ k_grad(GradSegs segs, void* __restrict__ out, int ot, const float* __restrict__ 
 // converted.  ks > 1: as in k_grad.
 //
 // Against tiles of 64 x 256: half the columns leave no split to be joined up to 512 rows of K =
-// 4096, and every weight costs 1.7 VALU operations (2.3 there, where a wave converts half
-// words).  M = 512, 4096 -> 4096: 24.7 us, 700 TFLOP/s (34 there).  A chunk takes 1.3 us, of
+// 4096, and every weight costs 1.6 VALU operations (2.0 there, where a wave converts half
+// words).  M = 512, 4096 -> 4096: 24.4 us, 700 TFLOP/s (34 there).  A chunk takes 1.27 us, of
 // which the matrix cores are busy 0.43: the two waves of a SIMD wait a third of the time for
 // each other, and what they issue does not overlap fully.  Reading the next operands before
 // the first half (double words) spills and gains nothing.
@@ -615,10 +615,40 @@ k_grad_narrow(GradSegs segs, void* __restrict__ out, int ot, const float* __rest
     for (int rb = 0; rb < 4; ++rb)
       af[slot][rb] = *(const f16x8*)(smem + st * Sh::A_BYTES + a_off + rb * 16 * (GN_BN * 2));
   };
-  auto decode = [&](int hf) __attribute__((always_inline)) {
+  // FP4: the even and the odd nibbles of neighbouring words in pairs, for both halves at once
+  // (PairWords' e and o, without picking bytes first; 512 rows, 14336 -> 4096 77.2 us with it, 75.0
+  // so).
+  uint32_t eo[2][4];
+  auto decode = [&](auto hfc) __attribute__((always_inline)) {
+    constexpr int hf = decltype(hfc)::value;
     if (hf == 0) grad_scales<INT4>(sv, zv, s2, nz2);
-    PairWords<INT4>::run(w, s2, nz2, hf ? 0x07060302u : 0x05040100u, bq[hf]);
+    if constexpr (INT4) {
+      PairWords<true>::run(w, s2, nz2, hf ? 0x07060302u : 0x05040100u, bq[hf]);
+    } else {
+      if (hf == 0) {
+        const uint32_t m = sgpr_const(0x0f0f0f0fu);
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const uint32_t x = w[p >> 1][2 * (p & 1)], y = w[p >> 1][2 * (p & 1) + 1];
+          eo[0][p] = (x & m) | ((y << 4) & ~m);
+          eo[1][p] = ((x >> 4) & m) | (y & ~m);
+        }
+      }
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        u32x4 lo, hi;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          lo[p] = __builtin_bit_cast(uint32_t, e2m1_pair_c<2 * hf>(eo[o][p]) * s2[p]);
+          hi[p] = __builtin_bit_cast(uint32_t, e2m1_pair_c<2 * hf + 1>(eo[o][p]) * s2[p]);
+        }
+        bq[hf][o] = __builtin_bit_cast(f16x8, lo);
+        bq[hf][2 + o] = __builtin_bit_cast(f16x8, hi);
+      }
+    }
   };
+  constexpr std::integral_constant<int, 0> first{};
+  constexpr std::integral_constant<int, 1> second{};
   auto half = [&](int slot, int hf) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -638,7 +668,7 @@ k_grad_narrow(GradSegs segs, void* __restrict__ out, int ot, const float* __rest
   auto chunk = [&](int ch, auto stc, int cur) __attribute__((always_inline)) {
     constexpr int st = decltype(stc)::value;
     half(cur, 0);
-    decode(1);
+    decode(second);
     order();
     // Every wave has read this chunk: its stage is refilled, and the next one, which has
     // landed once at most STAGES - 2 later ones are outstanding, is published.
@@ -649,13 +679,13 @@ k_grad_narrow(GradSegs segs, void* __restrict__ out, int ot, const float* __rest
     feed.issue(st);                                // behind the last chunk: again, never read
     frag(std::integral_constant<int, (st + 1) % STG>{}, cur ^ 1);
     half(cur, 1);
-    decode(0);
+    decode(first);
     order();
   };
   wait_vmcnt<(STG - 1) * Sh::LOADS>();
   __builtin_amdgcn_s_barrier();
   frag(std::integral_constant<int, 0>{}, 0);
-  decode(0);
+  decode(first);
   // an even number of stages in a round, so that the operand slots are constants
   for (int ch = c_beg; ch < c_end; ch += 2 * STG) {
     static_for(
@@ -1068,10 +1098,10 @@ GradPlan plan_grad(int nmat, const int* N, int M, int K) {
   // start, a time per chunk (more where all CUs share the memory) and its end, and the
   // hand-off of a split.  Measured, K = 4096, 64 x 128 tiles / 64 x 256 / 256 x 256, each at its
   // best split: M = 64, N = 4096 16.3 (4 ways) / 23 / 82; M = 300 24 / 28 / 89; M = 512 25 / 34 /
-  // 89, N = 14336 77 / 82 / 228; M = 1024, N = 4096 50 / 47 / 92; M = 2048 99 / 92 / 103, N =
+  // 89, N = 14336 75 / 82 / 228; M = 1024, N = 4096 50 / 47 / 92; M = 2048 99 / 92 / 103, N =
   // 14336 - / 292 / 266; M = 4096, N = 4096 - / 183 / 147.
   struct { int kind, bm, cols, bn; double start, chunk, full, split, each; } const kinds[] = {
-      {G_NARROW, GN_BM, GN_COLS, GN_BN, 3.6, 1.32, 1.32, 2.2, 1.25},
+      {G_NARROW, GN_BM, GN_COLS, GN_BN, 3.6, 1.27, 1.27, 2.2, 1.25},
       {G_64, 64, GR_COLS, 128, 7.8, 1.05, 1.21, 7, 0},
       {G_256, 256, GR_COLS, 64, 16, 1.75, 2.05, 20, 0}};
   double best = 0;
