@@ -256,19 +256,12 @@ def _plain(st):
 
 
 # ------------------------------------------------------------ the framework's
-_package = None
-
-
 def _mmfp4():
-    """The package, imported at the first call."""
-    global _package
-    if _package is None:
-        pkg = str(Path(__file__).resolve().parent.parent / "metal-marlin_amd")
-        if pkg not in sys.path:
-            sys.path.insert(0, pkg)
-        import mmfp4
-        _package = mmfp4
-    return _package
+    pkg = str(Path(__file__).resolve().parent.parent / "metal-marlin_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    import mmfp4
+    return mmfp4
 
 
 def _own(st):
