@@ -27,6 +27,10 @@ extern "C" {
 /* Message of the last failing call on this thread ("" if none). */
 const char* mm_last_error(void);
 
+/* The id of the capture that `stream` is in, 0 if it is not being captured.  A workspace whose
+ * counters were cleared within a capture belongs to that capture alone. */
+unsigned long long mm_capture_id(void* stream);
+
 /* ---------------------------------------------------------------- dequant */
 
 /* W[K,N] fp16 = fp16_RNE(E2M1[code] * scale), non-finite -> +0.

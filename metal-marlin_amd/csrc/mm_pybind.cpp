@@ -24,12 +24,34 @@ namespace {
 
 std::mutex g_mu;
 std::map<std::pair<int, int64_t>, at::Tensor> g_ws;   // (device index, stream) -> workspace
+struct Captured {
+  unsigned long long id;   // of the capture
+  at::Tensor buf;
+};
+std::map<std::pair<int, int64_t>, Captured> g_captured;
+constexpr int64_t COUNTER_BYTES = 65536;   // at the head of every workspace
 
 // One workspace per (device, stream), shared with the ctypes path (which
 // asks for it through workspace_for below); kept until release_workspaces().
+// Under capture one per capture and stream, from the graph's pool, its counters cleared by a
+// node of that graph: graphs never share one, with one another or with eager calls, and none
+// relies on a fill that only another one replays.  It is held until the stream is used again
+// outside that capture; the graph's pool keeps the memory as long as the graph lives.
 at::Tensor workspace_dev(int dev, int64_t stream, size_t nbytes, const at::TensorOptions& opt) {
   std::lock_guard<std::mutex> lock(g_mu);
   const auto key = std::make_pair(dev, stream);
+  if (const unsigned long long id = mm_capture_id((void*)stream)) {
+    Captured& c = g_captured[key];
+    if (c.id == id && (size_t)c.buf.numel() >= nbytes) return c.buf;
+    size_t size = std::max(nbytes, (size_t)1 << 20);
+    if (c.id == id) size = std::max(size, 2 * (size_t)c.buf.numel());
+    c = Captured{0, at::Tensor()};
+    at::Tensor buf = at::empty({(int64_t)size}, opt.dtype(at::kByte));
+    buf.narrow(0, 0, COUNTER_BYTES).zero_();
+    c = Captured{id, buf};
+    return buf;
+  }
+  if (!g_captured.empty()) g_captured.erase(key);
   auto it = g_ws.find(key);
   if (it != g_ws.end() && (size_t)it->second.numel() >= nbytes) return it->second;
   size_t size = nbytes < ((size_t)1 << 20) ? ((size_t)1 << 20) : nbytes;
@@ -53,6 +75,7 @@ at::Tensor workspace_for(int64_t device, int64_t stream, int64_t nbytes) {
 void release_workspaces() {
   std::lock_guard<std::mutex> lock(g_mu);
   g_ws.clear();
+  g_captured.clear();
 }
 
 [[noreturn]] void fail(int rc) {

@@ -20,6 +20,7 @@ _c_int, _c_size, _vp = ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p
 # name -> (restype, argtypes); must match include/mmfp4.h
 SIGNATURES: dict[str, tuple] = {
     "mm_last_error": (ctypes.c_char_p, []),
+    "mm_capture_id": (ctypes.c_ulonglong, [_vp]),
     "mm_fp4_dequant": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _vp]),
     "mm_u4_dequant": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp]),
     "mm_fp4_quantize": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp]),
@@ -239,20 +240,36 @@ def same_device_index(*tensors: torch.Tensor) -> int:
 
 # ---------------------------------------------------------------------------
 # Per-(device, stream) workspace.  Its head holds split-K arrival counters that
-# the kernels leave at zero, so it is allocated zeroed once and reused.
+# the kernels leave at zero, so it is allocated zeroed once and reused.  Under
+# graph capture: one per capture and stream.
 # ---------------------------------------------------------------------------
+_COUNTER_BYTES = 65536
 _ws: dict[tuple[int, int], torch.Tensor] = {}
+_captured_ws: dict[tuple[int, int], tuple[int, torch.Tensor]] = {}
 
 
 def workspace_on(index: int, stream: int, nbytes: int) -> torch.Tensor:
     """Workspace of at least `nbytes` for (device index, raw stream): one
     zero-initialised buffer per pair (at least 1 MiB, grown by doubling),
     held by the per-call binding when it is built (so both call paths share
-    it), else here.  Buffers are kept until release_workspaces()."""
+    it), else here.  Buffers are kept until release_workspaces().
+
+    Under graph capture: one per capture and stream, from the graph's pool, whose counters a
+    node of that graph clears.  Graphs never share one, with one another or with eager calls."""
     b = binding()
     if b:
         return b.workspace(index, stream, nbytes)
     key = (index, stream)
+    capture = load().mm_capture_id(stream)
+    if capture:
+        held, buf = _captured_ws.get(key, (0, None))
+        if held != capture or buf.numel() < nbytes:
+            size = max(nbytes, 1 << 20, 2 * buf.numel() if held == capture else 0)
+            buf = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", index))
+            buf[:_COUNTER_BYTES].zero_()
+            _captured_ws[key] = capture, buf
+        return buf
+    _captured_ws.pop(key, None)
     buf = _ws.get(key)
     if buf is None or buf.numel() < nbytes:
         size = max(nbytes, 1 << 20)
@@ -272,14 +289,15 @@ def release_workspaces() -> None:
     if b:
         b.release_workspaces()
     _ws.clear()
+    _captured_ws.clear()
 
 
 def fast(name: str, tensor: torch.Tensor, *args):
     """The per-call binding's entry `name` on the current stream of the tensor's device: its
-    result, or None when the binding is absent, the stream is being captured (call_workspace)
-    or the operands are not in the plain form it takes."""
+    result, or None when the binding is absent or the operands are not in the plain form it
+    takes."""
     b = binding()
-    if b is None or tensor.get_device() < 0 or torch.cuda.is_current_stream_capturing():
+    if b is None or tensor.get_device() < 0:
         return None
     try:
         return getattr(b, name)(*args, _raw_stream(tensor.get_device()))
@@ -287,14 +305,6 @@ def fast(name: str, tensor: torch.Tensor, *args):
         if type(e) is RuntimeError:
             raise MMError(str(e)) from None
         raise
-
-
-def call_workspace(index: int, stream: int, nbytes: int) -> torch.Tensor:
-    """workspace_on, or under graph capture a zeroed buffer of the call's own (from the
-    graph's memory pool): two captured graphs never share it, so they may replay at once."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
-    return workspace_on(index, stream, nbytes)
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:

@@ -120,8 +120,8 @@ def _add(base, x, lora_a, lora_b, adapter_ids, scaling, out=None):
         if T == 0:
             return out
         stream = _lib.raw_stream(dev.index)
-        ws = _lib.call_workspace(dev.index, stream,
-                                 _lib.load().mm_lora_workspace_bytes(T, K, N, r, L, 0))
+        ws = _lib.workspace_on(dev.index, stream,
+                               _lib.load().mm_lora_workspace_bytes(T, K, N, r, L, 0))
         _lib.call("mm_lora_add", _lib.ptr(xf), _TYPES[dt], _lib.ptr(bf), _TYPES[bf.dtype],
                   _lib.ptr(out), _lib.ptr(a), _lib.ptr(b), _lib.ptr(ids),
                   int(ids is not None and ids.dtype == torch.int64), _lib.ptr(st), factor, T, K,
@@ -199,8 +199,8 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_
         gt = dt if lora_a.dtype == lora_b.dtype == dt else torch.float32
         da, db = torch.empty_like(ac, dtype=gt), torch.empty_like(bc, dtype=gt)
         stream = _lib.raw_stream(dev.index)
-        ws = _lib.call_workspace(dev.index, stream,
-                                 _lib.load().mm_lora_workspace_bytes(T, K, N, r, L, 1))
+        ws = _lib.workspace_on(dev.index, stream,
+                               _lib.load().mm_lora_workspace_bytes(T, K, N, r, L, 1))
         _lib.call("mm_lora_backward", _lib.ptr(dyf), _lib.ptr(xf), _TYPES[dt], _lib.ptr(ac),
                   _lib.ptr(bc), _lib.ptr(ids), int(ids is not None and ids.dtype == torch.int64),
                   _lib.ptr(st), factor, _lib.ptr(dxb), _lib.ptr(dx), _lib.ptr(da), _lib.ptr(db),

@@ -93,7 +93,7 @@ def _launch(dC: list[torch.Tensor], ldc: list[int], row_mul: torch.Tensor | None
     zeros = table([z for _, _, z in mats]) if mats[0][2] is not None else None
     stream = _lib.raw_stream(dev.index)
     need = _lib.load().mm_gemm_backward_workspace_bytes(n, Ns, M, K)
-    ws = _lib.call_workspace(dev.index, stream, need)
+    ws = _lib.workspace_on(dev.index, stream, need)
     _lib.call("mm_gemm_backward", table(dC), (ctypes.c_int * n)(*ldc),
               _lib.ptr(row_mul), n, table([w for w, _, _ in mats]),
               table([s for _, s, _ in mats]), zeros, Ns, layout, _lib.ptr(out), _TYPES[dtype], M,
@@ -280,7 +280,7 @@ def fused_gate_up_swiglu(x: torch.Tensor, gate_packed: torch.Tensor, gate_scales
         gate_up = torch.empty((*lead, 2 * N), dtype=torch.float16, device=dev)
         if M > 0:
             stream = _lib.raw_stream(dev.index)
-            ws = _lib.call_workspace(dev.index, stream, kernels._ws_bytes(M, 2 * N, K))
+            ws = _lib.workspace_on(dev.index, stream, kernels._ws_bytes(M, 2 * N, K))
             ops = [plain(t) for t in (kernels._packed(gate_packed), kernels._half(gate_scales),
                                       kernels._packed(up_packed), kernels._half(up_scales))]
             _lib.call("mm_fp4_gate_up_keep", _lib.ptr(a), *map(_lib.ptr, ops), _lib.ptr(h),
