@@ -31,6 +31,10 @@ const char* mm_last_error(void);
  * counters were cleared within a capture belongs to that capture alone. */
 unsigned long long mm_capture_id(void* stream);
 
+/* 1 if what was recorded into `event` (a hipEvent_t, recorded outside any capture) is done, 0 if
+ * not or not known; does not disturb a capture under way. */
+int mm_event_done(void* event);
+
 /* ---------------------------------------------------------------- dequant */
 
 /* W[K,N] fp16 = fp16_RNE(E2M1[code] * scale), non-finite -> +0.

@@ -12,3 +12,17 @@ extern "C" unsigned long long mm_capture_id(void* stream) {
   }
   return status == hipStreamCaptureStatusNone ? 0 : id;
 }
+
+// Also while a stream is being captured: an event recorded before that is no part of it, and the
+// relaxed mode is the one that may ask.
+extern "C" int mm_event_done(void* event) {
+  hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+  if (hipThreadExchangeStreamCaptureMode(&mode) != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  const hipError_t e = hipEventQuery((hipEvent_t)event);
+  (void)hipThreadExchangeStreamCaptureMode(&mode);
+  if (e != hipSuccess) (void)hipGetLastError();
+  return e == hipSuccess;
+}

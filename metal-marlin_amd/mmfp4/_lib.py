@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
+import weakref
 from pathlib import Path
 
 import torch
@@ -21,6 +22,7 @@ _c_int, _c_size, _vp = ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p
 SIGNATURES: dict[str, tuple] = {
     "mm_last_error": (ctypes.c_char_p, []),
     "mm_capture_id": (ctypes.c_ulonglong, [_vp]),
+    "mm_event_done": (_c_int, [_vp]),
     "mm_fp4_dequant": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _vp]),
     "mm_u4_dequant": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp]),
     "mm_fp4_quantize": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp]),
@@ -155,7 +157,64 @@ def call(name: str, *args) -> None:
 
 
 def _stamp(t: torch.Tensor) -> tuple:
-    return (t._version, t.data_ptr(), tuple(t.shape), t.dtype)
+    return (t._version, t.data_ptr(), t.shape, t.dtype)
+
+
+class _Made:
+    """The making of a kept copy: its event until that is known to be done, the streams whose
+    later work is ordered behind it, and whether a graph was captured with it."""
+    __slots__ = ("ref", "index", "event", "streams", "captured")
+
+    def __init__(self, ref, index: int, event, stream: int) -> None:
+        self.ref, self.index, self.event = ref, index, event
+        self.streams, self.captured = {stream}, False
+
+
+_made: dict[int, _Made] = {}      # by the id of the copy, as long as it lives
+
+
+def keep(out: torch.Tensor) -> None:
+    """Note that `out`, whose making was just queued on the current stream, will be used by later
+    calls."""
+    if not out.is_cuda:
+        return
+    index, key = out.get_device(), id(out)
+    event = torch.cuda.Event()
+    event.record(torch.cuda.current_stream(index))
+    _made[key] = _Made(weakref.ref(out, lambda _: _made.pop(key, None)), index, event,
+                       _raw_stream(index))
+
+
+def usable(out: torch.Tensor) -> bool:
+    """Whether what is queued next on the current stream may read the kept copy `out`.  Another
+    stream than the copy's own is made to wait for its making, and the allocator is told of it;
+    a stream under capture, whose replays wait for nothing that was queued before, may once the
+    copy is known to be there."""
+    made = _made.get(id(out))
+    if made is None:
+        return not out.is_cuda
+    raw = _raw_stream(made.index)
+    capturing = raw != 0 and torch.cuda.is_current_stream_capturing()
+    if made.event is not None:
+        if load().mm_event_done(made.event.cuda_event):
+            made.event = None
+        elif capturing:
+            return False
+    if raw not in made.streams:
+        stream = torch.cuda.current_stream(made.index)
+        if made.event is not None:
+            stream.wait_event(made.event)
+        out.record_stream(stream)
+        made.streams.add(raw)
+    if capturing:
+        made.captured = True
+    return True
+
+
+def in_a_graph(out: torch.Tensor) -> bool:
+    """Whether a graph was captured that reads the kept copy `out`."""
+    made = _made.get(id(out))
+    return made is not None and made.captured
 
 
 def derived(src: torch.Tensor, key: str, build, also: torch.Tensor | None = None):
@@ -163,20 +222,30 @@ def derived(src: torch.Tensor, key: str, build, also: torch.Tensor | None = None
     when src (or `also`, a second input of build) is written in place (its
     version counter) or points at other storage.  The copy lives exactly as
     long as the source tensor object; a caller that passes a fresh view each
-    time gets no caching."""
+    time gets no caching.
+
+    The copy may be used on any stream (usable).  Under graph capture one that is known to be
+    there is used, and otherwise the call's own is made within the graph and not kept: it holds
+    nothing before a replay.  A graph reads the copy that it was captured with, which is kept as
+    long as src is."""
     cache = getattr(src, "_mmfp4_derived", None)
     stamp = _stamp(src) + (_stamp(also) if also is not None else ())
     hit = cache.get(key) if cache is not None else None
-    if hit is not None and hit[0] == stamp:
+    if hit is not None and hit[0] == stamp and usable(hit[1]):
         return hit[1]
     out = build(src)
+    if out.is_cuda and torch.cuda.is_current_stream_capturing():
+        return out
     if cache is None:
         cache = {}
         try:
             src._mmfp4_derived = cache
         except (AttributeError, RuntimeError):
             return out
+    if hit is not None and in_a_graph(hit[1]):
+        cache.setdefault("captured", []).append(hit[1])
     cache[key] = (stamp, out)
+    keep(out)
     return out
 
 

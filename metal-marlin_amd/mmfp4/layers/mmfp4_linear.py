@@ -21,7 +21,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
-from .. import autograd, backward, kernels
+from .. import _lib, autograd, backward, kernels
 
 __all__ = ["MMFP4Linear", "mmfp4_gemm", "rowpacked_to_marlin"]
 
@@ -118,22 +118,30 @@ class MMFP4Linear(nn.Module):
         source buffers' identity and version counters, so load_state_dict /
         copy_ into packed_weights or scales (or new tensors assigned to them)
         rebuilds it.  With out_features % 4 != 0 the words and scales are
-        padded to a multiple of 4 columns here, once, instead of per call."""
+        padded to a multiple of 4 columns here, once, instead of per call.
+        Streams and graph capture: as _lib.derived."""
         src, sc = self.packed_weights, self.scales
         pad = -self.out_features % 4
         key = (src.data_ptr(), src._version, device) + \
             ((sc.data_ptr(), sc._version) if pad else ())
-        kp = self._kernel_packed_weights
-        if kp is None or getattr(self, "_kernel_key", None) != key:
-            kp = rowpacked_to_marlin(src.to(device))
-            self._kernel_scales = None
-            if pad:
-                kp = torch.nn.functional.pad(kp.view(torch.int32), (0, pad))
-                self._kernel_scales = torch.nn.functional.pad(
-                    sc.to(device=device, dtype=torch.float16), (0, pad), value=1.0)
-            self._kernel_packed_weights = kp
-            self._kernel_key = key
-        return kp, self._kernel_scales
+        kept = [t for t in (self._kernel_packed_weights, self._kernel_scales) if t is not None]
+        if kept and getattr(self, "_kernel_key", None) == key and \
+                all([_lib.usable(t) for t in kept]):
+            return self._kernel_packed_weights, self._kernel_scales
+        kp, ks = rowpacked_to_marlin(src.to(device)), None
+        if pad:
+            kp = torch.nn.functional.pad(kp.view(torch.int32), (0, pad))
+            ks = torch.nn.functional.pad(sc.to(device=device, dtype=torch.float16), (0, pad),
+                                         value=1.0)
+        if kp.is_cuda and torch.cuda.is_current_stream_capturing():
+            return kp, ks
+        self._captured_weights = [t for t in kept if _lib.in_a_graph(t)] + \
+            getattr(self, "_captured_weights", [])
+        self._kernel_packed_weights, self._kernel_scales, self._kernel_key = kp, ks, key
+        for t in (kp, ks):
+            if t is not None:
+                _lib.keep(t)
+        return kp, ks
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.shape[-1] != self.in_features:
