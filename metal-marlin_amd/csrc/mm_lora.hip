@@ -1283,6 +1283,16 @@ Records record_at(const LoraPlan& p, char* at) {
   return Records{(uint16_t*)at, (uint16_t*)(at + h), (float*)(at + 2 * h), p.rp, p.nrc};
 }
 
+// Bytes of a problem's partial sums: `sums` of them if each is split, none otherwise.
+size_t part_bytes(size_t sums, int ks) { return ks > 1 ? sums * ks : 0; }
+size_t down_part(const LoraPlan& p, int ks) {
+  return part_bytes((size_t)p.tiles * p.nrc * LO_TM * p.rp * 4, ks);
+}
+size_t wgrad_part(const LoraPlan& p, int T, int L, int C) {
+  return part_bytes((size_t)L * p.nrc * mm_cdiv(C, LO_WG_COLS) * LO_WG_COLS * p.rp * 4,
+                    wgrad_split(T, L, p.nrc, C));
+}
+
 // Workspace: counters, the plan, the records of both problems, partial sums (of k_down and
 // then of wgrad, one after the other in the same memory).
 LoraPlan plan_lora(int T, int K, int N, int r, int L, bool backward) {
@@ -1297,18 +1307,12 @@ LoraPlan plan_lora(int T, int K, int N, int r, int L, bool backward) {
   p.rec[0] = p.first + align256(((size_t)L + 2) * 4);
   p.rec[1] = p.rec[0] + record_bytes(p);
   p.part = p.rec[1] + (backward ? record_bytes(p) : 0);
-  const size_t tile = (size_t)p.tiles * p.nrc * LO_TM * p.rp * 4;
   const int px = mm_cdiv(K, 64), py = backward ? mm_cdiv(N, 64) : 0;
   p.per = down_range((long)p.tiles * p.nrc, px + py);
   p.kx = mm_cdiv(px, p.per);
   p.ky = mm_cdiv(py, p.per);
-  size_t part = tile * p.kx;
-  if (backward) {
-    part += tile * p.ky;
-    const size_t col = (size_t)L * p.nrc * LO_WG_COLS * p.rp * 4;
-    part = std::max(part, col * (mm_cdiv(K, LO_WG_COLS) * (size_t)wgrad_split(T, L, p.nrc, K) +
-                                 mm_cdiv(N, LO_WG_COLS) * (size_t)wgrad_split(T, L, p.nrc, N)));
-  }
+  size_t part = down_part(p, p.kx) + down_part(p, p.ky);
+  if (backward) part = std::max(part, wgrad_part(p, T, L, K) + wgrad_part(p, T, L, N));
   p.total = p.part + align256(part);
   return p;
 }
@@ -1465,12 +1469,11 @@ extern "C" int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type,
   if (const int rc = make_plan(who, p, ids, ids64, T, L, ws, st, &plan, &own)) return rc;
   const int down_tiles = own.ids.p != nullptr ? p.all : p.tiles;
   const Records rx = record_at(p, (char*)ws + p.rec[0]), ry = record_at(p, (char*)ws + p.rec[1]);
-  float* part = (float*)((char*)ws + p.part);
+  char* part = (char*)ws + p.part;
   uint32_t* counters = (uint32_t*)ws;
   const int kx = p.kx, ky = p.ky;
-  const size_t tile = (size_t)p.tiles * p.nrc * LO_TM * p.rp;
-  const DownProblem px{x, A, K, kx, p.per, rx, part, counters, 0, 1};
-  const DownProblem py{dy, B, N, ky, p.per, ry, part + tile * kx,
+  const DownProblem px{x, A, K, kx, p.per, rx, (float*)part, counters, 0, 1};
+  const DownProblem py{dy, B, N, ky, p.per, ry, (float*)(part + down_part(p, kx)),
                        counters + LO_SPLIT_BELOW, 1, 1};
 #define MM_DOWN(RTV, TV)                                                                       \
   hipLaunchKernelGGL((k_down<TV, RTV>), dim3(down_tiles, std::max(kx, ky), 2 * p.nrc),             \
@@ -1482,9 +1485,9 @@ extern "C" int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type,
   const int ca = mm_cdiv(K, wa ? 4 * LO_WG_COLS : LO_WG_COLS);
   const int cb = mm_cdiv(N, wb ? 4 * LO_WG_COLS : LO_WG_COLS);
   const int ga = wgrad_split(T, L, p.nrc, K), gb = wgrad_split(T, L, p.nrc, N);
-  const GradProblem pa{x, dA, K, ga, grad_type == 0, wa, ry, part, counters};
-  const GradProblem pb{dy, dB, N, gb, grad_type == 0, wb, rx, part + (size_t)L * p.nrc * ca * ga * LO_WG_COLS * p.rp,
-                       counters + LO_SPLIT_BELOW};
+  const GradProblem pa{x, dA, K, ga, grad_type == 0, wa, ry, (float*)part, counters};
+  const GradProblem pb{dy, dB, N, gb, grad_type == 0, wb, rx,
+                       (float*)(part + wgrad_part(p, T, L, K)), counters + LO_SPLIT_BELOW};
   const UpProblem pu{A, dx_base, dx, K, ry};
   const long na = (long)ca * L * p.nrc * ga, nb = (long)cb * L * p.nrc * gb;
   const long nu = (long)p.all * mm_cdiv(K, LO_UP_COLS);
