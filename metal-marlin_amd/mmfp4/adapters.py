@@ -144,7 +144,8 @@ def lora_add(base: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     base is fp16, as the products return it, or of x's type; out has x's type.  With `out`
     (contiguous, of x's type; base itself will do) the result is written there.  Any number of
     tokens and any width or rank, at most 1024 adapters.  Differentiable in base, x, lora_a and
-    lora_b; `lora_backward` is the backward pass as a call."""
+    lora_b (the products and layers that make a base are differentiable in x as well);
+    `lora_backward` is the backward pass as a call."""
     if torch.is_grad_enabled() and any(t.requires_grad for t in (base, x, lora_a, lora_b)
                                        if isinstance(t, torch.Tensor)):
         from .autograd import LoraAdd

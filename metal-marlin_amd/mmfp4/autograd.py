@@ -1,7 +1,8 @@
 """Autograd over the quantized products: gradients of the input through frozen 4-bit weights,
-and of low-rank adapters.  The layers (QuantizedLinear, MarlinLinear, MMFP4Linear, LoRALinear)
-and lora_add use these by themselves where an operand requires a gradient; calls that need
-none take the same path as ever.  They are differentiable once: a gradient of a gradient is
+and of low-rank adapters.  The layers (QuantizedLinear, MarlinLinear, MMFP4Linear, LoRALinear),
+the products (marlin_gemm_fp4, marlin_gemm_int4, mmfp4_gemm_rowpacked, mmfp4_fused_qkv and what
+is made of them), fused_gate_up_swiglu and lora_add use these by themselves where an operand
+requires a gradient; calls that need none take the same path as ever.  They are differentiable once: a gradient of a gradient is
 an error, not a silent zero.
 
 A backward pass may be captured into a graph.  torch then refuses, by ending the process, one
@@ -16,9 +17,10 @@ from collections.abc import Callable
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _lib, adapters, backward
+from . import _lib, adapters, backward, kernels
 
-__all__ = ["linear", "gate_up_swiglu", "LoraAdd", "LoraLinear"]
+__all__ = ["linear", "marlin_gemm", "rowpacked_gemm", "gate_up_swiglu", "FusedQKV", "GateUp",
+           "LoraAdd", "LoraLinear"]
 
 
 def refuse_foreign_leaf(*tensors: torch.Tensor | None) -> None:
@@ -62,46 +64,92 @@ def wants_grad(*tensors: torch.Tensor | None) -> bool:
 
 
 class _Linear(torch.autograd.Function):
-    """y = forward(x) in x's type, dx = input_grad(dy); neither depends on anything trained."""
+    """y = forward(x) as it comes or in x's type, dx = input_grad(dy); neither depends on
+    anything trained."""
 
     @staticmethod
-    def forward(ctx, x, product, input_grad):
+    def forward(ctx, x, product, input_grad, cast):
         refuse_foreign_leaf(x)
         ctx.input_grad, ctx.dtype, ctx.shape = input_grad, x.dtype, x.shape
-        y = product(x).to(x.dtype)
+        y = product(x)
+        y = y.to(x.dtype) if cast else y
         # a view (columns of a padded product) could not be changed in place, as a bias is added
         return y.clone() if y._is_view() else y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return ctx.input_grad(dy, ctx.dtype).view(ctx.shape), None, None
+        return ctx.input_grad(dy, ctx.dtype).view(ctx.shape), None, None, None
 
 
 def linear(x: torch.Tensor, product: Callable, input_grad: Callable) -> torch.Tensor:
     """product(x) in x's type, differentiable in x: input_grad(dy, dtype) is its gradient."""
     if wants_grad(x):
-        return _Linear.apply(x, product, input_grad)
+        return _Linear.apply(x, product, input_grad, True)
     return product(x).to(x.dtype)
 
 
-class _GateUp(torch.autograd.Function):
+def marlin_gemm(kind: str, A: torch.Tensor, B_packed: torch.Tensor, scales: torch.Tensor,
+                zeros: torch.Tensor | None, group_size: int) -> torch.Tensor:
+    """marlin_gemm_fp4 / marlin_gemm_int4, differentiable in A."""
+    def input_grad(dy, dtype):
+        if kind == "fp4":
+            return backward.marlin_gemm_fp4_backward(dy, B_packed, scales, group_size, dtype)
+        return backward.marlin_gemm_int4_backward(dy, B_packed, scales, zeros, group_size, dtype)
+    return _Linear.apply(A, lambda x: kernels._gemm(kind, x, B_packed, scales, zeros, group_size),
+                         input_grad, False)
+
+
+def rowpacked_gemm(A: torch.Tensor, B_rows: torch.Tensor, scales: torch.Tensor,
+                   group_size: int) -> torch.Tensor:
+    """mmfp4_gemm_rowpacked, differentiable in A."""
+    return _Linear.apply(
+        A, lambda x: kernels.mmfp4_gemm_rowpacked(x, B_rows, scales, group_size),
+        lambda dy, dt: backward.mmfp4_gemm_rowpacked_backward(dy, B_rows, scales, group_size, dt),
+        False)
+
+
+class FusedQKV(torch.autograd.Function):
+    """mmfp4_fused_qkv, differentiable in A: the three gradients meet in one product."""
+
     @staticmethod
-    def forward(ctx, x, gate_packed, gate_scales, up_packed, up_scales, group_size, row_packed):
+    def forward(ctx, A, group_size, *weights):
+        refuse_foreign_leaf(A)
+        ctx.save_for_backward(*weights)
+        ctx.group_size, ctx.dtype, ctx.shape = group_size, A.dtype, A.shape
+        out = kernels.mmfp4_fused_qkv(A, *weights, group_size)
+        return tuple(t.clone() if t._is_view() else t for t in out)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk, dv):
+        dx = backward.mmfp4_fused_qkv_backward(dq, dk, dv, *ctx.saved_tensors, ctx.group_size,
+                                               out_dtype=ctx.dtype)
+        return (dx.view(ctx.shape), None, *[None] * 6)
+
+
+class GateUp(torch.autograd.Function):
+    """fused_gate_up_swiglu, its h as it comes or in x's type; h is differentiable in x, what is
+    kept is not."""
+
+    @staticmethod
+    def forward(ctx, x, gate_packed, gate_scales, up_packed, up_scales, group_size, row_packed,
+                cast):
         refuse_foreign_leaf(x)
         h, gate_up = backward.fused_gate_up_swiglu(x, gate_packed, gate_scales, up_packed,
                                                    up_scales, group_size, row_packed)
         ctx.save_for_backward(gate_up, gate_packed, gate_scales, up_packed, up_scales)
         ctx.group_size, ctx.row_packed, ctx.dtype = group_size, row_packed, x.dtype
-        return h.to(x.dtype)
+        ctx.mark_non_differentiable(gate_up)
+        return h.to(x.dtype) if cast else h, gate_up
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dh):
+    def backward(ctx, dh, _):
         gate_up, *weights = ctx.saved_tensors
         dx = backward.fused_gate_up_swiglu_backward(dh, gate_up, *weights, ctx.group_size,
                                                     ctx.row_packed, out_dtype=ctx.dtype)
-        return dx, None, None, None, None, None, None
+        return (dx, *[None] * 7)
 
 
 def gate_up_swiglu(x: torch.Tensor, gate_packed: torch.Tensor, gate_scales: torch.Tensor,
@@ -109,8 +157,8 @@ def gate_up_swiglu(x: torch.Tensor, gate_packed: torch.Tensor, gate_scales: torc
                    row_packed: bool = False) -> torch.Tensor:
     """silu(x @ Wg) * (x @ Wu) in x's type, differentiable in x: fused_gate_up_swiglu and its
     backward pass as one differentiable call."""
-    return _GateUp.apply(x, gate_packed, gate_scales, up_packed, up_scales, group_size,
-                         row_packed)
+    return GateUp.apply(x, gate_packed, gate_scales, up_packed, up_scales, group_size,
+                        row_packed, True)[0]
 
 
 class LoraAdd(torch.autograd.Function):

@@ -252,7 +252,12 @@ def fused_gate_up_swiglu(x: torch.Tensor, gate_packed: torch.Tensor, gate_scales
     one launch.  Marlin words [K/8, N], or with row_packed [N, K/8]; scales [K/group_size, N].
     Shapes that the one-launch kernels do not take (N % 8 != 0; above 32 rows K % 64 != 0;
     row-packed words whose group size is no multiple of 32, or 64 above 32 rows) run two
-    products, and SiLU then sees the fp16 ones."""
+    products, and SiLU then sees the fp16 ones.  Where x requires a gradient, h is
+    differentiable in x, and gate_up is not."""
+    if kernels._wants_grad(x):
+        from .autograd import GateUp
+        return GateUp.apply(x, gate_packed, gate_scales, up_packed, up_scales, group_size,
+                            row_packed, False)
     dev = _lib.require_device(x, gate_packed, gate_scales, up_packed, up_scales)
     if x.dim() == 0 or not x.is_floating_point():
         raise ValueError(f"x must be a floating tensor [*, K], got {x.dtype} {tuple(x.shape)}")

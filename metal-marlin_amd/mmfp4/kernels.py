@@ -4,7 +4,10 @@
 Same names, argument meaning and errors as metal_marlin/kernels_core.py;
 outputs are fp16 like the reference.  Calls are asynchronous on the current
 torch stream (the reference blocks on `waitUntilCompleted`); there is no CPU
-fallback: host tensors raise.
+fallback: host tensors raise.  marlin_gemm_fp4, marlin_gemm_int4 (and their aliases, the
+decode products and mmfp4_gemm, which call them), mmfp4_gemm_rowpacked and mmfp4_fused_qkv are
+differentiable in their activations; the weights are frozen.  The gate/up products here are
+not (their results are detached): gate_up_swiglu is the differentiable form.
 """
 
 from __future__ import annotations
@@ -176,6 +179,15 @@ def _gemm_ctypes(kind: str, A: torch.Tensor, B_packed: torch.Tensor, scales: tor
     return out.view(*A.shape[:-1], N)
 
 
+def _wants_grad(A: torch.Tensor) -> bool:
+    return getattr(A, "requires_grad", False) and torch.is_grad_enabled()
+
+
+def _autograd():
+    from . import autograd
+    return autograd
+
+
 def marlin_gemm_fp4(A: torch.Tensor, B_packed: torch.Tensor, scales: torch.Tensor,
                     group_size: int = 32) -> torch.Tensor:
     """C = A @ dequant(B_packed, scales) -- kernels_core.py:1830-1937.
@@ -185,6 +197,8 @@ def marlin_gemm_fp4(A: torch.Tensor, B_packed: torch.Tensor, scales: torch.Tenso
     the decode kernels, larger M the MFMA mid-sized or prefill kernel, whichever is
     faster (metal_dispatch.py:4083-4098 chooses by M too).
     """
+    if _wants_grad(A):
+        return _autograd().marlin_gemm("fp4", A, B_packed, scales, None, group_size)
     return _gemm("fp4", A, B_packed, scales, None, group_size)
 
 
@@ -214,6 +228,8 @@ def mmfp4_gemm_rowpacked(A: torch.Tensor, B_rows: torch.Tensor, scales: torch.Te
     runs the decode kernels; larger M the mid-sized or the pipelined prefill
     kernel, which read the words in place too but take [K/group_size, N] scales
     (the other layout is transposed here, K/group_size x N halves)."""
+    if _wants_grad(A):
+        return _autograd().rowpacked_gemm(A, B_rows, scales, group_size)
     if isinstance(A, torch.Tensor) and A.dim() == 2 and B_rows.dim() == 2 and \
             scales.dim() == 2 and scales.shape[1] == B_rows.shape[0]:
         out = _fast("rowpacked", A, B_rows, scales, group_size)
@@ -252,6 +268,8 @@ def marlin_gemm_fused_fp4(A, B_packed, scales, group_size: int = 32):
 def marlin_gemm_int4(A: torch.Tensor, B_packed: torch.Tensor, scales: torch.Tensor,
                      zeros: torch.Tensor, group_size: int = 32) -> torch.Tensor:
     """C = A @ ((q - zeros) * scales) -- kernels_core.py:1959-2066."""
+    if _wants_grad(A):
+        return _autograd().marlin_gemm("u4", A, B_packed, scales, zeros, group_size)
     return _gemm("u4", A, B_packed, scales, zeros, group_size)
 
 
@@ -289,6 +307,7 @@ def _gate_up(x: torch.Tensor, gate_packed: torch.Tensor, gate_scales: torch.Tens
         # stream 64-k chunks; other shapes take two GEMM launches (any N, and
         # the tile kernel for K % 64 tails), and SiLU then sees the fp16
         # products, as in the reference's kernel.
+        x = x.detach()      # as in the one-launch form: gate_up_swiglu is the differentiable one
         g = marlin_gemm_fp4(x, gate_packed, gate_scales, group_size)
         u = marlin_gemm_fp4(x, up_packed, up_scales, group_size)
         if not act:
@@ -388,6 +407,9 @@ def mmfp4_fused_qkv(A: torch.Tensor, Q_packed: torch.Tensor, Q_scales: torch.Ten
     and mid-sized M run one launch over all three matrices' column tiles;
     larger M one launch per matrix (the reference falls back to separate GEMMs
     for M > 1)."""
+    if _wants_grad(A):
+        return _autograd().FusedQKV.apply(A, group_size, Q_packed, Q_scales, K_packed, K_scales,
+                                          V_packed, V_scales)
     if isinstance(A, torch.Tensor) and A.dim() == 2:
         out = _fast("qkv", A, (Q_packed, K_packed, V_packed), (Q_scales, K_scales, V_scales),
                     group_size)
@@ -413,9 +435,9 @@ def mmfp4_fused_qkv(A: torch.Tensor, Q_packed: torch.Tensor, Q_scales: torch.Ten
     if any(n % 4 for n in Ns):
         # the one-launch form stores 4 adjacent columns per lane; other widths
         # take one (padded) GEMM per matrix
-        return tuple(marlin_gemm_fp4(a, p, sc, group_size).reshape(*lead, n)
-                     for (p, sc), n in zip(mats, Ns))
-    outs = [torch.empty((M, n), dtype=torch.float16, device=dev) for n in Ns]
+        a = a.view(*lead, Kdim)
+        return tuple(marlin_gemm_fp4(a, p, sc, group_size) for p, sc in mats)
+    outs = [torch.empty((*lead, n), dtype=torch.float16, device=dev) for n in Ns]
     lib = _lib.load()
     ws_bytes = max([int(lib.mm_gemm_workspace_bytes(M, sum(Ns), Kdim))] +
                    [int(lib.mm_gemm_workspace_bytes(M, n, Kdim)) for n in Ns])
@@ -427,7 +449,7 @@ def mmfp4_fused_qkv(A: torch.Tensor, Q_packed: torch.Tensor, Q_scales: torch.Ten
     Nt = (ctypes.c_int * 3)(*Ns)
     _lib.call("mm_fp4_gemm_multi", _lib.ptr(a), 3, Bt, St, Ct, Nt, M, Kdim, group_size,
               _lib.ptr(ws), ws.numel(), _lib.stream_of(a))
-    return tuple(o.reshape(*lead, n) for o, n in zip(outs, Ns))
+    return tuple(outs)
 
 
 def dequant_fp4(B_packed: torch.Tensor, scales: torch.Tensor, K: int, N: int,
@@ -503,7 +525,8 @@ def mmfp4_gemm(A: torch.Tensor, B_packed: torch.Tensor, B_scales: torch.Tensor,
     M = 1
     for d in A.shape[:-1]:
         M *= d
-    if 0 < M <= 16 and A.shape[-1] == K and N % 4 == 0 and group_size % 8 == 0:
+    if 0 < M <= 16 and A.shape[-1] == K and N % 4 == 0 and group_size % 8 == 0 and \
+            not _wants_grad(A):
         # decode sizes: the [N, K/g] scales are read in place (mm_fp4_gemm_mmfp4)
         dev = _lib.require_device(A, B_packed, B_scales)
         a = _half(A.reshape(M, K))

@@ -20,14 +20,15 @@ def dispatch_gemm_fp4(lib: Any, A: torch.Tensor, B_packed: torch.Tensor, scales:
                       out: torch.Tensor | None = None) -> torch.Tensor:
     """C[M, N] = A[M, K] @ dequant(B_packed [K/8, N], scales [K/g, N]).
     `enable_padding` is accepted and unused: the kernels take any M and
-    N % 4 == 0 without padding.  With `out`, the result is written there."""
+    N % 4 == 0 without padding.  With `out`, the result is written there and takes no part in
+    autograd."""
     if tuple(A.shape[-2:]) != (M, K) and not (A.dim() == 1 and M == 1 and A.shape[0] == K):
         raise ValueError(f"A shape {tuple(A.shape)} does not match M={M}, K={K}")
     if B_packed.shape[-1] != N:
         raise ValueError(f"B_packed has {B_packed.shape[-1]} columns, expected N={N}")
     C = kernels.marlin_gemm_fp4(A.reshape(M, K), B_packed, scales, group_size)
     if out is not None:
-        out.copy_(C)
+        out.copy_(C.detach())
         return out
     return C
 
