@@ -184,16 +184,26 @@ class LoraAdd(torch.autograd.Function):
         return dy.to(ctx.base_dtype), dx, da, db, None, None
 
 
+def _column_sums(t: torch.Tensor) -> torch.Tensor:
+    """[M, N] -> [N] in fp32.  At most 128 rows at a time: sums of more are shared out over
+    blocks, whose counters torch clears in a way that a graph must not replay."""
+    while t.shape[0] > 128:
+        n = t.shape[0] // 128 * 128
+        blocks = t[:n].view(-1, 128, t.shape[1]).sum(1, dtype=torch.float32)
+        t = torch.cat([blocks, t[n:].float()])
+    return t.sum(0, dtype=torch.float32)
+
+
 class LoraLinear(torch.autograd.Function):
-    """A layer and its adapters in one node, so that the two gradients of x are added before
-    they are rounded."""
+    """A layer and its adapters in one node.  `bias` is the layer's, for its gradient."""
 
     @staticmethod
-    def forward(ctx, x, lora_a, lora_b, adapter_ids, scaling, layer):
-        refuse_foreign_leaf(x, lora_a, lora_b)
+    def forward(ctx, x, lora_a, lora_b, adapter_ids, scaling, layer, bias):
+        refuse_foreign_leaf(x, lora_a, lora_b, bias)
         ctx.save_for_backward(x, lora_a, lora_b, adapter_ids,
                               scaling if isinstance(scaling, torch.Tensor) else None)
         ctx.scaling, ctx.layer = scaling, layer
+        ctx.bias_dtype = None if bias is None else bias.dtype
         return adapters._add(layer(x), x, lora_a, lora_b, adapter_ids, scaling).to(x.dtype)
 
     @staticmethod
@@ -201,8 +211,12 @@ class LoraLinear(torch.autograd.Function):
     def backward(ctx, dy):
         x, a, b, ids, scaling = ctx.saved_tensors
         dy = dy.contiguous()
-        base = ctx.layer.input_grad(dy, x.dtype) if ctx.needs_input_grad[0] else None
-        dx, da, db = adapters.lora_backward(dy, x, a, b, ids,
-                                            ctx.scaling if scaling is None else scaling,
-                                            dx_base=base)
-        return (dx if ctx.needs_input_grad[0] else None), da, db, None, None, None
+        dx = da = db = dbias = None
+        if any(ctx.needs_input_grad[:3]):
+            base = ctx.layer.input_grad(dy, x.dtype) if ctx.needs_input_grad[0] else None
+            dx, da, db = adapters.lora_backward(dy, x, a, b, ids,
+                                                ctx.scaling if scaling is None else scaling,
+                                                dx_base=base)
+        if ctx.needs_input_grad[6]:
+            dbias = _column_sums(dy.view(-1, dy.shape[-1])).to(ctx.bias_dtype)
+        return (dx if ctx.needs_input_grad[0] else None), da, db, None, None, None, dbias

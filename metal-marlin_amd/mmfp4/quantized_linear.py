@@ -179,9 +179,10 @@ class LoRALinear(nn.Module):
     """A quantized layer (QuantizedLinear, MarlinLinear, MMFP4Linear) with low-rank adapters of
     several requests or users beside it: y = layer(x) + scaling[a] * (x @ lora_a[a]^T) @
     lora_b[a]^T with a = adapter_ids[t], one id per token; ids outside [0, num_adapters) mean
-    no adapter.  The layer is frozen, lora_a [num_adapters, rank, in] (normal) and lora_b
-    [num_adapters, out, rank] (zeros) are the parameters.  `scaling`: a number, or one per
-    adapter.  fp16 or bf16 inputs; fp32 ones are computed as fp16, as the layer does."""
+    no adapter.  The layer's weights are frozen (a bias that requires a gradient gets it);
+    lora_a [num_adapters, rank, in] (normal) and lora_b [num_adapters, out, rank] (zeros) are
+    the parameters.  `scaling`: a number, or one per adapter.  fp16 or bf16 inputs; fp32 ones
+    are computed as fp16, as the layer does."""
 
     def __init__(self, layer, rank: int, num_adapters: int = 1,
                  scaling: float | torch.Tensor = 1.0, dtype: torch.dtype = torch.float16,
@@ -204,9 +205,10 @@ class LoRALinear(nn.Module):
             self.scaling = float(scaling)
 
     def forward(self, x: torch.Tensor, adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
-        if autograd.wants_grad(x, self.lora_a, self.lora_b):
+        bias = getattr(self.layer, "bias", None)
+        if autograd.wants_grad(x, self.lora_a, self.lora_b, bias):
             return autograd.LoraLinear.apply(x, self.lora_a, self.lora_b, adapter_ids,
-                                             self.scaling, self.layer)
+                                             self.scaling, self.layer, bias)
         return adapters.lora_add(self.layer(x), x, self.lora_a, self.lora_b, adapter_ids,
                                  self.scaling).to(x.dtype)
 
