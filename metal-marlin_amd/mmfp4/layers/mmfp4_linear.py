@@ -149,6 +149,8 @@ class MMFP4Linear(nn.Module):
         if not x.is_floating_point():
             raise ValueError(f"x must be a floating tensor, got dtype={x.dtype}")
         x2 = x.reshape(-1, self.in_features)
+        if self.bias is not None and self.bias.requires_grad and torch.is_grad_enabled():
+            autograd.refuse_foreign_leaf(self.bias)
         if self.bias is not None and self.bias.requires_grad and autograd.wants_grad(x):
             out = autograd.linear(x2, self._product, self.input_grad)
             out = out + self.bias.to(device=out.device, dtype=out.dtype)

@@ -97,6 +97,8 @@ class QuantizedLinear(nn.Module):
             x_flat = x_flat @ self.hadamard.to(x.device, x.dtype)
         out = self._dispatch_quantized_gemm(x_flat)
         if self.bias is not None:
+            if self.bias.requires_grad and torch.is_grad_enabled():
+                autograd.refuse_foreign_leaf(self.bias)
             out.add_(self.bias)
         return out.view(*batch_shape, self.out_features)
 
@@ -152,6 +154,8 @@ class MarlinLinear:
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
         out = quantized_linear(x, self.weight_packed, self.scales, self.group_size)
         if self.bias is not None:
+            if self.bias.requires_grad and torch.is_grad_enabled():
+                autograd.refuse_foreign_leaf(self.bias)
             out.add_(self.bias)
         return out
 

@@ -79,3 +79,26 @@ def test_beside_adapters_captured():
         torch.cuda.synchronize()
         for a, b in zip(held, step()):
             assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("wants", [False, True])
+def test_capture_beside_a_living_graph_is_refused(wants):
+    """An eager graph of the bias is alive on another stream: the captured forward pass raises
+    (a backward pass would end the process)."""
+    gen = torch.Generator().manual_seed(3)
+    for name, layer in layers(gen, 64, 64, 64, F16):
+        layer.bias.requires_grad_(True)
+        x = torch.randn((4, 64), generator=gen).to(DEV, F16)
+        alive = layer(x)
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            y = x.clone().requires_grad_(wants)
+            for f in (layer, mmfp4.LoRALinear(layer, 4)):
+                with pytest.raises(RuntimeError, match="another stream"):
+                    with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                        f(y)
+                with torch.no_grad(), torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                    f(y)                             # nothing to go back through
+        torch.cuda.synchronize()
+        assert alive.isfinite().all()
