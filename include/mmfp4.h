@@ -228,7 +228,7 @@ int mm_gemm_backward(const uint16_t* const* dC, const int* ldc, const float* row
                      int M, int K, int group_size, void* ws, size_t ws_bytes, void* stream);
 
 /* Gradients carried in fp16 under one power of two per row: Y = X * 2^e with the row's
- * largest magnitude in [2^14, 2^15), row_mul = 2^-e (a zero or non-finite row: e = 0).
+ * largest finite magnitude in [2^14, 2^15), row_mul = 2^-e (none: e = 0; at most 149).
  * type 0 fp32, 1 fp16, 2 bf16; N % 8 == 0. */
 int mm_grad_rows(const void* X, int type, uint16_t* Y, float* row_mul, int M, int N,
                  void* stream);

@@ -10,8 +10,12 @@
 //
 // Gradients have a wider range than activations.  bf16 and fp32 ones, and those of the
 // gate/up pair, are carried in fp16 with one power of two per row (k_grad_rows,
-// k_swiglu_grad): a row's largest value lands in [2^14, 2^15), so what is lost lies 2^-40
-// below it, and the power of two is taken out of the fp32 sums exactly.
+// k_swiglu_grad): a row's largest finite value lands in [2^14, 2^15), so what is lost lies
+// 2^-40 below it, and the power of two is taken out of the fp32 sums exactly.  11 bits of each
+// value are held: all of a bf16 one's 8, and of fp32 ones and the pair's dg and du the nearest
+// (a second fp16 term of each would double the matrix work; the fp16 gradients of the gated
+// block are off by 1.4 times the half step that the result's own rounding costs, bf16 ones by
+// no more than that).
 #include <algorithm>
 
 #include "mm_common.h"
@@ -893,21 +897,11 @@ k_grad_skinny(GradSegs segs, void* __restrict__ out, int ot, const float* __rest
 }
 
 // ---------------------------------------------------------------------------
-// Row conversion: fp16 values v * 2^e with the row's largest in [2^14, 2^15), and
-// rowmul[row] = 2^-e.  A zero or non-finite row keeps e = 0.
+// Row conversion: fp16 values v * 2^e with the row's largest finite one in [2^14, 2^15), and
+// rowmul[row] = 2^-e.
 // ---------------------------------------------------------------------------
 constexpr int RW_NT = 512;
 constexpr int RW_HOLD = 4;      // 8-value pieces of a row that a thread keeps in registers
-
-MM_DEV float row_exponent(float m, float& inv) {
-  int e = 0;
-  if (m > 0.0f && m < __builtin_inff()) {
-    (void)frexpf(m, &e);          // m = f * 2^e, f in [0.5, 1)
-    e = max(-110, min(110, 15 - e));
-  }
-  inv = ldexpf(1.0f, -e);
-  return ldexpf(1.0f, e);
-}
 
 MM_DEV float block_max(float m, float* red) {
 #pragma unroll
@@ -917,6 +911,33 @@ MM_DEV float block_max(float m, float* red) {
   m = red[0];
 #pragma unroll
   for (int i = 1; i < RW_NT / 64; ++i) m = fmaxf(m, red[i]);
+  return m;
+}
+// The row's factor from largest(finite), its largest magnitude, of the finite values alone or of
+// all: a non-finite value stays what it is and leaves the others theirs.  A row that has one
+// is looked through twice, so that the others are spared the test of every value.  2^e is up
+// to 2^149, so it comes as two factors, the second mostly 1.
+struct RowScale {
+  float mul, more;
+};
+template <typename F>
+MM_DEV RowScale row_scale(F largest, float* rowmul) {
+  float m = largest(std::false_type{});
+  if (m == __builtin_inff()) {
+    __syncthreads();            // every wave has the first maximum
+    m = largest(std::true_type{});
+  }
+  const int e = carry_exponent(m);
+  if (threadIdx.x == 0) rowmul[blockIdx.x] = ldexpf(1.0f, -e);
+  return RowScale{ldexpf(1.0f, min(e, 126)), ldexpf(1.0f, max(0, e - 126))};
+}
+template <bool FINITE>
+MM_DEV float max8(float m, const float (&v)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float a = fabsf(v[k]);
+    m = !FINITE || a < __builtin_inff() ? fmaxf(m, a) : m;
+  }
   return m;
 }
 
@@ -943,10 +964,15 @@ MM_DEV void load8(const void* p, size_t at, float (&v)[8]) {
     }
   }
 }
-MM_DEV void store8(f16* p, const float (&v)[8], float mul) {
+MM_DEV void store8(f16* p, const float (&v)[8], RowScale s) {
   f16x8 o;
+  if (s.more == 1.0f) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = (f16)(v[i] * mul);
+    for (int i = 0; i < 8; ++i) o[i] = (f16)(v[i] * s.mul);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (f16)(v[i] * s.mul * s.more);
+  }
   *(f16x8*)p = o;
 }
 
@@ -968,34 +994,34 @@ k_grad_rows(RowParts parts, f16* __restrict__ Y, float* __restrict__ rowmul) {
   __shared__ float red[RW_NT / 64];
   const int row = blockIdx.x, np = parts.end[2];
   const size_t base = 8 * (size_t)row * np;
-  float hold[RW_HOLD][8], m = 0.0f;
+  float hold[RW_HOLD][8];
 #pragma unroll
   for (int i = 0; i < RW_HOLD; ++i) {
     const int p = threadIdx.x + i * RW_NT;
-    if (p < np) {
-      parts.load<T>(row, p, hold[i]);
+    if (p < np) parts.load<T>(row, p, hold[i]);
+  }
+  auto largest = [&](auto finite) {
+    float m = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(hold[i][k]));
+    for (int i = 0; i < RW_HOLD; ++i)
+      if (threadIdx.x + i * RW_NT < np) m = max8<finite.value>(m, hold[i]);
+    for (int p = threadIdx.x + RW_HOLD * RW_NT; p < np; p += RW_NT) {
+      float v[8];
+      parts.load<T>(row, p, v);
+      m = max8<finite.value>(m, v);
     }
-  }
-  for (int p = threadIdx.x + RW_HOLD * RW_NT; p < np; p += RW_NT) {
-    float v[8];
-    parts.load<T>(row, p, v);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(v[k]));
-  }
-  float inv;
-  const float mul = row_exponent(block_max(m, red), inv);
-  if (threadIdx.x == 0) rowmul[blockIdx.x] = inv;
+    return block_max(m, red);
+  };
+  const RowScale scale = row_scale(largest, rowmul);
 #pragma unroll
   for (int i = 0; i < RW_HOLD; ++i) {
     const int p = threadIdx.x + i * RW_NT;
-    if (p < np) store8(Y + base + 8 * (size_t)p, hold[i], mul);
+    if (p < np) store8(Y + base + 8 * (size_t)p, hold[i], scale);
   }
   for (int p = threadIdx.x + RW_HOLD * RW_NT; p < np; p += RW_NT) {
     float v[8];
     parts.load<T>(row, p, v);
-    store8(Y + base + 8 * (size_t)p, v, mul);
+    store8(Y + base + 8 * (size_t)p, v, scale);
   }
 }
 
@@ -1025,38 +1051,39 @@ k_swiglu_grad(const void* __restrict__ dH, const f16* __restrict__ GU, f16* __re
 #pragma unroll
     for (int k = 0; k < 8; ++k) swiglu_grad(dh[k], g[k], u[k], dg[k], du[k]);
   };
-  float hg[RW_HOLD][8], hu[RW_HOLD][8], m = 0.0f;
+  float hg[RW_HOLD][8], hu[RW_HOLD][8];
+#pragma unroll
+  for (int i = 0; i < RW_HOLD; ++i) {
+    const int p = threadIdx.x + i * RW_NT;
+    if (p < np) grads(p, hg[i], hu[i]);
+  }
+  auto largest = [&](auto finite) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < RW_HOLD; ++i)
+      if (threadIdx.x + i * RW_NT < np)
+        m = max8<finite.value>(max8<finite.value>(m, hg[i]), hu[i]);
+    for (int p = threadIdx.x + RW_HOLD * RW_NT; p < np; p += RW_NT) {
+      float dg[8], du[8];
+      grads(p, dg, du);
+      m = max8<finite.value>(max8<finite.value>(m, dg), du);
+    }
+    return block_max(m, red);
+  };
+  const RowScale scale = row_scale(largest, rowmul);
 #pragma unroll
   for (int i = 0; i < RW_HOLD; ++i) {
     const int p = threadIdx.x + i * RW_NT;
     if (p < np) {
-      grads(p, hg[i], hu[i]);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) m = fmaxf(m, fmaxf(fabsf(hg[i][k]), fabsf(hu[i][k])));
+      store8(Y + gb + 8 * (size_t)p, hg[i], scale);
+      store8(Y + gb + N + 8 * (size_t)p, hu[i], scale);
     }
   }
   for (int p = threadIdx.x + RW_HOLD * RW_NT; p < np; p += RW_NT) {
     float dg[8], du[8];
     grads(p, dg, du);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) m = fmaxf(m, fmaxf(fabsf(dg[k]), fabsf(du[k])));
-  }
-  float inv;
-  const float mul = row_exponent(block_max(m, red), inv);
-  if (threadIdx.x == 0) rowmul[blockIdx.x] = inv;
-#pragma unroll
-  for (int i = 0; i < RW_HOLD; ++i) {
-    const int p = threadIdx.x + i * RW_NT;
-    if (p < np) {
-      store8(Y + gb + 8 * (size_t)p, hg[i], mul);
-      store8(Y + gb + N + 8 * (size_t)p, hu[i], mul);
-    }
-  }
-  for (int p = threadIdx.x + RW_HOLD * RW_NT; p < np; p += RW_NT) {
-    float dg[8], du[8];
-    grads(p, dg, du);
-    store8(Y + gb + 8 * (size_t)p, dg, mul);
-    store8(Y + gb + N + 8 * (size_t)p, du, mul);
+    store8(Y + gb + 8 * (size_t)p, dg, scale);
+    store8(Y + gb + N + 8 * (size_t)p, du, scale);
   }
 }
 

@@ -83,6 +83,19 @@ MM_DEV f16x8 dq_u4_word(uint32_t w, f16x2 negz2, f16x2 s2) {
 }
 
 // ---------------------------------------------------------------------------
+// Values carried in 16 bits under a power of two 2^e that puts the largest magnitude m of those
+// that share it into [2^14, 2^15).  e = 0 where there is none.  For the smallest m 2^-e has to be
+// an fp32 number too (the subnormal 2^-149): there all values are multiples of 2^-149 and
+// below 2^15 of them, so nothing is lost but what 11 bits do not hold.
+// ---------------------------------------------------------------------------
+MM_DEV int carry_exponent(float m) {
+  if (!(m > 0.0f)) return 0;
+  int e;
+  (void)frexpf(m, &e);            // m = f * 2^e, f in [0.5, 1)
+  return min(149, 15 - e);
+}
+
+// ---------------------------------------------------------------------------
 // Error reporting shared by every C entry point.
 // ---------------------------------------------------------------------------
 void mm_set_error(const char* fmt, ...);

@@ -5,8 +5,8 @@ has no backward pass (metal_marlin/quantized_linear.py:36-55 is forward only).
 
 Gradients are fp16, bf16 or fp32, and the result has the gradient's type unless
 `out_dtype` says otherwise.  fp16 ones are multiplied as they are; bf16 and fp32 ones, and
-those inside the gate/up block, are carried in fp16 under one power of two per row (22
-bits below a row's largest value are kept, so nothing underflows that bf16 can hold), the
+those inside the gate/up block, are carried in fp16 under one power of two per row: bf16 ones
+exactly and the others to 11 bits, but for what lies 2^-40 below a row's largest value.  The
 products are fp16 x fp16 in fp32 sums, and the sum is rounded once.
 """
 
