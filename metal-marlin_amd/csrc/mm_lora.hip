@@ -9,10 +9,12 @@
 // of one adapter (k_plan, or up to 2048 tokens each block of k_down for its own tile), and
 //   k_down   H of a tile, over the whole width: 16x16x32 MFMAs, the width split over the
 //            waves and over blocks.  The block that finishes a tile leaves a record of it:
-//            H as hi + lo in the operands' type, under one power of two per tile that puts
-//            the tile's largest value in [2^14, 2^15): 16 (bf16) or 22 (fp16) bits of H
-//            reach the second product, whatever its size.  The record has H by token and
-//            by rank, the operand orders of the two kernels that follow.
+//            H as hi + lo in the operands' type, under a power of two that puts the largest
+//            value in [2^14, 2^15), so that 16 (bf16) or 22 (fp16) bits of H reach the second
+//            product.  The record has H by token and by rank, the operand orders of the two
+//            kernels that follow: by token each token has a power of two of its own (in fp16
+//            another request's large values would cost it bits), by rank, where the tokens
+//            of a tile are summed, the tile has one.
 //   up       out of a tile: MFMAs over [hi | lo] of 16 ranks at a time.
 //   wgrad    dA_a or dB_a: MFMAs over 32 tokens at a time, tile after tile; the tiles are shared
 //            out over a block's waves, or a wave has them all where an adapter has few tokens.
@@ -390,7 +392,8 @@ MM_DEV TileInfo own_tile(const PlanOut& o, int T, int b, bool write, int* cnt, i
 struct Records {
   uint16_t* by_token;   // [tile][chunk][hi, lo][64][rp]
   uint16_t* by_rank;    // [tile][chunk][hi, lo][rp][64]
-  float* scale;         // [tile][chunk]: H = scale * (hi + lo)
+  float* token_scale;   // [tile][chunk][64]: H of a token = token_scale * (hi + lo) by token
+  float* scale;         // [tile][chunk]: H = scale * (hi + lo) by rank
   int rp, nrc;
 };
 
@@ -640,57 +643,68 @@ MM_DEV void down_tile(const DownProblem& p, const Plan& plan, const int* list, T
           for (int k = 0; k < PER; ++k) h[k] += ld[z][k];
     }
   }
-  // The record.  Ranks and rows past the last are zero.
+  // The record.  Ranks and rows past the last are zero.  The RP / 4 threads of a token lie side
+  // by side.  A non-finite token leaves the others their bits.
   const float s = scaling.at(t.e);
   float m = 0.0f;
+  int row_ex[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int it = threadIdx.x + k * NT, row = 4 * it / RP, rank = 4 * it % RP;
+    float rm = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       h[k][i] = row < t.rows && r0 + rank + i < r ? h[k][i] * s : 0.0f;
       const float a = fabsf(h[k][i]);
-      m = a < __builtin_inff() ? fmaxf(m, a) : m;   // a non-finite token leaves the others their bits
+      rm = a < __builtin_inff() ? fmaxf(rm, a) : rm;
     }
+#pragma unroll
+    for (int d = RP / 8; d > 0; d >>= 1) rm = fmaxf(rm, __shfl_xor(rm, d));
+    row_ex[k] = carry_exponent(rm);
+    m = fmaxf(m, rm);
   }
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-  if (lane == 0) s_max[wave] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < LO_DW; ++w) m = fmaxf(m, s_max[w]);
   int ex = 0;
-  if (m > 0.0f) {
-    (void)frexpf(m, &ex);                      // m = f * 2^ex, f in [0.5, 1)
-    ex = max(-110, min(110, 15 - ex));
+  if (p.by_rank) {
+#pragma unroll
+    for (int d = 32; d > RP / 8; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    if (lane == 0) s_max[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < LO_DW; ++w) m = fmaxf(m, s_max[w]);
+    ex = carry_exponent(m);
+    if (threadIdx.x == 0) p.rec.scale[slot] = ldexpf(1.0f, -ex);
   }
-  const float up = ldexpf(1.0f, ex);
   uint16_t* bt = p.rec.by_token + (size_t)slot * 2 * LO_TM * RP;
   uint16_t* br = p.rec.by_rank + (size_t)slot * 2 * LO_TM * RP;
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int it = threadIdx.x + k * NT, row = 4 * it / RP, rank = 4 * it % RP;
     if (it >= ITEMS) continue;
-    u16x4 hi, lo;
+    auto split = [&](int e, u16x4& hi, u16x4& lo) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float v = h[k][i] * up;
-      hi[i] = from_f32<T>(v);
-      const float f = to_f32<T>(hi[i]);
-      lo[i] = __builtin_isfinite(f) ? from_f32<T>(v - f) : (uint16_t)0;
-    }
+      for (int i = 0; i < 4; ++i) {
+        const float v = ldexpf(h[k][i], e);
+        hi[i] = from_f32<T>(v);
+        const float f = to_f32<T>(hi[i]);
+        lo[i] = __builtin_isfinite(f) ? from_f32<T>(v - f) : (uint16_t)0;
+      }
+    };
+    u16x4 hi, lo;
     if (p.by_token) {
+      split(row_ex[k], hi, lo);
       *(u16x4*)(bt + row * RP + rank) = hi;
       *(u16x4*)(bt + LO_TM * RP + row * RP + rank) = lo;
+      if (rank == 0) p.rec.token_scale[(size_t)slot * LO_TM + row] = ldexpf(1.0f, -row_ex[k]);
     }
-    if (p.by_rank)
+    if (p.by_rank) {
+      split(ex, hi, lo);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         br[(rank + i) * LO_TM + row] = hi[i];
         br[LO_TM * RP + (rank + i) * LO_TM + row] = lo[i];
       }
+    }
   }
-  if (threadIdx.x == 0) p.rec.scale[slot] = ldexpf(1.0f, -ex);
 }
 
 template <int T, int RT>
@@ -762,7 +776,10 @@ MM_DEV void up_rows(const UpProblem& p, const Plan& plan, TileInfo t, int r, int
       const size_t slot = (size_t)b * rec.nrc + ch;
       const uint16_t* H = rec.by_token + slot * 2 * LO_TM * RP + (q >> 1) * LO_TM * RP +
                           (16 * i0 + c) * RP + 8 * (q & 1);
-      const float f = rec.scale[slot];
+      f32x4 f[NI];   // of tokens 4q + k
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        f[i] = *(const f32x4*)(rec.token_scale + slot * LO_TM + 16 * (i0 + i) + 4 * q);
       u16x8 hv[NI][RT];
 #pragma unroll
       for (int i = 0; i < NI; ++i)
@@ -794,7 +811,7 @@ MM_DEV void up_rows(const UpProblem& p, const Plan& plan, TileInfo t, int r, int
           f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
           for (int k = 0; k < RT; ++k) acc = mfma<T>(hv[i][k], w[k][j], acc);
-          sum[i][j] += f * acc;
+          sum[i][j] += f[i] * acc;
         }
     }
 #pragma unroll
@@ -1276,11 +1293,14 @@ int wgrad_split(int T, int L, int nrc, int C) {
 
 size_t record_bytes(const LoraPlan& p) {
   const size_t h = (size_t)p.tiles * p.nrc * 2 * LO_TM * p.rp * 2;
-  return 2 * align256(h) + align256((size_t)p.tiles * p.nrc * 4);
+  const size_t n = (size_t)p.tiles * p.nrc;
+  return 2 * align256(h) + n * LO_TM * 4 + align256(n * 4);
 }
 Records record_at(const LoraPlan& p, char* at) {
   const size_t h = align256((size_t)p.tiles * p.nrc * 2 * LO_TM * p.rp * 2);
-  return Records{(uint16_t*)at, (uint16_t*)(at + h), (float*)(at + 2 * h), p.rp, p.nrc};
+  float* scales = (float*)(at + 2 * h);
+  return Records{(uint16_t*)at, (uint16_t*)(at + h), scales,
+                 scales + (size_t)p.tiles * p.nrc * LO_TM, p.rp, p.nrc};
 }
 
 // Bytes of a problem's partial sums: `sums` of them if each is split, none otherwise.
