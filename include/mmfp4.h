@@ -268,6 +268,14 @@ int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type, const uint
                      int grad_type, int T, int K, int N, int rank, int adapters, void* ws,
                      size_t ws_bytes, void* stream);
 
+/* mm_lora_backward of fp16 tokens for gradients of a wider range: dy[t] stands for row_mul[t] *
+ * dy[t] (mm_grad_rows; NULL: ones), dx_base and dx are fp32. */
+int mm_lora_backward_f32(const uint16_t* dy, const float* row_mul, const uint16_t* x,
+                         const uint16_t* A, const uint16_t* B, const void* ids, int ids64,
+                         const float* scaling, float scale, const float* dx_base, float* dx,
+                         void* dA, void* dB, int grad_type, int T, int K, int N, int rank,
+                         int adapters, void* ws, size_t ws_bytes, void* stream);
+
 /* -------------------------------------------------------------------- MoE */
 
 /* Stable counting sort of the T*k (token, slot) assignments by expert.

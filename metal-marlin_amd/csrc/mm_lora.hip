@@ -21,6 +21,7 @@
 // All sums are fp32 and in a fixed order.  All of them stream activations that are read
 // once (x, dy) or read and written once (out): HBM bounds them, the factors stay in L2.
 #include <algorithm>
+#include <type_traits>
 
 #include "mm_common.h"
 #include "mmfp4.h"
@@ -102,6 +103,28 @@ template <bool WHOLE>
 MM_DEV void st4(uint16_t* p, u16x4 v, int n) {
   if constexpr (WHOLE) *(u16x4_any*)p = v;
   else store4(p, v, n);
+}
+
+// The same of fp32 rows, which start at any multiple of four bytes.
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+template <bool WHOLE>
+MM_DEV f32x4 ld4f(const float* p, int n) {
+  if (WHOLE || n >= 4) return *(const f32x4_any*)p;
+  f32x4 v = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (i < n) v[i] = p[i];
+  return v;
+}
+template <bool WHOLE>
+MM_DEV void st4f(float* p, f32x4 v, int n) {
+  if (WHOLE || n >= 4) {
+    *(f32x4_any*)p = v;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (i < n) p[i] = v[i];
 }
 
 // Eight rows of four values -> four columns of eight (the MFMA operand of each column).
@@ -426,6 +449,7 @@ struct DownProblem {
   float* part;             // [tile][chunk][ks][64 * rp]
   uint32_t* counters;      // [tile][chunk]
   int by_token, by_rank;   // which records are wanted
+  const float* row_mul;    // [T] or nullptr: factors of the tokens' dy, taken into H and dH
 };
 
 // LDS of a wave: its pair's activations, 64 rows of 128 bytes, 16-byte piece (row, p) at
@@ -651,10 +675,16 @@ MM_DEV void down_tile(const DownProblem& p, const Plan& plan, const int* list, T
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int it = threadIdx.x + k * NT, row = 4 * it / RP, rank = 4 * it % RP;
-    float rm = 0.0f;
+    float rm = 0.0f, f = s;
+    if (p.row_mul != nullptr) {
+      const int at[1] = {min(row, LO_TM - 1)};
+      int token[1];
+      tokens_of(plan, list, b, at, token);
+      f *= p.row_mul[token[0]];
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      h[k][i] = row < t.rows && r0 + rank + i < r ? h[k][i] * s : 0.0f;
+      h[k][i] = row < t.rows && r0 + rank + i < r ? h[k][i] * f : 0.0f;
       const float a = fabsf(h[k][i]);
       rm = a < __builtin_inff() ? fmaxf(rm, a) : rm;
     }
@@ -733,11 +763,14 @@ k_down(DownProblem p0, DownProblem p1, Plan plan, PlanOut own, Scaling scaling, 
 // ---------------------------------------------------------------------------
 // up.  Block (tile, 256 columns): wave: 64 columns, lane (c, q): columns 4c .. 4c + 3 of
 // tokens 16 i + 4 q + k.  CR: the factor is [C, r] (B), else [r, C] (A).  BT: the base's
-// type (0: no base, zeros).  Group L (no adapter) copies the base.
+// type (0: no base, zeros), BT_F32: base (or none) and out are fp32.  Group L (no adapter)
+// copies the base.
 // ---------------------------------------------------------------------------
+constexpr int BT_F32 = 3;
 struct UpProblem {
-  const uint16_t *W, *base;
-  uint16_t* out;
+  const uint16_t* W;
+  const void* base;
+  void* out;
   int C;
   Records rec;
 };
@@ -753,15 +786,19 @@ MM_DEV void up_rows(const UpProblem& p, const Plan& plan, TileInfo t, int r, int
   const uint16_t* W = p.W + (none ? 0 : (size_t)t.e * r * C);
   // The bases of all rows are on their way before anything else.
   constexpr int NR = LO_TM / 16;
-  u16x4 bv[NR * 4];
+  typename std::conditional<BT == BT_F32, f32x4, u16x4>::type bv[NR * 4];
   int at[NR * 4], token[NR * 4];
 #pragma unroll
   for (int i = 0; i < NR * 4; ++i) at[i] = 16 * (i / 4) + 4 * q + i % 4;
   plan.get(b, at, token);
 #pragma unroll
-  for (int i = 0; i < NR * 4; ++i)
-    if constexpr (BT != 0) bv[i] = ld4<WHOLE>(p.base + (size_t)token[i] * C + n0, left);
+  for (int i = 0; i < NR * 4; ++i) {
+    const size_t from = (size_t)token[i] * C + n0;
+    if constexpr (BT == BT_F32)
+      bv[i] = p.base != nullptr ? ld4f<WHOLE>((const float*)p.base + from, left) : f32x4{0, 0, 0, 0};
+    else if constexpr (BT != 0) bv[i] = ld4<WHOLE>((const uint16_t*)p.base + from, left);
     else bv[i] = u16x4{0, 0, 0, 0};
+  }
   constexpr int NI = 2;   // blocks of 16 rows at a time (all four take the registers of a wave)
   u16x8 w[RT][4];
 #pragma unroll
@@ -820,12 +857,20 @@ MM_DEV void up_rows(const UpProblem& p, const Plan& plan, TileInfo t, int r, int
       for (int k = 0; k < 4; ++k) {
         const int row = 4 * (i0 + i) + k;
         if (16 * (i0 + i) + 4 * q + k >= t.rows) continue;
-        u16x4 o;
+        const size_t to = (size_t)token[row] * C + n0;
+        if constexpr (BT == BT_F32) {
+          f32x4 o = bv[row];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          o[j] = from_f32<T>(BT != 0 ? to_f32<BT != 0 ? BT : T>(bv[row][j]) + sum[i][j][k]
-                                     : sum[i][j][k]);
-        st4<WHOLE>(p.out + (size_t)token[row] * C + n0, o, left);
+          for (int j = 0; j < 4; ++j) o[j] += sum[i][j][k];
+          st4f<WHOLE>((float*)p.out + to, o, left);
+        } else {
+          u16x4 o;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            o[j] = from_f32<T>(BT != 0 ? to_f32<BT != 0 ? BT : T>(bv[row][j]) + sum[i][j][k]
+                                       : sum[i][j][k]);
+          st4<WHOLE>((uint16_t*)p.out + to, o, left);
+        }
       }
   }
 }
@@ -1449,7 +1494,7 @@ extern "C" int mm_lora_add(const uint16_t* x, int type, const uint16_t* base, in
   const Records rec = record_at(p, (char*)ws + p.rec[0]);
   const int ks = p.kx;
   const DownProblem d{x, A, K, ks, p.per, rec, (float*)((char*)ws + p.part),
-                      (uint32_t*)ws, 1, 0};
+                      (uint32_t*)ws, 1, 0, nullptr};
 #define MM_DOWN(RTV, TV)                                                                       \
   hipLaunchKernelGGL((k_down<TV, RTV>), dim3(down_tiles, ks, p.nrc), dim3(64 * LO_DW), 0, st, d,  \
                      d, plan, own, sc, r)
@@ -1468,12 +1513,12 @@ extern "C" int mm_lora_add(const uint16_t* x, int type, const uint16_t* base, in
   return 0;
 }
 
-extern "C" int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type,
-                                const uint16_t* A, const uint16_t* B, const void* ids, int ids64,
-                                const float* scaling, float scale, const uint16_t* dx_base,
-                                uint16_t* dx, void* dA, void* dB, int grad_type, int T, int K,
-                                int N, int r, int L, void* ws, size_t ws_bytes, void* stream) {
-  const char* who = "mm_lora_backward";
+// wide: dx_base and dx are fp32, else of the type of x.
+static int lora_backward(const char* who, const uint16_t* dy, const float* row_mul,
+                         const uint16_t* x, int type, const uint16_t* A, const uint16_t* B,
+                         const void* ids, int ids64, const float* scaling, float scale, bool wide,
+                         const void* dx_base, void* dx, void* dA, void* dB, int grad_type, int T,
+                         int K, int N, int r, int L, void* ws, size_t ws_bytes, void* stream) {
   if (const int rc = check_common(who, type, T, K, N, r, L, ids, ids64)) return rc;
   MM_CHECK_ARG(grad_type == 0 || grad_type == type,
                "%s: grad_type=%d must be 0 (fp32) or the type of x", who, grad_type);
@@ -1492,9 +1537,9 @@ extern "C" int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type,
   char* part = (char*)ws + p.part;
   uint32_t* counters = (uint32_t*)ws;
   const int kx = p.kx, ky = p.ky;
-  const DownProblem px{x, A, K, kx, p.per, rx, (float*)part, counters, 0, 1};
+  const DownProblem px{x, A, K, kx, p.per, rx, (float*)part, counters, 0, 1, row_mul};
   const DownProblem py{dy, B, N, ky, p.per, ry, (float*)(part + down_part(p, kx)),
-                       counters + LO_SPLIT_BELOW, 1, 1};
+                       counters + LO_SPLIT_BELOW, 1, 1, row_mul};
 #define MM_DOWN(RTV, TV)                                                                       \
   hipLaunchKernelGGL((k_down<TV, RTV>), dim3(down_tiles, std::max(kx, ky), 2 * p.nrc),             \
                      dim3(64 * LO_DW), 0, st, px, py, plan, own, sc, r)
@@ -1516,7 +1561,9 @@ extern "C" int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type,
 #define MM_BACK(RTV, TV, BV)                                                                   \
   hipLaunchKernelGGL((k_back<TV, RTV, BV>), dim3((unsigned)(na + nb + nu)), dim3(LO_NT), 0, st, pa, \
                      pb, pu, plan, r, (int)na, (int)nb)
-  if (dx_base != nullptr) {
+  if (wide) {
+    MM_LORA_RT(MM_BACK, 1, BT_F32)
+  } else if (dx_base != nullptr) {
     if (type == 1) { MM_LORA_RT(MM_BACK, 1, 1) } else { MM_LORA_RT(MM_BACK, 2, 2) }
   } else {
     if (type == 1) { MM_LORA_RT(MM_BACK, 1, 0) } else { MM_LORA_RT(MM_BACK, 2, 0) }
@@ -1524,4 +1571,26 @@ extern "C" int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type,
 #undef MM_BACK
   MM_CHECK_LAUNCH(who);
   return 0;
+}
+
+extern "C" int mm_lora_backward(const uint16_t* dy, const uint16_t* x, int type,
+                                const uint16_t* A, const uint16_t* B, const void* ids, int ids64,
+                                const float* scaling, float scale, const uint16_t* dx_base,
+                                uint16_t* dx, void* dA, void* dB, int grad_type, int T, int K,
+                                int N, int r, int L, void* ws, size_t ws_bytes, void* stream) {
+  return lora_backward("mm_lora_backward", dy, nullptr, x, type, A, B, ids, ids64, scaling, scale,
+                       false, dx_base, dx, dA, dB, grad_type, T, K, N, r, L, ws, ws_bytes, stream);
+}
+
+extern "C" int mm_lora_backward_f32(const uint16_t* dy, const float* row_mul, const uint16_t* x,
+                                    const uint16_t* A, const uint16_t* B, const void* ids,
+                                    int ids64, const float* scaling, float scale,
+                                    const float* dx_base, float* dx, void* dA, void* dB,
+                                    int grad_type, int T, int K, int N, int r, int L, void* ws,
+                                    size_t ws_bytes, void* stream) {
+  const char* who = "mm_lora_backward_f32";
+  MM_CHECK_ARG((((uintptr_t)row_mul | (uintptr_t)dx_base | (uintptr_t)dx) & 3) == 0,
+               "%s: row_mul, dx_base and dx must be 4-byte aligned", who);
+  return lora_backward(who, dy, row_mul, x, 1, A, B, ids, ids64, scaling, scale, true, dx_base, dx,
+                       dA, dB, grad_type, T, K, N, r, L, ws, ws_bytes, stream);
 }

@@ -61,6 +61,8 @@ SIGNATURES: dict[str, tuple] = {
                              ctypes.c_float] + [_c_int] * 5 + [_vp, _c_size, _vp]),
     "mm_lora_backward": (_c_int, [_vp, _vp, _c_int, _vp, _vp, _vp, _c_int, _vp,
                                   ctypes.c_float, _vp, _vp, _vp, _vp] + [_c_int] * 6 + [_vp, _c_size, _vp]),
+    "mm_lora_backward_f32": (_c_int, [_vp] * 6 + [_c_int, _vp, ctypes.c_float] + [_vp] * 4 +
+                             [_c_int] * 6 + [_vp, _c_size, _vp]),
     "mm_moe_sort": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp]),
     "mm_moe_sort_i64": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp]),
     "mm_moe_router_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),

@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .backward import _TYPES, on_device, plain
+from .backward import _TYPES, _carried, _pad_to, on_device, plain
 
 __all__ = ["lora_add", "lora_backward"]
 
@@ -140,9 +140,10 @@ def lora_add(base: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     token, int32 or int64: an id outside [0, adapters) means no adapter, and that token's out
     is its base.  scaling: a number, or one per adapter.
 
-    fp16 and bf16 (fp32 is computed as fp16): factors of another type are converted to x's;
-    base is fp16, as the products return it, or of x's type; out has x's type.  With `out`
-    (contiguous, of x's type; base itself will do) the result is written there.  Any number of
+    fp16 and bf16: factors of another type are converted to x's; base is fp16, as the products
+    return it, or of x's type; out has x's type.  fp32 tokens are computed as fp16, and out is
+    fp16, as the products return it.  With `out` (contiguous, of that type; base itself will do)
+    the result is written there.  Any number of
     tokens and any width or rank, at most 1024 adapters.  Differentiable in base, x, lora_a and
     lora_b (the products and layers that make a base are differentiable in x as well);
     `lora_backward` is the backward pass as a call."""
@@ -163,9 +164,10 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_
     """The gradients of lora_add for dy [*, N]: (dx [*, K], da, db), da and db shaped and typed
     as lora_a and lora_b (zeros for adapters without tokens), dx of x's type.  dx_base, the
     gradient that reached x through the projection itself (marlin_gemm_fp4_backward), is
-    added to dx before it is rounded (in fp32 for an fp32 x).  dy is rounded to the type that x is computed in: fp32
-    gradients are computed as fp16 and want a loss scale, fp32 factors beside fp16 or bf16
-    tokens get fp32 gradients."""
+    added to dx before it is rounded.  fp32 tokens are computed as fp16, and their dx is fp32.
+    dy of a wider type than fp16 tokens (or fp32 ones) is carried in fp16 under one power of two
+    per token, 11 bits of each value; dy beside bf16 tokens is rounded to bf16.  fp32 factors
+    beside fp16 or bf16 tokens get fp32 gradients."""
     if isinstance(x, torch.Tensor):
         got = _lib.fast("lora_backward", x, dy, x, lora_a, lora_b, adapter_ids,
                         *_plain_scaling(scaling), dx_base)
@@ -185,16 +187,23 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_
     ids = _ids(adapter_ids, x.shape[:-1], L)
     with on_device(dev):
         st, factor = _scaling(scaling, L, dev)
-        xf, dyf = (t.reshape(-1, t.shape[-1]).to(dt).contiguous() for t in (x, dy))
+        xf, dyf = x.reshape(-1, K).to(dt).contiguous(), dy.reshape(-1, N)
         T = xf.shape[0]
-        # an fp32 x: its own gradient has come through fp16, what arrives beside it has not
-        late = dx_base if x.dtype == torch.float32 else None
-        dxb = None if dx_base is None or late is not None else \
-            dx_base.reshape(T, K).to(dt).contiguous()
         ac, bc = a.to(dt).contiguous(), b.to(dt).contiguous()
         if T == 0:
             return x.new_empty(x.shape), torch.zeros_like(lora_a), torch.zeros_like(lora_b)
-        dx = torch.empty((T, K), dtype=dt, device=dev)
+        # where dx is fp32, or dy has a wider range than the tokens
+        wide = dt == torch.float16 and (x.dtype == torch.float32 or dy.dtype != dt)
+        mul = None
+        if wide and dy.dtype != dt:
+            dyf = dyf if dyf.dtype in _TYPES else dyf.float()
+            dyf, mul = _carried(plain(_pad_to(dyf, N + -N % 8)))
+            dyf = dyf[:, :N].contiguous()
+        else:
+            dyf = dyf.to(dt).contiguous()
+        dxt = torch.float32 if wide else dt
+        dxb = None if dx_base is None else dx_base.reshape(T, K).to(dxt).contiguous()
+        dx = torch.empty((T, K), dtype=dxt, device=dev)
         # factors that are not of the type they are computed in (fp32 masters) get their
         # gradients from the fp32 sums
         gt = dt if lora_a.dtype == lora_b.dtype == dt else torch.float32
@@ -202,10 +211,13 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, lora_a: torch.Tensor, lora_
         stream = _lib.raw_stream(dev.index)
         ws = _lib.workspace_on(dev.index, stream,
                                _lib.load().mm_lora_workspace_bytes(T, K, N, r, L, 1))
-        _lib.call("mm_lora_backward", _lib.ptr(dyf), _lib.ptr(xf), _TYPES[dt], _lib.ptr(ac),
-                  _lib.ptr(bc), _lib.ptr(ids), int(ids is not None and ids.dtype == torch.int64),
-                  _lib.ptr(st), factor, _lib.ptr(dxb), _lib.ptr(dx), _lib.ptr(da), _lib.ptr(db),
-                  _TYPES[gt], T, K, N, r, L, _lib.ptr(ws), ws.numel(), stream)
-    dx = dx.view(x.shape).to(x.dtype)
-    return (dx if late is None else dx + late, da.view(lora_a.shape).to(lora_a.dtype),
+        tokens = (_lib.ptr(ac), _lib.ptr(bc), _lib.ptr(ids),
+                  int(ids is not None and ids.dtype == torch.int64), _lib.ptr(st), factor,
+                  _lib.ptr(dxb), _lib.ptr(dx), _lib.ptr(da), _lib.ptr(db), _TYPES[gt], T, K, N, r,
+                  L, _lib.ptr(ws), ws.numel(), stream)
+        if wide:
+            _lib.call("mm_lora_backward_f32", _lib.ptr(dyf), _lib.ptr(mul), _lib.ptr(xf), *tokens)
+        else:
+            _lib.call("mm_lora_backward", _lib.ptr(dyf), _lib.ptr(xf), _TYPES[dt], *tokens)
+    return (dx.view(x.shape).to(x.dtype), da.view(lora_a.shape).to(lora_a.dtype),
             db.view(lora_b.shape).to(lora_b.dtype))
