@@ -278,6 +278,11 @@ int64_t plain_rows(const at::Tensor& t, int dev, int64_t n) {
     return -1;
   return t.numel() / n;
 }
+// Whether t is [*, n] with x's leading axes, plain but for its alignment.
+bool same_rows(const at::Tensor& t, const at::Tensor& x, int64_t n) {
+  return t.dim() == x.dim() && t.get_device() == x.get_device() && t.is_contiguous() &&
+         t.size(-1) == n && t.sizes().slice(0, t.dim() - 1) == x.sizes().slice(0, x.dim() - 1);
+}
 at::Tensor rows_like(const at::Tensor& t, int64_t n, at::ScalarType type) {
   std::vector<int64_t> shape(t.sizes().begin(), t.sizes().end());
   shape.back() = n;
@@ -427,7 +432,7 @@ pybind11::object gate_up_backward(const at::Tensor& dH, const at::Tensor& keep,
                        plain_matrix(Wu, Su, c10::nullopt, rows, g, dev)};
   const int64_t N = m[0].N, M = N ? plain_rows(dH, dev, N) : -1;
   if (M <= 0 || m[1].N != N || m[1].K != m[0].K || keep.scalar_type() != at::kHalf ||
-      keep.dim() != dH.dim() || plain_rows(keep, dev, 2 * N) != M)
+      !same_rows(keep, dH, 2 * N) || !aligned(keep))
     return pybind11::none();
   at::Tensor d = at::empty({M, 2 * N}, keep.options());
   at::Tensor mul = at::empty({M}, keep.options().dtype(at::kFloat));
@@ -479,10 +484,6 @@ bool plain_lora(const at::Tensor& x, const at::Tensor& a, const at::Tensor& b,
     l->scaling = (const float*)scaling->data_ptr();
   }
   return l->T > 0;
-}
-bool same_rows(const at::Tensor& t, const at::Tensor& x, int64_t n) {
-  return t.dim() == x.dim() && t.get_device() == x.get_device() && t.is_contiguous() &&
-         t.size(-1) == n && t.sizes().slice(0, t.dim() - 1) == x.sizes().slice(0, x.dim() - 1);
 }
 
 pybind11::object lora_add(const at::Tensor& base, const at::Tensor& x, const at::Tensor& a,
