@@ -31,6 +31,9 @@ const char* mm_last_error(void);
  * counters were cleared within a capture belongs to that capture alone. */
 unsigned long long mm_capture_id(void* stream);
 
+/* Clears a workspace's counters by a kernel on `stream` (also a node of a captured graph). */
+int mm_clear_counters(void* ws, size_t ws_bytes, void* stream);
+
 /* 1 if what was recorded into `event` (a hipEvent_t, recorded outside any capture) is done, 0 if
  * not or not known; does not disturb a capture under way. */
 int mm_event_done(void* event);

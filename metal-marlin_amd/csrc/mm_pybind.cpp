@@ -22,6 +22,12 @@
 
 namespace {
 
+[[noreturn]] void fail(int rc) {
+  const char* msg = mm_last_error();
+  if (rc == 1) throw pybind11::value_error(msg);
+  throw std::runtime_error(msg);
+}
+
 std::mutex g_mu;
 std::map<std::pair<int, int64_t>, at::Tensor> g_ws;   // (device index, stream) -> workspace
 struct Captured {
@@ -29,7 +35,6 @@ struct Captured {
   at::Tensor buf;
 };
 std::map<std::pair<int, int64_t>, Captured> g_captured;
-constexpr int64_t COUNTER_BYTES = 65536;   // at the head of every workspace
 
 // One workspace per (device, stream), shared with the ctypes path (which
 // asks for it through workspace_for below); kept until release_workspaces().
@@ -47,7 +52,7 @@ at::Tensor workspace_dev(int dev, int64_t stream, size_t nbytes, const at::Tenso
     if (c.id == id) size = std::max(size, 2 * (size_t)c.buf.numel());
     c = Captured{0, at::Tensor()};
     at::Tensor buf = at::empty({(int64_t)size}, opt.dtype(at::kByte));
-    buf.narrow(0, 0, COUNTER_BYTES).zero_();
+    if (const int rc = mm_clear_counters(buf.data_ptr(), size, (void*)stream)) fail(rc);
     c = Captured{id, buf};
     return buf;
   }
@@ -76,12 +81,6 @@ void release_workspaces() {
   std::lock_guard<std::mutex> lock(g_mu);
   g_ws.clear();
   g_captured.clear();
-}
-
-[[noreturn]] void fail(int rc) {
-  const char* msg = mm_last_error();
-  if (rc == 1) throw pybind11::value_error(msg);
-  throw std::runtime_error(msg);
 }
 
 void check_groups(const char* name, const at::Tensor& t, int64_t K, int64_t N, int64_t g) {

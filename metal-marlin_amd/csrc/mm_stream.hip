@@ -26,3 +26,19 @@ extern "C" int mm_event_done(void* event) {
   if (e != hipSuccess) (void)hipGetLastError();
   return e == hipSuccess;
 }
+
+// 64 KiB by one wave of every fourth CU, 16 bytes a lane.
+constexpr int CC_BYTES = 65536, CC_NT = 64;
+__global__ void __launch_bounds__(CC_NT) k_clear_counters(u32x4* ws) {
+  ws[blockIdx.x * CC_NT + threadIdx.x] = u32x4{0, 0, 0, 0};
+}
+
+extern "C" int mm_clear_counters(void* ws, size_t ws_bytes, void* stream) {
+  MM_CHECK_ARG(ws != nullptr && ((uintptr_t)ws & 15) == 0 && ws_bytes >= CC_BYTES,
+               "mm_clear_counters: a workspace of %zu bytes must have %d, 16-byte aligned", ws_bytes,
+               CC_BYTES);
+  hipLaunchKernelGGL(k_clear_counters, dim3(CC_BYTES / (16 * CC_NT)), dim3(CC_NT), 0,
+                     (hipStream_t)stream, (u32x4*)ws);
+  MM_CHECK_LAUNCH("mm_clear_counters");
+  return 0;
+}

@@ -23,6 +23,7 @@ SIGNATURES: dict[str, tuple] = {
     "mm_last_error": (ctypes.c_char_p, []),
     "mm_capture_id": (ctypes.c_ulonglong, [_vp]),
     "mm_event_done": (_c_int, [_vp]),
+    "mm_clear_counters": (_c_int, [_vp, _c_size, _vp]),
     "mm_fp4_dequant": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _vp]),
     "mm_u4_dequant": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp]),
     "mm_fp4_quantize": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp]),
@@ -314,7 +315,6 @@ def same_device_index(*tensors: torch.Tensor) -> int:
 # the kernels leave at zero, so it is allocated zeroed once and reused.  Under
 # graph capture: one per capture and stream.
 # ---------------------------------------------------------------------------
-_COUNTER_BYTES = 65536
 _ws: dict[tuple[int, int], torch.Tensor] = {}
 _captured_ws: dict[tuple[int, int], tuple[int, torch.Tensor]] = {}
 
@@ -337,7 +337,7 @@ def workspace_on(index: int, stream: int, nbytes: int) -> torch.Tensor:
         if held != capture or buf.numel() < nbytes:
             size = max(nbytes, 1 << 20, 2 * buf.numel() if held == capture else 0)
             buf = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", index))
-            buf[:_COUNTER_BYTES].zero_()
+            call("mm_clear_counters", ptr(buf), buf.numel(), stream)
             _captured_ws[key] = capture, buf
         return buf
     _captured_ws.pop(key, None)

@@ -14,6 +14,12 @@ def test_the_default_stream_is_in_no_capture():
     assert _lib.load().mm_capture_id(None) == 0
 
 
+def test_counters_are_cleared_in_a_whole_workspace():
+    for ws, size in ((None, 1 << 20), (8, 1 << 20), (16, 65535)):
+        with pytest.raises(ValueError, match="16-byte aligned"):
+            _lib.call("mm_clear_counters", ws, size, None)
+
+
 class Stream:
     def __init__(self, raw):
         self.raw, self.waits = raw, []
