@@ -18,8 +18,10 @@
 //   up       out of a tile: MFMAs over [hi | lo] of 16 ranks at a time.
 //   wgrad    dA_a or dB_a: MFMAs over 32 tokens at a time, tile after tile; the tiles are shared
 //            out over a block's waves, or a wave has them all where an adapter has few tokens.
-// All sums are fp32 and in a fixed order.  All of them stream activations that are read
-// once (x, dy) or read and written once (out): HBM bounds them, the factors stay in L2.
+// All sums are fp32 and in a fixed order.  They stream activations, the factors stay in L2: the
+// forward reads x and the base once and writes out; the backward reads x and dy twice, in k_down
+// and in wgrad (one pass over dy could give dH and dB, were H there before it).  HBM bounds long
+// batches, the latency of the chain sort, loads, hand-off short ones.
 #include <algorithm>
 #include <type_traits>
 

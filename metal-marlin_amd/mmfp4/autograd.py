@@ -195,7 +195,8 @@ def _column_sums(t: torch.Tensor) -> torch.Tensor:
 
 
 class LoraLinear(torch.autograd.Function):
-    """A layer and its adapters in one node.  `bias` is the layer's, for its gradient."""
+    """A layer and its adapters in one node: the layer's gradient of x, of x's type, is the
+    dx_base that the adapters' is added to in fp32.  `bias` is the layer's, for its gradient."""
 
     @staticmethod
     def forward(ctx, x, lora_a, lora_b, adapter_ids, scaling, layer, bias):
