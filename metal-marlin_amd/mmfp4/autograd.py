@@ -2,8 +2,8 @@
 and of low-rank adapters.  The layers (QuantizedLinear, MarlinLinear, MMFP4Linear, LoRALinear),
 the products (marlin_gemm_fp4, marlin_gemm_int4, mmfp4_gemm_rowpacked, mmfp4_fused_qkv and what
 is made of them), fused_gate_up_swiglu and lora_add use these by themselves where an operand
-requires a gradient; calls that need none take the same path as ever.  They are differentiable once: a gradient of a gradient is
-an error, not a silent zero.
+requires a gradient; calls that need none take the same path as ever.  They are differentiable
+once: a gradient of a gradient is an error, not a silent zero.
 
 A backward pass may be captured into a graph.  torch then refuses, by ending the process, one
 thing that a caller cannot see: a leaf whose gradient accumulator belongs to another stream
