@@ -279,6 +279,31 @@ int mm_lora_backward_f32(const uint16_t* dy, const float* row_mul, const uint16_
                          void* dA, void* dB, int grad_type, int T, int K, int N, int rank,
                          int adapters, void* ws, size_t ws_bytes, void* stream);
 
+/* ------------------------------------------ microscaled 4-bit floating point */
+
+/* MXFP4 (OCP microscaling format): rows of E2M1 codes, words [rows, K/8] (value 8j+i of a row in
+ * bits 4i..4i+3 of its word j), one E8M0 scale per 32 values, scales [rows, K/32]: byte c stands
+ * for 2^(c - 127), 255 for a block of NaNs.  Quantization: c - 127 = floor(log2(largest
+ * magnitude)) - 2, at least -127; codes rounded to nearest, ties to even, saturating at 6; a
+ * block that holds a NaN or an infinity gets scale 255.  X [rows, K] contiguous, type 0 fp32,
+ * 1 fp16, 2 bf16; K % 32 == 0; X and words 16-byte aligned.  The reference has no such format
+ * (its FP4 groups have fp16 scales: metal_marlin/quantize_fp4.py:131-284). */
+int mm_mxfp4_quantize(const void* X, int type, long long rows, int K, uint32_t* words,
+                      uint8_t* scales, void* stream);
+/* The values, in `type`, each rounded once; out 16-byte aligned. */
+int mm_mxfp4_dequantize(const uint32_t* words, const uint8_t* scales, long long rows, int K,
+                        void* out, int type, void* stream);
+
+/* Bytes of workspace mm_mxfp4_gemm needs (its first 64 KiB are left as they are: it may be the
+ * other products'). */
+size_t mm_mxfp4_gemm_workspace_bytes(int M, int N, int K);
+
+/* C[M, N] = q(X) . W^T with X [M, K] quantized as mm_mxfp4_quantize does and W [N, K] given so:
+ * words [N, K/8], scales [N, K/32].  fp32 sums, C of out_type rounded once.  Types as above;
+ * K % 32 == 0, any M and N; X, W and C 16-byte aligned. */
+int mm_mxfp4_gemm(const void* X, int type, const uint32_t* W, const uint8_t* scales, void* C,
+                  int out_type, int M, int N, int K, void* ws, size_t ws_bytes, void* stream);
+
 /* -------------------------------------------------------------------- MoE */
 
 /* Stable counting sort of the T*k (token, slot) assignments by expert.

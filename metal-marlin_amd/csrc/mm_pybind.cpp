@@ -528,6 +528,73 @@ pybind11::object lora_backward(const at::Tensor& dy, const at::Tensor& x, const 
   return pybind11::make_tuple(dx, da, db);
 }
 
+// ---------------------------------------------------------------------------
+// Microscaled 4-bit floating point: plain operands on the current device, or None.
+// ---------------------------------------------------------------------------
+// The words [.., N, K/8] and scales [.., N, K/32] of weights, of n axes.
+bool plain_mx(const at::Tensor& W, const at::Tensor& S, int dev, int n) {
+  if (W.dim() != n || S.dim() != n || W.get_device() != dev || S.get_device() != dev ||
+      (W.scalar_type() != at::kInt && W.scalar_type() != at::kUInt32) ||
+      S.scalar_type() != at::kByte || !W.is_contiguous() || !S.is_contiguous() || !aligned(W) ||
+      W.numel() == 0 || W.size(n - 1) != 4 * S.size(n - 1))
+    return false;
+  return W.sizes().slice(0, n - 1) == S.sizes().slice(0, n - 1);
+}
+at::ScalarType scalar_type_of(int64_t code) {
+  return code == 0 ? at::kFloat : (code == 1 ? at::kHalf : at::kBFloat16);
+}
+
+// out_type: 0 fp32, 1 fp16, 2 bf16, -1 x's.
+pybind11::object mx_gemm(const at::Tensor& x, const at::Tensor& W, const at::Tensor& S,
+                         int64_t out_type, int64_t stream) {
+  const int dev = (int)x.get_device();
+  if (!on_current_device(dev) || !plain_mx(W, S, dev, 2)) return pybind11::none();
+  const int64_t N = W.size(0), K = 8 * W.size(1), M = plain_rows(x, dev, K);
+  if (M < 0 || M > INT32_MAX || N > INT32_MAX) return pybind11::none();
+  const int type = type_code(x.scalar_type()), ot = out_type < 0 ? type : (int)out_type;
+  at::Tensor out = rows_like(x, N, scalar_type_of(ot));
+  if (M == 0) return pybind11::cast(out);
+  const size_t need = mm_mxfp4_gemm_workspace_bytes((int)M, (int)N, (int)K);
+  at::Tensor ws;
+  if (need) ws = workspace(x, stream, need);
+  const int rc = mm_mxfp4_gemm(x.data_ptr(), type, (const uint32_t*)W.data_ptr(),
+                               (const uint8_t*)S.data_ptr(), out.data_ptr(), ot, (int)M, (int)N,
+                               (int)K, need ? ws.data_ptr() : nullptr, need ? ws.numel() : 0,
+                               (void*)stream);
+  if (rc) fail(rc);
+  return pybind11::cast(out);
+}
+
+pybind11::object mx_quantize(const at::Tensor& x, int64_t stream) {
+  const int dev = (int)x.get_device();
+  if (!on_current_device(dev) || x.dim() < 1 || x.size(-1) == 0 || x.size(-1) % 32 != 0)
+    return pybind11::none();
+  const int64_t K = x.size(-1), rows = plain_rows(x, dev, K);
+  if (rows < 0 || K > INT32_MAX) return pybind11::none();
+  at::Tensor words = rows_like(x, K / 8, at::kInt), scales = rows_like(x, K / 32, at::kByte);
+  if (rows == 0) return pybind11::make_tuple(words, scales);
+  const int rc = mm_mxfp4_quantize(x.data_ptr(), type_code(x.scalar_type()), rows, (int)K,
+                                   (uint32_t*)words.data_ptr(), (uint8_t*)scales.data_ptr(),
+                                   (void*)stream);
+  if (rc) fail(rc);
+  return pybind11::make_tuple(words, scales);
+}
+
+pybind11::object mx_dequantize(const at::Tensor& W, const at::Tensor& S, int64_t type,
+                               int64_t stream) {
+  const int dev = (int)W.get_device();
+  if (!on_current_device(dev) || W.dim() < 1 || !plain_mx(W, S, dev, (int)W.dim()))
+    return pybind11::none();
+  const int64_t K = 8 * W.size(-1);
+  if (K > INT32_MAX) return pybind11::none();
+  at::Tensor out = rows_like(W, K, scalar_type_of(type));
+  const int rc = mm_mxfp4_dequantize((const uint32_t*)W.data_ptr(), (const uint8_t*)S.data_ptr(),
+                                     W.numel() / W.size(-1), (int)K, out.data_ptr(), (int)type,
+                                     (void*)stream);
+  if (rc) fail(rc);
+  return pybind11::cast(out);
+}
+
 // Stream id of a leaf's gradient accumulator, or -1 where it has none (yet).
 int64_t accumulator_stream(const at::Tensor& leaf) {
   const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
@@ -553,6 +620,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "mm_swiglu_grad and mm_gemm_backward on plain operands, else None");
   m.def("lora_add", &lora_add, "mm_lora_add on plain operands, else None");
   m.def("lora_backward", &lora_backward, "mm_lora_backward on plain operands, else None");
+  m.def("mx_gemm", &mx_gemm, "mm_mxfp4_gemm on plain operands, else None");
+  m.def("mx_quantize", &mx_quantize, "mm_mxfp4_quantize on a plain operand, else None");
+  m.def("mx_dequantize", &mx_dequantize, "mm_mxfp4_dequantize on plain operands, else None");
   m.def("accumulator_stream", &accumulator_stream,
         "stream id of a leaf's gradient accumulator, -1 without one");
   m.def("workspace", &workspace_for,

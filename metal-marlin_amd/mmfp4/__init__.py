@@ -15,6 +15,7 @@ from .fp4_metal import FP4Metal, dequantize_fp4_metal, quantize_fp4_metal
 from .backward import (fused_gate_up_swiglu, fused_gate_up_swiglu_backward,
                        marlin_gemm_fp4_backward, marlin_gemm_int4_backward,
                        mmfp4_fused_qkv_backward, mmfp4_gemm_rowpacked_backward)
+from .mxfp4 import mxfp4_dequantize, mxfp4_gemm, mxfp4_quantize
 from .adapters import lora_add, lora_backward
 from .autograd import gate_up_swiglu
 from .layers import MMFP4Linear

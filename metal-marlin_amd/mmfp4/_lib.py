@@ -64,6 +64,10 @@ SIGNATURES: dict[str, tuple] = {
                                   ctypes.c_float, _vp, _vp, _vp, _vp] + [_c_int] * 6 + [_vp, _c_size, _vp]),
     "mm_lora_backward_f32": (_c_int, [_vp] * 6 + [_c_int, _vp, ctypes.c_float] + [_vp] * 4 +
                              [_c_int] * 6 + [_vp, _c_size, _vp]),
+    "mm_mxfp4_quantize": (_c_int, [_vp, _c_int, ctypes.c_longlong, _c_int, _vp, _vp, _vp]),
+    "mm_mxfp4_dequantize": (_c_int, [_vp, _vp, ctypes.c_longlong, _c_int, _vp, _c_int, _vp]),
+    "mm_mxfp4_gemm_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
+    "mm_mxfp4_gemm": (_c_int, [_vp, _c_int, _vp, _vp, _vp] + [_c_int] * 4 + [_vp, _c_size, _vp]),
     "mm_moe_sort": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp]),
     "mm_moe_sort_i64": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp]),
     "mm_moe_router_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
