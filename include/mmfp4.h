@@ -358,6 +358,23 @@ int mm_moe_router_p16(const uint16_t* X, const uint16_t* W, const float* bias, i
 int mm_softmax_topk_p16(const void* logits, int logits_f32, int T, int E, int k, int renorm,
                         int64_t* ids, uint16_t* probs, void* stream);
 
+/* Routing from given logits [T, E] (type 0 fp32, 1 fp16, 2 bf16) with sigmoid (softmax 0) or
+ * softmax scores s, a balance bias b fp32 [E] or NULL, and groups of E / groups experts side by
+ * side: c = s + b; the `keep` groups with the largest sums of their two largest c stay; ids
+ * int64 [T, k] are the k largest c among their experts, in that order, ties to the lower index
+ * (decided in 64 bits); weights fp32 [T, k] = scale * s[ids], with renorm / (sum s[ids] + 1e-20).
+ * NaNs rank last; a softmax row without a value above -inf has s = 0.  E <= 1024, k <= 64,
+ * groups <= 64.  Beside mm_softmax_topk (metal_marlin/moe_dispatch.py:99-151), which knows
+ * neither bias nor groups. */
+int mm_moe_route(const void* logits, int type, const float* bias, int T, int E, int k, int softmax,
+                 int groups, int keep, int renorm, float scale, int64_t* ids, float* weights,
+                 void* stream);
+/* Its gradient: dweights fp32 [T, k] to dlogits [T, E] of the logits' type, for the same logits
+ * and ids (those outside [0, E) get nothing).  The bias gets none: it moves no weight. */
+int mm_moe_route_backward(const float* dweights, const void* logits, int type, const int64_t* ids,
+                          int T, int E, int k, int softmax, int renorm, float scale, void* dlogits,
+                          void* stream);
+
 /* Grouped expert GEMM over expert-sorted rows.  For expert e, rows
  * r in [offsets[e], offsets[e+1]) compute Y[r] = X[row(r)] . dequant(B[e], S[e]),
  * where row(r) = sorted_idx[r] / k when gather != 0 (rows of X are tokens)

@@ -595,6 +595,51 @@ pybind11::object mx_dequantize(const at::Tensor& W, const at::Tensor& S, int64_t
   return pybind11::cast(out);
 }
 
+// Routing: logits [*, E] and a bias [E] in plain form, or None.
+pybind11::object moe_route(const at::Tensor& logits, int64_t k, bool softmax,
+                           const c10::optional<at::Tensor>& bias, int64_t groups, int64_t keep,
+                           bool renorm, double scale, int64_t stream) {
+  const int dev = (int)logits.get_device();
+  const int type = type_code(logits.scalar_type());
+  if (!on_current_device(dev) || logits.dim() < 1 || type < 0 || !logits.is_contiguous() ||
+      logits.size(-1) == 0)
+    return pybind11::none();
+  const int64_t E = logits.size(-1), T = logits.numel() / E;
+  if (T > INT32_MAX || E > INT32_MAX || k < 0 || k > INT32_MAX || groups < 0 ||
+      groups > INT32_MAX || keep < 0 || keep > INT32_MAX ||
+      (bias && (bias->dim() != 1 || bias->numel() != E || bias->get_device() != dev ||
+                bias->scalar_type() != at::kFloat || !bias->is_contiguous())))
+    return pybind11::none();
+  at::Tensor w = rows_like(logits, k, at::kFloat), ids = rows_like(logits, k, at::kLong);
+  const int rc = mm_moe_route(logits.data_ptr(), type, bias ? (const float*)bias->data_ptr() : nullptr,
+                              (int)T, (int)E, (int)k, softmax, (int)groups, (int)keep, renorm,
+                              (float)scale, (int64_t*)ids.data_ptr(), (float*)w.data_ptr(),
+                              (void*)stream);
+  if (rc) fail(rc);
+  return pybind11::make_tuple(w, ids);
+}
+
+pybind11::object moe_route_backward(const at::Tensor& dw, const at::Tensor& logits,
+                                    const at::Tensor& ids, bool softmax, bool renorm, double scale,
+                                    int64_t stream) {
+  const int dev = (int)logits.get_device();
+  const int type = type_code(logits.scalar_type());
+  if (!on_current_device(dev) || logits.dim() < 1 || type < 0 || !logits.is_contiguous() ||
+      logits.size(-1) == 0 || dw.dim() != logits.dim() || dw.get_device() != dev ||
+      ids.get_device() != dev || dw.scalar_type() != at::kFloat || ids.scalar_type() != at::kLong ||
+      !dw.is_contiguous() || !ids.is_contiguous() || dw.sizes() != ids.sizes() ||
+      dw.sizes().slice(0, dw.dim() - 1) != logits.sizes().slice(0, dw.dim() - 1))
+    return pybind11::none();
+  const int64_t E = logits.size(-1), T = logits.numel() / E, k = dw.size(-1);
+  if (T > INT32_MAX || E > INT32_MAX || k > INT32_MAX) return pybind11::none();
+  at::Tensor dl = at::empty_like(logits);
+  const int rc = mm_moe_route_backward((const float*)dw.data_ptr(), logits.data_ptr(), type,
+                                       (const int64_t*)ids.data_ptr(), (int)T, (int)E, (int)k,
+                                       softmax, renorm, (float)scale, dl.data_ptr(), (void*)stream);
+  if (rc) fail(rc);
+  return pybind11::cast(dl);
+}
+
 // Stream id of a leaf's gradient accumulator, or -1 where it has none (yet).
 int64_t accumulator_stream(const at::Tensor& leaf) {
   const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
@@ -623,6 +668,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mx_gemm", &mx_gemm, "mm_mxfp4_gemm on plain operands, else None");
   m.def("mx_quantize", &mx_quantize, "mm_mxfp4_quantize on a plain operand, else None");
   m.def("mx_dequantize", &mx_dequantize, "mm_mxfp4_dequantize on plain operands, else None");
+  m.def("moe_route", &moe_route, "mm_moe_route on plain operands, else None");
+  m.def("moe_route_backward", &moe_route_backward,
+        "mm_moe_route_backward on plain operands, else None");
   m.def("accumulator_stream", &accumulator_stream,
         "stream id of a leaf's gradient accumulator, -1 without one");
   m.def("workspace", &workspace_for,

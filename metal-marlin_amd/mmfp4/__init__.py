@@ -16,6 +16,7 @@ from .backward import (fused_gate_up_swiglu, fused_gate_up_swiglu_backward,
                        marlin_gemm_fp4_backward, marlin_gemm_int4_backward,
                        mmfp4_fused_qkv_backward, mmfp4_gemm_rowpacked_backward)
 from .mxfp4 import mxfp4_dequantize, mxfp4_gemm, mxfp4_quantize
+from .routing import moe_route, moe_route_backward
 from .adapters import lora_add, lora_backward
 from .autograd import gate_up_swiglu
 from .layers import MMFP4Linear

@@ -74,6 +74,9 @@ SIGNATURES: dict[str, tuple] = {
     "mm_moe_router": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp,
                                _vp, _c_size, _vp]),
     "mm_softmax_topk": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp]),
+    "mm_moe_route": (_c_int, [_vp, _c_int, _vp] + [_c_int] * 7 + [ctypes.c_float, _vp, _vp, _vp]),
+    "mm_moe_route_backward": (_c_int, [_vp, _vp, _c_int, _vp] + [_c_int] * 5 +
+                              [ctypes.c_float, _vp, _vp]),
     "mm_moe_grouped_gemm": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp, _c_int,
                                      _c_int, _c_int, _c_int, _c_int, _vp, _vp]),
     "mm_moe_combine": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp]),

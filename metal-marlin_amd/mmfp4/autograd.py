@@ -20,7 +20,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib, adapters, backward, kernels
 
 __all__ = ["linear", "marlin_gemm", "rowpacked_gemm", "gate_up_swiglu", "FusedQKV", "GateUp",
-           "LoraAdd", "LoraLinear"]
+           "LoraAdd", "LoraLinear", "Route"]
 
 
 def refuse_foreign_leaf(*tensors: torch.Tensor | None) -> None:
@@ -221,3 +221,25 @@ class LoraLinear(torch.autograd.Function):
         if ctx.needs_input_grad[6]:
             dbias = _column_sums(dy.view(-1, dy.shape[-1])).to(ctx.bias_dtype)
         return (dx if ctx.needs_input_grad[0] else None), da, db, None, None, None, dbias
+
+
+class Route(torch.autograd.Function):
+    """moe_route, its weights differentiable in logits."""
+
+    @staticmethod
+    def forward(ctx, logits, top_k, softmax, bias, num_groups, topk_groups, renormalize, scale):
+        from .routing import _route
+        refuse_foreign_leaf(logits)
+        w, ids = _route(logits, top_k, softmax, bias, num_groups, topk_groups, renormalize, scale)
+        ctx.save_for_backward(logits, ids)
+        ctx.how = {"scoring": "softmax" if softmax else "sigmoid", "renormalize": renormalize,
+                   "scale": scale}
+        ctx.mark_non_differentiable(ids)
+        return w, ids
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dw, _):
+        from .routing import moe_route_backward
+        logits, ids = ctx.saved_tensors
+        return (moe_route_backward(dw.contiguous(), logits, ids, **ctx.how), *[None] * 7)

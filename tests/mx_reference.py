@@ -64,3 +64,43 @@ def check(out: torch.Tensor, ref: torch.Tensor, bound: torch.Tensor, what: str =
     off = torch.where(nan, 0.0, (out - ref).abs() - bound)
     worst = float(off.max()) if off.numel() else 0.0
     assert worst <= 0, f"{what}: beyond its bound by {worst:.3g} at {int(off.argmax())}"
+
+
+def route(logits, k, softmax=False, bias=None, groups=1, keep=1, renorm=True, scale=1.0):
+    """(weights fp64 [T, k], ids int64 [T, k]) token by token, from the definition."""
+    T, E = logits.shape
+    n = E // groups
+    l = logits.double().cpu()
+    if softmax:
+        s = torch.softmax(l, 1)
+        s[(l == -math.inf).all(1)] = 0.0
+    else:
+        s = torch.sigmoid(l)
+    c = s + (0 if bias is None else bias.double().cpu())
+    c = torch.where(torch.isnan(c), -math.inf, c)
+    ids = torch.empty(T, k, dtype=torch.int64)
+    for t in range(T):
+        row = c[t].tolist()
+        tops = []
+        for g in range(groups):
+            best = sorted(row[g * n:(g + 1) * n], reverse=True)[:2]
+            tops.append(sum(best))
+        kept = sorted(range(groups), key=lambda g: (-tops[g], g))[:keep]
+        free = [e for g in kept for e in range(g * n, (g + 1) * n)]
+        ids[t] = torch.tensor(sorted(free, key=lambda e: (-row[e], e))[:k])
+    w = s.gather(1, ids)
+    if renorm:
+        w = w / (w.sum(1, keepdim=True) + 1e-20)
+    return (w * scale).to(logits.device), ids.to(logits.device)
+
+
+def route_grad(dw, logits, ids, softmax=False, renorm=True, scale=1.0):
+    """dlogits fp64 by torch's own differentiation of the weights."""
+    leaf = logits.double().detach().requires_grad_(True)
+    s = torch.softmax(leaf, 1) if softmax else torch.sigmoid(leaf)
+    live = (ids >= 0) & (ids < logits.shape[1])
+    w = torch.where(live, s.gather(1, ids.clamp(0, logits.shape[1] - 1)), 0.0)
+    if renorm:
+        w = w / (w.sum(1, keepdim=True) + 1e-20)
+    (w * scale * dw.double()).sum().backward()
+    return leaf.grad
