@@ -300,9 +300,20 @@ size_t mm_mxfp4_gemm_workspace_bytes(int M, int N, int K);
 
 /* C[M, N] = q(X) . W^T with X [M, K] quantized as mm_mxfp4_quantize does and W [N, K] given so:
  * words [N, K/8], scales [N, K/32].  fp32 sums, C of out_type rounded once.  Types as above;
- * K % 32 == 0, any M and N; X, W and C 16-byte aligned. */
+ * K % 32 == 0, any M and N; X, W, scales and C 16-byte aligned. */
 int mm_mxfp4_gemm(const void* X, int type, const uint32_t* W, const uint8_t* scales, void* C,
                   int out_type, int M, int N, int K, void* ws, size_t ws_bytes, void* stream);
+
+/* Its input gradient, straight through the rounding of X:
+ *   dX[M, K] = dY[M, N] . W[N, K]
+ * dY of `type` with row stride ldy, a multiple of 16 bytes, and zeros between column N and the
+ * next such multiple; dX of out_type.  Weights and every dY enter exactly, products accumulate in
+ * fp32, rounded once.  K % 32 == 0; dY, W and dX 16-byte aligned.  Workspace as above,
+ * mm_mxfp4_gemm_backward_workspace_bytes. */
+size_t mm_mxfp4_gemm_backward_workspace_bytes(int M, int N, int K, int type);
+int mm_mxfp4_gemm_backward(const void* dY, int type, int ldy, const uint32_t* W,
+                           const uint8_t* scales, void* dX, int out_type, int M, int N, int K, void* ws, size_t ws_bytes,
+                           void* stream);
 
 /* -------------------------------------------------------------------- MoE */
 
@@ -449,6 +460,21 @@ int mm_moe_mlp_shared_fp4_p16(const uint16_t* X, const void* expert_ids, int ids
                               const uint32_t* Bsdn, const uint16_t* Ssdn, float shared_weight,
                               const uint16_t* base, int group_size, uint16_t* act_buf,
                               uint16_t* y_buf, int32_t* sort_buf, uint16_t* out, void* stream);
+
+/* Bytes of scratch that mm_moe_mlp_mxfp4 needs (no initial contents, nothing kept in it). */
+size_t mm_moe_mlp_mxfp4_scratch_bytes(int T, int k, int E, int H, int I, int type);
+
+/* mm_moe_mlp_fp4 on MXFP4 weights, both products with both sides in MXFP4:
+ *   (g | u) = q(X[t]) . Wgu[e]^T;  a = q(silu(g) * u), quantized from its fp32 values;
+ *   out[t] = sum_j probs[t, j] * (a . Wdn[e]^T)     (fp32, slot order, rounded once)
+ * Wgu words [E, 2I, H/8] and scales [E, 2I, H/32], the gate's I rows first; Wdn [E, H, I/8] and
+ * [E, H, I/32].  X [T, H] and out of type 0 fp32, 1 fp16, 2 bf16; what each expert gives a token
+ * is rounded to that type before the sum.  expert_ids [T, k] int32 or (ids_i64) int64; ids outside
+ * [0, E) contribute nothing.  probs fp32 [T, k].  H, I % 32 == 0, E <= 1024. */
+int mm_moe_mlp_mxfp4(const void* X, int type, const void* expert_ids, int ids_i64,
+                     const float* probs, int T, int k, int E, int H, int I, const uint32_t* Wgu,
+                     const uint8_t* Sgu, const uint32_t* Wdn, const uint8_t* Sdn, void* scratch,
+                     size_t scratch_bytes, void* out, void* stream);
 
 /* Shared + routed aggregation of one FP4 projection (no MLP):
  *   out[t] = X[t] . W_sh + sum_j probs[t, j] * (X[t] . W_routed[e(t, j)])

@@ -162,12 +162,13 @@ inline const char* type_name(int t) {
   return t == F32 ? "fp32" : (t == F16 ? "fp16" : (t == BF16 ? "bf16" : "?"));
 }
 
-// Quantized rows in a workspace: words [rows, kp/8] and scales [rows, kp/32], kp = K padded to
-// whole units with zeros.
-inline size_t padded(int K) { return ((size_t)K + UNIT - 1) / UNIT * UNIT; }
+// Quantized rows in a workspace: words [rows, kp/8] and scales [rows, kp/32], kp = K padded to a
+// multiple of 512 with zeros, so that a row's scales are whole 16-byte pieces; behind the last row
+// there is room for the scales of 63 more, which kernels may read and never use.
+inline size_t padded(int K) { return ((size_t)K + 511) / 512 * 512; }
 inline size_t codes_bytes(size_t rows, int K) { return rows * padded(K) / 2; }
 inline size_t packed_bytes(size_t rows, int K) {
-  return codes_bytes(rows, K) + (rows * padded(K) / BLOCK + 255) / 256 * 256;
+  return codes_bytes(rows, K) + (rows + 63) * padded(K) / BLOCK;
 }
 // x [rows, K] of `type` to words and scales whose rows are kp values long (kp >= K, zeros behind
 // K).

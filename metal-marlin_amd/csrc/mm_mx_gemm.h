@@ -19,137 +19,301 @@ MM_DEV void repeat(F&& f) {
   static_for(f, std::make_integer_sequence<int, N>{});
 }
 
-// ---------------------------------------------------------------------------
-// Few rows: bound by the weights' bytes.  NW waves share out the units of 256 k; a lane's 16-byte
-// loads are the matrix operand as it lies in memory (a 16-row tile's 1 KiB per instruction), so
-// weights go from HBM to the matrix cores without LDS.  The 16 rows of x per instruction are
-// quantized in registers by every wave for its own k (a lane holds whole blocks: no exchange), or
-// come as codes (T == CODES, rows padded to whole units).
-// ---------------------------------------------------------------------------
-template <int T, int MT>
-struct XUnit {
-  Vals<T> v[MT][2][4];
-};
-template <int MT>
-struct XUnit<CODES, MT> {
-  u32x4 v[MT][2];
-  uint8_t s[MT][2];
-};
-template <int NT>
-struct WUnit {
-  u32x4 v[NT][2];
-  uint8_t s[NT][2];
-};
-
-MM_DEV u32x4 load_once(const uint8_t* p) {   // weights: each is read once per launch
-  return __builtin_nontemporal_load((const u32x4*)p);
+typedef __attribute__((address_space(3))) void* lds_ptr;
+// 16 bytes per lane straight to LDS, the lanes' pieces side by side from lds_uniform on.
+MM_DEV void copy16(const void* src, void* lds_uniform) {
+  __builtin_amdgcn_global_load_lds(src, (lds_ptr)lds_uniform, 16, 0, 0);
+}
+// Waits until at most N vector memory operations are in flight.
+template <int N>
+MM_DEV void wait_loads() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+  __builtin_amdgcn_sched_barrier(0);
 }
 
-// x: this lane's row of each 16-row tile; xs: its scales (CODES).  w, s: its weight rows.
-// acc[mt][nt][i] is D[16 nt + 4 (lane / 16) + i, 16 mt + lane % 16].
-template <int T, int MT, int NT, int NW>
-MM_DEV void skinny(const char* const (&x)[MT], const uint8_t* const (&xs)[MT],
-                   const uint8_t* const (&w)[NT], const uint8_t* const (&s)[NT], int K,
-                   f32x4 (&acc)[MT][NT]) {
-  const int lane = threadIdx.x & 63, q = lane >> 4;
+// Stores to LDS beside copies to other parts of it: the compiler has a store of its own wait for
+// all copies in flight, which may be to the same place for all that it knows.  stores_done()
+// before what relies on them.
+MM_DEV uint32_t lds_at(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+MM_DEV void lds_store4(void* p, uint32_t v) {
+  asm volatile("ds_write_b32 %0, %1" ::"v"(lds_at(p)), "v"(v) : "memory");
+}
+MM_DEV void lds_store1(void* p, uint32_t v) {
+  asm volatile("ds_write_b8 %0, %1" ::"v"(lds_at(p)), "v"(v) : "memory");
+}
+MM_DEV void stores_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// A barrier that waits for no copy in flight (__syncthreads waits for them all).
+MM_DEV void block_barrier() {
+  stores_done();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: bound by the weights' bytes.  The NW waves of a block share out the units of 256 k.
+// A wave copies its units' rows global -> LDS, 128 bytes of 8 rows per instruction (a matrix
+// operand taken straight from memory would ask for 64 bytes of 16 rows, and a CU then gets 13
+// GB/s where it gets 29 from whole lines), DEPTH units ahead, in a ring of its own: it waits for
+// its own loads only, never for another wave.  Piece p of row r lies at p ^ (r / 2 % 8): the 16
+// rows that an operand read takes at once spread over all banks.
+// The rows are 16 NT of W, then (XT > 0) 16 XT of x's codes.
+// ---------------------------------------------------------------------------
+template <int NT, int XT, int NW, int DEPTH>
+struct Ring {
+  static constexpr int ROWS = 16 * (NT + XT), LOADS = ROWS / 8, STAGE = ROWS * 128;
+  static constexpr int BYTES = NW * DEPTH * STAGE;
+  static_assert(LOADS * (DEPTH - 1) < 64, "loads in flight");
+  static_assert(STAGE >= NT * 1024, "the waves' sums take its place");
+  uint32_t off[LOADS];
+  const uint8_t *W, *X;
+  char* mine;
+  int k;               // bytes per row of W
+
+  // wrow(r), xrow(r): the row, from W and X on, of row r of the tile.
+  template <class WRow, class XRow>
+  MM_DEV Ring(char* lds, const uint8_t* w, int K, WRow&& wrow, const uint8_t* x, int kp, XRow&& xrow)
+      : W(w), X(x), k(K / 2) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    mine = lds + wave * DEPTH * STAGE;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int r = i * 8 + lane / 8;
+      off[i] = i < 2 * NT ? wrow(r) * (uint32_t)k : xrow(r - 16 * NT) * (uint32_t)(kp / 2);
+    }
+  }
+  MM_DEV void issue(int u, int d) const {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      int at = 16 * ((lane & 7) ^ (4 * (i & 1) + (lane >> 4)));
+      // behind K the row's last piece, which meets zeros of x
+      if (i < 2 * NT) at = min(at, k - 16 - u * 128);
+      copy16((i < 2 * NT ? W : X) + (size_t)u * 128 + (off[i] + (uint32_t)at),
+             mine + d * STAGE + i * 1024);
+    }
+  }
+  // Blocks 4 j + lane / 16 of row 16 t + lane % 16, t counting the weights' tiles, then x's.
+  MM_DEV u32x4 operand(int d, int t, int j) const {
+    const int lane = threadIdx.x & 63, r = lane & 15, p = (4 * j + (lane >> 4)) ^ (r >> 1);
+    return *(const u32x4*)(mine + d * STAGE + (16 * t + r) * 128 + p * 16);
+  }
+};
+
+// Bytes to LDS by the whole block, 16 per lane and copy: the last piece again where a wave has
+// lanes to spare, so dst has room for whole KiB.  bytes a multiple of 16, both ends aligned so.
+template <int NTHR>
+MM_DEV void copy_to_lds(const uint8_t* src, char* dst, int bytes) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int b = wave * 1024; b < bytes; b += NTHR * 16)
+    copy16(src + min(b + lane * 16, bytes - 16), dst + b);
+}
+constexpr int whole_kib(int bytes) { return (bytes + 1023) / 1024 * 1024; }
+
+// Scales of rows that lie side by side, of whose `bytes` the first `valid` are there: copied, or,
+// for the last rows of W, stored byte by byte (before any copy is in flight).
+template <int NTHR>
+MM_DEV void scales_to_lds(const uint8_t* src, char* dst, int bytes, int valid) {
+  if (valid == bytes) {
+    copy_to_lds<NTHR>(src, dst, bytes);
+  } else {
+    for (int i = threadIdx.x; i < bytes; i += NTHR) dst[i] = i < valid ? (char)src[i] : (char)0;
+  }
+}
+
+// Rows of x in LDS, `lds_stride` bytes of codes each (an odd number of 16-byte pieces:
+// consecutive rows in different banks), then their scales.
+constexpr int lds_stride(int kp) { return kp / 2 + 16; }
+__host__ __device__ constexpr int lds_x_bytes(int rows, int kp) {
+  return rows * (lds_stride(kp) + kp / BLOCK);
+}
+
+// Exchange within groups of four lanes.
+MM_DEV uint32_t quad_max(uint32_t m) {
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, true));
+  return max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, true));
+}
+
+// The block quantizes `rows` <= 16 rows of K values into LDS, zeros from K to kp, U pieces of 8
+// values per thread and batch, four lanes to a block of 32.  The values come through LDS as well
+// (raw: raw_bytes of it): a value in a register would be waited for together with every copy in
+// flight.  A lane reads what it copied itself.
+// base(m): where row m begins.  first() issues the first batch; finish() expects it there and
+// leaves no copy in flight if there are more.
+template <int T, int NTHR, int U, class Base>
+struct QuantizeRows {
+  static constexpr int PARTS = T == F32 ? 2 : 1;
+  static constexpr int RAW = U * PARTS * NTHR * 16;
+  char *raw, *out;
+  int rows, K, kp;
+  Base base;
+  // row and column (in pieces) of piece p; exact for the few rows there are
+  MM_DEV void place(int p, int& m, int& c) const {
+    const int w = kp / 8;
+    m = (int)(((float)p + 0.5f) * (1.0f / (float)w));
+    c = p - m * w;
+  }
+  MM_DEV void issue(int p0) const {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      int m, c;
+      place(p0 + i * NTHR + threadIdx.x, m, c);
+      const char* src = base(min(m, rows - 1)) + (size_t)min(c, K / 8 - 1) * 8 * kBytes<T>;
+#pragma unroll
+      for (int h = 0; h < PARTS; ++h)
+        copy16(src + 16 * h, raw + ((i * PARTS + h) * (NTHR / 64) + wave) * 1024);
+    }
+  }
+  MM_DEV void store(int p0) const {
+    const int stride = lds_stride(kp);
+    char* const scales = out + rows * stride;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      int m, c;
+      place(p0 + i * NTHR + threadIdx.x, m, c);
+      Vals<T> v;
+      if constexpr (T == F32) {
+        v.v[0] = *(const f32x4*)(raw + (2 * i * NTHR + threadIdx.x) * 16);
+        v.v[1] = *(const f32x4*)(raw + ((2 * i + 1) * NTHR + threadIdx.x) * 16);
+      } else {
+        v.v = *(const u32x4*)(raw + (i * NTHR + threadIdx.x) * 16);
+      }
+      if (c >= K / 8) v = zero8<T>();
+      const uint32_t code = scale_code(amax_bits<T>(quad_max(amax8<T>(v))));
+      const uint32_t w = pack8<T>(v, scale_of(code));
+      if (m < rows) {
+        lds_store4(out + m * stride + c * 4, w);
+        if ((c & 3) == 0) lds_store1(scales + m * (kp / BLOCK) + c / 4, code);
+      }
+    }
+  }
+  MM_DEV void first() const { issue(0); }
+  MM_DEV void finish() const {
+    store(0);
+    for (int p = U * NTHR; p < rows * (kp / 8); p += U * NTHR) {
+      stores_done();                                 // and reads: raw is free again
+      issue(p);
+      wait_loads<0>();
+      store(p);
+    }
+    stores_done();
+  }
+};
+
+// A block's weights' scales in LDS, and x there or in the ring.
+struct LdsX {
+  const char* codes;       // of this lane's row
+  const uint8_t* scales;
+  template <class R>
+  MM_DEV void get(const R&, int, int, int, int b, u32x4& v, uint32_t& c) const {
+    v = *(const u32x4*)(codes + b * 16);
+    c = scales[b];
+  }
+};
+template <int NT>
+struct RingX {
+  const uint8_t* scales;   // of this lane's row of the first tile, in LDS
+  int tile;                // bytes from tile to tile
+  template <class R>
+  MM_DEV void get(const R& ring, int d, int mt, int j, int b, u32x4& v, uint32_t& c) const {
+    v = ring.operand(d, NT + mt, j);
+    c = scales[mt * tile + b];
+  }
+};
+
+// This wave's units; those of the first DEPTH are issued by skinny_begin.
+struct Span {
+  int beg, end;
+};
+template <int NW>
+MM_DEV Span skinny_span(int K) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kb = K / BLOCK, units = K / UNIT;
+  const int units = (K + UNIT - 1) / UNIT, upw = (units + NW - 1) / NW;
+  return {min(units, wave * upw), min(units, wave * upw + upw)};
+}
+// Always DEPTH of them, the last one again where the wave has fewer: what is loaded before can
+// then be waited for by counting.
+template <int DEPTH, class R>
+MM_DEV void skinny_begin(const R& ring, Span sp) {
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) ring.issue(max(0, min(sp.beg + d, sp.end - 1)), d);
+  __builtin_amdgcn_sched_barrier(0);
+}
+// ws: the scales in LDS of this lane's row of the first weight tile, woff(nt) bytes before tile
+// nt's.  acc[mt][nt][i] is D[16 nt + 4 (lane / 16) + i, 16 mt + lane % 16].
+template <int MT, int NT, int DEPTH, class R, class X, class WOff>
+MM_DEV void skinny(const R& ring, const X& x, const uint8_t* ws, WOff&& woff, int kb, Span sp,
+                   f32x4 (&acc)[MT][NT]) {
+  const int q = (threadIdx.x & 63) >> 4;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x4{0, 0, 0, 0};
-  // b: this lane's block of the instruction
-  auto load_w = [&](int b, int j, bool live, WUnit<NT>& o) {
+  for (int u0 = sp.beg; u0 < sp.end; u0 += DEPTH) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      o.v[nt][j] = live ? load_once(w[nt] + (size_t)b * 16) : u32x4{0, 0, 0, 0};
-      o.s[nt][j] = live ? s[nt][b] : (uint8_t)0;
-    }
-  };
-  auto load_x = [&](int b, int j, bool live, XUnit<T, MT>& o) {
+    for (int d = 0; d < DEPTH; ++d) {
+      const int u = u0 + d;
+      if (u >= sp.end) break;
+      if (u + DEPTH <= sp.end) wait_loads<R::LOADS * (DEPTH - 1)>();
+      else wait_loads<0>();
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      if constexpr (T == CODES) {
-        o.v[mt][j] = *(const u32x4*)(x[mt] + (size_t)b * 16);    // padded: always there
-        o.s[mt][j] = xs[mt][b];
-      } else {
+      for (int j = 0; j < 2; ++j) {
+        const int b = 8 * u + 4 * j + q, bw = min(b, kb - 1);
+        u32x4 wv[NT];
+        uint32_t wc[NT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          o.v[mt][j][i] =
-              live ? load8<T>(x[mt] + ((size_t)b * BLOCK + 8 * i) * kBytes<T>) : zero8<T>();
-      }
-    }
-  };
-  auto compute = [&](const WUnit<NT>& wu, const XUnit<T, MT>& xu) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        u32x4 xv;
-        uint32_t xc;
-        if constexpr (T == CODES) {
-          xv = xu.v[mt][j];
-          xc = xu.s[mt][j];
-        } else {
-          xv = pack_block<T>(xu.v[mt][j], xc);
+        for (int nt = 0; nt < NT; ++nt) {
+          wv[nt] = ring.operand(d, nt, j);
+          wc[nt] = ws[woff(nt) + bw];
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          acc[mt][nt] = mfma16<0, 0>(wu.v[nt][j], wu.s[nt][j], xv, xc, acc[mt][nt]);
+        for (int mt = 0; mt < MT; ++mt) {
+          u32x4 xv;
+          uint32_t xc;
+          x.get(ring, d, mt, j, b, xv, xc);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            acc[mt][nt] = mfma16<0, 0>(wv[nt], wc[nt], xv, xc, acc[mt][nt]);
+        }
       }
-  };
-  int u = wave;
-  if (u < units) {
-    WUnit<NT> wu;
-    XUnit<T, MT> xu;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) load_w(8 * u + 4 * j + q, j, true, wu);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) load_x(8 * u + 4 * j + q, j, true, xu);
-    for (; u + NW < units; u += NW) {
-      WUnit<NT> wn;
-      XUnit<T, MT> xn;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) load_w(8 * (u + NW) + 4 * j + q, j, true, wn);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) load_x(8 * (u + NW) + 4 * j + q, j, true, xn);
-      compute(wu, xu);
-      wu = wn;
-      xu = xn;
+      __builtin_amdgcn_sched_barrier(0);
+      if (u + DEPTH < sp.end) {
+        stores_done();                               // reads of what is overwritten, that is
+        ring.issue(u + DEPTH, d);
+      }
     }
-    compute(wu, xu);
-  }
-  if (K % UNIT != 0 && wave == units % NW) {   // the last blocks, fewer than 8
-    WUnit<NT> wu;
-    XUnit<T, MT> xu;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int b = 8 * units + 4 * j + q;
-      load_w(b, j, b < kb, wu);
-      load_x(b, j, b < kb, xu);
-    }
-    compute(wu, xu);
   }
 }
 
 // Sums of the waves: every wave parks its tiles, then fn(nn, mm, sum) gets D[nn, mm] of the
 // 16 NT x rows block, each from one thread, summed in wave order.
-template <int MT, int NT, int NW, class F>
-MM_DEV void skinny_reduce(const f32x4 (&acc)[MT][NT], float* red, int rows, F&& fn) {
+template <int MT, int NT, int NW>
+MM_DEV void skinny_park(const f32x4 (&acc)[MT][NT], float* red) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   f32x4* mine = (f32x4*)red + (size_t)wave * MT * NT * 64 + lane;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) mine[(mt * NT + nt) * 64] = acc[mt][nt];
+}
+template <int MT, int NT, int NW>
+MM_DEV float skinny_sum(const float* red, int nn, int mm) {
+  const int at = (((mm / 16) * NT + nn / 16) * 64 + (nn % 16 / 4) * 16 + mm % 16) * 4 + nn % 4;
+  float sum = red[at];
+#pragma unroll
+  for (int v = 1; v < NW; ++v) sum += red[v * MT * NT * 256 + at];
+  return sum;
+}
+template <int MT, int NT, int NW, class F>
+MM_DEV void skinny_reduce(const f32x4 (&acc)[MT][NT], float* red, int rows, F&& fn) {
+  skinny_park<MT, NT, NW>(acc, red);
   __syncthreads();
   for (int o = threadIdx.x; o < 16 * NT * rows; o += NW * 64) {
     const int mm = o / (16 * NT), nn = o % (16 * NT);
-    const int at = (((mm / 16) * NT + nn / 16) * 64 + (nn % 16 / 4) * 16 + mm % 16) * 4 + nn % 4;
-    float sum = red[at];
-#pragma unroll
-    for (int v = 1; v < NW; ++v) sum += red[v * MT * NT * 256 + at];
-    fn(nn, mm, sum);
+    fn(nn, mm, skinny_sum<MT, NT, NW>(red, nn, mm));
   }
 }
 
@@ -162,11 +326,6 @@ MM_DEV void skinny_reduce(const f32x4 (&acc)[MT][NT], float* red, int rows, F&& 
 // Rows of x are padded to whole units with zeros; what a weight row's last stage reads behind K
 // is some of its own blocks, times those zeros.
 // ---------------------------------------------------------------------------
-typedef __attribute__((address_space(3))) void* lds_ptr;
-MM_DEV void copy16(const void* src, void* lds_uniform) {
-  __builtin_amdgcn_global_load_lds(src, (lds_ptr)lds_uniform, 16, 0, 0);
-}
-
 template <int WM_, int WN_, int MB_, int NB_>
 struct Tile {
   static constexpr int WM = WM_, WN = WN_, MB = MB_, NB = NB_;

@@ -536,6 +536,7 @@ bool plain_mx(const at::Tensor& W, const at::Tensor& S, int dev, int n) {
   if (W.dim() != n || S.dim() != n || W.get_device() != dev || S.get_device() != dev ||
       (W.scalar_type() != at::kInt && W.scalar_type() != at::kUInt32) ||
       S.scalar_type() != at::kByte || !W.is_contiguous() || !S.is_contiguous() || !aligned(W) ||
+      !aligned(S) ||
       W.numel() == 0 || W.size(n - 1) != 4 * S.size(n - 1))
     return false;
   return W.sizes().slice(0, n - 1) == S.sizes().slice(0, n - 1);
@@ -561,6 +562,28 @@ pybind11::object mx_gemm(const at::Tensor& x, const at::Tensor& W, const at::Ten
                                (const uint8_t*)S.data_ptr(), out.data_ptr(), ot, (int)M, (int)N,
                                (int)K, need ? ws.data_ptr() : nullptr, need ? ws.numel() : 0,
                                (void*)stream);
+  if (rc) fail(rc);
+  return pybind11::cast(out);
+}
+
+// The gradient of x for dy [*, N].
+pybind11::object mx_gemm_backward(const at::Tensor& dy, const at::Tensor& W, const at::Tensor& S,
+                                  int64_t out_type, int64_t stream) {
+  const int dev = (int)dy.get_device();
+  if (!on_current_device(dev) || !plain_mx(W, S, dev, 2)) return pybind11::none();
+  const int64_t N = W.size(0), K = 8 * W.size(1), M = plain_rows(dy, dev, N);
+  if (M < 0 || M > INT32_MAX || N > INT32_MAX || N * dy.element_size() % 16 != 0)
+    return pybind11::none();
+  const int type = type_code(dy.scalar_type()), ot = out_type < 0 ? type : (int)out_type;
+  at::Tensor out = rows_like(dy, K, scalar_type_of(ot));
+  if (M == 0) return pybind11::cast(out);
+  const size_t need = mm_mxfp4_gemm_backward_workspace_bytes((int)M, (int)N, (int)K, type);
+  at::Tensor ws;
+  if (need) ws = workspace(dy, stream, need);
+  const int rc = mm_mxfp4_gemm_backward(dy.data_ptr(), type, (int)N, (const uint32_t*)W.data_ptr(),
+                                        (const uint8_t*)S.data_ptr(), out.data_ptr(), ot, (int)M,
+                                        (int)N, (int)K, need ? ws.data_ptr() : nullptr,
+                                        need ? ws.numel() : 0, (void*)stream);
   if (rc) fail(rc);
   return pybind11::cast(out);
 }
@@ -591,6 +614,36 @@ pybind11::object mx_dequantize(const at::Tensor& W, const at::Tensor& S, int64_t
   const int rc = mm_mxfp4_dequantize((const uint32_t*)W.data_ptr(), (const uint8_t*)S.data_ptr(),
                                      W.numel() / W.size(-1), (int)K, out.data_ptr(), (int)type,
                                      (void*)stream);
+  if (rc) fail(rc);
+  return pybind11::cast(out);
+}
+
+// The experts' block on MXFP4 weights: plain operands, ids and probs [T, k].
+pybind11::object mx_moe_mlp(const at::Tensor& x, const at::Tensor& Wgu, const at::Tensor& Sgu,
+                            const at::Tensor& Wdn, const at::Tensor& Sdn, const at::Tensor& ids,
+                            const at::Tensor& probs, int64_t stream) {
+  const int dev = (int)x.get_device();
+  if (!on_current_device(dev) || x.dim() != 2 || !plain_mx(Wgu, Sgu, dev, 3) ||
+      !plain_mx(Wdn, Sdn, dev, 3) || ids.dim() != 2 || probs.sizes() != ids.sizes() ||
+      ids.get_device() != dev || probs.get_device() != dev || !ids.is_contiguous() ||
+      !probs.is_contiguous() || probs.scalar_type() != at::kFloat ||
+      (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt))
+    return pybind11::none();
+  const int64_t E = Wgu.size(0), I = 8 * Wdn.size(2), H = 8 * Wgu.size(2);
+  const int64_t T = plain_rows(x, dev, H), k = ids.size(1);
+  if (T <= 0 || k == 0 || ids.size(0) != T || Wgu.size(1) != 2 * I || Wdn.size(0) != E ||
+      Wdn.size(1) != H || std::max({E, I, H, T, T * k}) > INT32_MAX)
+    return pybind11::none();
+  const int type = type_code(x.scalar_type());
+  at::Tensor out = at::empty_like(x);
+  const size_t need = mm_moe_mlp_mxfp4_scratch_bytes((int)T, (int)k, (int)E, (int)H, (int)I, type);
+  at::Tensor scratch = at::empty({(int64_t)need}, x.options().dtype(at::kByte));
+  const int rc = mm_moe_mlp_mxfp4(
+      x.data_ptr(), type, ids.data_ptr(), ids.scalar_type() == at::kLong,
+      (const float*)probs.data_ptr(), (int)T, (int)k, (int)E, (int)H, (int)I,
+      (const uint32_t*)Wgu.data_ptr(), (const uint8_t*)Sgu.data_ptr(),
+      (const uint32_t*)Wdn.data_ptr(), (const uint8_t*)Sdn.data_ptr(), scratch.data_ptr(), need,
+      out.data_ptr(), (void*)stream);
   if (rc) fail(rc);
   return pybind11::cast(out);
 }
@@ -666,8 +719,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("lora_add", &lora_add, "mm_lora_add on plain operands, else None");
   m.def("lora_backward", &lora_backward, "mm_lora_backward on plain operands, else None");
   m.def("mx_gemm", &mx_gemm, "mm_mxfp4_gemm on plain operands, else None");
+  m.def("mx_gemm_backward", &mx_gemm_backward, "mm_mxfp4_gemm_backward on plain operands, else None");
   m.def("mx_quantize", &mx_quantize, "mm_mxfp4_quantize on a plain operand, else None");
   m.def("mx_dequantize", &mx_dequantize, "mm_mxfp4_dequantize on plain operands, else None");
+  m.def("mx_moe_mlp", &mx_moe_mlp, "mm_moe_mlp_mxfp4 on plain operands, else None");
   m.def("moe_route", &moe_route, "mm_moe_route on plain operands, else None");
   m.def("moe_route_backward", &moe_route_backward,
         "mm_moe_route_backward on plain operands, else None");

@@ -15,11 +15,12 @@ from .fp4_metal import FP4Metal, dequantize_fp4_metal, quantize_fp4_metal
 from .backward import (fused_gate_up_swiglu, fused_gate_up_swiglu_backward,
                        marlin_gemm_fp4_backward, marlin_gemm_int4_backward,
                        mmfp4_fused_qkv_backward, mmfp4_gemm_rowpacked_backward)
-from .mxfp4 import mxfp4_dequantize, mxfp4_gemm, mxfp4_quantize
+from .mxfp4 import (moe_mlp_mxfp4, mxfp4_dequantize, mxfp4_gemm, mxfp4_gemm_backward,
+                    mxfp4_quantize)
 from .routing import moe_route, moe_route_backward
 from .adapters import lora_add, lora_backward
 from .autograd import gate_up_swiglu
-from .layers import MMFP4Linear
+from .layers import MMFP4Linear, MXFP4Linear
 from .ops import GemmFp4, dispatch_gemm_fp4
 from .loader import QuantizedModel, convert_safetensors_to_fp4, load_and_quantize_safetensors
 from .moe_dispatch import (FusedMoEDispatcher, MoEDispatcher, _fused_expert_mlp,

@@ -68,6 +68,9 @@ SIGNATURES: dict[str, tuple] = {
     "mm_mxfp4_dequantize": (_c_int, [_vp, _vp, ctypes.c_longlong, _c_int, _vp, _c_int, _vp]),
     "mm_mxfp4_gemm_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
     "mm_mxfp4_gemm": (_c_int, [_vp, _c_int, _vp, _vp, _vp] + [_c_int] * 4 + [_vp, _c_size, _vp]),
+    "mm_mxfp4_gemm_backward_workspace_bytes": (_c_size, [_c_int] * 4),
+    "mm_mxfp4_gemm_backward": (_c_int, [_vp, _c_int, _c_int, _vp, _vp, _vp] + [_c_int] * 4 +
+                               [_vp, _c_size, _vp]),
     "mm_moe_sort": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp]),
     "mm_moe_sort_i64": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp]),
     "mm_moe_router_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
@@ -82,6 +85,9 @@ SIGNATURES: dict[str, tuple] = {
     "mm_moe_combine": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp]),
     "mm_moe_mlp_fp4": (_c_int, [_vp, _vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_int,
                                 _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _vp, _vp, _vp]),
+    "mm_moe_mlp_mxfp4_scratch_bytes": (_c_size, [_c_int] * 6),
+    "mm_moe_mlp_mxfp4": (_c_int, [_vp, _c_int, _vp, _c_int, _vp] + [_c_int] * 5 + [_vp] * 5 +
+                         [_c_size, _vp, _vp]),
     "mm_moe_mlp_shared_fp4": (_c_int, [_vp, _vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int,
                                        _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                        ctypes.c_float, _vp, _c_int, _vp, _vp, _vp, _vp, _vp]),

@@ -109,6 +109,15 @@ def rowpacked_gemm(A: torch.Tensor, B_rows: torch.Tensor, scales: torch.Tensor,
         False)
 
 
+def mxfp4_product(x: torch.Tensor, words: torch.Tensor, scales: torch.Tensor,
+                  out_dtype: torch.dtype | None) -> torch.Tensor:
+    """mxfp4_gemm, differentiable in x."""
+    from . import mxfp4
+    return _Linear.apply(
+        x, lambda t: mxfp4._gemm(t, words, scales, out_dtype),
+        lambda dy, dt: mxfp4.mxfp4_gemm_backward(dy, words, scales, dt), False)
+
+
 class FusedQKV(torch.autograd.Function):
     """mmfp4_fused_qkv, differentiable in A: the three gradients meet in one product."""
 

@@ -2,5 +2,6 @@
 `metal_marlin.layers` surface for this path)."""
 
 from .mmfp4_linear import MMFP4Linear, mmfp4_gemm, rowpacked_to_marlin
+from .mxfp4_linear import MXFP4Linear
 
-__all__ = ["MMFP4Linear", "mmfp4_gemm", "rowpacked_to_marlin"]
+__all__ = ["MMFP4Linear", "MXFP4Linear", "mmfp4_gemm", "rowpacked_to_marlin"]

@@ -16,10 +16,11 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib
+from . import _lib, kernels
 from .backward import _TYPES, _type, on_device, plain
 
-__all__ = ["mxfp4_quantize", "mxfp4_dequantize", "mxfp4_gemm"]
+__all__ = ["mxfp4_quantize", "mxfp4_dequantize", "mxfp4_gemm", "mxfp4_gemm_backward",
+           "moe_mlp_mxfp4"]
 
 BLOCK = 32
 
@@ -84,7 +85,7 @@ def mxfp4_dequantize(words: torch.Tensor, scales: torch.Tensor,
     words, scales = _weights(words, scales)
     K = 8 * words.shape[-1]
     with on_device(dev):
-        w, s = plain(words), scales.contiguous()
+        w, s = plain(words), plain(scales)
         out = torch.empty((*words.shape[:-1], K), dtype=dtype, device=dev)
         _lib.call("mm_mxfp4_dequantize", _lib.ptr(w), _lib.ptr(s), out.numel() // K, K,
                   _lib.ptr(out), _TYPES[dtype], _lib.stream_of(w))
@@ -93,20 +94,20 @@ def mxfp4_dequantize(words: torch.Tensor, scales: torch.Tensor,
 
 def _gemm(x: torch.Tensor, words: torch.Tensor, scales: torch.Tensor,
           out_dtype: torch.dtype | None) -> torch.Tensor:
+    out = _lib.fast("mx_gemm", x, x, words, scales, -1 if out_dtype is None else _type(
+        "out_dtype", out_dtype))
+    if out is not None:
+        return out
     dev = _lib.require_device(x, words, scales)
     _type("x", x.dtype)
     dtype = out_dtype or x.dtype
-    _type("out_dtype", dtype)
-    out = _lib.fast("mx_gemm", x, x, words, scales, _TYPES[dtype])
-    if out is not None:
-        return out
     words, scales = _weights(words, scales, 2)
     N, K = words.shape[0], 8 * words.shape[1]
     if x.dim() == 0 or x.shape[-1] != K:
         raise ValueError(f"x shape {tuple(x.shape)} must end in K={K}")
     with on_device(dev):
         a = plain(x.reshape(-1, K))
-        w, s = plain(words), scales.contiguous()
+        w, s = plain(words), plain(scales)
         M = a.shape[0]
         out = torch.empty((*x.shape[:-1], N), dtype=dtype, device=dev)
         if out.numel() == 0:
@@ -123,5 +124,103 @@ def mxfp4_gemm(x: torch.Tensor, words: torch.Tensor, scales: torch.Tensor,
                out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """q(x) @ W^T [*, N] in x's type or out_dtype: x [*, K] fp16, bf16 or fp32 is quantized as
     mxfp4_quantize does, W [N, K] is given so (words [N, K/8], scales [N, K/32]); fp32 sums,
-    rounded once."""
-    return _gemm(x, words, scales, out_dtype)
+    rounded once.  Differentiable in x, straight through its rounding (mxfp4_gemm_backward)."""
+    if isinstance(x, torch.Tensor):
+        if kernels._wants_grad(x):
+            from . import autograd
+            return autograd.mxfp4_product(x, words, scales, out_dtype)
+        return _gemm(x, words, scales, out_dtype)
+    raise TypeError(f"expected torch.Tensor, got {type(x).__name__}")
+
+
+def mxfp4_gemm_backward(dy: torch.Tensor, words: torch.Tensor, scales: torch.Tensor,
+                        out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """dx = dy @ W, the gradient of mxfp4_gemm's input for dy [*, N] -> [*, K] in dy's type or
+    out_dtype: x's rounding counts as the identity.  dy (fp16, bf16 or fp32) and W enter exactly,
+    sums are fp32, rounded once."""
+    if not isinstance(dy, torch.Tensor):
+        raise TypeError(f"expected torch.Tensor, got {type(dy).__name__}")
+    out = _lib.fast("mx_gemm_backward", dy, dy, words, scales, -1 if out_dtype is None else _type(
+        "out_dtype", out_dtype))
+    if out is not None:
+        return out
+    dev = _lib.require_device(dy, words, scales)
+    _type("dy", dy.dtype)
+    dtype = out_dtype or dy.dtype
+    words, scales = _weights(words, scales, 2)
+    N, K = words.shape[0], 8 * words.shape[1]
+    if dy.dim() == 0 or dy.shape[-1] != N:
+        raise ValueError(f"dy shape {tuple(dy.shape)} must end in N={N}")
+    with on_device(dev):
+        out = torch.empty((*dy.shape[:-1], K), dtype=dtype, device=dev)
+        if out.numel() == 0:
+            return out
+        if N == 0:
+            return out.zero_()
+        w, s = plain(words), plain(scales)
+        d, pad = dy.reshape(-1, N), -N % (4 if dy.dtype == torch.float32 else 8)
+        if pad:                 # rows of whole 16-byte pieces
+            d = torch.nn.functional.pad(d, (0, pad))
+        d = plain(d)
+        M = d.shape[0]
+        stream = _lib.raw_stream(dev.index)
+        need = _lib.load().mm_mxfp4_gemm_backward_workspace_bytes(M, N, K, _TYPES[d.dtype])
+        ws = _lib.workspace_on(dev.index, stream, need)
+        _lib.call("mm_mxfp4_gemm_backward", _lib.ptr(d), _TYPES[d.dtype], N + pad,
+                  _lib.ptr(w), _lib.ptr(s), _lib.ptr(out), _TYPES[dtype], M, N, K, _lib.ptr(ws),
+                  ws.numel(), stream)
+    return out
+
+
+def moe_mlp_mxfp4(hidden: torch.Tensor, gate_up_words: torch.Tensor, gate_up_scales: torch.Tensor,
+                  down_words: torch.Tensor, down_scales: torch.Tensor, expert_ids: torch.Tensor,
+                  expert_probs: torch.Tensor) -> torch.Tensor:
+    """moe_mlp_fp4 on MXFP4 weights (metal_marlin/moe_dispatch.py:1241-1431 per expert, combined
+    as :812-925): for hidden [T, H] of fp16, bf16 or fp32 and its experts [T, k] (as moe_route or
+    router_softmax_topk give them),
+        (g | u) = q(x) @ W_gu[e]^T;  a = q(silu(g) * u);  y = a @ W_dn[e]^T
+        out[t] = sum_j p[t, j] * y                        [T, H] in hidden's type
+    gate_up_words [E, 2I, H/8] and scales [E, 2I, H/32], the gate's I rows first; down_words
+    [E, H, I/8] and scales [E, H, I/32].  silu(g) * u is quantized from its fp32 value.  Ids
+    outside [0, E) contribute nothing.  Not differentiable, as the other products of experts."""
+    dev = _lib.require_device(hidden, gate_up_words, gate_up_scales, down_words, down_scales,
+                              expert_ids, expert_probs)
+    _type("hidden", hidden.dtype)
+    out = _lib.fast("mx_moe_mlp", hidden, hidden, gate_up_words, gate_up_scales, down_words,
+                    down_scales, expert_ids, expert_probs)
+    if out is not None:
+        return out
+    gu, gus = _weights(gate_up_words, gate_up_scales, 3, "gate_up_words")
+    dn, dns = _weights(down_words, down_scales, 3, "down_words")
+    E, N2, H = gu.shape[0], gu.shape[1], 8 * gu.shape[2]
+    I = 8 * dn.shape[2]
+    if N2 != 2 * I or tuple(dn.shape[:2]) != (E, H):
+        raise ValueError(f"down_words shape {tuple(dn.shape)} != ({E}, {H}, {N2 // 16}) for "
+                         f"gate_up_words {tuple(gu.shape)}")
+    if hidden.dim() != 2 or hidden.shape[1] != H:
+        raise ValueError(f"hidden shape {tuple(hidden.shape)} must be [T, {H}]")
+    T = hidden.shape[0]
+    if expert_ids.dim() != 2 or expert_ids.shape[0] != T or expert_ids.shape[1] == 0 or \
+            expert_probs.shape != expert_ids.shape:
+        raise ValueError(f"expert_ids {tuple(expert_ids.shape)} and expert_probs "
+                         f"{tuple(expert_probs.shape)} must be [{T}, top_k]")
+    if expert_ids.is_floating_point() or expert_ids.dtype in (torch.bool, torch.uint64):
+        raise TypeError(f"expert_ids must be integers, got {expert_ids.dtype}")
+    k = expert_ids.shape[1]
+    with on_device(dev):
+        x = plain(hidden)
+        ids = expert_ids if expert_ids.dtype == torch.int64 else expert_ids.to(torch.int32)
+        ids, p = ids.contiguous(), expert_probs.to(torch.float32).contiguous()
+        gu, gus, dn, dns = map(plain, (gu, gus, dn, dns))
+        out = torch.empty((T, H), dtype=hidden.dtype, device=dev)
+        if T == 0:
+            return out
+        if E == 0:
+            return out.zero_()
+        need = _lib.load().mm_moe_mlp_mxfp4_scratch_bytes(T, k, E, H, I, _TYPES[x.dtype])
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev)
+        _lib.call("mm_moe_mlp_mxfp4", _lib.ptr(x), _TYPES[x.dtype], _lib.ptr(ids),
+                  int(ids.dtype == torch.int64), _lib.ptr(p), T, k, E, H, I, _lib.ptr(gu),
+                  _lib.ptr(gus), _lib.ptr(dn), _lib.ptr(dns), _lib.ptr(scratch), need,
+                  _lib.ptr(out), _lib.stream_of(x))
+    return out

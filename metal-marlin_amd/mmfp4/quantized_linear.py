@@ -180,8 +180,8 @@ class MarlinLinear:
 
 
 class LoRALinear(nn.Module):
-    """A quantized layer (QuantizedLinear, MarlinLinear, MMFP4Linear) with low-rank adapters of
-    several requests or users beside it: y = layer(x) + scaling[a] * (x @ lora_a[a]^T) @
+    """A quantized layer (QuantizedLinear, MarlinLinear, MMFP4Linear, MXFP4Linear) with low-rank
+    adapters of several requests or users beside it: y = layer(x) + scaling[a] * (x @ lora_a[a]^T) @
     lora_b[a]^T with a = adapter_ids[t], one id per token; ids outside [0, num_adapters) mean
     no adapter.  The layer's weights are frozen (a bias that requires a gradient gets it);
     lora_a [num_adapters, rank, in] (normal) and lora_b [num_adapters, out, rank] (zeros) are
