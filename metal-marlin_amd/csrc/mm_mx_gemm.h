@@ -52,6 +52,12 @@ MM_DEV void block_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// Nothing moves across this, loads of LDS least of all.
+MM_DEV void in_order() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // ---------------------------------------------------------------------------
 // Few rows: bound by the weights' bytes.  The NW waves of a block share out the units of 256 k.
 // A wave copies its units' rows global -> LDS, 128 bytes of 8 rows per instruction (a matrix
@@ -342,7 +348,8 @@ struct Tile {
 // The 8 scales from `at` on, of `blocks` >= 8; those behind the end are zero.
 MM_DEV u32x2 load_scales(const uint8_t* p, int at, int blocks) {
   u32x2 v;
-  __builtin_memcpy(&v, p + min(at, blocks - 8), 8);    // one load, whatever its alignment
+  // one load, whatever its alignment
+  __builtin_memcpy(&v, p + max(0, min(at, blocks - 8)), 8);
   return v;
 }
 MM_DEV u32x2 shift_scales(u32x2 v, int at, int blocks) {
@@ -411,39 +418,51 @@ MM_DEV void tile_loop(const Src& src, int u0, int u1, char* smem, f32x16 (&acc)[
             shift_scales(sc[i], 8 * u, blocks[i]);
     }
   };
-  auto compute = [&](int st) {
+  // Operands of quarter j (64 k) of a stage, and the lane's scales of a whole stage (half h's in
+  // every second byte from byte 0 on).
+  u32x4 a[2][Sh::NB], b[2][Sh::MB];
+  u32x2 sw[Sh::NB], sx[Sh::MB];
+  auto read = [&](int st, int j, int to) {
     const char* const d = smem + st * Sh::STAGE;
+    const int p = 16 * ((2 * j + h) ^ ((l32 >> 1) & 7));
+#pragma unroll
+    for (int n = 0; n < Sh::NB; ++n)
+      a[to][n] = *(const u32x4*)(d + ((wn * Sh::NB + n) * 32 + l32) * 128 + p);
+#pragma unroll
+    for (int m = 0; m < Sh::MB; ++m)
+      b[to][m] = *(const u32x4*)(d + (Sh::TN + (wm * Sh::MB + m) * 32 + l32) * 128 + p);
+  };
+  auto read_sc = [&](int st) {
     const char* const s = smem + 2 * Sh::STAGE + st * Sh::SSTAGE;
-    u32x2 sw[Sh::NB], sx[Sh::MB];
 #pragma unroll
     for (int n = 0; n < Sh::NB; ++n)
       sw[n] = *(const u32x2*)(s + ((wn * Sh::NB + n) * 32 + l32) * 8) >> (uint32_t)(8 * h);
 #pragma unroll
     for (int m = 0; m < Sh::MB; ++m)
       sx[m] = *(const u32x2*)(s + (Sh::TN + (wm * Sh::MB + m) * 32 + l32) * 8) >> (uint32_t)(8 * h);
-    // The operands of a quarter are read while the quarter before it is multiplied.
-    u32x4 a[2][Sh::NB], b[2][Sh::MB];
-    auto read = [&](int j, u32x4 (&av)[Sh::NB], u32x4 (&bv)[Sh::MB]) {
-      const int p = 16 * ((2 * j + h) ^ ((l32 >> 1) & 7));
+  };
+  // Quarter j; `between` runs after its first products: what it reads is not waited for by them.
+  auto multiply = [&](auto jc, const u32x2 (&w)[Sh::NB], const u32x2 (&x)[Sh::MB], auto&& between) {
+    constexpr int j = decltype(jc)::value;
 #pragma unroll
-      for (int n = 0; n < Sh::NB; ++n)
-        av[n] = *(const u32x4*)(d + ((wn * Sh::NB + n) * 32 + l32) * 128 + p);
+    for (int n = 0; n < Sh::NB; ++n) {
 #pragma unroll
       for (int m = 0; m < Sh::MB; ++m)
-        bv[m] = *(const u32x4*)(d + (Sh::TN + (wm * Sh::MB + m) * 32 + l32) * 128 + p);
-    };
-    read(0, a[0], b[0]);
-    repeat<4>([&](auto jc) {
+        acc[n][m] = mfma32<j % 2 * 2, j % 2 * 2>(a[j & 1][n], w[n][j / 2], b[j & 1][m], x[m][j / 2],
+                                                 acc[n][m]);
+      if (n == 0) {
+        in_order();
+        between();
+        in_order();
+      }
+    }
+    in_order();
+  };
+  // Quarters 0 to 2 of a stage, each while the next one's operands are read.
+  auto quarters = [&](int st) {
+    repeat<3>([&](auto jc) {
       constexpr int j = decltype(jc)::value;
-      if constexpr (j < 3) read(j + 1, a[(j + 1) & 1], b[(j + 1) & 1]);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int n = 0; n < Sh::NB; ++n)
-#pragma unroll
-        for (int m = 0; m < Sh::MB; ++m)
-          acc[n][m] = mfma32<j % 2 * 2, j % 2 * 2>(a[j & 1][n], sw[n][j / 2], b[j & 1][m],
-                                                   sx[m][j / 2], acc[n][m]);
-      __builtin_amdgcn_sched_barrier(0);
+      multiply(jc, sw, sx, [&] { read(st, j + 1, (j + 1) & 1); });
     });
   };
   issue(u0, 0);
@@ -462,33 +481,90 @@ MM_DEV void tile_loop(const Src& src, int u0, int u1, char* smem, f32x16 (&acc)[
   }
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
+  issue(min(u0 + 1, u1 - 1), 1);
+  load_sc(min(u0 + 1, u1 - 1));
+  read_sc(0);
+  read(0, 0, 0);
   int st = 0;
+#pragma unroll 1
   for (int u = u0; u + 1 < u1; ++u) {
-    issue(u + 1, st ^ 1);
-    load_sc(u + 1);
-    __builtin_amdgcn_sched_barrier(0);
-    compute(st);
+    quarters(st);
+    // Every operand of this stage has been read, or is in flight to its registers: the next stage
+    // is made sure of, this one's memory given to the one after it, and the last quarter is
+    // multiplied while the next stage's first is read.
     store_sc(u + 1, st ^ 1);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
+    // (Past the last stage that one again, and nobody reads it: a branch here would let the
+    // compiler move the multiplications of this stage behind it.)
+    issue(min(u + 2, u1 - 1), st);
+    load_sc(min(u + 2, u1 - 1));
+    u32x2 w[Sh::NB], x[Sh::MB];
+#pragma unroll
+    for (int n = 0; n < Sh::NB; ++n) w[n] = sw[n];
+#pragma unroll
+    for (int m = 0; m < Sh::MB; ++m) x[m] = sx[m];
     st ^= 1;
+    multiply(std::integral_constant<int, 3>{}, w, x, [&] {
+      read_sc(st);
+      read(st, 0, 0);
+    });
   }
-  compute(st);
+  quarters(st);
+  multiply(std::integral_constant<int, 3>{}, sw, sx, [] {});
+  wait_loads<0>();
 }
 
-// fn(n, m, v): v[0..3] are D[n..n+3, m] of the tile, n a multiple of 4.
-template <class Sh, class F>
-MM_DEV void tile_out(const f32x16 (&acc)[Sh::NB][Sh::MB], F&& fn) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// The tile's results to C, row m of which begins at row_at(m) (row m of the tile, an index into C),
+// columns n0 .. N: through LDS, 32 rows of a wave at a time, so that stores are whole lines (a
+// lane holds 4 results of a row, and stores of those took a sixth of the time of a large
+// product: 2048 x 14336 x 4096 93 us, 77 without them).  Every wave of the block has to be done
+// with the tile's memory.  rows: rows of the tile that are there.
+template <class Sh, class RowAt>
+MM_DEV void tile_out(const f32x16 (&acc)[Sh::NB][Sh::MB], char* smem, void* C, int type, int rows,
+                     int n0, int N, RowAt&& row_at) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / Sh::WN, wn = wave % Sh::WN, l32 = lane & 31, h = lane >> 5;
+  constexpr int COLS = Sh::NB * 32;
+  const int size = type == F32 ? 4 : 2, pitch = COLS * size + 16;
+  static_assert(Sh::NWAVE * 32 * (COLS * 4 + 16) <= Sh::LDS, "the waves' rows take the tile's place");
+  char* const mine = smem + wave * 32 * (COLS * 4 + 16);
+  const int c0 = n0 + wn * COLS, cols = min(COLS, N - c0);
+  if (cols <= 0) return;
+  const bool whole = N * size % 16 == 0;      // pieces of 16 bytes lie whole and aligned
 #pragma unroll
-  for (int m = 0; m < Sh::MB; ++m)
+  for (int m = 0; m < Sh::MB; ++m) {
+    const int m0 = (wm * Sh::MB + m) * 32;
+    if (m0 >= rows) break;
+    stores_done();                            // and the reads of the rows before
 #pragma unroll
     for (int n = 0; n < Sh::NB; ++n)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        fn((wn * Sh::NB + n) * 32 + 8 * g + 4 * h, (wm * Sh::MB + m) * 32 + l32,
-           f32x4{acc[n][m][4 * g], acc[n][m][4 * g + 1], acc[n][m][4 * g + 2], acc[n][m][4 * g + 3]});
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 v = {acc[n][m][4 * g], acc[n][m][4 * g + 1], acc[n][m][4 * g + 2],
+                         acc[n][m][4 * g + 3]};
+        store4(mine + l32 * pitch, type, n * 32 + 8 * g + 4 * h, v);
+      }
+    stores_done();
+    const int rn = min(32, rows - m0);
+    if (whole) {
+      const int per = cols * size / 16;       // pieces per row
+      for (int p = lane; p < 32 * (COLS * size / 16); p += 64) {
+        const int r = p / (COLS * size / 16), c = p % (COLS * size / 16);
+        if (r < rn && c < per)
+          *(u32x4*)((char*)C + (row_at(m0 + r) + c0) * size + 16 * c) =
+              *(const u32x4*)(mine + r * pitch + 16 * c);
+      }
+    } else {
+      for (int p = lane; p < 32 * COLS; p += 64) {
+        const int r = p / COLS, c = p % COLS;
+        if (r >= rn || c >= cols) continue;
+        const size_t at = row_at(m0 + r) + c0 + c;
+        if (type == F32) ((float*)C)[at] = *(const float*)(mine + r * pitch + 4 * c);
+        else ((uint16_t*)C)[at] = *(const uint16_t*)(mine + r * pitch + 2 * c);
+      }
+    }
+  }
 }
 
 }  // namespace mmmx

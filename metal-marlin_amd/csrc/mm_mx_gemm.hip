@@ -1,6 +1,7 @@
 // C[M, N] = q(X) . W^T: X [M, K] fp32, fp16 or bf16 is quantized to MXFP4 (mm_mx.h), W is kept so,
 // words [N, K/8] and scales [N, K/32].  The cores are in mm_mx_gemm.h.
 #include <algorithm>
+#include <cstdlib>
 
 #include "mm_mx_gemm.h"
 #include "mmfp4.h"
@@ -107,20 +108,9 @@ k_mx_tile(const uint8_t* __restrict__ X, const uint8_t* __restrict__ XS, int kp,
                      K, kp, N - 1 - n0, M - 1 - m0};
   f32x16 acc[Sh::NB][Sh::MB];
   tile_loop<Sh>(src, 0, (K + UNIT - 1) / UNIT, smem, acc);
-  const bool whole = N % 4 == 0;
-  tile_out<Sh>(acc, [&](int n, int m, f32x4 v) {
-    m += m0;
-    n += n0;
-    if (m >= M || n >= N) return;
-    const size_t at = (size_t)m * N + n;
-    if (whole) {
-      store4(C, out_type, at, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i < N) store1(C, out_type, at + i, v[i]);
-    }
-  });
+  __syncthreads();
+  tile_out<Sh>(acc, smem, C, out_type, M - m0, n0, N,
+               [=](int m) { return (size_t)(m0 + m) * N; });
 }
 
 constexpr int SKINNY_M = 16;    // rows that the kernel may quantize itself
@@ -166,7 +156,7 @@ void launch_tile(const uint8_t* xq, const uint8_t* xs, int kp, const uint32_t* W
                  void* C, int out_type, int M, int N, int K, hipStream_t st) {
   const int gm = mm_cdiv(M, Sh::TM), gn = mm_cdiv(N, Sh::TN);
   hipLaunchKernelGGL((k_mx_tile<Sh>), dim3((unsigned)(gm * gn)), dim3(Sh::NTHR), 0, st, xq, xs, kp,
-                     (const uint8_t*)W, S, C, out_type, M, N, K, gm, gn, std::min(gm, 8));
+                     (const uint8_t*)W, S, C, out_type, M, N, K, gm, gn, std::min(gm, 4));
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -214,7 +204,13 @@ extern "C" int mm_mxfp4_gemm(const void* X, int type, const uint32_t* W, const u
     return 0;
   }
   const long big = (long)mm_cdiv(M, 256) * mm_cdiv(N, 256);
-  if (big >= 200) launch_tile<Tile<4, 2, 2, 4>>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
+  static const int cfg = getenv("MX_CFG") ? atoi(getenv("MX_CFG")) : 0;
+  if (cfg == 1) launch_tile<Tile<2, 2, 4, 4>>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
+  else if (cfg == 2) launch_tile<Tile<2, 2, 2, 2>>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
+  else if (cfg == 3) launch_tile<Tile<2, 2, 2, 4>>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
+  else if (cfg == 4) launch_tile<Tile<2, 2, 1, 4>>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
+  else if (cfg == 5) launch_tile<Tile<2, 4, 2, 2>>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
+  else if (big >= 200) launch_tile<Tile<4, 2, 2, 4>>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
   else launch_tile<Tile<2, 2, 2, 2>>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
   MM_CHECK_LAUNCH("mm_mxfp4_gemm");
   return 0;

@@ -201,20 +201,9 @@ k_mx_moe_tile(const uint8_t* __restrict__ X, const uint8_t* __restrict__ XS, int
   f32x16 acc[Sh::NB][Sh::MB];
   if (!ACT || n0 < half) tile_loop<Sh>(src, 0, (K + UNIT - 1) / UNIT, smem, acc);
   if constexpr (!ACT) {
-    const bool whole = N % 4 == 0;
-    tile_out<Sh>(acc, [&](int n, int m, f32x4 v) {
-      m += m0;
-      n += n0;
-      if (m >= r1 || n >= N) return;
-      const size_t at = (size_t)m * N + n;
-      if (whole) {
-        store4(y, type, at, v);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (n + i < N) store1(y, type, at + i, v[i]);
-      }
-    });
+    __syncthreads();
+    tile_out<Sh>(acc, smem, y, type, r1 - m0, n0, N,
+                 [=](int m) { return (size_t)(m0 + m) * N; });
   } else {
     // A block of h is 16 values in each of lanes l and l + 32: n = 8 g + 4 h + i.
     const int wave = tid >> 6, wm = wave / Sh::WN, wn = wave % Sh::WN, l32 = lane & 31;
