@@ -175,4 +175,21 @@ inline size_t packed_bytes(size_t rows, int K) {
 int launch_quantize(const void* x, int type, size_t rows, int K, size_t kp, uint32_t* words,
                     uint8_t* scales, hipStream_t stream);
 
+// The same for tiles, which take scales by units of 256 values, 8 of each row side by side and
+// unit_pitch(rows) from unit to unit (there is room for the rows of whole tiles); in the same
+// launch the scales S of the weights [N, K] go to `units` in that order.
+inline __host__ __device__ size_t unit_pitch(size_t rows) { return (rows + 255) / 256 * 2048; }
+int launch_quantize_units(const void* x, int type, size_t rows, int K, size_t kp, uint32_t* words,
+                          uint8_t* scales, const uint8_t* S, size_t N, uint8_t* units,
+                          hipStream_t stream);
+
+// Rows of `kb` scales to rows of `ks` >= kb, zeros behind: where kb is no multiple of 4, the tiles,
+// which copy four at a time, take such a copy.
+inline int scale_stride(int K) { return K / BLOCK % 4 == 0 ? K / BLOCK : (K / BLOCK + 3) / 4 * 4; }
+int launch_pad_scales(const uint8_t* s, size_t rows, int kb, int ks, uint8_t* out, hipStream_t stream);
+
+// out[i] = sum over s of part[s][i], in order, rounded once; part[s] begins s * sum_pitch(n) on.
+__host__ __device__ inline size_t sum_pitch(size_t n) { return (n + 3) / 4 * 4; }
+int launch_sum(const float* part, int splits, size_t n, void* out, int type, hipStream_t stream);
+
 }  // namespace mmmx

@@ -237,16 +237,6 @@ __global__ void __launch_bounds__(Sh::NTHR) k_mx_grad(Grad a, int gm, int gk) {
   }
 }
 
-// Partial sums [splits, n] in split order, rounded once; n % 4 == 0.
-__global__ void __launch_bounds__(256)
-k_mx_grad_sum(const float* __restrict__ part, int splits, size_t n, void* __restrict__ out, int type) {
-  const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= n) return;
-  f32x4 v = *(const f32x4*)(part + i);
-  for (int s = 1; s < splits; ++s) v += *(const f32x4*)(part + (size_t)s * n + i);
-  store4(out, type, i, v);
-}
-
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 constexpr size_t COUNTERS = 65536;
 
@@ -317,11 +307,6 @@ extern "C" int mm_mxfp4_gemm_backward(const void* dY, int type, int ldy, const u
   if (type == F32) launch_t<F32>(a, p, st);
   else if (type == F16) launch_t<F16>(a, p, st);
   else launch_t<BF16>(a, p, st);
-  if (part) {
-    const size_t n = (size_t)M * K;
-    hipLaunchKernelGGL(k_mx_grad_sum, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, part,
-                       p.splits, n, dX, out_type);
-  }
   MM_CHECK_LAUNCH("mm_mxfp4_gemm_backward");
-  return 0;
+  return part ? launch_sum(part, p.splits, (size_t)M * K, dX, out_type, st) : 0;
 }

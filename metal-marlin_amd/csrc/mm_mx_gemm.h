@@ -24,6 +24,9 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 MM_DEV void copy16(const void* src, void* lds_uniform) {
   __builtin_amdgcn_global_load_lds(src, (lds_ptr)lds_uniform, 16, 0, 0);
 }
+MM_DEV void copy4(const void* src, void* lds_uniform) {
+  __builtin_amdgcn_global_load_lds(src, (lds_ptr)lds_uniform, 4, 0, 0);
+}
 // Waits until at most N vector memory operations are in flight.
 template <int N>
 MM_DEV void wait_loads() {
@@ -325,43 +328,35 @@ MM_DEV void skinny_reduce(const f32x4 (&acc)[MT][NT], float* red, int rows, F&& 
 
 // ---------------------------------------------------------------------------
 // More rows: tiles of TM x-rows by TN weight rows, bound by the matrix cores and LDS.  A stage is
-// one unit of 256 k: 128 bytes of every row, copied global -> LDS directly in 16-byte pieces, the
-// next stage while this one is multiplied.  Piece p of row r lies at p ^ (r / 2 % 8), so that the
-// 16 rows that an operand read takes at once spread over all banks.  The 8 scales per row go
-// through registers.  Each wave owns 32 NB x 32 MB of the tile.
+// one unit of 256 k: 128 bytes and 8 scales of every row, copied global -> LDS directly into a
+// ring of S stages, S - 1 of them ahead of the one that is multiplied.  Piece p of row r lies at
+// p ^ (r / 2 % 8), so that the 16 rows that an operand read takes at once spread over all banks.
+// Each wave owns 32 NB x 32 MB of the tile.
 // Rows of x are padded to whole units with zeros; what a weight row's last stage reads behind K
 // is some of its own blocks, times those zeros.
 // ---------------------------------------------------------------------------
-template <int WM_, int WN_, int MB_, int NB_>
+template <int WM_, int WN_, int MB_, int NB_, int S_ = 2>
 struct Tile {
-  static constexpr int WM = WM_, WN = WN_, MB = MB_, NB = NB_;
+  static constexpr int WM = WM_, WN = WN_, MB = MB_, NB = NB_, S = S_;
   static constexpr int NTHR = WM * WN * 64, NWAVE = WM * WN;
   static constexpr int TM = WM * MB * 32, TN = WN * NB * 32, ROWS = TM + TN;
-  static constexpr int STAGE = ROWS * 128, SSTAGE = ROWS * 8;
-  static constexpr int LDS = 2 * (STAGE + SSTAGE);
-  static constexpr int IT = ROWS / 8 / NWAVE;          // 1 KiB copies per wave and stage
-  static constexpr int SIT = (ROWS + NTHR - 1) / NTHR; // scale rows per thread
-  static_assert(ROWS % (8 * NWAVE) == 0, "copies per wave");
-  static_assert(TN % 8 == 0 && TM % 8 == 0, "a copy's rows are all of W or all of x");
+  static constexpr int STAGE = ROWS * 128;
+  static constexpr int SW = (TN + 127) / 128, SX = (TM + 127) / 128;   // KiB of scales of a stage
+  static constexpr int SSTAGE = (SW + SX) * 1024;
+  static constexpr int LDS = S * (STAGE + SSTAGE);
+  static constexpr int IT = ROWS / 8 / NWAVE;            // 1 KiB copies per wave and stage
+  static_assert(ROWS % (8 * NWAVE) == 0 && NWAVE % 2 == 0, "copies per wave");
+  static_assert(TN % 32 == 0 && TM % 32 == 0, "a copy's rows are all of W or all of x");
 };
-
-// The 8 scales from `at` on, of `blocks` >= 8; those behind the end are zero.
-MM_DEV u32x2 load_scales(const uint8_t* p, int at, int blocks) {
-  u32x2 v;
-  // one load, whatever its alignment
-  __builtin_memcpy(&v, p + max(0, min(at, blocks - 8)), 8);
-  return v;
-}
-MM_DEV u32x2 shift_scales(u32x2 v, int at, int blocks) {
-  const uint64_t q = (uint64_t)v.y << 32 | v.x;
-  const uint64_t r = q >> (8 * max(0, at + 8 - blocks));
-  return u32x2{(uint32_t)r, (uint32_t)(r >> 32)};
-}
 
 // Stages [u0, u1) into acc.  src: W, S, X, XS (the bases of the weights' and x's words and
 // scales), K and kp (values per row of W and of x), wrow(r) and xrow(r): the row, counted from
 // those bases, of row r of the tile; every one must be readable, and rows times K / 2 or kp / 2
-// stay below 2^32.
+// stay below 2^32.  Scales: Src::BY_UNIT: those of a unit lie together, 8 of each row, spitch and
+// xpitch bytes from unit to unit, readable for all rows of the tile.
+// Else rows of ks scales of W, a multiple of 4, and of kp / 32 of x: each of them is a line of
+// memory for 8 bytes, which cost as much as the words (4096 x 14336, 128 rows, tiles of 64 x 128:
+// 34.3 us, 28.5 without any scales).
 template <class Sh, class Src>
 MM_DEV void tile_loop(const Src& src, int u0, int u1, char* smem, f32x16 (&acc)[Sh::NB][Sh::MB]) {
   const int tid = threadIdx.x, lane = tid & 63;
@@ -375,14 +370,28 @@ MM_DEV void tile_loop(const Src& src, int u0, int u1, char* smem, f32x16 (&acc)[
       for (int i = 0; i < 16; ++i) acc[n][m][i] = 0.0f;
   if (u0 >= u1) return;
 
-  uint32_t off[Sh::IT];
+  constexpr int PIECES = Src::BY_UNIT ? Sh::SW + Sh::SX : Sh::ROWS / 32;    // copies of scales
+  constexpr int SIT = (PIECES + Sh::NWAVE - 1) / Sh::NWAVE, COPIES = Sh::IT + SIT;
+  static_assert(COPIES * (Sh::S - 2) < 64, "copies in flight");
+  uint32_t off[Sh::IT], soff[SIT];
 #pragma unroll
   for (int i = 0; i < Sh::IT; ++i) {
     const int r0 = (i * Sh::NWAVE + wave) * 8, r = r0 + lane / 8;
     off[i] = r0 < Sh::TN ? src.wrow(r) * (uint32_t)(src.K / 2)
                          : src.xrow(r - Sh::TN) * (uint32_t)(src.kp / 2);
   }
-  static_assert(Sh::NWAVE % 2 == 0, "a lane's pieces lie alike in all its copies");
+#pragma unroll
+  for (int i = 0; i < SIT; ++i) {          // waves to spare copy the last piece again
+    const int c = min(i * Sh::NWAVE + wave, PIECES - 1);
+    if constexpr (Src::BY_UNIT) {
+      soff[i] = c < Sh::SW ? min(c * 1024 + lane * 16, Sh::TN * 8 - 16)
+                           : min((c - Sh::SW) * 1024 + lane * 16, Sh::TM * 8 - 16);
+    } else {
+      const int r = c * 32 + lane / 2;
+      soff[i] = c * 32 < Sh::TN ? src.wrow(r) * (uint32_t)src.ks
+                                : src.xrow(r - Sh::TN) * (uint32_t)(src.kp / BLOCK);
+    }
+  }
   const int at = 16 * ((lane & 7) ^ ((wave * 4 + (lane >> 4)) & 7));
   auto issue = [&](int u, int st) {
 #pragma unroll
@@ -393,31 +402,99 @@ MM_DEV void tile_loop(const Src& src, int u0, int u1, char* smem, f32x16 (&acc)[
       copy16(base + (off[i] + (uint32_t)min(at, left)),
              smem + st * Sh::STAGE + (i * Sh::NWAVE + wave) * 1024);
     }
-  };
-  const uint8_t* scale[Sh::SIT];
-  int blocks[Sh::SIT];
+    char* const to = smem + Sh::S * Sh::STAGE + st * Sh::SSTAGE;
 #pragma unroll
-  for (int i = 0; i < Sh::SIT; ++i) {
-    const int r = min(tid + i * Sh::NTHR, Sh::ROWS - 1);
-    const bool isw = r < Sh::TN;
-    blocks[i] = (isw ? src.K : src.kp) / BLOCK;
-    scale[i] = isw ? src.S + (size_t)src.wrow(r) * blocks[i]
-                   : src.XS + (size_t)src.xrow(r - Sh::TN) * blocks[i];
-  }
-  u32x2 sc[Sh::SIT];
-  auto load_sc = [&](int u) {
-#pragma unroll
-    for (int i = 0; i < Sh::SIT; ++i) sc[i] = load_scales(scale[i], 8 * u, blocks[i]);
-  };
-  auto store_sc = [&](int u, int st) {
-#pragma unroll
-    for (int i = 0; i < Sh::SIT; ++i) {
-      const int r = tid + i * Sh::NTHR;
-      if (Sh::ROWS % Sh::NTHR == 0 || r < Sh::ROWS)
-        *(u32x2*)(smem + 2 * Sh::STAGE + st * Sh::SSTAGE + r * 8) =
-            shift_scales(sc[i], 8 * u, blocks[i]);
+    for (int i = 0; i < SIT; ++i) {
+      const int c = min(i * Sh::NWAVE + wave, PIECES - 1);
+      if constexpr (Src::BY_UNIT) {
+        copy16((c < Sh::SW ? src.S + (size_t)u * src.spitch : src.XS + (size_t)u * src.xpitch) + soff[i],
+               to + c * 1024);
+      } else {
+        const bool isw = c * 32 < Sh::TN;
+        const int left = (isw ? src.ks : src.kp / BLOCK) - 4 - u * 8;
+        copy4((isw ? src.S : src.XS) + u * 8 + (soff[i] + (uint32_t)min(4 * (lane & 1), left)),
+              to + (isw ? c * 256 : Sh::SW * 1024 + (c - Sh::TN / 32) * 256));
+      }
     }
   };
+  // Deep rings are for few blocks: one on a CU, with registers to spare.  A stage's operands are
+  // read whole while the stage before is multiplied, so that a wave waits for LDS and for the others
+  // only where the copies are late.
+  if constexpr (Sh::S > 2) {
+    u32x4 a[2][4][Sh::NB], b[2][4][Sh::MB];
+    u32x2 sw[2][Sh::NB], sx[2][Sh::MB];
+    auto read = [&](int st, auto to_) {
+      constexpr int to = decltype(to_)::value;
+      const char* const s = smem + Sh::S * Sh::STAGE + st * Sh::SSTAGE;
+      const char* const d = smem + st * Sh::STAGE;
+#pragma unroll
+      for (int n = 0; n < Sh::NB; ++n)
+        sw[to][n] = *(const u32x2*)(s + ((wn * Sh::NB + n) * 32 + l32) * 8);
+#pragma unroll
+      for (int m = 0; m < Sh::MB; ++m)
+        sx[to][m] = *(const u32x2*)(s + Sh::SW * 1024 + ((wm * Sh::MB + m) * 32 + l32) * 8);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int p = 16 * ((2 * j + h) ^ ((l32 >> 1) & 7));
+#pragma unroll
+        for (int n = 0; n < Sh::NB; ++n)
+          a[to][j][n] = *(const u32x4*)(d + ((wn * Sh::NB + n) * 32 + l32) * 128 + p);
+#pragma unroll
+        for (int m = 0; m < Sh::MB; ++m)
+          b[to][j][m] = *(const u32x4*)(d + (Sh::TN + (wm * Sh::MB + m) * 32 + l32) * 128 + p);
+      }
+    };
+    auto multiply = [&](auto of_) {
+      constexpr int of = decltype(of_)::value;
+      u32x2 w[Sh::NB], x[Sh::MB];
+#pragma unroll
+      for (int n = 0; n < Sh::NB; ++n) w[n] = sw[of][n] >> (uint32_t)(8 * h);
+#pragma unroll
+      for (int m = 0; m < Sh::MB; ++m) x[m] = sx[of][m] >> (uint32_t)(8 * h);
+      repeat<4>([&](auto jc) {
+        constexpr int j = decltype(jc)::value;
+#pragma unroll
+        for (int n = 0; n < Sh::NB; ++n)
+#pragma unroll
+          for (int m = 0; m < Sh::MB; ++m)
+            acc[n][m] = mfma32<j % 2 * 2, j % 2 * 2>(a[of][j][n], w[n][j / 2], b[of][j][m],
+                                                     x[m][j / 2], acc[n][m]);
+      });
+      in_order();
+    };
+#pragma unroll
+    for (int d = 0; d < Sh::S; ++d) issue(min(u0 + d, u1 - 1), d);
+    wait_loads<COPIES * (Sh::S - 1)>();
+    block_barrier();
+    read(0, std::integral_constant<int, 0>{});
+    int st = 0, u = u0;
+    // One stage: what it reads of the next is not waited for before the next one's turn.
+    auto step = [&](auto of_) {
+      constexpr int of = decltype(of_)::value;
+      stores_done();                        // this stage's operands are in registers
+      wait_loads<COPIES * (Sh::S - 2)>();
+      block_barrier();
+      issue(min(u + Sh::S, u1 - 1), st);
+      st = st + 1 == Sh::S ? 0 : st + 1;
+      read(st, std::integral_constant<int, 1 - of>{});
+      in_order();
+      multiply(of_);
+      ++u;
+    };
+#pragma unroll 1
+    for (; u + 2 < u1;) {
+      step(std::integral_constant<int, 0>{});
+      step(std::integral_constant<int, 1>{});
+    }
+    if (u + 1 < u1) {
+      step(std::integral_constant<int, 0>{});
+      multiply(std::integral_constant<int, 1>{});
+    } else {
+      multiply(std::integral_constant<int, 0>{});
+    }
+    wait_loads<0>();
+    return;
+  }
   // Operands of quarter j (64 k) of a stage, and the lane's scales of a whole stage (half h's in
   // every second byte from byte 0 on).
   u32x4 a[2][Sh::NB], b[2][Sh::MB];
@@ -433,13 +510,13 @@ MM_DEV void tile_loop(const Src& src, int u0, int u1, char* smem, f32x16 (&acc)[
       b[to][m] = *(const u32x4*)(d + (Sh::TN + (wm * Sh::MB + m) * 32 + l32) * 128 + p);
   };
   auto read_sc = [&](int st) {
-    const char* const s = smem + 2 * Sh::STAGE + st * Sh::SSTAGE;
+    const char* const s = smem + Sh::S * Sh::STAGE + st * Sh::SSTAGE;
 #pragma unroll
     for (int n = 0; n < Sh::NB; ++n)
       sw[n] = *(const u32x2*)(s + ((wn * Sh::NB + n) * 32 + l32) * 8) >> (uint32_t)(8 * h);
 #pragma unroll
     for (int m = 0; m < Sh::MB; ++m)
-      sx[m] = *(const u32x2*)(s + (Sh::TN + (wm * Sh::MB + m) * 32 + l32) * 8) >> (uint32_t)(8 * h);
+      sx[m] = *(const u32x2*)(s + Sh::SW * 1024 + ((wm * Sh::MB + m) * 32 + l32) * 8) >> (uint32_t)(8 * h);
   };
   // Quarter j; `between` runs after its first products: what it reads is not waited for by them.
   auto multiply = [&](auto jc, const u32x2 (&w)[Sh::NB], const u32x2 (&x)[Sh::MB], auto&& between) {
@@ -465,46 +542,29 @@ MM_DEV void tile_loop(const Src& src, int u0, int u1, char* smem, f32x16 (&acc)[
       multiply(jc, sw, sx, [&] { read(st, j + 1, (j + 1) & 1); });
     });
   };
-  issue(u0, 0);
-  if (src.K >= UNIT) {
-    load_sc(u0);
-    store_sc(u0, 0);
-  } else {                        // one stage, fewer than 8 blocks in a row of W
+  // Past the last stage that one again, and nobody reads it: the copies in flight can be counted,
+  // and no branch lets the compiler move the multiplications of a stage behind it.
 #pragma unroll
-    for (int i = 0; i < Sh::SIT; ++i) {
-      const int r = tid + i * Sh::NTHR;
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        if (r < Sh::ROWS)
-          smem[2 * Sh::STAGE + r * 8 + c] = c < blocks[i] ? (char)scale[i][c] : (char)0;
-    }
-  }
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  issue(min(u0 + 1, u1 - 1), 1);
-  load_sc(min(u0 + 1, u1 - 1));
+  for (int d = 0; d < Sh::S; ++d) issue(min(u0 + d, u1 - 1), d);
+  wait_loads<COPIES * (Sh::S - 1)>();
+  block_barrier();
   read_sc(0);
   read(0, 0, 0);
   int st = 0;
 #pragma unroll 1
   for (int u = u0; u + 1 < u1; ++u) {
     quarters(st);
-    // Every operand of this stage has been read, or is in flight to its registers: the next stage
-    // is made sure of, this one's memory given to the one after it, and the last quarter is
-    // multiplied while the next stage's first is read.
-    store_sc(u + 1, st ^ 1);
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    // (Past the last stage that one again, and nobody reads it: a branch here would let the
-    // compiler move the multiplications of this stage behind it.)
-    issue(min(u + 2, u1 - 1), st);
-    load_sc(min(u + 2, u1 - 1));
+    // Once every wave has the last operands of this stage in registers, its memory goes to the
+    // stage S further on; the last quarter is multiplied while the next stage's first is read.
+    wait_loads<COPIES * (Sh::S - 2)>();
+    block_barrier();
+    issue(min(u + Sh::S, u1 - 1), st);
     u32x2 w[Sh::NB], x[Sh::MB];
 #pragma unroll
     for (int n = 0; n < Sh::NB; ++n) w[n] = sw[n];
 #pragma unroll
     for (int m = 0; m < Sh::MB; ++m) x[m] = sx[m];
-    st ^= 1;
+    st = st + 1 == Sh::S ? 0 : st + 1;
     multiply(std::integral_constant<int, 3>{}, w, x, [&] {
       read_sc(st);
       read(st, 0, 0);

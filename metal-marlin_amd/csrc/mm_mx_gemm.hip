@@ -1,7 +1,6 @@
 // C[M, N] = q(X) . W^T: X [M, K] fp32, fp16 or bf16 is quantized to MXFP4 (mm_mx.h), W is kept so,
 // words [N, K/8] and scales [N, K/32].  The cores are in mm_mx_gemm.h.
 #include <algorithm>
-#include <cstdlib>
 
 #include "mm_mx_gemm.h"
 #include "mmfp4.h"
@@ -79,6 +78,8 @@ k_mx_skinny_codes(const uint8_t* __restrict__ X, const uint8_t* __restrict__ XS,
 struct DenseSrc {
   const uint8_t *W, *S, *X, *XS;
   int K, kp, n_last, m_last;
+  size_t spitch, xpitch;
+  static constexpr bool BY_UNIT = true;
   MM_DEV uint32_t wrow(int r) const { return min(r, n_last); }
   MM_DEV uint32_t xrow(int r) const { return min(r, m_last); }
 };
@@ -94,23 +95,26 @@ MM_DEV void tile_of(int id, int gm, int gn, int grp, int& tm, int& tn) {
   tn = in / rows;
 }
 
+// grid (tiles, splits of K): with more than one, each split's fp32 sums go to C, sum_pitch(M * N)
+// apart.
 template <class Sh>
 __global__ void __launch_bounds__(Sh::NTHR)
 k_mx_tile(const uint8_t* __restrict__ X, const uint8_t* __restrict__ XS, int kp,
           const uint8_t* __restrict__ W, const uint8_t* __restrict__ S, void* __restrict__ C,
-          int out_type, int M, int N, int K, int gm, int gn, int grp) {
+          int out_type, int M, int N, int K, int gm, int gn, int grp, int per) {
   __shared__ __attribute__((aligned(16))) char smem[Sh::LDS];
   int tm, tn;
   tile_of(blockIdx.x, gm, gn, grp, tm, tn);
   const int m0 = tm * Sh::TM, n0 = tn * Sh::TN;
-  const DenseSrc src{W + (size_t)n0 * (K / 2), S + (size_t)n0 * (K / BLOCK),
-                     X + (size_t)m0 * (kp / 2), XS + (size_t)m0 * (kp / BLOCK),
-                     K, kp, N - 1 - n0, M - 1 - m0};
+  const DenseSrc src{W + (size_t)n0 * (K / 2), S + (size_t)n0 * 8, X + (size_t)m0 * (kp / 2),
+                     XS + (size_t)m0 * 8, K, kp, N - 1 - n0, M - 1 - m0, unit_pitch(N), unit_pitch(M)};
   f32x16 acc[Sh::NB][Sh::MB];
-  tile_loop<Sh>(src, 0, (K + UNIT - 1) / UNIT, smem, acc);
+  const int u0 = blockIdx.y * per, u1 = min((K + UNIT - 1) / UNIT, u0 + per);
+  tile_loop<Sh>(src, u0, u1, smem, acc);
   __syncthreads();
+  const size_t base = blockIdx.y * sum_pitch((size_t)M * N);
   tile_out<Sh>(acc, smem, C, out_type, M - m0, n0, N,
-               [=](int m) { return (size_t)(m0 + m) * N; });
+               [=](int m) { return base + (size_t)(m0 + m) * N; });
 }
 
 constexpr int SKINNY_M = 16;    // rows that the kernel may quantize itself
@@ -141,32 +145,105 @@ void launch_skinny(const void* X, const uint32_t* W, const uint8_t* S, void* C, 
   else launch_skinny_as<T, 1, 8, 2, 4>(X, W, S, C, out_type, M, N, K, st);
 }
 
-template <int MT, int NT, int D>
+constexpr int CODES_WAVES = 8, LDS_BYTES = 160 * 1024, CUS = 256;
+template <int MT>
+long codes_lds(int K) {
+  return Ring<1, MT, CODES_WAVES, 1>::BYTES + (long)whole_kib(16 * (K / BLOCK)) +
+         whole_kib(16 * MT * (int)(padded(K) / BLOCK));
+}
+template <int MT>
 void launch_codes(const uint8_t* xq, const uint8_t* xs, int kp, const uint32_t* W, const uint8_t* S,
                   void* C, int out_type, int M, int N, int K, hipStream_t st) {
-  hipLaunchKernelGGL((k_mx_skinny_codes<MT, NT, 8, D>),
-                     dim3(mm_cdiv(N, 16 * NT), mm_cdiv(M, 16 * MT)), dim3(512),
-                     (Ring<NT, MT, 8, D>::BYTES + whole_kib(16 * NT * (K / BLOCK)) +
-                      whole_kib(16 * MT * (kp / BLOCK))),
-                     st, xq, xs, kp, (const uint8_t*)W, S, C, out_type, M, N, K);
+  hipLaunchKernelGGL((k_mx_skinny_codes<MT, 1, CODES_WAVES, 1>), dim3(mm_cdiv(N, 16), mm_cdiv(M, 16 * MT)),
+                     dim3(CODES_WAVES * 64), codes_lds<MT>(K), st, xq, xs, kp, (const uint8_t*)W, S, C,
+                     out_type, M, N, K);
+}
+// Rows that stream the weights, from codes: 16, 32 or 64 a block, as long as a block's scales fit
+// LDS.  More than 32 rows only while the CUs hold all blocks at once, two each: us, streamed against
+// tiles, M = 64 4096 -> 4096 9.0 / 10.8, 14336 -> 4096 14.0 / 17.5, 4096 -> 14336 24.4 / 14.1.
+bool streams(int M, int N, int K) {
+  if (M > CODES_M || (M > 32 && N > 2 * CUS * 16)) return false;
+  return (M <= 16 ? codes_lds<1>(K) : M <= 32 ? codes_lds<2>(K) : codes_lds<4>(K)) <= LDS_BYTES;
+}
+
+// Tiles.  A block is alone on its CU, or (64 x 64) one of two that take turns; a stage of it takes
+// `stage` us and its beginning and end `ends`, measured at 65 .. 2048 rows of 14336 x 4096, 4096 x
+// 14336 and 4096 x 4096.  The estimate picked the fastest tile and split of those (65, 128, 333,
+// 512, 1024, 2048 rows: 14, 15, 26, 28, 42, 78 us; 17, 18, 31, 34, 50, 85; 11, 11, 14, 16, 22, 31;
+// the largest tiles alone: 34 .. 78; 89 .. 103; 33 .. 39).
+using Tile256 = Tile<4, 2, 2, 4, 2>;       // 256 x 256, 8 waves
+using Tile128w = Tile<2, 4, 2, 2, 3>;      // 128 x 256, 8 waves
+using Tile128 = Tile<4, 2, 1, 2, 4>;       // 128 x 128, 8 waves
+using Tile64w = Tile<2, 4, 1, 1, 5>;       // 64 x 128, 8 waves
+using Tile64 = Tile<2, 2, 1, 1, 4>;        // 64 x 64, 4 waves
+struct Cost {
+  int tm, tn;
+  float stage, ends;
+};
+constexpr Cost COSTS[] = {{256, 256, 1.75f, 6.0f}, {128, 256, 1.2f, 4.0f}, {128, 128, 0.7f, 3.0f},
+                          {64, 128, 0.45f, 2.5f}, {64, 64, 0.28f, 2.0f}};
+constexpr int MAX_SPLITS = 8;
+
+struct Plan {
+  int tile;           // which tiles; -1: a kernel that streams the weights
+  int splits, per;    // splits of K and their stages
+};
+// With few tiles K is split, and the splits' sums are joined by another launch: 2.5 us and their
+// bytes at about 3 TB/s.
+Plan plan_of(int M, int N, int K) {
+  const int stages = mm_cdiv(K, UNIT);
+  if (streams(M, N, K)) return Plan{-1, 1, stages};
+  Plan best{0, 1, stages};
+  float least = 0;
+  for (int t = 0; t < 5; ++t) {
+    const long tiles = (long)mm_cdiv(M, COSTS[t].tm) * mm_cdiv(N, COSTS[t].tn);
+    for (int s = 1; s <= MAX_SPLITS && (s == 1 || (tiles * s <= 2 * CUS && stages >= 4 * s)); ++s) {
+      const int per = mm_cdiv(stages, s), splits = mm_cdiv(stages, per);
+      float us = (float)((tiles * splits + CUS - 1) / CUS) * (per * COSTS[t].stage + COSTS[t].ends);
+      if (splits > 1) us += 2.5f + (float)M * N * 4 * (splits + 1) / 3e6f;
+      if (least == 0 || us < least) {
+        least = us;
+        best = Plan{t, splits, per};
+      }
+    }
+  }
+  return best;
 }
 
 template <class Sh>
-void launch_tile(const uint8_t* xq, const uint8_t* xs, int kp, const uint32_t* W, const uint8_t* S,
-                 void* C, int out_type, int M, int N, int K, hipStream_t st) {
+void launch_tile(const Plan& p, const uint8_t* xq, const uint8_t* xs, int kp, const uint32_t* W,
+                 const uint8_t* S, void* C, int out_type, int M, int N, int K, hipStream_t st) {
   const int gm = mm_cdiv(M, Sh::TM), gn = mm_cdiv(N, Sh::TN);
-  hipLaunchKernelGGL((k_mx_tile<Sh>), dim3((unsigned)(gm * gn)), dim3(Sh::NTHR), 0, st, xq, xs, kp,
-                     (const uint8_t*)W, S, C, out_type, M, N, K, gm, gn, std::min(gm, 4));
+  hipLaunchKernelGGL((k_mx_tile<Sh>), dim3((unsigned)(gm * gn), p.splits), dim3(Sh::NTHR), 0, st, xq,
+                     xs, kp, (const uint8_t*)W, S, C, out_type, M, N, K, gm, gn,
+                     std::min(gm, 4), p.per);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+// x's codes and scales; for tiles W's scales by units; the splits' sums.
+struct Space {
+  size_t xs, scales, part, total;
+};
+Space space_of(const Plan& p, int M, int N, int K) {
+  Space s;
+  const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  s.xs = COUNTERS + codes_bytes(M, K);
+  if (p.tile < 0) {
+    s.scales = s.part = s.total = COUNTERS + up(packed_bytes(M, K));
+    return s;
+  }
+  s.scales = s.xs + mm_cdiv(K, UNIT) * unit_pitch(M);
+  s.part = s.scales + mm_cdiv(K, UNIT) * unit_pitch(N);
+  s.total = s.part + (p.splits > 1 ? p.splits * sum_pitch((size_t)M * N) * sizeof(float) : 0);
+  return s;
+}
+
 }  // namespace
 
 extern "C" size_t mm_mxfp4_gemm_workspace_bytes(int M, int N, int K) {
-  (void)N;
-  if (M <= 0 || K <= 0 || quantizes_itself(M, K)) return 0;
-  return COUNTERS + packed_bytes(M, K);
+  if (M <= 0 || N <= 0 || K <= 0 || quantizes_itself(M, K)) return 0;
+  return space_of(plan_of(M, N, K), M, N, K).total;
 }
 
 extern "C" int mm_mxfp4_gemm(const void* X, int type, const uint32_t* W, const uint8_t* S, void* C,
@@ -178,6 +255,8 @@ extern "C" int mm_mxfp4_gemm(const void* X, int type, const uint32_t* W, const u
   MM_CHECK_ARG(type >= F32 && type <= BF16 && out_type >= F32 && out_type <= BF16,
                "mm_mxfp4_gemm: unknown type %d or %d", type, out_type);
   if (M == 0) return 0;
+  MM_CHECK_ARG(K < (1 << 24) && (size_t)mm_cdiv(M, 64) * mm_cdiv(N, 64) < ((size_t)1 << 31),
+               "mm_mxfp4_gemm: M=%d, N=%d, K=%d is too large", M, N, K);
   MM_CHECK_ARG(X && W && S && C && aligned16(X) && aligned16(W) && aligned16(S) && aligned16(C),
                "mm_mxfp4_gemm: X, W, scales and C must be 16-byte aligned and nothing null");
   const size_t need = mm_mxfp4_gemm_workspace_bytes(M, N, K);
@@ -193,25 +272,31 @@ extern "C" int mm_mxfp4_gemm(const void* X, int type, const uint32_t* W, const u
     return 0;
   }
   const int kp = (int)padded(K);
-  uint8_t* const xq = (uint8_t*)ws + COUNTERS;
-  uint8_t* const xs = xq + codes_bytes(M, K);
-  if (const int rc = launch_quantize(X, type, M, K, kp, (uint32_t*)xq, xs, st)) return rc;
-  if (M <= CODES_M) {
-    if (M <= 16) launch_codes<1, 1, 1>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
-    else if (M <= 32) launch_codes<2, 1, 1>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
-    else launch_codes<4, 1, 1>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
+  const Plan p = plan_of(M, N, K);
+  const Space sp = space_of(p, M, N, K);
+  uint8_t *const xq = (uint8_t*)ws + COUNTERS, *const xs = (uint8_t*)ws + sp.xs;
+  if (p.tile < 0) {
+    if (const int rc = launch_quantize(X, type, M, K, kp, (uint32_t*)xq, xs, st)) return rc;
+    if (M <= 16) launch_codes<1>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
+    else if (M <= 32) launch_codes<2>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
+    else launch_codes<4>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
     MM_CHECK_LAUNCH("mm_mxfp4_gemm");
     return 0;
   }
-  const long big = (long)mm_cdiv(M, 256) * mm_cdiv(N, 256);
-  static const int cfg = getenv("MX_CFG") ? atoi(getenv("MX_CFG")) : 0;
-  if (cfg == 1) launch_tile<Tile<2, 2, 4, 4>>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
-  else if (cfg == 2) launch_tile<Tile<2, 2, 2, 2>>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
-  else if (cfg == 3) launch_tile<Tile<2, 2, 2, 4>>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
-  else if (cfg == 4) launch_tile<Tile<2, 2, 1, 4>>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
-  else if (cfg == 5) launch_tile<Tile<2, 4, 2, 2>>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
-  else if (big >= 200) launch_tile<Tile<4, 2, 2, 4>>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
-  else launch_tile<Tile<2, 2, 2, 2>>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
+  uint8_t* const s = (uint8_t*)ws + sp.scales;
+  if (const int rc = launch_quantize_units(X, type, M, K, kp, (uint32_t*)xq, xs, S, N, s, st)) return rc;
+  void* const to = p.splits > 1 ? (void*)((char*)ws + sp.part) : C;
+  const int to_type = p.splits > 1 ? (int)F32 : out_type;
+  const auto run = [&](auto sh) {
+    launch_tile<decltype(sh)>(p, xq, xs, kp, W, s, to, to_type, M, N, K, st);
+  };
+  switch (p.tile) {
+    case 0: run(Tile256{}); break;
+    case 1: run(Tile128w{}); break;
+    case 2: run(Tile128{}); break;
+    case 3: run(Tile64w{}); break;
+    default: run(Tile64{}); break;
+  }
   MM_CHECK_LAUNCH("mm_mxfp4_gemm");
-  return 0;
+  return p.splits > 1 ? launch_sum((const float*)to, p.splits, (size_t)M * N, C, out_type, st) : 0;
 }

@@ -136,9 +136,10 @@ k_mx_moe_down(const uint8_t* __restrict__ hw, const uint8_t* __restrict__ hs, in
 // rows of the gate and the same 32 of up (I rows on).
 struct GroupSrc {
   const uint8_t *W, *S, *X, *XS;
-  int K, kp;
+  int K, kp, ks;
   const int32_t* sorted;    // null: rows of x in sorted order
   int k, m0, m_last, n0, n_last, half;
+  static constexpr bool BY_UNIT = false;
   MM_DEV uint32_t wrow(int r) const {
     if (half == 0) return min(n0 + r, n_last);
     return min(n0 + r / 64 * 32 + r % 32, half - 1) + (r % 64 / 32) * half;
@@ -154,8 +155,8 @@ struct GroupSrc {
 template <class Sh, bool ACT>
 __global__ void __launch_bounds__(Sh::NTHR)
 k_mx_moe_tile(const uint8_t* __restrict__ X, const uint8_t* __restrict__ XS, int kp,
-              const uint8_t* __restrict__ W, const uint8_t* __restrict__ S, Rows rows, int E, int N,
-              int K, int gn, int np, void* __restrict__ y, int type, uint32_t* __restrict__ hw,
+              const uint8_t* __restrict__ W, const uint8_t* __restrict__ S, int ks, Rows rows, int E,
+              int N, int K, int gn, int np, void* __restrict__ y, int type, uint32_t* __restrict__ hw,
               uint8_t* __restrict__ hs) {
   __shared__ __attribute__((aligned(16))) char smem[Sh::LDS];
   static_assert(Sh::LDS >= (MAX_E + 1) * 4, "the prefix sums use the tiles' memory");
@@ -196,7 +197,7 @@ k_mx_moe_tile(const uint8_t* __restrict__ X, const uint8_t* __restrict__ XS, int
   const int m0 = __builtin_amdgcn_readfirstlane(rows.offsets[e] + (tile - tp[e]) * Sh::TM);
   __syncthreads();
   const int half = ACT ? N / 2 : 0, n0 = bx * (ACT ? Sh::TN / 2 : Sh::TN);
-  const GroupSrc src{W + (size_t)e * N * (K / 2), S + (size_t)e * N * (K / BLOCK), X, XS, K, kp,
+  const GroupSrc src{W + (size_t)e * N * (K / 2), S + (size_t)e * N * ks, X, XS, K, kp, ks,
                      ACT ? rows.sorted : nullptr, rows.k, m0, r1 - 1, n0, N - 1, half};
   f32x16 acc[Sh::NB][Sh::MB];
   if (!ACT || n0 < half) tile_loop<Sh>(src, 0, (K + UNIT - 1) / UNIT, smem, acc);
@@ -294,14 +295,20 @@ void launch_gate_up(const void* X, const uint8_t* W, const uint8_t* S, Rows rows
 }
 
 struct Scratch {
-  size_t sort, xq, hq, y, total;
+  size_t sort, xq, gs, ds, hq, y, total;
 };
 Scratch scratch_of(int T, int k, int E, int H, int I, int type) {
   const size_t R = (size_t)T * k;
+  const bool tiles = takes_tiles((long)R, E, H);
+  const auto anew = [&](size_t rows, int K) {      // scales that the tiles take from a copy
+    return tiles && scale_stride(K) != K / BLOCK ? up(rows * scale_stride(K)) : 0;
+  };
   Scratch s;
   s.sort = 0;
   s.xq = up((E + 1 + 2 * R) * sizeof(int32_t));
-  s.hq = s.xq + (takes_tiles((long)R, E, H) ? up(packed_bytes(T, H)) : 0);
+  s.gs = s.xq + (tiles ? up(packed_bytes(T, H)) : 0);
+  s.ds = s.gs + anew((size_t)E * 2 * I, H);
+  s.hq = s.ds + anew((size_t)E * H, I);
   s.y = s.hq + up(packed_bytes(R, I));
   s.total = s.y + up(R * H * (type == F32 ? 4 : 2));
   return s;
@@ -358,14 +365,27 @@ extern "C" int mm_moe_mlp_mxfp4(const void* X, int type, const void* expert_ids,
     uint8_t* const xs = xq + codes_bytes(T, H);
     if (const int rc = launch_quantize(X, type, T, H, hp, (uint32_t*)xq, xs, st)) return rc;
     using Sh = Tile<2, 2, 1, 2>;
+    const uint8_t *gs = Sgu, *ds = Sdn;
+    if (scale_stride(H) != H / BLOCK) {
+      uint8_t* const s = (uint8_t*)base + sc.gs;
+      if (const int rc = launch_pad_scales(gs, (size_t)E * 2 * I, H / BLOCK, scale_stride(H), s, st))
+        return rc;
+      gs = s;
+    }
+    if (scale_stride(I) != I / BLOCK) {
+      uint8_t* const s = (uint8_t*)base + sc.ds;
+      if (const int rc = launch_pad_scales(ds, (size_t)E * H, I / BLOCK, scale_stride(I), s, st))
+        return rc;
+      ds = s;
+    }
     const long tiles = (R + Sh::TM - 1) / Sh::TM + std::min(E, R);
     const int g1 = mm_cdiv(ip, Sh::TN / 2), g2 = mm_cdiv(H, Sh::TN);
     MM_CHECK_ARG(tiles * std::max(g1, g2) < (1L << 30), "mm_moe_mlp_mxfp4: too many tiles");
     hipLaunchKernelGGL((k_mx_moe_tile<Sh, true>), dim3((unsigned)((tiles * g1 + 7) / 8 * 8)),
-                       dim3(Sh::NTHR), 0, st, xq, xs, hp, gw, Sgu, rows, E, 2 * I, H, g1, ip,
+                       dim3(Sh::NTHR), 0, st, xq, xs, hp, gw, gs, scale_stride(H), rows, E, 2 * I, H, g1, ip,
                        nullptr, type, hw, hs);
     hipLaunchKernelGGL((k_mx_moe_tile<Sh, false>), dim3((unsigned)((tiles * g2 + 7) / 8 * 8)),
-                       dim3(Sh::NTHR), 0, st, (const uint8_t*)hw, hs, ip, dw, Sdn, rows, E, H, I,
+                       dim3(Sh::NTHR), 0, st, (const uint8_t*)hw, hs, ip, dw, ds, scale_stride(I), rows, E, H, I,
                        g2, 0, y, type, nullptr, nullptr);
   } else {
     if (type == F32) launch_gate_up<F32>(X, gw, Sgu, rows, R, E, H, I, hw, hs, st);
