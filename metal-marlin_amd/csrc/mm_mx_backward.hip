@@ -4,12 +4,14 @@
 // The contraction runs along N, across the rows of W, whose scales change from row to row: the
 // scaled matrix instructions cannot take them.  Every MXFP4 value is a bf16 number, though (2 bits
 // of E2M1 and bf16 has E8M0's exponents), so weights are converted exactly, 64 rows of a stage at
-// a time, into an LDS tile [n][k], from which ds_read_b64_tr_b16 takes columns as 32x32x16 bf16
-// operands.  dY is bf16, or the exact sum of bf16 terms: fp16 is two of them (11 bits in 8 + 8),
-// fp32 three (24 bits), each of which is multiplied: products are exact, sums fp32, rounded once.
+// a time, into an LDS tile [n][k], from which ds_read_b64_tr_b16 takes columns as 32x32x16
+// operands.  bf16 dY is multiplied as it is.  fp16 dY is, too, in stages whose weights are normal
+// fp16 numbers, as those of a trained matrix are; in others it is two bf16 terms (11 bits in 8 +
+// 8).  fp32 is three (24 bits).  Products are exact, sums fp32, rounded once.
 //
-// Bound by the matrix cores and LDS together; 16-bit conversions (16 per 32 weights) are small
-// beside them from 64 rows of dY on.
+// Bound by LDS and the matrix cores in turn: a stage of a 128 x 256 tile reads 128 KiB of operands
+// and writes 58, about 0.5 us, and multiplies for 0.43; it takes 1.17 (2048 x 14336 x 4096: 268 us
+// of bf16, 0.9 PFLOP/s; 324 of fp16, 588 with two terms throughout).
 #include <algorithm>
 
 #include "mm_mx_gemm.h"
@@ -27,26 +29,34 @@ typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 __device__ __attribute__((aligned(16))) const uint32_t mx_zeros[4] = {0, 0, 0, 0};
 
 // WK x WM waves of 32 KB x 32 MB each.  A stage is 128 bytes of every row of dY: BN = 64 columns
-// (32 of fp32).
+// (32 of fp32), and as many rows of W.  LDS holds three stages of dY, three of W's words and scales
+// and two of converted weights: what is copied has two stages' time to arrive.
 template <int T, int WK_, int WM_, int KB_, int MB_>
 struct GradTile {
   static constexpr int WK = WK_, WM = WM_, KB = KB_, MB = MB_;
+  static constexpr int WN = WK, NB = KB;                  // as the results' columns
   static constexpr int NWAVE = WK * WM, NTHR = NWAVE * 64;
   static constexpr int TK = WK * KB * 32, TM = WM * MB * 32;
   static constexpr int BN = 128 / kBytes<T>, STEPS = BN / 16;
-  static constexpr int A = TM * 128, B = BN * TK * 2;     // bytes of a stage of dY and of W
-  static constexpr int LDS = 2 * (A + B);
-  static constexpr int IT = TM / 8 / NWAVE;               // copies of dY per wave and stage
   static constexpr int BLOCKS = BN * TK / 32;             // of W per stage
-  static constexpr int WIT = (BLOCKS + NTHR - 1) / NTHR;  // of those per thread
+  static constexpr int A = TM * 128, B = BN * TK * 2;     // bytes of a stage of dY and of W in bf16
+  static constexpr int WP = BLOCKS / 64, SP = (BLOCKS + 255) / 256;   // copies of words, of scales
+  static constexpr int RAW = WP * 1024 + SP * 256;
+  static constexpr int STAGES = 3 * (A + RAW) + 2 * B, OUT = NWAVE * 32 * (KB * 128 + 16);
+  static constexpr int LDS = (STAGES > OUT ? STAGES : OUT) + 16;      // and which stages are wide
+  static constexpr int IT = TM / 8 / NWAVE, WIT = (WP + NWAVE - 1) / NWAVE,
+                       SIT = (SP + NWAVE - 1) / NWAVE;    // copies per wave and stage
+  static constexpr int COPIES = IT + WIT + SIT;
   static constexpr int TERMS = T == BF16 ? 1 : (T == F16 ? 2 : 3);
-  static_assert(TM % (8 * NWAVE) == 0 && NWAVE % 2 == 0, "copies per wave");
+  static_assert(TM % (8 * NWAVE) == 0 && NWAVE % 2 == 0 && BLOCKS <= NTHR && BLOCKS % 64 == 0,
+                "copies per wave, blocks per thread");
 };
 
 struct Grad {
   const uint8_t *dY, *W, *S;
   void* out;           // dX, or (split) fp32 partial sums [splits, M, K]
-  int out_type, M, N, K, ldy, stages, per;   // ldy: row stride of dY; per: stages of a split
+  // ldy: row stride of dY; ks: of the scales, a multiple of 4; per: stages of a split
+  int out_type, M, N, K, ldy, ks, stages, per;
 };
 
 // Columns n .. n + 7 of a row of dY as bf16 terms whose sum they are: each term is the leading 8
@@ -88,18 +98,27 @@ MM_DEV void terms(const char* p0, const char* p1, bf16x8 (&t)[T == BF16 ? 1 : (T
   }
 }
 
+// Weights 2 I, 2 I + 1 of a word as fp16 or bf16.
+template <bool HALF, int I>
+MM_DEV uint32_t two(uint32_t w, float s) {
+  if constexpr (HALF)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, I));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, I));
+}
+
 template <class Sh, int T>
 __global__ void __launch_bounds__(Sh::NTHR) k_mx_grad(Grad a, int gm, int gk) {
   __shared__ __attribute__((aligned(16))) char smem[Sh::LDS];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wk = wave / Sh::WM, wm = wave % Sh::WM, l32 = lane & 31, h = lane >> 5;
+  const int wm = wave / Sh::WK, wk = wave % Sh::WK, l32 = lane & 31, h = lane >> 5;
   // each XCD takes a stretch of tiles, row tiles innermost: they share their weights
   const int total = gm * gk, q = total >> 3, rem = total & 7, xcd = blockIdx.x & 7;
   const int lin = xcd * q + min(xcd, rem) + (int)(blockIdx.x >> 3);
   const int m0 = lin % gm * Sh::TM, k0 = lin / gm * Sh::TK;
   const int u0 = blockIdx.y * a.per, u1 = min(a.stages, u0 + a.per);
-  const int kb = a.K / BLOCK, row_bytes = (a.N * kBytes<T> + 15) / 16 * 16;
+  const int row_bytes = (a.N * kBytes<T> + 15) / 16 * 16;
 
   const uint8_t* src[Sh::IT];
 #pragma unroll
@@ -108,50 +127,79 @@ __global__ void __launch_bounds__(Sh::NTHR) k_mx_grad(Grad a, int gm, int gk) {
     src[i] = a.dY + (size_t)min(m0 + r, a.M - 1) * a.ldy * kBytes<T>;
   }
   const int at = 16 * ((lane & 7) ^ ((wave * 4 + (lane >> 4)) & 7));
-  auto issue = [&](int u, int st) {
+  // Stages past the last one: that one again, which nobody uses.
+  auto issue_dy = [&](int v, int slot) {
+    const int u = min(v, u1 - 1);
 #pragma unroll
     for (int i = 0; i < Sh::IT; ++i) {
       const int b = u * 128 + at;
       copy16(b < row_bytes ? src[i] + b : (const uint8_t*)mx_zeros,
-             smem + st * Sh::A + (i * Sh::NWAVE + wave) * 1024);
+             smem + slot * Sh::A + (i * Sh::NWAVE + wave) * 1024);
     }
   };
-  // Thread t converts blocks t, t + NTHR, .. of a stage: row t / (TK / 32), block t % (TK / 32).
+  // Block b of a stage is block b % RB of row b / RB; rows past N meet zeros of dY, blocks past K
+  // are not stored.
   constexpr int RB = Sh::TK / 32;
-  u32x4 wreg[Sh::WIT];
-  uint32_t sreg[Sh::WIT];
-  auto load = [&](int u) {
+  char* const raw = smem + 3 * Sh::A;
+  char* const conv = raw + 3 * Sh::RAW;
+  auto issue_w = [&](int v, int slot) {
+    const int u = min(v, u1 - 1);
 #pragma unroll
-    for (int i = 0; i < Sh::WIT; ++i) {
-      const int b = tid + i * Sh::NTHR;
-      // rows past N meet zeros of dY, blocks past K are not stored
-      const size_t n = min(u * Sh::BN + b / RB, a.N - 1);
-      const int c = min(k0 / 32 + b % RB, kb - 1);
-      wreg[i] = *(const u32x4*)(a.W + n * (a.K / 2) + c * 16);
-      sreg[i] = a.S[n * kb + c];
+    for (int i = 0; i < Sh::WIT; ++i) {      // waves to spare copy the last piece again
+      const int c = min(i * Sh::NWAVE + wave, Sh::WP - 1), b = c * 64 + lane;
+      const int n = min(u * Sh::BN + b / RB, a.N - 1);
+      copy16(a.W + (size_t)n * (a.K / 2) + min(k0 / 2 + b % RB * 16, a.K / 2 - 16),
+             raw + slot * Sh::RAW + c * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < Sh::SIT; ++i) {
+      const int c = min(i * Sh::NWAVE + wave, Sh::SP - 1), b = min((c * 64 + lane) * 4, Sh::BLOCKS - 4);
+      const int n = min(u * Sh::BN + b / RB, a.N - 1);
+      copy4(a.S + (size_t)n * a.ks + min(k0 / 32 + b % RB, a.ks - 4),
+            raw + slot * Sh::RAW + Sh::WP * 1024 + c * 256);
     }
   };
-  // [n][k] in 64-byte blocks, block c of row n at c ^ (n % 4): the 4 rows that a transposed read
-  // takes lie in different banks.
-  auto store = [&](int st) {
+  // Thread b converts block b.  [n][k] in 64-byte blocks, block c of row n at c ^ (n % 4): the 4
+  // rows that a transposed read takes lie in different banks.
+  const bool idle = Sh::BLOCKS != Sh::NTHR && tid >= Sh::BLOCKS;
+  auto store = [&](u32x4 wv, uint32_t code, int half_of, auto half) __attribute__((always_inline)) {
+    constexpr bool HALF = decltype(half)::value;
+    if (idle) return;
+    const int n = tid / RB, c = tid % RB;
+    char* const d = conv + half_of * Sh::B + n * (Sh::TK * 2) + (c ^ (n & 3)) * 64;
+    const float s = scale_of(code);
+    const uint32_t nan = !HALF && code == 255u ? 0x7fc07fc0u : 0u;
+    // lanes of one round write all of the 16 pieces that banks tell apart
+    const int turn = (tid >> 2) & 3;
+    if (turn & 1) wv = u32x4{wv[1], wv[2], wv[3], wv[0]};
+    if (turn & 2) wv = u32x4{wv[2], wv[3], wv[0], wv[1]};
 #pragma unroll
-    for (int i = 0; i < Sh::WIT; ++i) {
-      const int b = tid + i * Sh::NTHR;
-      if (Sh::BLOCKS % Sh::NTHR != 0 && b >= Sh::BLOCKS) break;
-      const int n = b / RB, c = b % RB;
-      char* const d = smem + 2 * Sh::A + st * Sh::B + n * (Sh::TK * 2) + (c ^ (n & 3)) * 64;
-      const float s = scale_of(sreg[i]);
-      const uint32_t nan = sreg[i] == 255u ? 0x7fc07fc0u : 0u;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t w = wreg[i][j];
-        *(u32x4*)(d + 16 * j) =
-            u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0)) | nan,
-                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1)) | nan,
-                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2)) | nan,
-                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3)) | nan};
-      }
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w = wv[j];
+      lds_store16(d + 16 * ((j + turn) & 3), u32x4{two<HALF, 0>(w, s) | nan, two<HALF, 1>(w, s) | nan,
+                                    two<HALF, 2>(w, s) | nan, two<HALF, 3>(w, s) | nan});
     }
+  };
+  // A stage of fp16 dY is wide, two bf16 terms, if one of its weights is no normal fp16 number: 0.5
+  // .. 6 times 2^-13 .. 2^13, or zeros under any scale but NaN.  Whoever finds one leaves the
+  // stage's number in its half's word.
+  int* const wide = (int*)(smem + Sh::LDS - 16);
+  constexpr std::true_type HALF{};
+  constexpr std::false_type BF{};
+  const auto convert = [&](int u, int slot, int half_of) __attribute__((always_inline)) {
+    const char* const r = raw + slot * Sh::RAW;
+    const int b = min(tid, Sh::BLOCKS - 1);
+    const u32x4 wv = *(const u32x4*)(r + b * 16);
+    const uint32_t code = *(const uint8_t*)(r + Sh::WP * 1024 + b);
+    if constexpr (T == F16) {
+      const u32x4 m = wv & 0x77777777u;
+      if (code - 114u > 26u && (code == 255u || (m.x | m.y | m.z | m.w) != 0u))
+        lds_store4(wide + half_of, (uint32_t)u);
+      stores_done();
+      block_barrier();
+      if (wide[half_of] != u) return store(wv, code, half_of, HALF);
+    }
+    store(wv, code, half_of, BF);
   };
   f32x16 acc[Sh::KB][Sh::MB];
 #pragma unroll
@@ -164,9 +212,10 @@ __global__ void __launch_bounds__(Sh::NTHR) k_mx_grad(Grad a, int gm, int gk) {
   // A transposed read: lane s of a group of 16 points at row s / 4, columns 4 (s % 4) on, of a
   // 4 x 16 block, and gets column s of it.  Groups 2 h + g take rows 8 h (+ 4) and columns 16 g.
   const int tr_n = 8 * h + (lane & 15) / 4, tr_c = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-  auto compute = [&](int st) {
-    const char* const dA = smem + st * Sh::A;
-    const char* const dB = smem + 2 * Sh::A + st * Sh::B;
+  auto compute = [&](int slot, int half_of, auto half) __attribute__((always_inline)) {
+    constexpr bool HALF = decltype(half)::value;
+    const char* const dA = smem + slot * Sh::A;
+    char* const dB = conv + half_of * Sh::B;
 #pragma unroll
     for (int j = 0; j < Sh::STEPS; ++j) {
       bf16x8 wv[Sh::KB];
@@ -187,6 +236,14 @@ __global__ void __launch_bounds__(Sh::NTHR) k_mx_grad(Grad a, int gm, int gk) {
       for (int m = 0; m < Sh::MB; ++m) {
         const int r = (wm * Sh::MB + m) * 32 + l32, sw = (r >> 1) & 7;
         const char* const row = dA + r * 128;
+        if constexpr (HALF) {
+          const f16x8 v = *(const f16x8*)(row + 16 * ((2 * j + h) ^ sw));
+#pragma unroll
+          for (int k = 0; k < Sh::KB; ++k)
+            acc[k][m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, wv[k]), v,
+                                                               acc[k][m], 0, 0, 0);
+          continue;
+        }
         bf16x8 t[Sh::TERMS];
         if constexpr (T == F32)
           terms<T>(row + 16 * ((4 * j + 2 * h) ^ sw), row + 16 * ((4 * j + 2 * h + 1) ^ sw), t);
@@ -201,62 +258,82 @@ __global__ void __launch_bounds__(Sh::NTHR) k_mx_grad(Grad a, int gm, int gk) {
     }
   };
   if (u0 < u1) {
-    issue(u0, 0);
-    load(u0);
-    store(0);
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    int st = 0;
-    for (int u = u0; u + 1 < u1; ++u) {
-      issue(u + 1, st ^ 1);
-      load(u + 1);
-      __builtin_amdgcn_sched_barrier(0);
-      compute(st);
-      store(st ^ 1);
-      __builtin_amdgcn_s_waitcnt(0);
-      __syncthreads();
-      st ^= 1;
+    if (T == F16 && tid < 2) wide[tid] = -1;
+    issue_w(u0, 0);
+    issue_dy(u0, 0);
+    issue_w(u0 + 1, 1);
+    issue_dy(u0 + 1, 1);
+    issue_w(u0 + 2, 2);
+    wait_loads<2 * Sh::COPIES>();
+    stores_done();
+    block_barrier();
+    convert(u0, 0, 0);
+    int slot = 0, half_of = 0;
+#pragma unroll 1
+    for (int u = u0; u < u1; ++u) {
+      // dY of this stage, words of the next and this stage's converted weights are there, and all
+      // have done with the stage before
+      wait_loads<Sh::COPIES>();
+      stores_done();
+      block_barrier();
+      const int next = slot == 2 ? 0 : slot + 1;
+      issue_dy(u + 2, next == 2 ? 0 : next + 1);
+      issue_w(u + 3, slot);
+      convert(u + 1, next, half_of ^ 1);
+      if (T == F16 && wide[half_of] != u) compute(slot, half_of, HALF);
+      else compute(slot, half_of, BF);
+      slot = next;
+      half_of ^= 1;
     }
-    compute(st);
+    wait_loads<0>();
   }
-  const size_t base = (size_t)blockIdx.y * a.M * a.K;      // 0 unless split
-#pragma unroll
-  for (int m = 0; m < Sh::MB; ++m) {
-    const int mm = m0 + (wm * Sh::MB + m) * 32 + l32;
-    if (mm >= a.M) continue;
-#pragma unroll
-    for (int k = 0; k < Sh::KB; ++k)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int kk = k0 + (wk * Sh::KB + k) * 32 + 8 * g + 4 * h;
-        if (kk < a.K)                                       // K % 32 == 0: all four or none
-          store4(a.out, a.out_type, base + (size_t)mm * a.K + kk,
-                 f32x4{acc[k][m][4 * g], acc[k][m][4 * g + 1], acc[k][m][4 * g + 2],
-                       acc[k][m][4 * g + 3]});
-      }
-  }
+  __syncthreads();
+  const size_t base = blockIdx.y * sum_pitch((size_t)a.M * a.K);      // 0 unless split
+  tile_out<Sh>(acc, smem, a.out, a.out_type, a.M - m0, k0, a.K,
+               [=, K = a.K](int m) { return base + (size_t)(m0 + m) * K; });
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 constexpr size_t COUNTERS = 65536;
 
-// Splits of N: while the tiles leave CUs idle and every split keeps four stages.
-struct Plan {
-  int big, splits, per, stages;
+// Tiles of dX: a stage of the only block on a CU takes `one` us, of two that share it `two`, a
+// block's beginning and end `ends` (bf16; measured at 64 .. 2048 rows of 14336 x 4096, 4096 x 14336
+// and 4096 x 4096; fp16 takes 1.2 times as long, which changes no choice).
+struct Cost {
+  int tm, tk;
+  float one, two, ends;
 };
+constexpr Cost COSTS[] = {{128, 256, 1.2f, 2.4f, 4.0f}, {64, 128, 0.83f, 1.15f, 2.5f},
+                          {32, 128, 0.6f, 0.85f, 2.0f}};
+constexpr int CUS = 256, MAX_SPLITS = 16;
+
+struct Plan {
+  int tile, splits, per, stages;
+};
+// With few tiles N is split, and the splits' sums are joined by another launch: 2.5 us and their
+// bytes at about 3 TB/s.  us, best tile and split: 2048 x 14336 x 4096 268 (of 64 x 128 524, in two
+// splits 298), 509 x 4096 x 4096 35 in four (unsplit 79), 128 x 4096 x 4096 22 (30 of 128 x 256).
 Plan plan_of(int M, int N, int K, int type) {
-  Plan p;
-  const int bn = type == F32 ? 32 : 64;
-  p.stages = mm_cdiv(N, bn);
-  p.big = (long)mm_cdiv(M, 256) * mm_cdiv(K, 256) >= 200;
-  p.splits = 1;
-  if (!p.big) {
-    const long tiles = (long)mm_cdiv(M, M <= 32 ? 32 : 128) * mm_cdiv(K, 128);
-    p.splits = (int)std::max(1L, std::min({512 / std::max(1L, tiles), (long)p.stages / 4, 16L}));
+  Plan best{0, 1, 0, mm_cdiv(N, type == F32 ? 32 : 64)};
+  float least = 0;
+  for (int t = 0; t < 3; ++t) {
+    const Cost& c = COSTS[t];
+    const long tiles = (long)mm_cdiv(M, c.tm) * mm_cdiv(K, c.tk);
+    for (int s = 1; s <= MAX_SPLITS && (s == 1 || (tiles * s <= 2 * CUS && best.stages >= 2 * s)); ++s) {
+      const int per = mm_cdiv(best.stages, s), splits = mm_cdiv(best.stages, per);
+      const long blocks = tiles * splits, rest = blocks % (2 * CUS);
+      float us = (float)(blocks / (2 * CUS)) * (per * c.two + c.ends);
+      if (rest) us += per * (rest > CUS ? c.two : c.one) + c.ends;
+      if (splits > 1) us += 2.5f + (float)M * K * 4 * (splits + 1) / 3e6f;
+      if (least == 0 || us < least) {
+        least = us;
+        best.tile = t;
+        best.splits = splits;
+        best.per = per;
+      }
+    }
   }
-  p.per = mm_cdiv(p.stages, p.splits);
-  p.splits = mm_cdiv(p.stages, p.per);
-  return p;
+  return best;
 }
 
 template <int T, class Sh>
@@ -267,17 +344,29 @@ void launch(Grad a, const Plan& p, hipStream_t st) {
 }
 template <int T>
 void launch_t(const Grad& a, const Plan& p, hipStream_t st) {
-  if (p.big) launch<T, GradTile<T, 2, 4, 4, 2>>(a, p, st);
-  else if (a.M <= 32) launch<T, GradTile<T, 4, 1, 1, 1>>(a, p, st);
-  else launch<T, GradTile<T, 2, 2, 2, 2>>(a, p, st);
+  if (p.tile == 0) launch<T, GradTile<T, 4, 2, 2, 2>>(a, p, st);
+  else if (p.tile == 1) launch<T, GradTile<T, 4, 2, 1, 1>>(a, p, st);
+  else launch<T, GradTile<T, 4, 1, 1, 1>>(a, p, st);
+}
+
+// W's scales where they have to be laid out anew; the splits' sums.
+struct Space {
+  size_t part, total;
+};
+Space space_of(const Plan& p, int M, int N, int K) {
+  Space s;
+  const bool anew = scale_stride(K) != K / BLOCK;
+  s.part = COUNTERS + (anew ? ((size_t)N * scale_stride(K) + 255) / 256 * 256 : 0);
+  s.total = s.part + (p.splits > 1 ? p.splits * sum_pitch((size_t)M * K) * sizeof(float) : 0);
+  if (s.total == COUNTERS) s.total = 0;
+  return s;
 }
 
 }  // namespace
 
 extern "C" size_t mm_mxfp4_gemm_backward_workspace_bytes(int M, int N, int K, int type) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const Plan p = plan_of(M, N, K, type);
-  return p.splits > 1 ? COUNTERS + (size_t)p.splits * M * K * sizeof(float) : 0;
+  return space_of(plan_of(M, N, K, type), M, N, K).total;
 }
 
 extern "C" int mm_mxfp4_gemm_backward(const void* dY, int type, int ldy, const uint32_t* W,
@@ -293,17 +382,23 @@ extern "C" int mm_mxfp4_gemm_backward(const void* dY, int type, int ldy, const u
   MM_CHECK_ARG(N < (1 << 28) && K < (1 << 28), "mm_mxfp4_gemm_backward: N=%d or K=%d is too large",
                N, K);
   if (M == 0) return 0;
-  MM_CHECK_ARG(dY && W && S && dX && aligned16(dY) && aligned16(W) && aligned16(dX),
-               "mm_mxfp4_gemm_backward: dY, W and dX must be 16-byte aligned and nothing null");
+  MM_CHECK_ARG(dY && W && S && dX && aligned16(dY) && aligned16(W) && aligned16(S) && aligned16(dX),
+               "mm_mxfp4_gemm_backward: dY, W, scales and dX must be 16-byte aligned and nothing null");
   const Plan p = plan_of(M, N, K, type);
-  const size_t need = mm_mxfp4_gemm_backward_workspace_bytes(M, N, K, type);
-  MM_CHECK_ARG(need == 0 || (ws && aligned16(ws) && ws_bytes >= need),
+  const Space sp = space_of(p, M, N, K);
+  MM_CHECK_ARG(sp.total == 0 || (ws && aligned16(ws) && ws_bytes >= sp.total),
                "mm_mxfp4_gemm_backward: needs a workspace of %zu bytes, 16-byte aligned, got %zu",
-               need, ws_bytes);
+               sp.total, ws_bytes);
   const hipStream_t st = (hipStream_t)stream;
-  float* const part = p.splits > 1 ? (float*)((char*)ws + COUNTERS) : nullptr;
+  const int ks = scale_stride(K);
+  if (ks != K / BLOCK) {
+    uint8_t* const s = (uint8_t*)ws + COUNTERS;
+    if (const int rc = launch_pad_scales(S, N, K / BLOCK, ks, s, st)) return rc;
+    S = s;
+  }
+  float* const part = p.splits > 1 ? (float*)((char*)ws + sp.part) : nullptr;
   const Grad a{(const uint8_t*)dY, (const uint8_t*)W, S, part ? part : dX, part ? (int)F32 : out_type,
-               M, N, K, ldy, p.stages, p.per};
+               M, N, K, ldy, ks, p.stages, p.per};
   if (type == F32) launch_t<F32>(a, p, st);
   else if (type == F16) launch_t<F16>(a, p, st);
   else launch_t<BF16>(a, p, st);

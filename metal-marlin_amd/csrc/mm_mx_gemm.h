@@ -44,6 +44,9 @@ MM_DEV uint32_t lds_at(const void* p) {
 MM_DEV void lds_store4(void* p, uint32_t v) {
   asm volatile("ds_write_b32 %0, %1" ::"v"(lds_at(p)), "v"(v) : "memory");
 }
+MM_DEV void lds_store16(void* p, u32x4 v) {
+  asm volatile("ds_write_b128 %0, %1" ::"v"(lds_at(p)), "v"(v) : "memory");
+}
 MM_DEV void lds_store1(void* p, uint32_t v) {
   asm volatile("ds_write_b8 %0, %1" ::"v"(lds_at(p)), "v"(v) : "memory");
 }

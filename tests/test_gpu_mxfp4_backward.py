@@ -98,6 +98,30 @@ def test_range(dtype):
         assert float(off.max()) <= 0
 
 
+@pytest.mark.parametrize("m", [7, 150])
+def test_fp16_exponents(m):
+    """fp16 gradients down to the subnormal ones, and weights whose scales leave fp16's range in some
+    rows and columns only: each product is exact however a stage takes them."""
+    announce(f"mxfp4_gemm_backward fp16 exponents m={m}")
+    dy = normal(m, 640, dtype=torch.float16)
+    dy = torch.ldexp(dy.float(), -(torch.arange(640, device=DEV) % 24).float()).half()
+    w, s = weight(640, 512)
+    s[64:128, 3] = 113                       # one stage of one column tile
+    s[300, :] = 141
+    s[450:460, 9:] = 90
+    s[500:600, :8] = 0                       # zeros under the least scale
+    w[500:600, :32] = 0
+    rw = values(w, s)
+    ref = dy.double() @ rw
+    dx = mmfp4.mxfp4_gemm_backward(dy, w, s, torch.float32)
+    check(dx, ref, bound_of(dy, rw, ref, torch.float32), f"m={m}")
+    tiny = torch.full((m, 640), 2.0 ** -24, dtype=torch.float16, device=DEV)     # the smallest one
+    one = torch.full_like(s, 127)
+    ref = tiny.double() @ values(w, one)
+    dx = mmfp4.mxfp4_gemm_backward(tiny, w, one, torch.float32)
+    assert torch.equal(dx.double(), ref)     # sums of multiples of 2^-25 below 2^-12: exact
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_not_finite(dtype):
     announce(f"mxfp4_gemm_backward not finite {dtype}")
