@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(NT) k_moe_route_grad(RouteGrad a) {
     const int j = j0 + l;
     const int64_t id = j < k ? a.ids[(size_t)t * k + j] : -1;
     const bool live = id >= 0 && id < E;
+    const int which = live ? (int)id : -1;
     double u = j < k ? (double)a.dw[(size_t)t * k + j] * (double)a.scale : 0.0;
     if (a.renorm) u = (u - us / sum) / sum;
     // the first lane of those with one index adds them up, in order
@@ -247,8 +248,7 @@ __global__ void __launch_bounds__(NT) k_moe_route_grad(RouteGrad a) {
     bool first = live;
     for (int o = 0; o < min(L, k - j0); ++o) {
       const double ou = __shfl(u, o, L);
-      const int oid = __shfl((int)id, o, L);
-      if (oid == (int)id) {
+      if (__shfl(which, o, L) == which) {
         mine_all += ou;
         first = first && o >= l;
       }

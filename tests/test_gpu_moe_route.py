@@ -137,6 +137,19 @@ def test_gradient_of_repeated_and_foreign_ids():
                 assert ((dl.double() - ref).abs() <= bound).all()
 
 
+def test_gradient_of_ids_beyond_32_bits():
+    """An id whose low 32 bits name an expert is foreign all the same."""
+    announce("moe_route_backward large ids")
+    for T in (3, 2200):
+        logits, dw = normal(T, 40, seed=4), normal(T, 4, seed=5)
+        ids = torch.tensor([3, 2 ** 32 + 3, 7, -2 ** 40 + 7], device=DEV).expand(T, 4)
+        want = mmfp4.moe_route_backward(dw, logits, torch.where(ids < 40, ids, -1).clamp(min=-1))
+        assert torch.equal(mmfp4.moe_route_backward(dw, logits, ids), want)
+        ref = route_grad(dw, logits, ids, False, True)
+        bound = half_step(ref, torch.float32) * (1 + 2.0 ** -20) + 1e-14
+        assert ((want.double() - ref).abs() <= bound).all()
+
+
 def test_autograd_and_differences():
     announce("moe_route autograd")
     logits = normal(7, 48, seed=8)
