@@ -462,14 +462,13 @@ int mm_moe_mlp_shared_fp4_p16(const uint16_t* X, const void* expert_ids, int ids
                               uint16_t* y_buf, int32_t* sort_buf, uint16_t* out, void* stream);
 
 /* Bytes of scratch that mm_moe_mlp_mxfp4 needs (no initial contents, nothing kept in it). */
-size_t mm_moe_mlp_mxfp4_scratch_bytes(int T, int k, int E, int H, int I, int type);
+size_t mm_moe_mlp_mxfp4_scratch_bytes(int T, int k, int E, int H, int I);
 
 /* mm_moe_mlp_fp4 on MXFP4 weights, both products with both sides in MXFP4:
  *   (g | u) = q(X[t]) . Wgu[e]^T;  a = q(silu(g) * u), quantized from its fp32 values;
  *   out[t] = sum_j probs[t, j] * (a . Wdn[e]^T)     (fp32, slot order, rounded once)
  * Wgu words [E, 2I, H/8] and scales [E, 2I, H/32], the gate's I rows first; Wdn [E, H, I/8] and
- * [E, H, I/32].  X [T, H] and out of type 0 fp32, 1 fp16, 2 bf16; what each expert gives a token
- * is rounded to that type before the sum.  expert_ids [T, k] int32 or (ids_i64) int64; ids outside
+ * [E, H, I/32].  X [T, H] and out of type 0 fp32, 1 fp16, 2 bf16.  expert_ids [T, k] int32 or (ids_i64) int64; ids outside
  * [0, E) contribute nothing.  probs fp32 [T, k].  H, I % 32 == 0, E <= 1024. */
 int mm_moe_mlp_mxfp4(const void* X, int type, const void* expert_ids, int ids_i64,
                      const float* probs, int T, int k, int E, int H, int I, const uint32_t* Wgu,

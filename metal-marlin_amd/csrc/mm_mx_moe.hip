@@ -101,7 +101,7 @@ template <int NT, int NW, int DEPTH>
 __global__ void __launch_bounds__(NW * 64)
 k_mx_moe_down(const uint8_t* __restrict__ hw, const uint8_t* __restrict__ hs, int ip,
               const uint8_t* __restrict__ W, const uint8_t* __restrict__ S, Rows rows, int H, int I,
-              void* __restrict__ y, int type) {
+              float* __restrict__ y) {
   using R = Ring<NT, 1, NW, DEPTH>;
   extern __shared__ __attribute__((aligned(16))) char lds[];   // ring (later sums), scales of W, of h
   const int e = blockIdx.y, r0 = rows.offsets[e], r1 = rows.offsets[e + 1];
@@ -127,7 +127,7 @@ k_mx_moe_down(const uint8_t* __restrict__ hw, const uint8_t* __restrict__ hs, in
                          acc);
     __syncthreads();
     skinny_reduce<1, NT, NW>(acc, (float*)lds, min(16, r1 - m0), [&](int nn, int mm, float v) {
-      if (n0 + nn < H) store1(y, type, (size_t)(m0 + mm) * H + n0 + nn, v);
+      if (n0 + nn < H) y[(size_t)(m0 + mm) * H + n0 + nn] = v;
     });
   }
 }
@@ -156,7 +156,7 @@ template <class Sh, bool ACT>
 __global__ void __launch_bounds__(Sh::NTHR)
 k_mx_moe_tile(const uint8_t* __restrict__ X, const uint8_t* __restrict__ XS, int kp,
               const uint8_t* __restrict__ W, const uint8_t* __restrict__ S, int ks, Rows rows, int E,
-              int N, int K, int gn, int np, void* __restrict__ y, int type, uint32_t* __restrict__ hw,
+              int N, int K, int gn, int np, float* __restrict__ y, uint32_t* __restrict__ hw,
               uint8_t* __restrict__ hs) {
   __shared__ __attribute__((aligned(16))) char smem[Sh::LDS];
   static_assert(Sh::LDS >= (MAX_E + 1) * 4, "the prefix sums use the tiles' memory");
@@ -203,7 +203,7 @@ k_mx_moe_tile(const uint8_t* __restrict__ X, const uint8_t* __restrict__ XS, int
   if (!ACT || n0 < half) tile_loop<Sh>(src, 0, (K + UNIT - 1) / UNIT, smem, acc);
   if constexpr (!ACT) {
     __syncthreads();
-    tile_out<Sh>(acc, smem, y, type, r1 - m0, n0, N,
+    tile_out<Sh>(acc, smem, y, F32, r1 - m0, n0, N,
                  [=](int m) { return (size_t)(m0 + m) * N; });
   } else {
     // A block of h is 16 values in each of lanes l and l + 32: n = 8 g + 4 h + i.
@@ -244,11 +244,11 @@ k_mx_moe_tile(const uint8_t* __restrict__ X, const uint8_t* __restrict__ XS, int
 }
 
 // out[t] = sum over j of p[t, j] * y[inverse[t, j]], in slot order; rows past the valid ones are
-// those of ids outside [0, E).  y has out's type: one rounding of y before the sum, as large as
-// the one after it, for half the bytes of fp32.
+// those of ids outside [0, E).  y is fp32: rounded to out's type it would add an error as large as
+// out's own rounding.
 template <int T>
 __global__ void __launch_bounds__(256)
-k_mx_moe_combine(const char* __restrict__ y, const float* __restrict__ probs,
+k_mx_moe_combine(const float* __restrict__ y, const float* __restrict__ probs,
                  const int32_t* __restrict__ inverse, const int32_t* __restrict__ valid, int k,
                  int H, void* __restrict__ out) {
   const size_t t = blockIdx.x;
@@ -259,15 +259,10 @@ k_mx_moe_combine(const char* __restrict__ y, const float* __restrict__ probs,
       const int row = inverse[t * k + j];
       if (row >= nv) continue;
       const float p = probs[t * k + j];
-      const Vals<T> v = load8<T>(y + ((size_t)row * H + c) * kBytes<T>);
+      const f32x4 v[2] = {*(const f32x4*)(y + (size_t)row * H + c),
+                          *(const f32x4*)(y + (size_t)row * H + c + 4)};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float f;
-        if constexpr (T == F32) f = v.v[i / 4][i % 4];
-        else if constexpr (T == F16) f = (float)as_f16x2(v.v[i / 2])[i % 2];
-        else f = (float)as_bf16x2(v.v[i / 2])[i % 2];
-        sum[i] += p * f;
-      }
+      for (int i = 0; i < 8; ++i) sum[i] += p * v[i / 4][i % 4];
     }
     store4(out, T, t * H + c, f32x4{sum[0], sum[1], sum[2], sum[3]});
     store4(out, T, t * H + c + 4, f32x4{sum[4], sum[5], sum[6], sum[7]});
@@ -278,9 +273,9 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
 // Whether an expert's rows are taken in tiles: from 4 of them on average (128 experts, T = 64: 93
-// us streamed; T = 128 116), or where 16 rows of x do not fit LDS.
-bool takes_tiles(long rows, int E, int H) {
-  return rows >= 4L * E || lds_x_bytes(16, (int)padded(H)) > 65536;
+// us streamed; T = 128 116), or where 16 rows of x, or an expert's scales, do not fit LDS.
+bool takes_tiles(long rows, int E, int H, int I) {
+  return rows >= 4L * E || I > 65536 || lds_x_bytes(16, (int)padded(H)) > 65536;
 }
 
 template <int T>
@@ -297,9 +292,9 @@ void launch_gate_up(const void* X, const uint8_t* W, const uint8_t* S, Rows rows
 struct Scratch {
   size_t sort, xq, gs, ds, hq, y, total;
 };
-Scratch scratch_of(int T, int k, int E, int H, int I, int type) {
+Scratch scratch_of(int T, int k, int E, int H, int I) {
   const size_t R = (size_t)T * k;
-  const bool tiles = takes_tiles((long)R, E, H);
+  const bool tiles = takes_tiles((long)R, E, H, I);
   const auto anew = [&](size_t rows, int K) {      // scales that the tiles take from a copy
     return tiles && scale_stride(K) != K / BLOCK ? up(rows * scale_stride(K)) : 0;
   };
@@ -310,15 +305,15 @@ Scratch scratch_of(int T, int k, int E, int H, int I, int type) {
   s.ds = s.gs + anew((size_t)E * 2 * I, H);
   s.hq = s.ds + anew((size_t)E * H, I);
   s.y = s.hq + up(packed_bytes(R, I));
-  s.total = s.y + up(R * H * (type == F32 ? 4 : 2));
+  s.total = s.y + up(R * H * sizeof(float));
   return s;
 }
 
 }  // namespace
 
-extern "C" size_t mm_moe_mlp_mxfp4_scratch_bytes(int T, int k, int E, int H, int I, int type) {
+extern "C" size_t mm_moe_mlp_mxfp4_scratch_bytes(int T, int k, int E, int H, int I) {
   if (T <= 0 || k <= 0 || E <= 0 || H <= 0 || I <= 0) return 0;
-  return scratch_of(T, k, E, H, I, type).total;
+  return scratch_of(T, k, E, H, I).total;
 }
 
 extern "C" int mm_moe_mlp_mxfp4(const void* X, int type, const void* expert_ids, int ids_i64,
@@ -335,9 +330,10 @@ extern "C" int mm_moe_mlp_mxfp4(const void* X, int type, const void* expert_ids,
                (long long)T * k);
   if (T == 0) return 0;
   MM_CHECK_ARG(X && expert_ids && probs && Wgu && Sgu && Wdn && Sdn && out && aligned16(X) &&
-                   aligned16(Wgu) && aligned16(Wdn) && aligned16(out),
-               "mm_moe_mlp_mxfp4: X, weights and out must be 16-byte aligned and nothing null");
-  const Scratch sc = scratch_of(T, k, E, H, I, type);
+                   aligned16(Wgu) && aligned16(Wdn) && aligned16(Sgu) && aligned16(Sdn) &&
+                   aligned16(out),
+               "mm_moe_mlp_mxfp4: X, weights, scales and out must be 16-byte aligned and nothing null");
+  const Scratch sc = scratch_of(T, k, E, H, I);
   MM_CHECK_ARG(scratch && aligned16(scratch) && scratch_bytes >= sc.total,
                "mm_moe_mlp_mxfp4: needs %zu bytes of scratch, 16-byte aligned, got %zu", sc.total,
                scratch_bytes);
@@ -358,9 +354,9 @@ extern "C" int mm_moe_mlp_mxfp4(const void* X, int type, const void* expert_ids,
   const Rows rows{offsets, sorted, k};
   uint32_t* const hw = (uint32_t*)(base + sc.hq);
   uint8_t* const hs = (uint8_t*)hw + codes_bytes(R, I);
-  void* const y = base + sc.y;
+  float* const y = (float*)(base + sc.y);
   const uint8_t *gw = (const uint8_t*)Wgu, *dw = (const uint8_t*)Wdn;
-  if (takes_tiles(R, E, H)) {
+  if (takes_tiles(R, E, H, I)) {
     uint8_t* const xq = (uint8_t*)base + sc.xq;
     uint8_t* const xs = xq + codes_bytes(T, H);
     if (const int rc = launch_quantize(X, type, T, H, hp, (uint32_t*)xq, xs, st)) return rc;
@@ -383,10 +379,10 @@ extern "C" int mm_moe_mlp_mxfp4(const void* X, int type, const void* expert_ids,
     MM_CHECK_ARG(tiles * std::max(g1, g2) < (1L << 30), "mm_moe_mlp_mxfp4: too many tiles");
     hipLaunchKernelGGL((k_mx_moe_tile<Sh, true>), dim3((unsigned)((tiles * g1 + 7) / 8 * 8)),
                        dim3(Sh::NTHR), 0, st, xq, xs, hp, gw, gs, scale_stride(H), rows, E, 2 * I, H, g1, ip,
-                       nullptr, type, hw, hs);
+                       nullptr, hw, hs);
     hipLaunchKernelGGL((k_mx_moe_tile<Sh, false>), dim3((unsigned)((tiles * g2 + 7) / 8 * 8)),
                        dim3(Sh::NTHR), 0, st, (const uint8_t*)hw, hs, ip, dw, ds, scale_stride(I), rows, E, H, I,
-                       g2, 0, y, type, nullptr, nullptr);
+                       g2, 0, y, nullptr, nullptr);
   } else {
     if (type == F32) launch_gate_up<F32>(X, gw, Sgu, rows, R, E, H, I, hw, hs, st);
     else if (type == F16) launch_gate_up<F16>(X, gw, Sgu, rows, R, E, H, I, hw, hs, st);
@@ -394,10 +390,10 @@ extern "C" int mm_moe_mlp_mxfp4(const void* X, int type, const void* expert_ids,
     using Rg = Ring<2, 1, 4, 1>;
     hipLaunchKernelGGL((k_mx_moe_down<2, 4, 1>), dim3(mm_cdiv(H, 32), E), dim3(256),
                        (Rg::BYTES + whole_kib(32 * (I / BLOCK)) + whole_kib(16 * (ip / BLOCK))), st,
-                       (const uint8_t*)hw, hs, ip, dw, Sdn, rows, H, I, y, type);
+                       (const uint8_t*)hw, hs, ip, dw, Sdn, rows, H, I, y);
   }
 #define MM_MX_COMBINE(T)                                                                         \
-  hipLaunchKernelGGL((k_mx_moe_combine<T>), dim3(T_), dim3(256), 0, st, (const char*)y, probs,     \
+  hipLaunchKernelGGL((k_mx_moe_combine<T>), dim3(T_), dim3(256), 0, st, y, probs,     \
                      inverse, offsets + E, k, H, out)
   const int T_ = T;
   if (type == F32) MM_MX_COMBINE(F32);

@@ -636,7 +636,7 @@ pybind11::object mx_moe_mlp(const at::Tensor& x, const at::Tensor& Wgu, const at
     return pybind11::none();
   const int type = type_code(x.scalar_type());
   at::Tensor out = at::empty_like(x);
-  const size_t need = mm_moe_mlp_mxfp4_scratch_bytes((int)T, (int)k, (int)E, (int)H, (int)I, type);
+  const size_t need = mm_moe_mlp_mxfp4_scratch_bytes((int)T, (int)k, (int)E, (int)H, (int)I);
   at::Tensor scratch = at::empty({(int64_t)need}, x.options().dtype(at::kByte));
   const int rc = mm_moe_mlp_mxfp4(
       x.data_ptr(), type, ids.data_ptr(), ids.scalar_type() == at::kLong,

@@ -85,7 +85,7 @@ SIGNATURES: dict[str, tuple] = {
     "mm_moe_combine": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp]),
     "mm_moe_mlp_fp4": (_c_int, [_vp, _vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_int,
                                 _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _vp, _vp, _vp]),
-    "mm_moe_mlp_mxfp4_scratch_bytes": (_c_size, [_c_int] * 6),
+    "mm_moe_mlp_mxfp4_scratch_bytes": (_c_size, [_c_int] * 5),
     "mm_moe_mlp_mxfp4": (_c_int, [_vp, _c_int, _vp, _c_int, _vp] + [_c_int] * 5 + [_vp] * 5 +
                          [_c_size, _vp, _vp]),
     "mm_moe_mlp_shared_fp4": (_c_int, [_vp, _vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int,

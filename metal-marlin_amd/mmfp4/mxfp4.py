@@ -34,6 +34,12 @@ def _scales(t: torch.Tensor, name: str = "scales") -> torch.Tensor:
     return t
 
 
+def _count(name: str, n: int) -> int:
+    if n >= 1 << 31:
+        raise ValueError(f"{name}={n} is too large: at most 2^31 - 1")
+    return n
+
+
 def _weights(words: torch.Tensor, scales: torch.Tensor, dims: int | None = None,
              name: str = "words") -> tuple[torch.Tensor, torch.Tensor]:
     """The checked pair: words [*, K/8] and scales [*, K/32] of as many axes as `dims`."""
@@ -102,13 +108,13 @@ def _gemm(x: torch.Tensor, words: torch.Tensor, scales: torch.Tensor,
     _type("x", x.dtype)
     dtype = out_dtype or x.dtype
     words, scales = _weights(words, scales, 2)
-    N, K = words.shape[0], 8 * words.shape[1]
+    N, K = _count("N", words.shape[0]), _count("K", 8 * words.shape[1])
     if x.dim() == 0 or x.shape[-1] != K:
         raise ValueError(f"x shape {tuple(x.shape)} must end in K={K}")
     with on_device(dev):
         a = plain(x.reshape(-1, K))
         w, s = plain(words), plain(scales)
-        M = a.shape[0]
+        M = _count("rows", a.shape[0])
         out = torch.empty((*x.shape[:-1], N), dtype=dtype, device=dev)
         if out.numel() == 0:
             return out
@@ -148,7 +154,7 @@ def mxfp4_gemm_backward(dy: torch.Tensor, words: torch.Tensor, scales: torch.Ten
     _type("dy", dy.dtype)
     dtype = out_dtype or dy.dtype
     words, scales = _weights(words, scales, 2)
-    N, K = words.shape[0], 8 * words.shape[1]
+    N, K = _count("N", words.shape[0]), _count("K", 8 * words.shape[1])
     if dy.dim() == 0 or dy.shape[-1] != N:
         raise ValueError(f"dy shape {tuple(dy.shape)} must end in N={N}")
     with on_device(dev):
@@ -162,7 +168,7 @@ def mxfp4_gemm_backward(dy: torch.Tensor, words: torch.Tensor, scales: torch.Ten
         if pad:                 # rows of whole 16-byte pieces
             d = torch.nn.functional.pad(d, (0, pad))
         d = plain(d)
-        M = d.shape[0]
+        M = _count("rows", d.shape[0])
         stream = _lib.raw_stream(dev.index)
         need = _lib.load().mm_mxfp4_gemm_backward_workspace_bytes(M, N, K, _TYPES[d.dtype])
         ws = _lib.workspace_on(dev.index, stream, need)
@@ -199,7 +205,7 @@ def moe_mlp_mxfp4(hidden: torch.Tensor, gate_up_words: torch.Tensor, gate_up_sca
                          f"gate_up_words {tuple(gu.shape)}")
     if hidden.dim() != 2 or hidden.shape[1] != H:
         raise ValueError(f"hidden shape {tuple(hidden.shape)} must be [T, {H}]")
-    T = hidden.shape[0]
+    T = _count("T", hidden.shape[0])
     if expert_ids.dim() != 2 or expert_ids.shape[0] != T or expert_ids.shape[1] == 0 or \
             expert_probs.shape != expert_ids.shape:
         raise ValueError(f"expert_ids {tuple(expert_ids.shape)} and expert_probs "
@@ -217,7 +223,7 @@ def moe_mlp_mxfp4(hidden: torch.Tensor, gate_up_words: torch.Tensor, gate_up_sca
             return out
         if E == 0:
             return out.zero_()
-        need = _lib.load().mm_moe_mlp_mxfp4_scratch_bytes(T, k, E, H, I, _TYPES[x.dtype])
+        need = _lib.load().mm_moe_mlp_mxfp4_scratch_bytes(T, k, E, H, I)
         scratch = torch.empty(need, dtype=torch.uint8, device=dev)
         _lib.call("mm_moe_mlp_mxfp4", _lib.ptr(x), _TYPES[x.dtype], _lib.ptr(ids),
                   int(ids.dtype == torch.int64), _lib.ptr(p), T, k, E, H, I, _lib.ptr(gu),

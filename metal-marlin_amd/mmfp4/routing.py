@@ -22,6 +22,16 @@ def _softmax(scoring: str) -> bool:
     return _SCORING[scoring]
 
 
+def _tokens(logits: torch.Tensor) -> int:
+    """The rows of logits [*, E]."""
+    if logits.dim() == 0 or logits.shape[-1] == 0:
+        raise ValueError(f"logits must be [*, num_experts], got {tuple(logits.shape)}")
+    T = logits.numel() // logits.shape[-1]
+    if T >= 1 << 31:
+        raise ValueError(f"{T} tokens are too many: at most 2^31 - 1")
+    return T
+
+
 def _route(logits, top_k, softmax, bias, num_groups, topk_groups, renormalize, scale):
     dev = _lib.require_device(logits, bias)
     _type("logits", logits.dtype)
@@ -29,8 +39,7 @@ def _route(logits, top_k, softmax, bias, num_groups, topk_groups, renormalize, s
                     renormalize, scale)
     if out is not None:
         return out
-    if logits.dim() == 0 or logits.shape[-1] == 0:
-        raise ValueError(f"logits must be [*, num_experts], got {tuple(logits.shape)}")
+    T = _tokens(logits)
     E = logits.shape[-1]
     if bias is not None and tuple(bias.shape) != (E,):
         raise ValueError(f"bias shape {tuple(bias.shape)} != ({E},)")
@@ -40,7 +49,7 @@ def _route(logits, top_k, softmax, bias, num_groups, topk_groups, renormalize, s
         shape = (*logits.shape[:-1], max(0, top_k))
         ids = torch.empty(shape, dtype=torch.int64, device=dev)
         w = torch.empty(shape, dtype=torch.float32, device=dev)
-        _lib.call("mm_moe_route", _lib.ptr(l), _TYPES[l.dtype], _lib.ptr(b), l.numel() // E, E,
+        _lib.call("mm_moe_route", _lib.ptr(l), _TYPES[l.dtype], _lib.ptr(b), T, E,
                   top_k, int(softmax), num_groups, topk_groups, int(renormalize), scale,
                   _lib.ptr(ids), _lib.ptr(w), _lib.stream_of(l))
     return w, ids
@@ -75,8 +84,7 @@ def moe_route_backward(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.
                     float(scale))
     if out is not None:
         return out
-    if logits.dim() == 0 or logits.shape[-1] == 0:
-        raise ValueError(f"logits must be [*, num_experts], got {tuple(logits.shape)}")
+    T = _tokens(logits)
     if ids.dim() != logits.dim() or ids.shape[:-1] != logits.shape[:-1] or \
             dweights.shape != ids.shape:
         raise ValueError(f"dweights {tuple(dweights.shape)} and ids {tuple(ids.shape)} must be "
@@ -90,6 +98,6 @@ def moe_route_backward(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.
         dw = dweights.to(torch.float32).contiguous()
         dl = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
         _lib.call("mm_moe_route_backward", _lib.ptr(dw), _lib.ptr(l), _TYPES[l.dtype],
-                  _lib.ptr(i), l.numel() // E, E, ids.shape[-1], int(softmax), int(renormalize),
+                  _lib.ptr(i), T, E, ids.shape[-1], int(softmax), int(renormalize),
                   float(scale), _lib.ptr(dl), _lib.stream_of(l))
     return dl
