@@ -300,7 +300,7 @@ size_t mm_mxfp4_gemm_workspace_bytes(int M, int N, int K);
 
 /* C[M, N] = q(X) . W^T with X [M, K] quantized as mm_mxfp4_quantize does and W [N, K] given so:
  * words [N, K/8], scales [N, K/32].  fp32 sums, C of out_type rounded once.  Types as above;
- * K % 32 == 0, any M and N; X, W, scales and C 16-byte aligned. */
+ * K % 32 == 0, K < 2^24, any M and N; X, W, scales and C 16-byte aligned. */
 int mm_mxfp4_gemm(const void* X, int type, const uint32_t* W, const uint8_t* scales, void* C,
                   int out_type, int M, int N, int K, void* ws, size_t ws_bytes, void* stream);
 
@@ -308,12 +308,12 @@ int mm_mxfp4_gemm(const void* X, int type, const uint32_t* W, const uint8_t* sca
  *   dX[M, K] = dY[M, N] . W[N, K]
  * dY of `type` with row stride ldy, a multiple of 16 bytes, and zeros between column N and the
  * next such multiple; dX of out_type.  Weights and every dY enter exactly, products accumulate in
- * fp32, rounded once.  K % 32 == 0; dY, W and dX 16-byte aligned.  Workspace as above,
+ * fp32, rounded once.  K % 32 == 0; dY, W, scales and dX 16-byte aligned.  Workspace as above,
  * mm_mxfp4_gemm_backward_workspace_bytes. */
 size_t mm_mxfp4_gemm_backward_workspace_bytes(int M, int N, int K, int type);
 int mm_mxfp4_gemm_backward(const void* dY, int type, int ldy, const uint32_t* W,
-                           const uint8_t* scales, void* dX, int out_type, int M, int N, int K, void* ws, size_t ws_bytes,
-                           void* stream);
+                           const uint8_t* scales, void* dX, int out_type, int M, int N, int K,
+                           void* ws, size_t ws_bytes, void* stream);
 
 /* -------------------------------------------------------------------- MoE */
 

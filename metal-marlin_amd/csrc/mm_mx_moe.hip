@@ -360,6 +360,8 @@ extern "C" int mm_moe_mlp_mxfp4(const void* X, int type, const void* expert_ids,
     uint8_t* const xq = (uint8_t*)base + sc.xq;
     uint8_t* const xs = xq + codes_bytes(T, H);
     if (const int rc = launch_quantize(X, type, T, H, hp, (uint32_t*)xq, xs, st)) return rc;
+    // 64 x 128: three blocks share a CU.  us of both products, 1000 tokens of 128 experts of 2048 ->
+    // 768: 71 + 43; of 128 x 128 73 + 47, with rings of three 76 + 51, of 64 x 256 104 + 54.
     using Sh = Tile<2, 2, 1, 2>;
     const uint8_t *gs = Sgu, *ds = Sdn;
     if (scale_stride(H) != H / BLOCK) {
