@@ -14,6 +14,8 @@
 //
 // L lanes share a token (16 where the token fits and there are many tokens, else 64), expert
 // l + L * slot to lane l.
+#include <type_traits>
+
 #include "mm_common.h"
 #include "mm_mx.h"
 #include "mmfp4.h"
@@ -25,19 +27,55 @@ constexpr int NT = 256;
 constexpr int MAX_E = 1024, MAX_K = 64, MAX_G = 64;
 constexpr double EPS = 1e-20;
 
+// Joins over groups of lanes, step D: a value of the other half of the lane's 2 D, for operands that
+// all D lanes of a half hold alike, as they do where a join goes D = 1, 2, 4, ..  Moves between
+// registers, mirrored where that is what there is: a selection of 8 among 256 waits for 48 such
+// steps (through LDS 11.3 us for 32 tokens).
+template <int D>
+MM_DEV uint32_t other(uint32_t v) {
+  static_assert(D == 1 || D == 2 || D == 4 || D == 8 || D == 16 || D == 32, "steps of a wave");
+  if constexpr (D == 1) return __builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 15, 15, true);
+  else if constexpr (D == 2) return __builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 15, 15, true);
+  else if constexpr (D == 4) return __builtin_amdgcn_update_dpp(0, (int)v, 0x141, 15, 15, true);
+  else if constexpr (D == 8) return __builtin_amdgcn_update_dpp(0, (int)v, 0x140, 15, 15, true);
+  else if constexpr (D == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? r[0] : r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? r[0] : r[1];
+  }
+}
+template <int D>
+MM_DEV float other(float v) {
+  return __builtin_bit_cast(float, other<D>(__builtin_bit_cast(uint32_t, v)));
+}
+template <int D>
+MM_DEV double other(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)other<D>((uint32_t)(u >> 32)) << 32 |
+                                        other<D>((uint32_t)u));
+}
+// f(D) for D = 1, 2, 4, .. below L.
+template <int L, int D = 1, class F>
+MM_DEV void steps(F&& f) {
+  if constexpr (D < L) {
+    f(std::integral_constant<int, D>{});
+    steps<L, 2 * D>(f);
+  }
+}
+
 template <int L>
 MM_DEV double all_sum(double v) {
-#pragma unroll
-  for (int d = 1; d < L; d <<= 1) v += __shfl_xor(v, d);
+  steps<L>([&](auto d) { v += other<decltype(d)::value>(v); });
   return v;
 }
 template <int L>
 MM_DEV float all_max(float v) {   // the largest, a NaN if there is one
-#pragma unroll
-  for (int d = 1; d < L; d <<= 1) {
-    const float o = __shfl_xor(v, d);
+  steps<L>([&](auto d) {
+    const float o = other<decltype(d)::value>(v);
     v = (o > v || o != o) ? o : v;
-  }
+  });
   return v;
 }
 
@@ -126,11 +164,13 @@ __global__ void __launch_bounds__(NT) k_moe_route(Route a) {
       b2 = v > b1 ? b1 : (v > b2 ? v : b2);
       b1 = v > b1 ? v : b1;
     }
-    for (int d = 1; d < P; d <<= 1) {
-      const double o1 = __shfl_xor(b1, d), o2 = __shfl_xor(b2, d);
+    steps<L>([&](auto d) {
+      constexpr int D = decltype(d)::value;
+      if (D >= P) return;
+      const double o1 = other<D>(b1), o2 = other<D>(b2);
       b2 = o1 > b1 ? (b1 > o2 ? b1 : o2) : (o1 > b2 ? o1 : b2);
       b1 = o1 > b1 ? o1 : b1;
-    }
+    });
     const double best = not_nan(n == 1 ? b1 : b1 + b2);
     int ahead = 0;
     for (int j = 0; j < G; ++j) {
@@ -157,14 +197,14 @@ __global__ void __launch_bounds__(NT) k_moe_route(Route a) {
         bv = c[i];
         bi = l + L * i;
       }
-#pragma unroll
-    for (int d = 1; d < L; d <<= 1) {
-      const double ov = __shfl_xor(bv, d);
-      const int oi = __shfl_xor(bi, d);
+    steps<L>([&](auto d) {
+      constexpr int D = decltype(d)::value;
+      const double ov = other<D>(bv);
+      const int oi = (int)other<D>((uint32_t)bi);
       const bool take = oi != 0x7fffffff && (bi == 0x7fffffff || ov > bv || (ov == bv && oi < bi));
       bv = take ? ov : bv;
       bi = take ? oi : bi;
-    }
+    });
     if (bi % L == l) out |= 1u << (bi / L);
     const double v = ls[bi];
     total += v;
