@@ -21,7 +21,6 @@
 #include "mmfp4.h"
 
 namespace {
-using mmmx::bf16;
 
 constexpr int NT = 256;
 constexpr int MAX_E = 1024, MAX_K = 64, MAX_G = 64;
@@ -79,10 +78,26 @@ MM_DEV float all_max(float v) {   // the largest, a NaN if there is one
   return v;
 }
 
-MM_DEV float load_logit(const void* p, int type, size_t i) {
-  if (type == mmmx::F32) return ((const float*)p)[i];
-  if (type == mmmx::F16) return (float)((const f16*)p)[i];
-  return (float)((const bf16*)p)[i];
+// The lane's logits, -inf past E.  All loads leave before one is waited for: one type for all, and
+// the last expert's again past E.
+template <int L, int SL>
+MM_DEV void load_logits(const void* p, int type, size_t base, int E, float (&x)[SL]) {
+  const int l = threadIdx.x % L;
+  if (type == mmmx::F32) {
+#pragma unroll
+    for (int i = 0; i < SL; ++i) x[i] = ((const float*)p)[base + min(l + L * i, E - 1)];
+  } else {
+    uint16_t v[SL];
+#pragma unroll
+    for (int i = 0; i < SL; ++i) v[i] = ((const uint16_t*)p)[base + min(l + L * i, E - 1)];
+#pragma unroll
+    for (int i = 0; i < SL; ++i)
+      x[i] = type == mmmx::F16 ? (float)__builtin_bit_cast(f16, v[i])
+                               : __builtin_bit_cast(float, (uint32_t)v[i] << 16);
+  }
+#pragma unroll
+  for (int i = 0; i < SL; ++i)
+    if (l + L * i >= E) x[i] = -__builtin_inff();
 }
 
 // s of the lane's experts; lanes past E get 0.
@@ -90,11 +105,7 @@ template <int L, int SL>
 MM_DEV void scores(const void* logits, int type, size_t base, int E, bool softmax, double (&s)[SL]) {
   const int l = threadIdx.x % L;
   float x[SL];
-#pragma unroll
-  for (int i = 0; i < SL; ++i) {
-    const int e = l + L * i;
-    x[i] = e < E ? load_logit(logits, type, base + e) : -__builtin_inff();
-  }
+  load_logits<L, SL>(logits, type, base, E, x);
   if (!softmax) {
 #pragma unroll
     for (int i = 0; i < SL; ++i) s[i] = 1.0 / (1.0 + exp(-(double)x[i]));
@@ -137,13 +148,19 @@ __global__ void __launch_bounds__(NT) k_moe_route(Route a) {
   double* const ls = lds + (size_t)mine * 2 * E;
   double* const lc = ls + E;
   double s[SL], c[SL];
+  float b[SL];
+#pragma unroll
+  for (int i = 0; i < SL; ++i) b[i] = 0.0f;
+  if (a.bias)
+#pragma unroll
+    for (int i = 0; i < SL; ++i) b[i] = a.bias[min(l + L * i, E - 1)];
   scores<L, SL>(a.logits, a.type, (size_t)t * E, E, a.softmax, s);
   uint32_t out = 0;                                  // slots that cannot be taken (any more)
 #pragma unroll
   for (int i = 0; i < SL; ++i) {
     const int e = l + L * i;
     if (e < E) {
-      c[i] = not_nan(a.bias ? s[i] + (double)a.bias[e] : s[i]);
+      c[i] = not_nan(s[i] + (double)b[i]);
       ls[e] = s[i];
       lc[e] = c[i];
     } else {
