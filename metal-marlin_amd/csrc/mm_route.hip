@@ -13,7 +13,8 @@
 // forms), and the bytes, 2 to 4 per logit, are what the kernels wait for.
 //
 // L lanes share a token (16 where the token fits and there are many tokens, else 64), expert
-// l + L * slot to lane l.
+// l + L * slot to lane l.  Bound by latency: 32 tokens of 256 experts, 8 of them, 8.7-10 us, 4096
+// of 128 9.8-11 and the gradient 5.5.
 #include <type_traits>
 
 #include "mm_common.h"
@@ -29,7 +30,7 @@ constexpr double EPS = 1e-20;
 // Joins over groups of lanes, step D: a value of the other half of the lane's 2 D, for operands that
 // all D lanes of a half hold alike, as they do where a join goes D = 1, 2, 4, ..  Moves between
 // registers, mirrored where that is what there is: a selection of 8 among 256 waits for 48 such
-// steps (through LDS 11.3 us for 32 tokens).
+// steps (the call of 32 tokens 10.3 us, through LDS 10.8).
 template <int D>
 MM_DEV uint32_t other(uint32_t v) {
   static_assert(D == 1 || D == 2 || D == 4 || D == 8 || D == 16 || D == 32, "steps of a wave");

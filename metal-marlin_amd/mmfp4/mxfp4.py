@@ -61,11 +61,12 @@ def _weights(words: torch.Tensor, scales: torch.Tensor, dims: int | None = None,
 def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """x [*, K] fp16, bf16 or fp32, K % 32 == 0 -> words int32 [*, K/8], scales uint8 [*, K/32].
     quantize_fp4 is its counterpart for groups with fp16 scales."""
+    if isinstance(x, torch.Tensor):
+        out = _lib.fast("mx_quantize", x, x)
+        if out is not None:
+            return out
     dev = _lib.require_device(x)
     _type("x", x.dtype)
-    out = _lib.fast("mx_quantize", x, x.detach())
-    if out is not None:
-        return out
     if x.dim() == 0 or x.shape[-1] == 0 or x.shape[-1] % BLOCK != 0:
         raise ValueError(f"x shape {tuple(x.shape)}: the last axis must be a positive multiple of "
                          f"{BLOCK}")

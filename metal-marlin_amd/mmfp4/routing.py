@@ -33,12 +33,13 @@ def _tokens(logits: torch.Tensor) -> int:
 
 
 def _route(logits, top_k, softmax, bias, num_groups, topk_groups, renormalize, scale):
+    if isinstance(logits, torch.Tensor) and (bias is None or isinstance(bias, torch.Tensor)):
+        out = _lib.fast("moe_route", logits, logits, top_k, softmax, bias, num_groups, topk_groups,
+                        renormalize, scale)
+        if out is not None:
+            return out
     dev = _lib.require_device(logits, bias)
     _type("logits", logits.dtype)
-    out = _lib.fast("moe_route", logits, logits, top_k, softmax, bias, num_groups, topk_groups,
-                    renormalize, scale)
-    if out is not None:
-        return out
     T = _tokens(logits)
     E = logits.shape[-1]
     if bias is not None and tuple(bias.shape) != (E,):
@@ -77,13 +78,14 @@ def moe_route_backward(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.
                        scoring: str = "sigmoid", renormalize: bool = True, scale: float = 1.0):
     """The gradient of moe_route's weights: dweights [*, top_k] -> dlogits [*, E] of the logits'
     type, for the logits and ids of the forward pass.  Ids outside [0, E) get nothing."""
-    dev = _lib.require_device(dweights, logits, ids)
     softmax = _softmax(scoring)
+    if all(isinstance(t, torch.Tensor) for t in (dweights, logits, ids)):
+        out = _lib.fast("moe_route_backward", logits, dweights, logits, ids, softmax, renormalize,
+                        float(scale))
+        if out is not None:
+            return out
+    dev = _lib.require_device(dweights, logits, ids)
     _type("logits", logits.dtype)
-    out = _lib.fast("moe_route_backward", logits, dweights, logits, ids, softmax, renormalize,
-                    float(scale))
-    if out is not None:
-        return out
     T = _tokens(logits)
     if ids.dim() != logits.dim() or ids.shape[:-1] != logits.shape[:-1] or \
             dweights.shape != ids.shape:
