@@ -123,8 +123,8 @@ constexpr size_t COUNTERS = 65536;   // head of every workspace: other products'
 
 // Whether the blocks quantize x themselves.  Each of them does it anew, so from about 16384 values
 // on (4 rows of 4096) a launch that does it once is faster: us, in the kernel against apart,
-// 4096 -> 14336 M = 4 8.8 / 10.9, M = 8 11.5 / 11.1, M = 16 17.4 / 11.1; 14336 -> 4096 M = 1
-// 7.1 / 9.3, M = 2 8.4 / 9.4, M = 4 12.8 / 9.5.
+// 4096 -> 14336 M = 8 11.5 / 10.1, M = 16 17.4 / 10.4, M = 4 8.8 in the kernel; 14336 -> 4096 M = 1
+// 7.1 / 9.2, M = 2 8.4 / 9.3, M = 4 12.8 / 9.3.
 bool quantizes_itself(int M, int K) { return M <= SKINNY_M && (long)M * K <= 16384 + 4096; }
 
 template <int T, int NT, int NW, int D, int U>
@@ -145,25 +145,35 @@ void launch_skinny(const void* X, const uint32_t* W, const uint8_t* S, void* C, 
   else launch_skinny_as<T, 1, 8, 2, 4>(X, W, S, C, out_type, M, N, K, st);
 }
 
-constexpr int CODES_WAVES = 8, LDS_BYTES = 160 * 1024, CUS = 256;
-template <int MT>
+constexpr int CODES_WAVES = 4, CODES_DEPTH = 2, LDS_BYTES = 160 * 1024, CUS = 256;
+template <int MT, int NT>
 long codes_lds(int K) {
-  return Ring<1, MT, CODES_WAVES, 1>::BYTES + (long)whole_kib(16 * (K / BLOCK)) +
+  return Ring<NT, MT, CODES_WAVES, CODES_DEPTH>::BYTES + (long)whole_kib(16 * NT * (K / BLOCK)) +
          whole_kib(16 * MT * (int)(padded(K) / BLOCK));
 }
-template <int MT>
-void launch_codes(const uint8_t* xq, const uint8_t* xs, int kp, const uint32_t* W, const uint8_t* S,
-                  void* C, int out_type, int M, int N, int K, hipStream_t st) {
-  hipLaunchKernelGGL((k_mx_skinny_codes<MT, 1, CODES_WAVES, 1>), dim3(mm_cdiv(N, 16), mm_cdiv(M, 16 * MT)),
-                     dim3(CODES_WAVES * 64), codes_lds<MT>(K), st, xq, xs, kp, (const uint8_t*)W, S, C,
-                     out_type, M, N, K);
+template <int MT, int NT>
+void launch_codes_as(const uint8_t* xq, const uint8_t* xs, int kp, const uint32_t* W,
+                     const uint8_t* S, void* C, int out_type, int M, int N, int K, hipStream_t st) {
+  hipLaunchKernelGGL((k_mx_skinny_codes<MT, NT, CODES_WAVES, CODES_DEPTH>),
+                     dim3(mm_cdiv(N, 16 * NT), mm_cdiv(M, 16 * MT)), dim3(CODES_WAVES * 64),
+                     (codes_lds<MT, NT>(K)), st, xq, xs, kp, (const uint8_t*)W, S, C, out_type, M, N,
+                     K);
 }
+// Up to 32 rows take 32 columns a block where 16 would make more blocks than the CUs hold at once,
+// two each: us, 32 columns against 16, M = 24 4096 -> 14336 11.8 / 13.6, 4096 -> 4096 8.2 / 7.0,
+// 14336 -> 4096 11.9 / 10.4.  (Eight waves and one unit ahead: 13.7, 7.7, 10.6.)
+bool wide_codes(int M, int N) { return M <= 32 && N > 2 * CUS * 16; }
+
 // Rows that stream the weights, from codes: 16, 32 or 64 a block, as long as a block's scales fit
-// LDS.  More than 32 rows only while the CUs hold all blocks at once, two each: us, streamed against
-// tiles, M = 64 4096 -> 4096 9.0 / 10.8, 14336 -> 4096 14.0 / 17.5, 4096 -> 14336 24.4 / 14.1.
+// LDS.  More than 32 rows only while the CUs hold all blocks at once: us, streamed against tiles,
+// M = 64 4096 -> 4096 9.1 / 10.8, 14336 -> 4096 14.3 / 17.5, 4096 -> 14336 24.4 / 12.3.
 bool streams(int M, int N, int K) {
   if (M > CODES_M || (M > 32 && N > 2 * CUS * 16)) return false;
-  return (M <= 16 ? codes_lds<1>(K) : M <= 32 ? codes_lds<2>(K) : codes_lds<4>(K)) <= LDS_BYTES;
+  const long lds = wide_codes(M, N) ? (M <= 16 ? codes_lds<1, 2>(K) : codes_lds<2, 2>(K))
+                   : M <= 16        ? codes_lds<1, 1>(K)
+                   : M <= 32        ? codes_lds<2, 1>(K)
+                                    : codes_lds<4, 1>(K);
+  return lds <= LDS_BYTES;
 }
 
 // Tiles.  A block is alone on its CU, or (64 x 64) one of two that take turns; a stage of it takes
@@ -277,9 +287,16 @@ extern "C" int mm_mxfp4_gemm(const void* X, int type, const uint32_t* W, const u
   uint8_t *const xq = (uint8_t*)ws + COUNTERS, *const xs = (uint8_t*)ws + sp.xs;
   if (p.tile < 0) {
     if (const int rc = launch_quantize(X, type, M, K, kp, (uint32_t*)xq, xs, st)) return rc;
-    if (M <= 16) launch_codes<1>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
-    else if (M <= 32) launch_codes<2>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
-    else launch_codes<4>(xq, xs, kp, W, S, C, out_type, M, N, K, st);
+    const auto run = [&](auto mt, auto nt) {
+      launch_codes_as<decltype(mt)::value, decltype(nt)::value>(xq, xs, kp, W, S, C, out_type, M, N,
+                                                                K, st);
+    };
+    constexpr std::integral_constant<int, 1> one{};
+    constexpr std::integral_constant<int, 2> two{};
+    if (wide_codes(M, N)) M <= 16 ? run(one, two) : run(two, two);
+    else if (M <= 16) run(one, one);
+    else if (M <= 32) run(two, one);
+    else run(std::integral_constant<int, 4>{}, one);
     MM_CHECK_LAUNCH("mm_mxfp4_gemm");
     return 0;
   }

@@ -139,6 +139,13 @@ def test_gemm_large(m, n, k):
     gemm_case(m, n, k, torch.bfloat16)
 
 
+@pytest.mark.parametrize("m", [6, 16, 17, 32, 33, 64])
+@pytest.mark.parametrize("n,k", [(8193, 5056), (8221, 736), (14336, 4096)])
+def test_gemm_wide(m, n, k):
+    announce(f"mxfp4_gemm {m} x {n} x {k}")
+    gemm_case(m, n, k, TYPES[(m + n) % 3], seed=m)
+
+
 @pytest.mark.parametrize("k", range(32, 800, 32))
 def test_gemm_every_tail(k):
     announce(f"mxfp4_gemm k={k}")
