@@ -307,8 +307,9 @@ int mm_mxfp4_gemm(const void* X, int type, const uint32_t* W, const uint8_t* sca
 /* Its input gradient, straight through the rounding of X:
  *   dX[M, K] = dY[M, N] . W[N, K]
  * dY of `type` with row stride ldy, a multiple of 16 bytes, and zeros between column N and the
- * next such multiple; dX of out_type.  Weights and every dY enter exactly, products accumulate in
- * fp32, rounded once.  K % 32 == 0; dY, W, scales and dX 16-byte aligned.  Workspace as above,
+ * next such multiple; dX of out_type.  Weights of every scale enter exactly, those beyond fp32
+ * (scales 253 and 254) too, and dY does, but for what of an fp32 value lies below 2^-133; products
+ * accumulate in fp32 and are rounded once.  K % 32 == 0; dY, W, scales and dX 16-byte aligned.  Workspace as above,
  * mm_mxfp4_gemm_backward_workspace_bytes. */
 size_t mm_mxfp4_gemm_backward_workspace_bytes(int M, int N, int K, int type);
 int mm_mxfp4_gemm_backward(const void* dY, int type, int ldy, const uint32_t* W,

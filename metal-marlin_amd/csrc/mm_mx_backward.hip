@@ -2,12 +2,15 @@
 // through the rounding of x.
 //
 // The contraction runs along N, across the rows of W, whose scales change from row to row: the
-// scaled matrix instructions cannot take them.  Every MXFP4 value is a bf16 number, though (2 bits
-// of E2M1 and bf16 has E8M0's exponents), so weights are converted exactly, 64 rows of a stage at
-// a time, into an LDS tile [n][k], from which ds_read_b64_tr_b16 takes columns as 32x32x16
-// operands.  bf16 dY is multiplied as it is.  fp16 dY is, too, in stages whose weights are normal
-// fp16 numbers, as those of a trained matrix are; in others it is two bf16 terms (11 bits in 8 +
-// 8).  fp32 is three (24 bits).  Products are exact, sums fp32, rounded once.
+// scaled matrix instructions cannot take them.  A quarter of every MXFP4 value is a bf16 number,
+// though: 2 bits of E2M1, and magnitudes from 2^-130, a subnormal one, to 1.5 * 2^127.  (Of the
+// values themselves those of scale codes 253 and 254 reach 1.5 * 2^129: infinities, which make NaNs
+// of zeros of dY.)  So quarters of the weights are converted exactly, 64 rows of a stage at a time,
+// into an LDS tile [n][k], from which ds_read_b64_tr_b16 takes columns as 32x32x16 operands, and the
+// sums are multiplied by 4.  bf16 dY is multiplied as it is.  fp16 dY is, too, in stages whose
+// quarters are normal fp16 numbers, as those of a trained matrix are; in others it is two bf16 terms
+// (11 bits in 8 + 8).  fp32 is three (24 bits; what lies below 2^-133, bf16's smallest step, is cut
+// off).  Products are exact, sums fp32, rounded once.
 //
 // Bound by LDS and the matrix cores in turn: a stage of a 128 x 256 tile reads 128 KiB of operands
 // and writes 58, about 0.5 us, and multiplies for 0.43; it takes 1.17 (2048 x 14336 x 4096: 268 us
@@ -98,13 +101,20 @@ MM_DEV void terms(const char* p0, const char* p1, bf16x8 (&t)[T == BF16 ? 1 : (T
   }
 }
 
-// Weights 2 I, 2 I + 1 of a word as fp16 or bf16.
+// Weights 2 I, 2 I + 1 of a word as fp16 or bf16 under the scale s.
 template <bool HALF, int I>
 MM_DEV uint32_t two(uint32_t w, float s) {
   if constexpr (HALF)
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, I));
   else
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, I));
+}
+// The same as bf16 under a scale below 2^-127, the least that the conversion knows: the leading
+// halves of fp32 products, which are multiples of 2^-130.
+template <int I>
+MM_DEV uint32_t two_small(uint32_t w, float s) {
+  const f32x2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, I);
+  return __builtin_amdgcn_perm(u32_of(v.y * s), u32_of(v.x * s), 0x07060302u);
 }
 
 template <class Sh, int T>
@@ -167,7 +177,7 @@ __global__ void __launch_bounds__(Sh::NTHR) k_mx_grad(Grad a, int gm, int gk) {
     if (idle) return;
     const int n = tid / RB, c = tid % RB;
     char* const d = conv + half_of * Sh::B + n * (Sh::TK * 2) + (c ^ (n & 3)) * 64;
-    const float s = scale_of(code);
+    const float s = scale_of(max(code, 2u) - 2u);        // a quarter
     const uint32_t nan = !HALF && code == 255u ? 0x7fc07fc0u : 0u;
     // lanes of one round write all of the 16 pieces that banks tell apart
     const int turn = (tid >> 2) & 3;
@@ -179,10 +189,19 @@ __global__ void __launch_bounds__(Sh::NTHR) k_mx_grad(Grad a, int gm, int gk) {
       lds_store16(d + 16 * ((j + turn) & 3), u32x4{two<HALF, 0>(w, s) | nan, two<HALF, 1>(w, s) | nan,
                                     two<HALF, 2>(w, s) | nan, two<HALF, 3>(w, s) | nan});
     }
+    if (!HALF && code < 2u) {
+      const float t = f32_of(0x00100000u << code);       // 2^-129, 2^-128
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t w = j == 0 ? wv[0] : (j == 1 ? wv[1] : (j == 2 ? wv[2] : wv[3]));
+        lds_store16(d + 16 * ((j + turn) & 3), u32x4{two_small<0>(w, t), two_small<1>(w, t),
+                                                     two_small<2>(w, t), two_small<3>(w, t)});
+      }
+    }
   };
-  // A stage of fp16 dY is wide, two bf16 terms, if one of its weights is no normal fp16 number: 0.5
-  // .. 6 times 2^-13 .. 2^13, or zeros under any scale but NaN.  Whoever finds one leaves the
-  // stage's number in its half's word.
+  // A stage of fp16 dY is wide, two bf16 terms, if a quarter of one of its weights is no normal
+  // fp16 number: 0.5 .. 6 times 2^-13 .. 2^13, or zeros under any scale but NaN.  Whoever finds one
+  // leaves the stage's number in its half's word.
   int* const wide = (int*)(smem + Sh::LDS - 16);
   constexpr std::true_type HALF{};
   constexpr std::false_type BF{};
@@ -193,7 +212,7 @@ __global__ void __launch_bounds__(Sh::NTHR) k_mx_grad(Grad a, int gm, int gk) {
     const uint32_t code = *(const uint8_t*)(r + Sh::WP * 1024 + b);
     if constexpr (T == F16) {
       const u32x4 m = wv & 0x77777777u;
-      if (code - 114u > 26u && (code == 255u || (m.x | m.y | m.z | m.w) != 0u))
+      if (code - 116u > 26u && (code == 255u || (m.x | m.y | m.z | m.w) != 0u))
         lds_store4(wide + half_of, (uint32_t)u);
       stores_done();
       block_barrier();
@@ -287,6 +306,12 @@ __global__ void __launch_bounds__(Sh::NTHR) k_mx_grad(Grad a, int gm, int gk) {
     }
     wait_loads<0>();
   }
+#pragma unroll
+  for (int k = 0; k < Sh::KB; ++k)
+#pragma unroll
+    for (int m = 0; m < Sh::MB; ++m)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[k][m][i] *= 4.0f;
   __syncthreads();
   const size_t base = blockIdx.y * sum_pitch((size_t)a.M * a.K);      // 0 unless split
   tile_out<Sh>(acc, smem, a.out, a.out_type, a.M - m0, k0, a.K,

@@ -143,8 +143,8 @@ def mxfp4_gemm(x: torch.Tensor, words: torch.Tensor, scales: torch.Tensor,
 def mxfp4_gemm_backward(dy: torch.Tensor, words: torch.Tensor, scales: torch.Tensor,
                         out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """dx = dy @ W, the gradient of mxfp4_gemm's input for dy [*, N] -> [*, K] in dy's type or
-    out_dtype: x's rounding counts as the identity.  dy (fp16, bf16 or fp32) and W enter exactly,
-    sums are fp32, rounded once."""
+    out_dtype: x's rounding counts as the identity.  dy (fp16, bf16, or fp32 but for what lies below
+    2^-133) and W enter exactly, sums are fp32, rounded once."""
     if not isinstance(dy, torch.Tensor):
         raise TypeError(f"expected torch.Tensor, got {type(dy).__name__}")
     out = _lib.fast("mx_gemm_backward", dy, dy, words, scales, -1 if out_dtype is None else _type(
