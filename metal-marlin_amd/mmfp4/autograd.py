@@ -20,7 +20,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib, adapters, backward, kernels
 
 __all__ = ["linear", "marlin_gemm", "rowpacked_gemm", "gate_up_swiglu", "FusedQKV", "GateUp",
-           "LoraAdd", "LoraLinear", "Route"]
+           "LoraAdd", "LoraLinear", "Route", "Undifferentiable"]
 
 
 def refuse_foreign_leaf(*tensors: torch.Tensor | None) -> None:
@@ -230,6 +230,21 @@ class LoraLinear(torch.autograd.Function):
         if ctx.needs_input_grad[6]:
             dbias = _column_sums(dy.view(-1, dy.shape[-1])).to(ctx.bias_dtype)
         return (dx if ctx.needs_input_grad[0] else None), da, db, None, None, None, dbias
+
+
+class Undifferentiable(torch.autograd.Function):
+    """call() of the operands `inputs`, which has no backward pass: where one reaches it through
+    other terms of a sum (a residual, another loss) it is an error, not a silent zero."""
+
+    @staticmethod
+    def forward(ctx, name, call, *inputs):
+        ctx.name = name
+        return call()
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError(f"{ctx.name} is not differentiable; detach its operands, or call it "
+                           "under torch.no_grad(), where no gradient through it is wanted")
 
 
 class Route(torch.autograd.Function):

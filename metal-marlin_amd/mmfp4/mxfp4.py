@@ -189,7 +189,20 @@ def moe_mlp_mxfp4(hidden: torch.Tensor, gate_up_words: torch.Tensor, gate_up_sca
         out[t] = sum_j p[t, j] * y                        [T, H] in hidden's type
     gate_up_words [E, 2I, H/8] and scales [E, 2I, H/32], the gate's I rows first; down_words
     [E, H, I/8] and scales [E, H, I/32].  silu(g) * u is quantized from its fp32 value.  Ids
-    outside [0, E) contribute nothing.  Not differentiable, as the other products of experts."""
+    outside [0, E) contribute nothing.  Not differentiable, as the other products of experts: a
+    backward pass that reaches its result raises."""
+    if kernels._wants_grad(hidden) or kernels._wants_grad(expert_probs):
+        from . import autograd
+        return autograd.Undifferentiable.apply(
+            "moe_mlp_mxfp4", lambda: _moe_mlp(hidden, gate_up_words, gate_up_scales, down_words,
+                                              down_scales, expert_ids, expert_probs),
+            hidden, expert_probs)
+    return _moe_mlp(hidden, gate_up_words, gate_up_scales, down_words, down_scales, expert_ids,
+                    expert_probs)
+
+
+def _moe_mlp(hidden, gate_up_words, gate_up_scales, down_words, down_scales, expert_ids,
+             expert_probs) -> torch.Tensor:
     dev = _lib.require_device(hidden, gate_up_words, gate_up_scales, down_words, down_scales,
                               expert_ids, expert_probs)
     _type("hidden", hidden.dtype)
