@@ -28,6 +28,18 @@ def weight(n, k, code):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_every_value(dtype):
+    """All 16 codes under all 256 scales, back to values: one rounding of a type that ends where
+    infinity begins."""
+    announce(f"mxfp4_dequantize every value {dtype}")
+    w = torch.tensor([0x76543210, -0x01234568], dtype=torch.int32, device=DEV).repeat(256, 2)
+    s = torch.arange(256, device=DEV).to(torch.uint8).unsqueeze(1)
+    got, want = mmfp4.mxfp4_dequantize(w, s, dtype), values(w, s).to(dtype)
+    assert torch.isnan(got[255]).all() and torch.equal(got[:255], want[:255])
+    assert torch.equal(torch.signbit(got[:255]), torch.signbit(want[:255]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n,k", [(3, 255, 96), (40, 255, 64), (255, 255, 320), (500, 2000, 256),
                                    (33, 2041, 64)])
 def test_gradient_of_every_scale(m, n, k, dtype):
