@@ -300,7 +300,8 @@ size_t mm_mxfp4_gemm_workspace_bytes(int M, int N, int K);
 
 /* C[M, N] = q(X) . W^T with X [M, K] quantized as mm_mxfp4_quantize does and W [N, K] given so:
  * words [N, K/8], scales [N, K/32].  fp32 sums, C of out_type rounded once.  Types as above;
- * K % 32 == 0, K < 2^24, any M and N; X, W, scales and C 16-byte aligned. */
+ * K % 32 == 0, K < 2^24, N < 2^29, any M that a launch of 2^32 threads holds (M times K, padded to
+ * 512s, below 2^37); X, W, scales and C 16-byte aligned. */
 int mm_mxfp4_gemm(const void* X, int type, const uint32_t* W, const uint8_t* scales, void* C,
                   int out_type, int M, int N, int K, void* ws, size_t ws_bytes, void* stream);
 
@@ -376,7 +377,7 @@ int mm_softmax_topk_p16(const void* logits, int logits_f32, int T, int E, int k,
  * int64 [T, k] are the k largest c among their experts, in that order, ties to the lower index
  * (decided in 64 bits); weights fp32 [T, k] = scale * s[ids], with renorm / (sum s[ids] + 1e-20).
  * NaNs rank last; a softmax row without a value above -inf has s = 0.  E <= 1024, k <= 64,
- * groups <= 64.  Beside mm_softmax_topk (metal_marlin/moe_dispatch.py:99-151), which knows
+ * groups <= 64, T < 2^26 (2^28 where E <= 256 and groups <= 16).  Beside mm_softmax_topk (metal_marlin/moe_dispatch.py:99-151), which knows
  * neither bias nor groups. */
 int mm_moe_route(const void* logits, int type, const float* bias, int T, int E, int k, int softmax,
                  int groups, int keep, int renorm, float scale, int64_t* ids, float* weights,
@@ -469,8 +470,10 @@ size_t mm_moe_mlp_mxfp4_scratch_bytes(int T, int k, int E, int H, int I);
  *   (g | u) = q(X[t]) . Wgu[e]^T;  a = q(silu(g) * u), quantized from its fp32 values;
  *   out[t] = sum_j probs[t, j] * (a . Wdn[e]^T)     (fp32, slot order, rounded once)
  * Wgu words [E, 2I, H/8] and scales [E, 2I, H/32], the gate's I rows first; Wdn [E, H, I/8] and
- * [E, H, I/32].  X [T, H] and out of type 0 fp32, 1 fp16, 2 bf16.  expert_ids [T, k] int32 or (ids_i64) int64; ids outside
- * [0, E) contribute nothing.  probs fp32 [T, k].  H, I % 32 == 0, E <= 1024. */
+ * [E, H, I/32].  X [T, H] and out of type 0 fp32, 1 fp16, 2 bf16.  expert_ids [T, k] int32 or
+ * (ids_i64) int64; ids outside [0, E) contribute nothing.  probs fp32 [T, k].  H, I % 32 == 0,
+ * E <= 1024, and below 4 GiB: an expert's words of either matrix, and the codes of the T tokens (H)
+ * and of the T*k rows of a (I), half a byte a value, rows padded to 512s. */
 int mm_moe_mlp_mxfp4(const void* X, int type, const void* expert_ids, int ids_i64,
                      const float* probs, int T, int k, int E, int H, int I, const uint32_t* Wgu,
                      const uint8_t* Sgu, const uint32_t* Wdn, const uint8_t* Sdn, void* scratch,

@@ -158,6 +158,11 @@ MM_DEV void store4(void* C, int type, size_t i, f32x4 v) {
   *(u32x2*)((uint16_t*)C + i) = p;
 }
 
+// A launch has fewer than 2^32 threads along an axis.
+inline bool launch_holds(size_t blocks, size_t threads) {
+  return blocks < ((size_t)1 << 32) / threads;
+}
+
 inline const char* type_name(int t) {
   return t == F32 ? "fp32" : (t == F16 ? "fp16" : (t == BF16 ? "bf16" : "?"));
 }

@@ -404,12 +404,14 @@ extern "C" int mm_mxfp4_gemm_backward(const void* dY, int type, int ldy, const u
                "mm_mxfp4_gemm_backward: unknown type %d or %d", type, out_type);
   MM_CHECK_ARG(ldy >= N && ldy % (type == F32 ? 4 : 8) == 0,
                "mm_mxfp4_gemm_backward: ldy=%d: rows of dY must be whole 16-byte pieces, N=%d", ldy, N);
-  MM_CHECK_ARG(N < (1 << 28) && K < (1 << 28), "mm_mxfp4_gemm_backward: N=%d or K=%d is too large",
-               N, K);
+  MM_CHECK_ARG(M <= INT32_MAX - 127 && N < (1 << 28) && K < (1 << 28),
+               "mm_mxfp4_gemm_backward: M=%d, N=%d or K=%d is too large", M, N, K);
   if (M == 0) return 0;
   MM_CHECK_ARG(dY && W && S && dX && aligned16(dY) && aligned16(W) && aligned16(S) && aligned16(dX),
                "mm_mxfp4_gemm_backward: dY, W, scales and dX must be 16-byte aligned and nothing null");
   const Plan p = plan_of(M, N, K, type);
+  MM_CHECK_ARG(launch_holds((size_t)mm_cdiv(M, COSTS[p.tile].tm) * mm_cdiv(K, COSTS[p.tile].tk), 512),
+               "mm_mxfp4_gemm_backward: M=%d, K=%d is too large", M, K);
   const Space sp = space_of(p, M, N, K);
   MM_CHECK_ARG(sp.total == 0 || (ws && aligned16(ws) && ws_bytes >= sp.total),
                "mm_mxfp4_gemm_backward: needs a workspace of %zu bytes, 16-byte aligned, got %zu",

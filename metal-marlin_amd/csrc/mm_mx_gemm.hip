@@ -265,7 +265,9 @@ extern "C" int mm_mxfp4_gemm(const void* X, int type, const uint32_t* W, const u
   MM_CHECK_ARG(type >= F32 && type <= BF16 && out_type >= F32 && out_type <= BF16,
                "mm_mxfp4_gemm: unknown type %d or %d", type, out_type);
   if (M == 0) return 0;
-  MM_CHECK_ARG(K < (1 << 24) && (size_t)mm_cdiv(M, 64) * mm_cdiv(N, 64) < ((size_t)1 << 31),
+  // rows and columns of whole tiles are counted in 31 bits, and a launch holds the blocks that
+  // stream the weights
+  MM_CHECK_ARG(K < (1 << 24) && M <= INT32_MAX - 255 && N < (1 << 29),
                "mm_mxfp4_gemm: M=%d, N=%d, K=%d is too large", M, N, K);
   MM_CHECK_ARG(X && W && S && C && aligned16(X) && aligned16(W) && aligned16(S) && aligned16(C),
                "mm_mxfp4_gemm: X, W, scales and C must be 16-byte aligned and nothing null");
@@ -300,6 +302,9 @@ extern "C" int mm_mxfp4_gemm(const void* X, int type, const uint32_t* W, const u
     MM_CHECK_LAUNCH("mm_mxfp4_gemm");
     return 0;
   }
+  const Cost& c = COSTS[p.tile];
+  MM_CHECK_ARG(launch_holds((size_t)mm_cdiv(M, c.tm) * mm_cdiv(N, c.tn), 512),
+               "mm_mxfp4_gemm: M=%d, N=%d is too large", M, N);
   uint8_t* const s = (uint8_t*)ws + sp.scales;
   if (const int rc = launch_quantize_units(X, type, M, K, kp, (uint32_t*)xq, xs, S, N, s, st)) return rc;
   void* const to = p.splits > 1 ? (void*)((char*)ws + sp.part) : C;

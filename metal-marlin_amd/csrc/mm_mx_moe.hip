@@ -378,7 +378,7 @@ extern "C" int mm_moe_mlp_mxfp4(const void* X, int type, const void* expert_ids,
     }
     const long tiles = (R + Sh::TM - 1) / Sh::TM + std::min(E, R);
     const int g1 = mm_cdiv(ip, Sh::TN / 2), g2 = mm_cdiv(H, Sh::TN);
-    MM_CHECK_ARG(tiles * std::max(g1, g2) < (1L << 30), "mm_moe_mlp_mxfp4: too many tiles");
+    MM_CHECK_ARG(launch_holds(tiles * std::max(g1, g2) + 7, Sh::NTHR), "mm_moe_mlp_mxfp4: too many tiles");
     hipLaunchKernelGGL((k_mx_moe_tile<Sh, true>), dim3((unsigned)((tiles * g1 + 7) / 8 * 8)),
                        dim3(Sh::NTHR), 0, st, xq, xs, hp, gw, gs, scale_stride(H), rows, E, 2 * I, H, g1, ip,
                        nullptr, hw, hs);

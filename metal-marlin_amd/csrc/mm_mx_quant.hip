@@ -172,12 +172,14 @@ k_mx_sum(const float* __restrict__ part, int splits, size_t n, void* __restrict_
   }
 }
 
+constexpr size_t PER = QT / 4 * QU;      // MX blocks per thread block
+
 template <int T>
 void quantize_t(const void* x, size_t rows, int K, size_t kp, uint32_t* words, uint8_t* scales,
                 Units g, hipStream_t stream) {
   const int kb = K / BLOCK, kbp = (int)(kp / BLOCK);
-  const size_t blocks = rows * kbp, per = QT / 4 * QU;
-  const uint32_t own = (uint32_t)((blocks + per - 1) / per);
+  const size_t blocks = rows * kbp;
+  const uint32_t own = (uint32_t)((blocks + PER - 1) / PER);
   if (g.pitch) {
     g.first = own;
     g.across = (g.units + 15) / 16;
@@ -193,6 +195,9 @@ void quantize_t(const void* x, size_t rows, int K, size_t kp, uint32_t* words, u
 }
 int quantize(const void* x, int type, size_t rows, int K, size_t kp, uint32_t* words, uint8_t* scales,
              const Units& g, hipStream_t stream) {
+  const size_t own = (rows * (kp / BLOCK) + PER - 1) / PER;
+  MM_CHECK_ARG(launch_holds(own + ((size_t)g.n + 63) / 64 * ((g.units + 15) / 16), QT),
+               "MXFP4 quantization: %zu rows of %d are too many", rows, K);
   if (type == F32) quantize_t<F32>(x, rows, K, kp, words, scales, g, stream);
   else if (type == F16) quantize_t<F16>(x, rows, K, kp, words, scales, g, stream);
   else quantize_t<BF16>(x, rows, K, kp, words, scales, g, stream);
@@ -202,8 +207,9 @@ int quantize(const void* x, int type, size_t rows, int K, size_t kp, uint32_t* w
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// Blocks that one launch takes: a grid has at most 2^31 - 1 thread blocks of 256 MX blocks.
-constexpr size_t MAX_BLOCKS = (size_t)1 << 38;
+// MX blocks that one launch takes: each has one thread.
+static_assert(PER == QT, "a thread per block");
+constexpr size_t MAX_BLOCKS = ((size_t)1 << 32) - 2 * QT;
 
 }  // namespace
 
@@ -222,6 +228,8 @@ int mmmx::launch_quantize_units(const void* x, int type, size_t rows, int K, siz
 int mmmx::launch_pad_scales(const uint8_t* s, size_t rows, int kb, int ks, uint8_t* out,
                             hipStream_t stream) {
   const size_t n = rows * (ks / 4);
+  MM_CHECK_ARG(launch_holds((n + QT - 1) / QT, QT), "MXFP4 scales: %zu rows of %d are too many", rows,
+               kb);
   hipLaunchKernelGGL(k_mx_pad_scales, dim3((unsigned)((n + QT - 1) / QT)), dim3(QT), 0, stream, s, n,
                      kb, ks, (uint32_t*)out);
   MM_CHECK_LAUNCH("MXFP4 scales");

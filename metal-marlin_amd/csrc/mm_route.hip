@@ -343,7 +343,9 @@ Shape shape_of(int T, int E, int groups) {
   do {                                                                                          \
     const Shape sh = shape_of(T, E, groups);                                                    \
     const int tok = NT / sh.L;                                                                  \
-    const dim3 grid((unsigned)mm_cdiv(T, tok));                                                 \
+    const size_t blocks = ((size_t)T + tok - 1) / tok;                                          \
+    MM_CHECK_ARG(mmmx::launch_holds(blocks, NT), "routing: %d tokens are too many", T);         \
+    const dim3 grid((unsigned)blocks);                                                          \
     const size_t bytes = (size_t)tok * 2 * E * sizeof(double);                                  \
     const hipStream_t st = (hipStream_t)stream;                                                 \
     if (sh.L == 16) {                                                                           \

@@ -65,7 +65,8 @@ def moe_route(logits: torch.Tensor, top_k: int, *, scoring: str = "sigmoid",
     the choice and no weight); with num_groups > 1 only those of the topk_groups groups (E /
     num_groups experts side by side) with the largest sums of their two best are eligible.  The
     weights are scale * s of the chosen, with renormalize divided by (their sum + 1e-20).  Ties go
-    to the lower index.  At most 1024 experts, 64 of them chosen, 64 groups.  NaNs rank last; a
+    to the lower index.  At most 1024 experts, 64 of them chosen, 64 groups, and fewer than 2^26
+    tokens (2^28 with up to 256 experts in up to 16 groups).  NaNs rank last; a
     softmax row of nothing but -inf has weights 0.  Differentiable in logits."""
     if isinstance(logits, torch.Tensor) and autograd.wants_grad(logits):
         return autograd.Route.apply(logits, top_k, _softmax(scoring), bias, num_groups,
