@@ -24,7 +24,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int BLOCK = 32;            // values that share a scale
 constexpr int UNIT = 256;            // k of one step of the products: 128 bytes of a row's words
-enum Type { F32 = 0, F16 = 1, BF16 = 2, CODES = 3 };
+enum Type { F32 = 0, F16 = 1, BF16 = 2 };
 
 MM_DEV uint32_t u32_of(float f) { return __builtin_bit_cast(uint32_t, f); }
 MM_DEV float f32_of(uint32_t u) { return __builtin_bit_cast(float, u); }
