@@ -13,8 +13,10 @@
 // off).  Products are exact, sums fp32, rounded once.
 //
 // Bound by LDS and the matrix cores in turn: a stage of a 128 x 256 tile reads 128 KiB of operands
-// and writes 58, about 0.5 us, and multiplies for 0.43; it takes 1.17 (2048 x 14336 x 4096: 268 us
-// of bf16, 0.9 PFLOP/s; 324 of fp16, 588 with two terms throughout).
+// and writes 58, about 0.5 us, and multiplies for 0.43; it takes 1.2 where the last-level cache
+// holds the operands (2048 x 14336 x 4096: 270 us of bf16, 0.89 PFLOP/s; 323 of fp16, 588 with two
+// terms throughout; 1093 of fp32).  Where they come out of HBM (eight sets of operands in turn) bf16
+// takes 326 us, 0.74 PFLOP/s.
 #include <algorithm>
 
 #include "mm_mx_gemm.h"
@@ -323,7 +325,8 @@ constexpr size_t COUNTERS = 65536;
 
 // Tiles of dX: a stage of the only block on a CU takes `one` us, of two that share it `two`, a
 // block's beginning and end `ends` (bf16; measured at 64 .. 2048 rows of 14336 x 4096, 4096 x 14336
-// and 4096 x 4096; fp16 takes 1.2 times as long, which changes no choice).
+// and 4096 x 4096, operands in the last-level cache; fp16 takes 1.2 times as long, which changes no
+// choice).
 struct Cost {
   int tm, tk;
   float one, two, ends;
@@ -336,7 +339,7 @@ struct Plan {
   int tile, splits, per, stages;
 };
 // With few tiles N is split, and the splits' sums are joined by another launch: 2.5 us and their
-// bytes at about 3 TB/s.  us, best tile and split: 2048 x 14336 x 4096 268 (of 64 x 128 524, in two
+// bytes at about 3 TB/s.  us, best tile and split: 2048 x 14336 x 4096 270 (of 64 x 128 524, in two
 // splits 298), 509 x 4096 x 4096 35 in four (unsplit 79), 128 x 4096 x 4096 22 (30 of 128 x 256).
 Plan plan_of(int M, int N, int K, int type) {
   Plan best{0, 1, 0, mm_cdiv(N, type == F32 ? 32 : 64)};

@@ -121,10 +121,11 @@ constexpr int SKINNY_M = 16;    // rows that the kernel may quantize itself
 constexpr int CODES_M = 64;     // rows that stream the weights from codes
 constexpr size_t COUNTERS = 65536;   // head of every workspace: other products' arrival counters
 
-// Whether the blocks quantize x themselves.  Each of them does it anew, so from about 16384 values
-// on (4 rows of 4096) a launch that does it once is faster: us, in the kernel against apart,
-// 4096 -> 14336 M = 8 11.5 / 10.1, M = 16 17.4 / 10.4, M = 4 8.8 in the kernel; 14336 -> 4096 M = 1
-// 7.1 / 9.2, M = 2 8.4 / 9.3, M = 4 12.8 / 9.3.
+// Whether the blocks quantize x themselves.  Each of them does it anew, so from some number of values
+// on a launch that does it once is faster: us, in the kernel against apart, 4096 -> 14336 M = 8
+// 11.5 / 10.1, M = 16 17.4 / 10.4, M = 4 8.8 in the kernel; 14336 -> 4096 M = 1 7.1 / 9.2, M = 2
+// 8.4 / 9.3, M = 4 12.8 / 9.3.  The border lies between 16384 and 28672 values; it is drawn at 20480,
+// which costs the last M = 2 (28672) 0.9 us.
 bool quantizes_itself(int M, int K) { return M <= SKINNY_M && (long)M * K <= 16384 + 4096; }
 
 template <int T, int NT, int NW, int D, int U>

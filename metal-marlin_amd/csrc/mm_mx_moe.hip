@@ -5,8 +5,12 @@
 // sum over a token's experts in slot order.  With many rows per expert a launch before them
 // quantizes the tokens once; with few the gate_up kernel does it on the way.
 //
-// Both products are bound by the weights' bytes until an expert has some hundred rows: every expert
-// that has a row is streamed once.
+// Both products are bound by the weights' bytes until an expert has some hundred rows.  Where the
+// weights are streamed (few rows per expert on average) a block takes an expert's rows sixteen at a
+// time, one sixteen after the other, and streams its part of the weights for each: once for most
+// experts, but where one expert has most of the rows that expert's blocks work alone.  128 experts of
+// 2048 -> 768, one per token: 64 tokens spread 35 us, all to one expert 55; 511 tokens 94 and 355,
+// where 512, in tiles, take 89 and 31.
 #include <algorithm>
 
 #include "mm_mx_gemm.h"

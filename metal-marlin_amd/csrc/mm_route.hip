@@ -1,8 +1,9 @@
-// Routing of tokens to experts as current mixtures do it, from given logits [T, E], and its
+// Routing of tokens to experts with a balance bias and groups, from given logits [T, E], and its
 // gradient.  For a token with logits l:
 //   s = sigmoid(l) or softmax(l);  c = s + b   (b: the experts' balance bias, may be null)
 //   experts lie in G groups of E / G side by side; a group's score is the sum of its two largest
-//   c; only experts of the best `keep` groups are eligible
+//   c, without a bias too (routing that ranks groups by their best expert alone is another rule);
+//   only experts of the best `keep` groups are eligible
 //   ids = the k eligible experts with the largest c, in that order; ties to the lower index
 //   w = scale * s[ids] (/ (sum of s[ids] + 1e-20))
 // A NaN c ranks below every other value; a row of softmax without a value above -inf has s = 0.
@@ -13,8 +14,8 @@
 // forms), and the bytes, 2 to 4 per logit, are what the kernels wait for.
 //
 // L lanes share a token (16 where the token fits and there are many tokens, else 64), expert
-// l + L * slot to lane l.  Bound by latency: 32 tokens of 256 experts, 8 of them, 8.7-10 us, 4096
-// of 128 9.8-11 and the gradient 5.5.
+// l + L * slot to lane l.  Bound by latency: 32 tokens of 256 experts, 8 of them, 9-10 us, 4096
+// of 128 10-11 and the gradient 5.6.
 #include <type_traits>
 
 #include "mm_common.h"

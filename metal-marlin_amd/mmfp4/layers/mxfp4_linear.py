@@ -13,7 +13,8 @@ __all__ = ["MXFP4Linear"]
 
 class MXFP4Linear(nn.Module):
     """y = q(x) @ W^T (+ bias) in x's type, W MXFP4: packed_weights [out, in/8] words and scales
-    uint8 [out, in/32].  Differentiable in x, straight through its rounding; the weights are
+    uint8 [out, in/32].  As in MMFP4Linear the bias is added to the product in its type: two
+    roundings.  Differentiable in x, straight through its rounding; the weights are
     frozen, and a bias that requires a gradient gets it."""
 
     def __init__(self, packed_weights: torch.Tensor, scales: torch.Tensor,

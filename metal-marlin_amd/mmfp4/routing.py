@@ -61,9 +61,11 @@ def moe_route(logits: torch.Tensor, top_k: int, *, scoring: str = "sigmoid",
               renormalize: bool = True, scale: float = 1.0):
     """logits [*, E] -> (weights fp32 [*, top_k], ids int64 [*, top_k]).
 
-    s = sigmoid(logits) or softmax(logits).  Experts are ranked by s + bias (bias [E], which moves
-    the choice and no weight); with num_groups > 1 only those of the topk_groups groups (E /
-    num_groups experts side by side) with the largest sums of their two best are eligible.  The
+    s = sigmoid(logits) or softmax(logits).  Experts are ranked by s + bias (bias [E], taken as
+    fp32, which moves the choice and no weight); with num_groups > 1 only those of the topk_groups
+    groups (E / num_groups experts side by side) with the largest sums of their two best s + bias
+    are eligible.  That is so without a bias too: where a model ranks its groups by their best
+    expert alone, these are not its experts.  The
     weights are scale * s of the chosen, with renormalize divided by (their sum + 1e-20).  Ties go
     to the lower index.  At most 1024 experts, 64 of them chosen, 64 groups, and fewer than 2^26
     tokens (2^28 with up to 256 experts in up to 16 groups).  NaNs rank last; a
